@@ -34,8 +34,10 @@ extern "C" {
 #define TCMI_ERR_HIP (-2)
 #define TCMI_C64 0
 #define TCMI_C128 1
-#define TCMI_F32 2   /* real dtypes: tcmi_allreduce_sum only */
+#define TCMI_F32 2   /* real dtypes: tcmi_allreduce_sum, the training operators */
 #define TCMI_F64 3
+#define TCMI_F16 4   /* the training operators only */
+#define TCMI_BF16 5
 
 /* library / runtime probes */
 int tcmi_version(void);
@@ -389,6 +391,58 @@ int tcmi_comm_unique_id(void* id_out_host);
 int tcmi_comm_init(const void* id_host, int rank, int world, void** comm_out_host);
 int tcmi_allreduce_sum(void* comm, void* buf, long long count, int dtype, void* stream);
 int tcmi_comm_destroy(void* comm);
+
+/* ---- training operators (matrix-shaped parameters and a head over many classes) --------------------------------------
+ * Newton-Schulz orthogonalisation: N = |G|_F + eps, X = G / N, then `steps` times A = X X^H, X <- a X + (b A + c A A) X with
+ * (a, b, c) = coef_host[3 i .. 3 i + 2] (host memory, float64).  g: [batch] matrices of rows x cols with element strides
+ * rs / cs / bs; out: contiguous, same dtype (TCMI_F32, TCMI_F16, TCMI_BF16 or TCMI_C64).  full = 1: two f16 pieces per
+ * operand (f32 accuracy), 0: one (results of bf16 accuracy).  saved (full only, may be NULL): what the gradient needs.
+ * Coefficients that let a singular value grow past 64 are refused.  Workspaces: tcmi_ns_work_bytes(.., what) bytes,
+ * 256-byte aligned, contents undefined; nothing is kept in them between calls.  A matrix with a non-finite entry gives NaN.
+ * No counterpart in the reference, whose orthogonal factors come from its backends' svd / qr
+ * (tensorcircuit/backends/abstract_backend.py `svd`, `qr`). */
+#define TCMI_NS_MAX_STEPS 16
+#define TCMI_NS_WORK 0          /* tcmi_newton_schulz without `saved`, tcmi_muon_step */
+#define TCMI_NS_WORK_SAVING 1   /* tcmi_newton_schulz with `saved` */
+#define TCMI_NS_SAVED 2         /* `saved` itself */
+#define TCMI_NS_WORK_GRAD 3     /* tcmi_newton_schulz_grad */
+long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full, int dtype, int what);
+int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long g_bs, void* out, int rows, int cols, int batch,
+                       int steps, const double* coef_host, double eps, int full, void* saved, long long saved_bytes, void* work,
+                       long long work_bytes, int dtype, void* stream);
+
+/* Its gradient: dg (contiguous) = the pullback of dout through the iteration that filled `saved` (same g, sizes, steps,
+ * coefficients and eps); complex: dL/dRe + i dL/dIm.  `saved` is only read. */
+int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long long g_bs, const void* dout, long long d_rs,
+                            long long d_cs, long long d_bs, void* dg, int rows, int cols, int batch, int steps,
+                            const double* coef_host, double eps, const void* saved, long long saved_bytes, void* work,
+                            long long work_bytes, int dtype, void* stream);
+
+/* One optimiser step in place: buf <- momentum buf + (1 - momentum) grad (f32), u = buf or, nesterov,
+ * (1 - momentum) grad + momentum buf; param <- keep param + rate * newton_schulz(u).  Real dtypes; param and grad share one. */
+int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, const void* grad, long long g_rs, long long g_cs,
+                   long long g_bs, float* buf, long long b_rs, long long b_cs, long long b_bs, int rows, int cols, int batch,
+                   double momentum, int nesterov, double keep, double rate, int steps, const double* coef_host, double eps,
+                   int full, void* work, long long work_bytes, int dtype, void* stream);
+
+/* Softmax cross entropy of a linear head, logits never stored: h [tokens][features], w [classes][features] (row strides
+ * h_rs, w_rs; features contiguous), bias [classes] or NULL, all of one dtype (TCMI_F32 / F16 / BF16); target int64.
+ * Writes lse[tokens], loss[tokens] (f32; 0 for target == ignore_index, NaN for any other target outside [0, classes)) and,
+ * with `total` given, the sum (mean = 0) or mean over the rows that count, and their number.
+ * No counterpart in the reference: it leaves classical heads to the host framework (tensorcircuit/torchnn.py). */
+long long tcmi_lce_work_bytes(const void* h, long long h_rs, const void* w, long long w_rs, int tokens, int features, int classes,
+                              int dtype, int backward_pass);
+int tcmi_linear_cross_entropy(const void* h, long long h_rs, const void* w, long long w_rs, const void* bias, const long long* target,
+                              long long ignore_index, int tokens, int features, int classes, float* lse, float* loss, float* total,
+                              float* count, int mean, void* work, long long work_bytes, int dtype, void* stream);
+
+/* Its gradients (contiguous, dtype of the inputs; NULL: not wanted).  dloss: f32 [tokens] (per_row = 1) or one value,
+ * divided by *count when count is given (mean).  lse from the forward call.  Ignored rows contribute nothing, whatever
+ * they hold, and get a zero gradient. */
+int tcmi_linear_cross_entropy_grad(const void* h, long long h_rs, const void* w, long long w_rs, const void* bias,
+                                   const long long* target, long long ignore_index, int tokens, int features, int classes,
+                                   const float* lse, const float* dloss, int per_row, const float* count, void* dh, void* dw, void* db,
+                                   void* work, long long work_bytes, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

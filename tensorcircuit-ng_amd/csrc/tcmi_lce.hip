@@ -1,0 +1,687 @@
+// Softmax cross entropy of a linear head over many classes, without its logits:
+//   l[t][v] = <h_t, w_v> + b_v,   loss_t = log sum_v exp l[t][v] - l[t][y_t],
+//   P = exp(l - lse) - onehot(y),  dh_t = r_t P_t w,  dw = P^T (r h),  db = P^T r      (r_t = dloss_t, 0 for ignored rows)
+// Forward: one product on the matrix pipe whose epilogue keeps, per row and tile of classes, the running maximum and the
+// sum of exponentials (T x V / 128 pairs instead of T x V logits).  Backward: per piece of the classes the logits are
+// formed again, become P (f16, row-major and transposed) in the epilogue, and two products use it while it is there.
+// Bound by the matrix pipe: 2 T D V multiply-adds forward, 6 T D V more backward.
+//
+// Operand precision.  bf16 / f16 heads: the logits from the inputs as they are (products exact in the f32 accumulator);
+// P is one f16 piece under 2^14 (2^-11 relative; bf16 would cost 2^-8), h and w enter the two gradient products as f16
+// under a power of two taken from their largest value (exact for 8- and 11-bit significands down to 2^-29 of it).
+// f32 heads: two f16 pieces everywhere (2^-22), three products per product.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include "../../include/tcmi.h"
+#include "tcmi_mm16.h"
+
+extern "C" int tcmi_set_error_(int code, const char* msg);
+
+namespace tcmi {
+namespace lce {
+
+using namespace mm16;
+
+constexpr float PSCALE = 16384.f;            // P lies in [-1, 1]
+constexpr int PARTS = 256;
+
+template <int DT>
+__device__ __forceinline__ float fetch(const void* p, long long at) {
+  if constexpr (DT == TCMI_F32) return ((const float*)p)[at];
+  else if constexpr (DT == TCMI_F16) return (float)((const f16*)p)[at];
+  else return (float)((const __bf16*)p)[at];
+}
+__device__ __forceinline__ float fetch_any(const void* p, int dt, long long at) {
+  return dt == TCMI_F32 ? ((const float*)p)[at] : dt == TCMI_F16 ? (float)((const f16*)p)[at] : (float)((const __bf16*)p)[at];
+}
+__device__ __forceinline__ void put(void* p, int dt, long long at, float v) {
+  if (dt == TCMI_F32) ((float*)p)[at] = v;
+  else if (dt == TCMI_F16) ((f16*)p)[at] = (f16)v;
+  else ((__bf16*)p)[at] = (__bf16)v;
+}
+
+// power of two that brings `top` into [2^14, 2^15); 1 for zero and for what is not finite
+__device__ __forceinline__ float scale_of(float top) {
+  const unsigned e = __float_as_uint(top) >> 23;
+  if (e == 0 || e >= 255) return 1.f;
+  const int k = 14 - ((int)e - 127);
+  return ldexpf(1.f, k > 100 ? 100 : k < -100 ? -100 : k);
+}
+
+// Rows of an operand, k padded to 64.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per
+// row, whose inverse goes to inv[row].  One wave per row, the second read comes from the cache.
+template <int DT>
+__global__ __launch_bounds__(256) void rows_kernel(const void* src, long long rs, int rows, int cols, int colsp, void* hi, f16* lo,
+                                                   float* inv) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const long long in = row * rs, out = (long long)row * colsp;
+  if constexpr (DT == TCMI_F32) {
+    const float* p = (const float*)src + in;
+    float top = 0.f;
+    for (int c = lane; c < cols; c += 64) top = fmaxf(top, fabsf(p[c]));
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float s = scale_of(top);
+    for (int c = lane; c < colsp; c += 64) {
+      f16 h, l;
+      two_pieces(c < cols ? p[c] * s : 0.f, h, l);
+      ((f16*)hi)[out + c] = h;
+      lo[out + c] = l;
+    }
+    if (lane == 0) inv[row] = 1.f / s;
+  } else {
+    const unsigned short* p = (const unsigned short*)src + in;
+    for (int c = lane; c < colsp; c += 64) ((unsigned short*)hi)[out + c] = c < cols ? p[c] : 0;
+  }
+}
+
+// r_t: the factor of row t in the gradients
+__global__ __launch_bounds__(256) void factor_kernel(const long long* y, long long ignore, const float* dloss, int per_row,
+                                                     const float* count, int T, float* r) {
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= T) return;
+  const float g = per_row ? dloss[t] : count ? dloss[0] / count[0] : dloss[0];
+  r[t] = y[t] == ignore ? 0.f : g;
+}
+
+// partial maxima of |x| (times a row factor; rows whose factor is zero do not count)
+template <int DT>
+__global__ __launch_bounds__(256) void top_kernel(const void* src, long long rs, int rows, int cols, const float* r, float* part) {
+  __shared__ float red[4];
+  float top = 0.f;
+  const int lane = threadIdx.x & 63;
+  for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4) {
+    const float f = r ? fabsf(r[row]) : 1.f;
+    if (f == 0.f) continue;
+    for (int c = lane; c < cols; c += 64) top = fmaxf(top, fabsf(fetch<DT>(src, row * rs + c)) * f);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// out[c][row] = src[row][c] * r[row] * scale as f16 pieces, rows padded to 64 with zeros.  A zero factor gives zero
+// whatever the row holds.
+template <int DT>
+__global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs, int rows, int cols, const float* r,
+                                                   const float* part, int nparts, f16* hi, f16* lo, long long ldt, float* inv) {
+  __shared__ float tile[64][65];
+  __shared__ float red[4];
+  const int tid = threadIdx.x, u = tid & 63, w = tid >> 6;
+  float top = 0.f;
+  for (int k = tid; k < nparts; k += 256) top = fmaxf(top, part[k]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (u == 0) red[w] = top;
+  __syncthreads();
+  const float s = scale_of(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  if (r0 == 0 && c0 == 0 && tid == 0) *inv = 1.f / s;
+#pragma unroll 4
+  for (int k = w; k < 64; k += 4) {
+    const int row = r0 + k, c = c0 + u;
+    float x = 0.f;
+    if (row < rows && c < cols) {
+      const float f = r ? r[row] : 1.f;
+      if (f != 0.f) x = fetch<DT>(src, row * rs + c) * f * s;
+    }
+    tile[k][u] = x;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int k = w; k < 64; k += 4) {
+    const int c = c0 + k, row = r0 + u;
+    if (c < cols) {                                  // the grid covers the padded rows exactly
+      f16 h, l;
+      two_pieces(tile[u][k], h, l);
+      hi[c * ldt + row] = h;
+      if (lo) lo[c * ldt + row] = l;
+    }
+  }
+}
+
+// logits of a tile: acc times the rows' scales plus the bias
+struct Logits {
+  const float *hs, *ws;          // f32: inverse scales of the rows of h and of w (null: 1)
+  const void* bias;              // null: none
+  int dtype;
+  int v0;                        // first class of the piece
+};
+
+template <class T>
+__device__ __forceinline__ void logits(const Logits& q, const Args& g, int m0, int n0, f32x4 (&acc)[T::MI][T::NI]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+#pragma unroll
+  for (int j = 0; j < T::NI; ++j) {
+    const int col = n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4);
+    f32x4 cs, cb;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = min(col + r, g.N - 1) + q.v0;
+      cs[r] = q.ws ? q.ws[c] : 1.f;
+      cb[r] = q.bias ? fetch_any(q.bias, q.dtype, c) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) {
+      const int row = min(m0 + wm * T::MI * 16 + i * 16 + (lane & 15), g.M - 1);
+      const float rs = q.hs ? q.hs[row] : 1.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(acc[i][j][r] * rs, cs[r], cb[r]);
+    }
+  }
+}
+
+// forward: per row the tile's maximum and sum of exponentials, and the target's logit where it lies in the tile
+struct EpiLse {
+  Logits q;
+  float2* part;                  // [T][tiles of classes]
+  float* target;                 // [T]
+  const long long* y;
+  template <class T>
+  __device__ void tile(const Args& g, int m0, int n0, int, bool, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
+    logits<T>(q, g, m0, n0, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+    float2* stat = reinterpret_cast<float2*>(lds);                    // [WN][BM]
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) {
+      const int rl = wm * T::MI * 16 + i * 16 + (lane & 15), row = m0 + rl;
+      const long long yt = row < g.M ? y[row] : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j) {
+        const int col = n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (col + r >= g.N) acc[i][j][r] = -INFINITY;
+          else if (col + r == yt) target[row] = acc[i][j][r];
+          top = fmaxf(top, acc[i][j][r]);
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float at = top == -INFINITY ? 0.f : top;                  // a row of -inf has sum 0, not NaN
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < T::NI; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += __expf(acc[i][j][r] - at);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (lane < 16) stat[wn * T::BM + rl] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int rl = threadIdx.x; rl < T::BM; rl += T::THREADS) {
+      if (m0 + rl >= g.M) continue;
+      float2 a = stat[rl];
+#pragma unroll
+      for (int k = 1; k < T::WN; ++k) {
+        const float2 b = stat[k * T::BM + rl];
+        const float top = fmaxf(a.x, b.x), at = top == -INFINITY ? 0.f : top;
+        a = make_float2(top, a.y * __expf(a.x - at) + b.y * __expf(b.x - at));
+      }
+      part[(long long)(m0 + rl) * g.tn + n0 / T::BN] = a;
+    }
+  }
+};
+
+// joins the tiles of a row: one wave per row
+__global__ __launch_bounds__(256) void join_kernel(const float2* part, int tiles, const float* target, const long long* y,
+                                                   long long ignore, int T, int V, float* lse, float* loss) {
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (t >= T) return;
+  const float2* p = part + (long long)t * tiles;
+  float top = -INFINITY, bad = 0.f;
+  for (int k = lane; k < tiles; k += 64) {
+    top = fmaxf(top, p[k].x);
+    if (p[k].y != p[k].y) bad = p[k].y;              // fmaxf drops a NaN, the sums do not
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float at = top == -INFINITY ? 0.f : top;
+  float sum = bad;
+  for (int k = lane; k < tiles; k += 64) sum += p[k].x == -INFINITY ? 0.f : p[k].y * expf(p[k].x - at);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) {
+    const float l = at + logf(sum);
+    lse[t] = l;
+    const long long yt = y[t];
+    loss[t] = yt == ignore ? 0.f : yt < 0 || yt >= V ? NAN : l - target[t];
+  }
+}
+
+// sum or mean over the rows that count, in f64 and a fixed order
+__global__ __launch_bounds__(1024) void total_kernel(const float* loss, const long long* y, long long ignore, int T, int mean,
+                                                     float* out, float* count) {
+  __shared__ double rs[16];
+  __shared__ int rc[16];
+  double s = 0.0;
+  int c = 0;
+  for (int t = threadIdx.x; t < T; t += 1024) {
+    s += loss[t];
+    c += y[t] != ignore;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    s += __shfl_xor(s, o);
+    c += __shfl_xor(c, o);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    rs[threadIdx.x >> 6] = s;
+    rc[threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    c = 0;
+    for (int k = 0; k < 16; ++k) {
+      s += rs[k];
+      c += rc[k];
+    }
+    *count = (float)c;
+    *out = (float)(mean ? s / c : s);                // no row counts: 0 / 0
+  }
+}
+
+// backward: P as f16 pieces, row-major for dh and transposed for dw, zero in the padding and in ignored rows
+struct EpiProb {
+  Logits q;
+  const float* lse;
+  const long long* y;
+  long long ignore;
+  int V;
+  f16 *hi, *lo, *thi, *tlo;
+  long long ld, ldt;             // padded classes of the piece, padded rows
+  template <class T>
+  __device__ void tile(const Args& g, int m0, int n0, int, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+    logits<T>(q, g, m0, n0, acc);
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 x) {
+      const bool in = row < g.M;
+      const long long yt = in ? y[row] : ignore;
+      const bool keep = in && yt != ignore, bad = keep && (yt < 0 || yt >= V);
+      const float l = keep ? lse[row] : 0.f;
+      f16x4 vh, vl;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float p = 0.f;
+        if (keep && col + r < g.N) {
+          p = __expf(x[r] - l);
+          if (col + r + q.v0 == yt) p -= 1.f;
+          if (bad) p = NAN;
+        }
+        f16 a, b;
+        two_pieces(p * PSCALE, a, b);
+        vh[r] = a;
+        vl[r] = b;
+      }
+      if (in && col < ld) {
+        *reinterpret_cast<f16x4*>(hi + row * ld + col) = vh;
+        if (lo) *reinterpret_cast<f16x4*>(lo + row * ld + col) = vl;
+      }
+      if (row < ldt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (col + r < g.N) {
+            thi[(col + r) * ldt + row] = vh[r];
+            if (tlo) tlo[(col + r) * ldt + row] = vl[r];
+          }
+      }
+    });
+  }
+};
+
+// a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor
+struct EpiGrad {
+  const float* inv;              // inverse of the other operand's scale, on the device
+  float* sum;                    // f32 [rows][N] (null: only one piece)
+  int first, last;
+  const float* r;                // null: 1
+  void* out;
+  int dtype;
+  template <class T>
+  __device__ void tile(const Args& g, int m0, int n0, int, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+    const float al = *inv * (1.f / PSCALE);
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
+      if (row >= g.M) return;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (col + k >= g.N) continue;
+        const long long at = (long long)row * g.N + col + k;
+        float x = al * v[k];
+        if (!first) x += sum[at];
+        if (!last) sum[at] = x;
+        else put(out, dtype, at, r ? (r[row] == 0.f ? 0.f : x * r[row]) : x);
+      }
+    });
+  }
+};
+
+// db_v = sum_t P[t][v] r_t from the transposed pieces: one wave per class
+__global__ __launch_bounds__(256) void bias_kernel(const f16* hi, const f16* lo, long long ldt, const float* r, int T, int vc, void* out,
+                                                   int dtype, int v0) {
+  const int v = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (v >= vc) return;
+  float s = 0.f;
+  for (int t = lane; t < T; t += 64) {
+    float p = (float)hi[v * ldt + t];
+    if (lo) p += (float)lo[v * ldt + t];
+    s = fmaf(p, r[t], s);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if (lane == 0) put(out, dtype, (long long)v0 + v, s * (1.f / PSCALE));
+}
+
+// ---------------------------------------------------------------------------------------------------------- host side
+using TileL = Tile<128, 128, 2, 2>;
+
+struct Arena {
+  char* base;
+  long long used = 0;
+  template <class P>
+  P* take(long long count) {
+    P* p = base ? reinterpret_cast<P*>(base + used) : nullptr;
+    used += (count * (long long)sizeof(P) + 255) & ~255ll;
+    return p;
+  }
+};
+
+struct Shape {
+  int T, D, V, dtype;
+  int dp, tp;                    // padded features, padded rows
+  bool split;                    // f32: two pieces
+  bool h_direct, w_direct;       // the operand is read where it lies
+};
+
+struct Rows {                    // the forward operands when they are not read in place
+  void *h, *w;
+  f16 *hl, *wl;
+  float *hs, *ws;
+};
+
+Rows take_rows(Arena& a, const Shape& s) {
+  Rows r{};
+  if (!s.h_direct) r.h = a.take<f16>((long long)s.T * s.dp);
+  if (!s.w_direct) r.w = a.take<f16>((long long)s.V * s.dp);
+  if (s.split) {
+    r.hl = a.take<f16>((long long)s.T * s.dp);
+    r.wl = a.take<f16>((long long)s.V * s.dp);
+    r.hs = a.take<float>(s.T);
+    r.ws = a.take<float>(s.V);
+  }
+  return r;
+}
+
+struct FwdWork {
+  Rows rows;
+  float2* part;
+  float* target;
+};
+
+FwdWork take_fwd(Arena& a, const Shape& s) {
+  FwdWork w{};
+  w.rows = take_rows(a, s);
+  w.part = a.take<float2>((long long)s.T * ((s.V + TileL::BN - 1) / TileL::BN));
+  w.target = a.take<float>(s.T);
+  return w;
+}
+
+// classes per piece of the backward: P and its transpose take at most about 1 GiB, pieces of equal size
+int piece_of(const Shape& s) {
+  const long long per = (long long)(s.T + s.tp) * 2 * (s.split ? 2 : 1);
+  long long most = (1ll << 30) / per / 256 * 256;
+  if (most < 1024) most = 1024;
+  const long long pieces = (s.V + most - 1) / most;
+  const long long c = ((s.V + pieces - 1) / pieces + 255) / 256 * 256;
+  return (int)(c < s.V ? c : s.V);
+}
+
+struct BwdWork {
+  Rows rows;
+  float *r, *parth, *partw, *invh, *invw, *sum;
+  f16 *ph, *pl, *qh, *ql, *th, *tl, *wh, *wl;      // P, P^T, h^T, w^T of the piece
+};
+
+BwdWork take_bwd(Arena& a, const Shape& s) {
+  BwdWork w{};
+  const long long vc = piece_of(s), vp = (vc + 63) & ~63ll;
+  w.rows = take_rows(a, s);
+  w.r = a.take<float>(s.T);
+  w.parth = a.take<float>(PARTS);
+  w.partw = a.take<float>(PARTS);
+  w.invh = a.take<float>(1);
+  w.invw = a.take<float>(1);
+  w.sum = vc < s.V ? a.take<float>((long long)s.T * s.D) : nullptr;
+  w.ph = a.take<f16>(s.T * vp);
+  w.qh = a.take<f16>(vc * s.tp);
+  w.th = a.take<f16>((long long)s.D * s.tp);
+  w.wh = a.take<f16>(s.D * vp);
+  if (s.split) {
+    w.pl = a.take<f16>(s.T * vp);
+    w.ql = a.take<f16>(vc * s.tp);
+    w.tl = a.take<f16>((long long)s.D * s.tp);
+    w.wl = a.take<f16>(s.D * vp);
+  }
+  return w;
+}
+
+#define TRY(x)                                   \
+  do {                                           \
+    const hipError_t e_ = (x);                   \
+    if (e_ != hipSuccess) return e_;             \
+  } while (0)
+
+#define BY_TYPE(dt, K, ...)                                                                        \
+  do {                                                                                             \
+    if ((dt) == TCMI_F32) hipLaunchKernelGGL(K<TCMI_F32>, __VA_ARGS__);                            \
+    else if ((dt) == TCMI_F16) hipLaunchKernelGGL(K<TCMI_F16>, __VA_ARGS__);                       \
+    else hipLaunchKernelGGL(K<TCMI_BF16>, __VA_ARGS__);                                            \
+  } while (0)
+
+template <class Epi>
+hipError_t run(Args& g, int dtype, const Epi& e, hipStream_t st) {
+  unsigned blocks;
+  if (!plan<TileL>(g, 1, false, &blocks)) return hipErrorInvalidValue;
+  if (dtype == TCMI_BF16) hipLaunchKernelGGL((product_kernel<bf16x8, TileL, Epi>), dim3(blocks), dim3(TileL::THREADS), 0, st, g, e);
+  else hipLaunchKernelGGL((product_kernel<f16x8, TileL, Epi>), dim3(blocks), dim3(TileL::THREADS), 0, st, g, e);
+  return hipGetLastError();
+}
+
+void pairs(Args& g, const void* ah, const void* al, const void* bh, const void* bl) {
+  auto add = [&](const void* a, const void* b) {
+    g.a[g.nseg] = a;
+    g.b[g.nseg] = b;
+    ++g.nseg;
+  };
+  add(ah, bh);
+  if (bl) add(ah, bl);
+  if (al) add(al, bh);
+}
+
+struct In {
+  const void *h, *w, *bias;
+  long long hrs, wrs;
+  const long long* y;
+  long long ignore;
+};
+
+hipError_t operands(const Shape& s, const In& in, const Rows& r, hipStream_t st) {
+  if (!s.h_direct) {
+    BY_TYPE(s.dtype, rows_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, s.dp, r.h, r.hl, r.hs);
+    TRY(hipGetLastError());
+  }
+  if (!s.w_direct) {
+    BY_TYPE(s.dtype, rows_kernel, dim3((s.V + 3) / 4), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, s.dp, r.w, r.wl, r.ws);
+    TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+// the logits' product for the classes [v0, v0 + vc)
+Args logit_args(const Shape& s, const In& in, const Rows& r, int v0, int vc) {
+  Args g{};
+  g.M = s.T;
+  g.N = vc;
+  g.K = s.dp;
+  g.lda = s.h_direct ? in.hrs : s.dp;
+  g.ldb = s.w_direct ? in.wrs : s.dp;
+  const void* h = s.h_direct ? in.h : r.h;
+  const f16* w = (const f16*)(s.w_direct ? in.w : r.w) + v0 * g.ldb;
+  pairs(g, h, r.hl, w, r.wl ? r.wl + v0 * g.ldb : nullptr);
+  return g;
+}
+
+hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, float* loss, float* total, float* count, int mean,
+                   hipStream_t st) {
+  TRY(operands(s, in, w.rows, st));
+  Args g = logit_args(s, in, w.rows, 0, s.V);
+  EpiLse e{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y};
+  TRY(run(g, s.dtype, e, st));
+  hipLaunchKernelGGL(join_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, w.part, g.tn, w.target, in.y, in.ignore, s.T, s.V, lse, loss);
+  TRY(hipGetLastError());
+  if (total) {
+    hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, in.y, in.ignore, s.T, mean, total, count);
+    TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float* lse, const float* dloss, int per_row, const float* count,
+                    void* dh, void* dw, void* db, hipStream_t st) {
+  TRY(operands(s, in, w.rows, st));
+  hipLaunchKernelGGL(factor_kernel, dim3((s.T + 255) / 256), dim3(256), 0, st, in.y, in.ignore, dloss, per_row, count, s.T, w.r);
+  TRY(hipGetLastError());
+  auto blocks = [](int rows) { return rows / 4 < 1 ? 1 : rows / 4 > PARTS ? PARTS : rows / 4; };
+  const float* none = nullptr;
+  if (dw) {
+    const int nb = blocks(s.T);
+    BY_TYPE(s.dtype, top_kernel, dim3(nb), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, w.r, w.parth);
+    TRY(hipGetLastError());
+    BY_TYPE(s.dtype, turn_kernel, dim3(s.tp / 64, (s.D + 63) / 64), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, w.r, w.parth, nb, w.th,
+            w.tl, (long long)s.tp, w.invh);
+    TRY(hipGetLastError());
+  }
+  const int nbw = blocks(s.V);
+  if (dh) {
+    BY_TYPE(s.dtype, top_kernel, dim3(nbw), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, none, w.partw);
+    TRY(hipGetLastError());
+  }
+  const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
+  for (int v0 = 0; v0 < s.V; v0 += vc) {
+    const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (n + 63) & ~63;
+    Args g = logit_args(s, in, w.rows, v0, n);
+    EpiProb e{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.ph, w.pl, w.qh, w.ql, np, s.tp};
+    TRY(run(g, s.dtype, e, st));
+    if (dh) {
+      BY_TYPE(s.dtype, turn_kernel, dim3(np / 64, (s.D + 63) / 64), dim3(256), 0, st, (const char*)in.w + v0 * in.wrs * size, in.wrs, n,
+              s.D, none, w.partw, nbw, w.wh, w.wl, (long long)np, w.invw);
+      TRY(hipGetLastError());
+      Args d{};
+      d.M = s.T;
+      d.N = s.D;
+      d.K = np;
+      d.lda = np;
+      d.ldb = np;
+      pairs(d, w.ph, w.pl, w.wh, w.wl);
+      EpiGrad eh{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype};
+      TRY(run(d, TCMI_F16, eh, st));
+    }
+    if (dw) {
+      Args d{};
+      d.M = n;
+      d.N = s.D;
+      d.K = s.tp;
+      d.lda = s.tp;
+      d.ldb = s.tp;
+      pairs(d, w.qh, w.ql, w.th, w.tl);
+      EpiGrad ew{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype};
+      TRY(run(d, TCMI_F16, ew, st));
+    }
+    if (db) {
+      hipLaunchKernelGGL(bias_kernel, dim3((n + 3) / 4), dim3(256), 0, st, w.qh, w.ql, (long long)s.tp, w.r, s.T, n, db, s.dtype, v0);
+      TRY(hipGetLastError());
+    }
+  }
+  return hipSuccess;
+}
+
+bool shape_ok(int T, int D, int V, int dtype) {
+  return T >= 1 && D >= 1 && V >= 1 && T <= (1 << 26) && D <= (1 << 20) && V <= (1 << 28) &&
+         (dtype == TCMI_F32 || dtype == TCMI_F16 || dtype == TCMI_BF16);
+}
+
+// an operand is read in place when its rows are whole k steps and 16-byte aligned
+bool direct(const void* p, long long rs, int D, int dtype) {
+  return dtype != TCMI_F32 && D % 64 == 0 && rs % 8 == 0 && rs < (1ll << 22) && ((uintptr_t)p & 15) == 0;
+}
+
+Shape shape_of(int T, int D, int V, int dtype, bool h_direct, bool w_direct) {
+  Shape s{};
+  s.T = T;
+  s.D = D;
+  s.V = V;
+  s.dtype = dtype;
+  s.dp = (D + 63) & ~63;
+  s.tp = (T + 63) & ~63;
+  s.split = dtype == TCMI_F32;
+  s.h_direct = h_direct;
+  s.w_direct = w_direct;
+  return s;
+}
+
+}  // namespace lce
+}  // namespace tcmi
+
+using namespace tcmi::lce;
+
+extern "C" {
+
+long long tcmi_lce_work_bytes(const void* h, long long h_rs, const void* w, long long w_rs, int tokens, int features, int classes,
+                              int dtype, int backward_pass) {
+  if (!shape_ok(tokens, features, classes, dtype)) return -1;
+  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype));
+  Arena a{nullptr};
+  if (backward_pass) take_bwd(a, s);
+  else take_fwd(a, s);
+  return a.used;
+}
+
+int tcmi_linear_cross_entropy(const void* h, long long h_rs, const void* w, long long w_rs, const void* bias, const long long* target,
+                              long long ignore_index, int tokens, int features, int classes, float* lse, float* loss, float* total,
+                              float* count, int mean, void* work, long long work_bytes, int dtype, void* stream) {
+  if (!shape_ok(tokens, features, classes, dtype) || !h || !w || !target || !lse || !loss || !work || (total && !count) || h_rs < features ||
+      w_rs < features)
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy: bad argument");
+  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype));
+  Arena a{(char*)work};
+  const FwdWork k = take_fwd(a, s);
+  if (a.used > work_bytes || ((uintptr_t)work & 255))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy: workspace too small or not 256-byte aligned");
+  const In in{h, w, bias, h_rs, w_rs, target, ignore_index};
+  const hipError_t e = forward(s, in, k, lse, loss, total, count, mean, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
+}
+
+int tcmi_linear_cross_entropy_grad(const void* h, long long h_rs, const void* w, long long w_rs, const void* bias,
+                                   const long long* target, long long ignore_index, int tokens, int features, int classes,
+                                   const float* lse, const float* dloss, int per_row, const float* count, void* dh, void* dw, void* db,
+                                   void* work, long long work_bytes, int dtype, void* stream) {
+  if (!shape_ok(tokens, features, classes, dtype) || !h || !w || !target || !lse || !dloss || !work || (!dh && !dw && !db) ||
+      h_rs < features || w_rs < features)
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy_grad: bad argument");
+  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype));
+  Arena a{(char*)work};
+  const BwdWork k = take_bwd(a, s);
+  if (a.used > work_bytes || ((uintptr_t)work & 255))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy_grad: workspace too small or not 256-byte aligned");
+  const In in{h, w, bias, h_rs, w_rs, target, ignore_index};
+  const hipError_t e = backward(s, in, k, lse, dloss, per_row, count, dh, dw, db, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
+}
+
+}  // extern "C"

@@ -1,0 +1,924 @@
+// Newton-Schulz orthogonalisation of (batches of) matrices, its gradient, and the optimiser step built on it.
+//
+//   N = |G|_F + eps,  X_0 = G / N;   A = X X^H,  B = b A + c A A,  X <- a X + B X        (steps times)
+// A and B are symmetric, so only the tiles on and below the diagonal are computed and written twice.  Singular values are
+// at most 1 at the start (Frobenius norm) and the polynomial bounds them afterwards, so every operand has a bound known
+// on the host: operands are f16 under a power-of-two scale, products run on the f16 matrix pipe (mm16.h).
+//
+// Precision.  X is carried in f32: a X is exact, the matrix pipe sees only B X.
+//   full (f32, f16, complex64, and everything that is differentiated): two f16 pieces per operand, three products.
+//   half (bf16 results): one f16 piece per operand.  Directions with small singular values are the ones a step amplifies
+//   (by a per step, a^5 = 485 for the default), and B is small on them: rounding X before B X costs 2^-11 of |B X| and
+//   does not reach them, where rounding the carried X would (1e-3 against 2e-2 of the result, five steps, random and
+//   low-rank-plus-noise matrices, against 64 bits; a bf16 result is itself rounded at 1.7e-3).
+// Complex matrices are real ones of twice the size, E(X) = [[Re, Im], [-Im, Re]], E(X Y) = E(X) E(Y), E(X)^T = E(X^H):
+// the two symmetric products run on E directly, the updates compute the upper block row only.
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include "../../include/tcmi.h"
+#include "tcmi_mm16.h"
+
+extern "C" int tcmi_set_error_(int code, const char* msg);
+
+namespace tcmi {
+namespace orth {
+
+using namespace mm16;
+
+enum { SRC_F32 = 0, SRC_F16 = 1, SRC_BF16 = 2, SRC_C64 = 3, SRC_PLANAR = 4 };
+
+struct Mat {                    // a batch of matrices as the caller holds them; strides in elements
+  const void* p;
+  long long rs, cs, bs;
+};
+
+template <int SRC>
+__device__ __forceinline__ float2 fetch(const void* p, long long at) {
+  if constexpr (SRC == SRC_F32 || SRC == SRC_PLANAR) return make_float2(((const float*)p)[at], 0.f);
+  if constexpr (SRC == SRC_F16) return make_float2((float)((const f16*)p)[at], 0.f);
+  if constexpr (SRC == SRC_BF16) return make_float2((float)((const __bf16*)p)[at], 0.f);
+  if constexpr (SRC == SRC_C64) return ((const float2*)p)[at];
+  return make_float2(0.f, 0.f);
+}
+
+__device__ __forceinline__ void put(void* p, int dtype, long long at, float v) {
+  if (dtype == TCMI_F32) ((float*)p)[at] = v;
+  else if (dtype == TCMI_F16) ((f16*)p)[at] = (f16)v;
+  else ((__bf16*)p)[at] = (__bf16)v;
+}
+
+__device__ __forceinline__ double block_sum(double v, double* red) {        // 256 threads, fixed order
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0] + red[1] + red[2] + red[3];
+  __syncthreads();
+  return v;
+}
+
+// Partial sums of squares (MODE 0), of x y (MODE 1: <D, G>), or the momentum update with the squares of its direction u
+// (MODE 2), in f64: an f32 square overflows from 1.8e19 on.  One read of the data; partial sums in a fixed order, so the
+// result does not depend on the order of the workgroups.  lanes: threads along the contiguous axis.
+struct SumArgs {
+  Mat x, y;
+  int outer, inner, lanes;
+  double* part;               // [batch][gridDim.x]
+  float* buf;                 // MODE 2: momentum, strides below
+  long long brs, bcs, bbs;
+  float rest;
+  int nesterov;
+};
+
+// `rest` = 1 - momentum, formed in f64: as 1 - 0.95f it would be off by 2^-22 of itself
+__device__ __forceinline__ float direction(float g, float v, float rest, int nesterov) {
+  return nesterov ? fmaf(rest, g - v, v) : v;
+}
+
+template <int SRC, int MODE>
+__global__ __launch_bounds__(256) void sums_kernel(SumArgs a) {
+  __shared__ double red[4];
+  const int per = 256 / a.lanes, r0 = threadIdx.x / a.lanes, c0 = threadIdx.x % a.lanes;
+  const long long bx = (long long)blockIdx.y * a.x.bs;
+  double s = 0.0;
+  for (int o = blockIdx.x * per + r0; o < a.outer; o += gridDim.x * per)
+    for (int i = c0; i < a.inner; i += a.lanes) {
+      const float2 v = fetch<SRC>(a.x.p, bx + o * a.x.rs + i * a.x.cs);
+      if constexpr (MODE == 1) {          // x: caller's G (complex: planar D holds re at i, im further on, see y strides)
+        const float* d = (const float*)a.y.p + (long long)blockIdx.y * a.y.bs + o * a.y.rs + i * a.y.cs;
+        s += (double)v.x * d[0];
+        if constexpr (SRC == SRC_C64) s += (double)v.y * d[a.brs];
+      } else if constexpr (MODE == 2) {
+        float* m = a.buf + (long long)blockIdx.y * a.bbs + o * a.brs + i * a.bcs;
+        const float nv = fmaf(a.rest, v.x - m[0], m[0]);
+        m[0] = nv;
+        const float u = direction(v.x, nv, a.rest, a.nesterov);
+        s += (double)u * u;
+      } else {
+        s += (double)v.x * v.x + (double)v.y * v.y;
+      }
+    }
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) a.part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
+}
+
+// Operand layout: a 64 x 64 tile of the source becomes f16 pieces, row-major and transposed (both k-contiguous for the
+// products that read them), zero beyond the matrix up to the next multiple of 64, and the f32 carry.  Bound by its
+// writes.  norm: the tile is divided by (sqrt(sum of part) + eps); every workgroup adds the partial sums itself.
+struct PackArgs {
+  Mat src;
+  int m, n, tx, ty, fast_rows;             // logical size, tiles, 1: the source is contiguous along rows
+  const double* part;
+  int npart;
+  float eps, scale;                        // pieces = value * scale
+  float* norm_out;                         // [batch] the norm without eps (may be null)
+  const float* buf;                        // momentum (null: none)
+  long long brs, bcs, bbs;
+  float rest;
+  int nesterov;
+  f16 *hi, *lo, *thi, *tlo;                // lo, tlo null: one piece
+  long long ld, os, ldt, ts;               // row strides and batch strides
+  float* carry;                            // f32 [m][ldc] (null: none); complex: im at column n + j
+  int carry_raw;                           // 1: the carry is not divided by the norm
+  long long ldc, cbs;
+  int embed;                               // complex as a real matrix of twice the size
+};
+
+template <int SRC>
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
+  __shared__ float tr[64][65], tim[SRC == SRC_C64 || SRC == SRC_PLANAR ? 64 : 1][65];
+  __shared__ double red[4];
+  constexpr bool MAYBE_COMPLEX = SRC == SRC_C64 || SRC == SRC_PLANAR;
+  const unsigned tiles = (unsigned)a.tx * a.ty;
+  const int bz = blockIdx.x / tiles, t = blockIdx.x % tiles, i0 = (t / a.tx) * 64, j0 = (t % a.tx) * 64;
+  float inv = 1.f;
+  if (a.part) {
+    double s = 0.0;
+    for (int k = threadIdx.x; k < a.npart; k += 256) s += a.part[(long long)bz * a.npart + k];
+    const double nrm = sqrt(block_sum(s, red));
+    if (a.norm_out && t == 0 && threadIdx.x == 0) a.norm_out[bz] = (float)nrm;
+    const double d = nrm + (double)a.eps;
+    inv = d == 0.0 ? 0.f : (float)(1.0 / d);
+  }
+  const long long base = (long long)bz * a.src.bs;
+  const int u = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll 4
+  for (int k = w; k < 64; k += 4) {
+    const int il = a.fast_rows ? u : k, jl = a.fast_rows ? k : u, i = i0 + il, j = j0 + jl;
+    float2 v = make_float2(0.f, 0.f);
+    if (i < a.m && j < a.n) {
+      const long long at = base + i * a.src.rs + j * a.src.cs;
+      v = fetch<SRC>(a.src.p, at);
+      if (SRC == SRC_PLANAR && a.embed) v.y = ((const float*)a.src.p)[at + a.n];
+      if (a.buf) v.x = direction(v.x, a.buf[(long long)bz * a.bbs + i * a.brs + j * a.bcs], a.rest, a.nesterov);
+    }
+    tr[il][jl] = v.x;
+    if (MAYBE_COMPLEX) tim[MAYBE_COMPLEX ? il : 0][jl] = v.y;
+  }
+  __syncthreads();
+  const float cinv = a.carry_raw ? 1.f : inv;
+  const bool twice = MAYBE_COMPLEX && a.embed;
+  const int mrows = twice ? a.m : (a.m + 63) & ~63, ncols = twice ? a.n : (a.n + 63) & ~63;
+  f16 *hi = a.hi + (long long)bz * a.os, *lo = a.lo ? a.lo + (long long)bz * a.os : nullptr;
+  f16 *thi = a.thi + (long long)bz * a.ts, *tlo = a.tlo ? a.tlo + (long long)bz * a.ts : nullptr;
+  auto store = [&](f16* ph, f16* pl, long long at, float x) {
+    f16 h, l;
+    two_pieces(x * inv * a.scale, h, l);
+    ph[at] = h;
+    if (pl) pl[at] = l;
+  };
+#pragma unroll 4
+  for (int k = w; k < 64; k += 4) {
+    {                                      // rows of X: lanes along j
+      const int i = i0 + k, j = j0 + u;
+      if (i < a.m && j < ncols) {
+        const float re = tr[k][u];
+        store(hi, lo, i * a.ld + j, re);
+        if (a.carry && j < a.n) a.carry[(long long)bz * a.cbs + i * a.ldc + j] = re * cinv;
+        if (twice) {
+          const float im = tim[MAYBE_COMPLEX ? k : 0][u];
+          store(hi, lo, i * a.ld + j + a.n, im);
+          store(hi, lo, (long long)(i + a.m) * a.ld + j, -im);
+          store(hi, lo, (long long)(i + a.m) * a.ld + j + a.n, re);
+          if (a.carry) a.carry[(long long)bz * a.cbs + i * a.ldc + j + a.n] = im * cinv;
+        }
+      }
+    }
+    {                                      // rows of X^T: lanes along i
+      const int i = i0 + u, j = j0 + k;
+      if (j < a.n && i < mrows) {
+        const float re = tr[u][k];
+        store(thi, tlo, j * a.ldt + i, re);
+        if (twice) {
+          const float im = tim[MAYBE_COMPLEX ? u : 0][k];
+          store(thi, tlo, (long long)(j + a.n) * a.ldt + i, im);
+          store(thi, tlo, j * a.ldt + i + a.m, -im);
+          store(thi, tlo, (long long)(j + a.n) * a.ldt + i + a.m, re);
+        }
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void clear_kernel(uint4* p, long long n) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = make_uint4(0, 0, 0, 0);
+}
+
+// A symmetric result as f16 pieces: value = alpha acc + beta (src hi + src lo), stored times `scale`; the tile below the
+// diagonal also writes its mirror image.  Columns up to the padded width get zeros.
+struct EpiSym {
+  f16 *hi, *lo;
+  const f16 *shi, *slo;
+  long long ld, bs;
+  float alpha, beta, scale;
+  template <class T>
+  __device__ void tile(const Args& g, int m0, int n0, int bz, bool mirror, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+    const int wide = (g.M + 63) & ~63;
+    f16 *h = hi + bz * bs, *l = lo ? lo + bz * bs : nullptr;
+    const f16 *sh = shi ? shi + bz * bs : nullptr, *sl = slo ? slo + bz * bs : nullptr;
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
+      f16x4 vh, vl, s4 = {}, t4 = {};
+      if (sh && row < g.M && col < wide) {
+        s4 = *reinterpret_cast<const f16x4*>(sh + (long long)row * ld + col);
+        if (sl) t4 = *reinterpret_cast<const f16x4*>(sl + (long long)row * ld + col);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = v[r] * alpha;
+        if (sh) x += beta * ((float)s4[r] + (float)t4[r]);
+        x = row < g.M && col + r < g.M ? x * scale : 0.f;
+        f16 a, b;
+        two_pieces(x, a, b);
+        vh[r] = a;
+        vl[r] = b;
+      }
+      if (row < g.M && col < wide) {
+        *reinterpret_cast<f16x4*>(h + (long long)row * ld + col) = vh;
+        if (l) *reinterpret_cast<f16x4*>(l + (long long)row * ld + col) = vl;
+      }
+      if (mirror && row < wide) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (col + r < g.M) {
+            h[(long long)(col + r) * ld + row] = vh[r];
+            if (l) l[(long long)(col + r) * ld + row] = vl[r];
+          }
+      }
+    });
+  }
+};
+
+// carry <- beta carry + alpha acc (f32, in place: a thread reads and writes the same element)
+struct EpiCarry {
+  float* carry;
+  long long ld, bs;
+  float alpha, beta;
+  const float* dev;              // [batch] further factor of acc held on the device (null: none)
+  template <class T>
+  __device__ void tile(const Args& g, int m0, int n0, int bz, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+    const float al = dev ? alpha * dev[bz] : alpha;
+    float* c = carry + bz * bs;
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
+      if (row >= g.M) return;
+      float* p = c + (long long)row * ld + col;
+      if (col + 3 < g.N) {
+        f32x4 x = *reinterpret_cast<f32x4*>(p);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = fmaf(al, v[r], beta * x[r]);
+        *reinterpret_cast<f32x4*>(p) = x;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (col + r < g.N) p[r] = fmaf(al, v[r], beta * p[r]);
+      }
+    });
+  }
+};
+
+// the last step: x = beta carry + alpha acc goes to the caller's matrix (out = x) or into a weight (out = keep out + rate x)
+struct EpiOut {
+  const float* carry;
+  long long ld, bs;
+  float alpha, beta;
+  void* out;
+  long long rs, cs, os;
+  int dtype, n;                  // n: columns; complex: columns of the imaginary part start there
+  int update;
+  float keep, rate;
+  template <class T>
+  __device__ void tile(const Args& g, int m0, int n0, int bz, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+    const float* c = carry + bz * bs;
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = col + r;
+        if (row >= g.M || j >= g.N) continue;
+        const float x = fmaf(alpha, v[r], beta * c[(long long)row * ld + j]);
+        if (dtype == TCMI_C64) {
+          const int im = j >= n;
+          ((float*)out)[2 * (bz * os + row * rs + (j - im * n) * cs) + im] = x;
+        } else {
+          const long long at = bz * os + row * rs + j * cs;
+          if (update) {
+            const float old = dtype == TCMI_F32 ? ((float*)out)[at] : dtype == TCMI_F16 ? (float)((f16*)out)[at] : (float)((__bf16*)out)[at];
+            put(out, dtype, at, fmaf(rate, x, keep * old));
+          } else {
+            put(out, dtype, at, x);
+          }
+        }
+      }
+    });
+  }
+};
+
+// dG = D / N - G <D, G> / (N^2 |G|)
+template <int SRC>
+__global__ __launch_bounds__(256) void grad_out_kernel(Mat gm, const float* d, long long ldd, long long dbs, int m, int n,
+                                                       const double* part, int npart, const float* norm, float eps, void* out,
+                                                       long long rs, long long cs, long long os, int dtype) {
+  __shared__ double red[4];
+  const int bz = blockIdx.y;
+  double s = 0.0;
+  for (int k = threadIdx.x; k < npart; k += 256) s += part[(long long)bz * npart + k];
+  const double inner = block_sum(s, red), nr = norm[bz], full = nr + (double)eps;
+  const float f1 = full == 0.0 ? 0.f : (float)(1.0 / full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * full * nr));
+  const long long total = (long long)m * n;
+  for (long long k = blockIdx.x * 256ll + threadIdx.x; k < total; k += gridDim.x * 256ll) {
+    // the source decides the order: consecutive threads along its contiguous axis
+    const long long i = gm.cs <= gm.rs ? k / n : k % m, j = gm.cs <= gm.rs ? k % n : k / m;
+    const float2 g = fetch<SRC>(gm.p, bz * gm.bs + i * gm.rs + j * gm.cs);
+    const float* dd = d + bz * dbs + i * ldd + j;
+    const long long at = bz * os + i * rs + j * cs;
+    if (SRC == SRC_C64) {
+      ((float2*)out)[at] = make_float2(dd[0] * f1 - g.x * f2, dd[n] * f1 - g.y * f2);
+    } else {
+      put(out, dtype, at, dd[0] * f1 - g.x * f2);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- host side
+using TileS = Tile<128, 128, 2, 2>;
+
+struct Shape {
+  int m, n;                       // min, max of the caller's two dimensions
+  bool flip;                      // the caller's matrix is taller than wide: X is its transpose
+  int cx;                         // 2 for complex
+  int mr, nc;                     // size of the (embedded) real matrix
+  long long mp, np;               // padded to 64
+  int batch;
+};
+
+Shape shape_of(int rows, int cols, int batch, int dtype) {
+  Shape s;
+  s.flip = rows > cols;
+  s.m = s.flip ? cols : rows;
+  s.n = s.flip ? rows : cols;
+  s.cx = dtype == TCMI_C64 ? 2 : 1;
+  s.mr = s.cx * s.m;
+  s.nc = s.cx * s.n;
+  s.mp = (s.mr + 63ll) & ~63ll;
+  s.np = (s.nc + 63ll) & ~63ll;
+  s.batch = batch;
+  return s;
+}
+
+struct Arena {                    // hands out 256-byte aligned pieces of a caller's buffer (base null: only counts)
+  char* base;
+  long long used = 0;
+  template <class P>
+  P* take(long long count) {
+    P* p = base ? reinterpret_cast<P*>(base + used) : nullptr;
+    used += (count * (long long)sizeof(P) + 255) & ~255ll;
+    return p;
+  }
+};
+
+struct Pieces {                   // one step's operands
+  f16 *xh, *xl, *th, *tl, *ah, *al, *bh, *bl;
+};
+
+Pieces take_pieces(Arena& w, const Shape& s, bool full) {
+  Pieces p{};
+  const long long x = s.mr * s.np * s.batch, t = s.nc * s.mp * s.batch, q = s.mr * s.mp * s.batch;
+  p.xh = w.take<f16>(x);
+  p.th = w.take<f16>(t);
+  p.ah = w.take<f16>(q);
+  p.bh = w.take<f16>(q);
+  if (full) {
+    p.xl = w.take<f16>(x);
+    p.tl = w.take<f16>(t);
+    p.al = w.take<f16>(q);
+    p.bl = w.take<f16>(q);
+  }
+  return p;
+}
+
+constexpr int MAX_PART = 256;
+
+struct Work {
+  double* part;
+  float* norm;
+  float* carry;
+  Pieces p;
+};
+
+Work take_work(Arena& w, const Shape& s, bool full, bool saved) {
+  Work k{};
+  k.part = w.take<double>((long long)s.batch * MAX_PART);
+  k.norm = w.take<float>(s.batch);
+  k.carry = w.take<float>(s.m * s.np * s.batch);
+  if (!saved) k.p = take_pieces(w, s, full);
+  return k;
+}
+
+struct Saved {
+  float* norm;
+  Pieces p[TCMI_NS_MAX_STEPS];
+};
+
+Saved take_saved(Arena& w, const Shape& s, int steps) {
+  Saved v{};
+  v.norm = w.take<float>(s.batch);
+  for (int i = 0; i < steps; ++i) v.p[i] = take_pieces(w, s, true);
+  return v;
+}
+
+struct GradWork {
+  double* part;
+  float* norm;
+  float* carry;
+  f16 *dh, *dl, *th, *tl, *sh, *sl, *qh, *ql;
+};
+
+GradWork take_grad(Arena& w, const Shape& s) {
+  GradWork k{};
+  k.part = w.take<double>((long long)s.batch * MAX_PART);
+  k.norm = w.take<float>(s.batch);
+  k.carry = w.take<float>(s.m * s.np * s.batch);
+  const long long x = s.mr * s.np * s.batch, t = s.nc * s.mp * s.batch, q = s.mr * s.mp * s.batch;
+  k.dh = w.take<f16>(x);
+  k.dl = w.take<f16>(x);
+  k.th = w.take<f16>(t);
+  k.tl = w.take<f16>(t);
+  k.sh = w.take<f16>(q);
+  k.sl = w.take<f16>(q);
+  k.qh = w.take<f16>(q);
+  k.ql = w.take<f16>(q);
+  return k;
+}
+
+// What bounds the operands of a step whose X has singular values in [0, s]: x for X, A = s^2, B = max |b t + c t^2|, next = max |p|.
+struct Bound {
+  double x, A, B, next;
+};
+
+Bound bound_of(double s, const double* co) {
+  const double a = co[0], b = co[1], c = co[2], t1 = s * s;
+  Bound r{s, t1, fabs(b * t1 + c * t1 * t1), 0.0};
+  if (c != 0.0) {
+    const double t = -b / (2 * c);
+    if (t > 0 && t < t1) r.B = fmax(r.B, fabs(b * t + c * t * t));
+  }
+  auto p = [&](double t) { return fabs(sqrt(t) * (a + b * t + c * t * t)); };
+  r.next = p(t1);
+  const double disc = 9 * b * b - 20 * a * c;
+  if (c != 0.0 && disc >= 0) {
+    const double u = (-3 * b + sqrt(disc)) / (10 * c), v = (-3 * b - sqrt(disc)) / (10 * c);
+    if (u > 0 && u < t1) r.next = fmax(r.next, p(u));
+    if (v > 0 && v < t1) r.next = fmax(r.next, p(v));
+  } else if (c == 0.0 && b != 0.0) {
+    const double u = -a / (3 * b);
+    if (u > 0 && u < t1) r.next = fmax(r.next, p(u));
+  }
+  return r;
+}
+
+// the largest power of two that keeps values up to `bound` below 2^15
+float scale_for(double bound) {
+  if (!(bound > 0)) return 1.f;
+  int e;
+  frexp(bound, &e);               // bound < 2^e
+  e = 15 - e;
+  return (float)ldexp(1.0, e > 30 ? 30 : e);
+}
+
+constexpr double SLACK = 1.02;    // rounding may carry a singular value past its bound
+constexpr double MAX_S = 64.0;
+
+struct Scales {
+  float x, A, B;
+};
+
+bool scales_of(int steps, const double* coef, Scales* out) {
+  double s = 1.0;
+  for (int i = 0; i < steps; ++i) {
+    const Bound b = bound_of(s * SLACK, coef + 3 * i);
+    if (!(b.x <= MAX_S) || !(b.B <= 1024.0) || !isfinite(b.next)) return false;
+    out[i] = {scale_for(b.x), scale_for(b.A), scale_for(b.B)};
+    s = b.next;
+  }
+  return s * SLACK <= MAX_S;
+}
+
+template <class T, class Epi>
+hipError_t run(Args& g, int batch, bool tri, const Epi& e, hipStream_t st) {
+  unsigned blocks;
+  if (!plan<T>(g, batch, tri, &blocks)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((product_kernel<f16x8, T, Epi>), dim3(blocks), dim3(T::THREADS), 0, st, g, e);
+  return hipGetLastError();
+}
+
+// segments of (ah + al)(bh + bl)^T without al bl; a null low piece drops its products
+void pairs(Args& g, const f16* ah, const f16* al, const f16* bh, const f16* bl) {
+  auto add = [&](const f16* a, const f16* b) {
+    g.a[g.nseg] = a;
+    g.b[g.nseg] = b;
+    ++g.nseg;
+  };
+  add(ah, bh);
+  if (bl) add(ah, bl);
+  if (al) add(al, bh);
+}
+
+int sum_blocks(const Shape& s) {
+  long long n = (long long)s.m * s.n / 2048;
+  const int cap = s.batch >= 64 ? 16 : s.batch >= 8 ? 64 : MAX_PART;
+  return (int)(n < 1 ? 1 : n > cap ? cap : n);
+}
+
+template <int MODE>
+hipError_t launch_sums(int src, SumArgs a, int blocks, int batch, hipStream_t st) {
+  // the contiguous axis inside; the sum does not care which of the two is called rows
+  if (a.x.rs < a.x.cs && a.outer > 0) {
+    long long t = a.x.rs; a.x.rs = a.x.cs; a.x.cs = t;
+    t = a.y.rs; a.y.rs = a.y.cs; a.y.cs = t;
+    if (MODE == 2) { t = a.brs; a.brs = a.bcs; a.bcs = t; }
+    const int o = a.outer; a.outer = a.inner; a.inner = o;
+  }
+  a.lanes = a.inner > 128 ? 256 : a.inner > 64 ? 128 : a.inner > 32 ? 64 : 32;
+  const dim3 grid(blocks, batch);
+  if (src == SRC_F32) hipLaunchKernelGGL((sums_kernel<SRC_F32, MODE>), grid, dim3(256), 0, st, a);
+  else if (src == SRC_F16) hipLaunchKernelGGL((sums_kernel<SRC_F16, MODE>), grid, dim3(256), 0, st, a);
+  else if (src == SRC_BF16) hipLaunchKernelGGL((sums_kernel<SRC_BF16, MODE>), grid, dim3(256), 0, st, a);
+  else if constexpr (MODE != 2) hipLaunchKernelGGL((sums_kernel<SRC_C64, MODE>), grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_pack(int src, PackArgs a, const Shape& s, hipStream_t st) {
+  a.m = s.m;
+  a.n = s.n;
+  a.tx = (s.n + 63) / 64;
+  a.ty = (s.m + 63) / 64;
+  a.embed = s.cx == 2;
+  a.fast_rows = a.src.rs < a.src.cs;
+  a.ld = s.np;
+  a.os = s.mr * s.np;
+  a.ldt = s.mp;
+  a.ts = s.nc * s.mp;
+  a.ldc = s.np;
+  a.cbs = s.m * s.np;
+  const long long blocks = (long long)a.tx * a.ty * s.batch;
+  if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)blocks);
+  if (src == SRC_F32) hipLaunchKernelGGL(pack_kernel<SRC_F32>, grid, dim3(256), 0, st, a);
+  else if (src == SRC_F16) hipLaunchKernelGGL(pack_kernel<SRC_F16>, grid, dim3(256), 0, st, a);
+  else if (src == SRC_BF16) hipLaunchKernelGGL(pack_kernel<SRC_BF16>, grid, dim3(256), 0, st, a);
+  else if (src == SRC_C64) hipLaunchKernelGGL(pack_kernel<SRC_C64>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(pack_kernel<SRC_PLANAR>, grid, dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+hipError_t clear(void* p, long long bytes, hipStream_t st) {
+  const long long n = bytes / 16;
+  const long long b = (n + 255) / 256;
+  hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(b > 4096 ? 4096 : b < 1 ? 1 : b)), dim3(256), 0, st, (uint4*)p, n);
+  return hipGetLastError();
+}
+
+Args base_args(const Shape& s, int M, int N, long long K, long long lda, long long ldb, long long sa, long long sb) {
+  Args g{};
+  g.M = M;
+  g.N = N;
+  g.K = (int)K;
+  g.lda = lda;
+  g.ldb = ldb;
+  g.sa = sa;
+  g.sb = sb;
+  return g;
+}
+
+#define TRY(x)                                   \
+  do {                                           \
+    const hipError_t e_ = (x);                   \
+    if (e_ != hipSuccess) return e_;             \
+  } while (0)
+
+// A, B and the update of one step from the pieces of X; the update's epilogue is the caller's
+template <class Epi>
+hipError_t ns_step(const Shape& s, const Pieces& p, const Scales& c, const double* co, bool full, const Epi& last, hipStream_t st) {
+  const long long xs = s.mr * s.np, ts = s.nc * s.mp, qs = s.mr * s.mp;
+  Args g = base_args(s, s.mr, s.mr, s.np, s.np, s.np, xs, xs);
+  pairs(g, p.xh, p.xl, p.xh, p.xl);
+  EpiSym ea{p.ah, full ? p.al : nullptr, nullptr, nullptr, s.mp, qs, 1.f / (c.x * c.x), 0.f, c.A};
+  TRY(run<TileS>(g, s.batch, true, ea, st));
+  g = base_args(s, s.mr, s.mr, s.mp, s.mp, s.mp, qs, qs);
+  pairs(g, p.ah, p.al, p.ah, p.al);
+  EpiSym eb{p.bh, full ? p.bl : nullptr, p.ah, p.al, s.mp, qs, (float)co[2] / (c.A * c.A), (float)co[1] / c.A, c.B};
+  TRY(run<TileS>(g, s.batch, true, eb, st));
+  g = base_args(s, s.m, s.nc, s.mp, s.mp, s.mp, qs, ts);
+  pairs(g, p.bh, p.bl, p.th, p.tl);
+  return run<TileS>(g, s.batch, false, last, st);
+}
+
+struct Problem {
+  Mat g;                          // caller's matrix with rows = the shorter axis
+  void* out;
+  long long ors, ocs, obs;
+  int src, dtype, steps;
+  const double* coef;
+  double eps;
+  bool full;
+  // optimiser step
+  float* buf;
+  long long brs, bcs, bbs;
+  float rest, keep, rate;
+  int nesterov;
+};
+
+hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
+  const int nb = sum_blocks(s);
+  SumArgs sa{};
+  sa.x = q.g;
+  sa.outer = s.m;
+  sa.inner = s.n;
+  sa.part = w.part;
+  if (q.buf) {
+    sa.buf = q.buf;
+    sa.brs = q.brs;
+    sa.bcs = q.bcs;
+    sa.bbs = q.bbs;
+    sa.rest = q.rest;
+    sa.nesterov = q.nesterov;
+    TRY(launch_sums<2>(q.src, sa, nb, s.batch, st));
+  } else {
+    TRY(launch_sums<0>(q.src, sa, nb, s.batch, st));
+  }
+  for (int i = 0; i < q.steps; ++i) {
+    const Pieces& p = sv ? sv->p[i] : w.p;
+    if (s.cx == 2 && (s.mp != s.mr || s.np != s.nc) && (sv || i == 0)) {     // the doubled matrix's padding
+      TRY(clear(p.xh, s.mr * s.np * s.batch * 2, st));
+      TRY(clear(p.th, s.nc * s.mp * s.batch * 2, st));
+      if (q.full) {
+        TRY(clear(p.xl, s.mr * s.np * s.batch * 2, st));
+        TRY(clear(p.tl, s.nc * s.mp * s.batch * 2, st));
+      }
+    }
+    PackArgs a{};
+    a.scale = sc[i].x;
+    a.hi = p.xh;
+    a.lo = p.xl;
+    a.thi = p.th;
+    a.tlo = p.tl;
+    if (i == 0) {
+      a.src = q.g;
+      a.part = w.part;
+      a.npart = nb;
+      a.eps = (float)q.eps;
+      a.norm_out = sv ? sv->norm : w.norm;
+      a.carry = w.carry;
+      a.buf = q.buf;
+      a.brs = q.brs;
+      a.bcs = q.bcs;
+      a.bbs = q.bbs;
+      a.rest = q.rest;
+      a.nesterov = q.nesterov;
+      TRY(launch_pack(q.src, a, s, st));
+    } else {
+      a.src = Mat{w.carry, s.np, 1, s.m * s.np};
+      TRY(launch_pack(SRC_PLANAR, a, s, st));
+    }
+    const float alpha = 1.f / (sc[i].B * sc[i].x), beta = (float)q.coef[3 * i];
+    if (i + 1 < q.steps) {
+      EpiCarry e{w.carry, s.np, s.m * s.np, alpha, beta, nullptr};
+      TRY(ns_step(s, p, sc[i], q.coef + 3 * i, q.full, e, st));
+    } else {
+      EpiOut e{w.carry, s.np, s.m * s.np, alpha, beta, q.out, q.ors, q.ocs, q.obs, q.dtype, s.n, q.buf != nullptr, q.keep, q.rate};
+      TRY(ns_step(s, p, sc[i], q.coef + 3 * i, q.full, e, st));
+    }
+  }
+  return hipSuccess;
+}
+
+hipError_t backward(const Shape& s, const Problem& q, const Mat& dy, const Scales* sc, GradWork& w, const Saved& sv, hipStream_t st) {
+  const long long xs = s.mr * s.np, ts = s.nc * s.mp, qs = s.mr * s.mp;
+  const int nb = sum_blocks(s);
+  if (s.cx == 2 && (s.mp != s.mr || s.np != s.nc)) {
+    TRY(clear(w.dh, xs * s.batch * 2, st));
+    TRY(clear(w.dl, xs * s.batch * 2, st));
+    TRY(clear(w.th, ts * s.batch * 2, st));
+    TRY(clear(w.tl, ts * s.batch * 2, st));
+  }
+  double bound[TCMI_NS_MAX_STEPS];
+  double sig = 1.0;
+  for (int i = 0; i < q.steps; ++i) {
+    bound[i] = sig * SLACK;
+    sig = bound_of(bound[i], q.coef + 3 * i).next;
+  }
+  for (int i = q.steps - 1; i >= 0; --i) {
+    const Pieces& p = sv.p[i];
+    const double x = bound[i], b = fabs(q.coef[3 * i + 1]), c = fabs(q.coef[3 * i + 2]);
+    // D is divided by its own norm before it is cut: |D|_F = 1, |S|_F <= 2 x, |Q|_F <= 2 x b + 4 x^3 c.  B D and Q X share an
+    // accumulator, so their scales have to agree: sB sD = sQ sX.
+    const float sS = scale_for(2 * x * SLACK), qmax = scale_for((2 * x * b + 4 * x * x * x * c) * SLACK);
+    float sD = scale_for(SLACK), sQ = sc[i].B * sD / sc[i].x;
+    if (sQ > qmax) {
+      sD *= qmax / sQ;
+      sQ = qmax;
+    }
+    // |D|
+    SumArgs sa{};
+    sa.outer = s.m;
+    sa.part = w.part;
+    const bool first = i == q.steps - 1;
+    if (first) {
+      sa.x = dy;
+      sa.inner = s.n;
+      TRY(launch_sums<0>(q.src, sa, nb, s.batch, st));
+    } else {
+      sa.x = Mat{w.carry, s.np, 1, s.m * s.np};
+      sa.inner = s.nc;
+      TRY(launch_sums<0>(SRC_F32, sa, nb, s.batch, st));
+    }
+    PackArgs a{};
+    a.part = w.part;
+    a.npart = nb;
+    a.norm_out = w.norm;
+    a.scale = sD;
+    a.hi = w.dh;
+    a.lo = w.dl;
+    a.thi = w.th;
+    a.tlo = w.tl;
+    if (first) {
+      a.src = dy;
+      a.carry = w.carry;
+      a.carry_raw = 1;                               // D itself; only its pieces are divided, the epilogue multiplies
+    } else {
+      a.src = Mat{w.carry, s.np, 1, s.m * s.np};
+    }
+    TRY(launch_pack(first ? q.src : SRC_PLANAR, a, s, st));
+    // S = D X^T + X D^T
+    Args g = base_args(s, s.mr, s.mr, s.np, s.np, s.np, xs, xs);
+    pairs(g, w.dh, w.dl, p.xh, p.xl);
+    pairs(g, p.xh, p.xl, w.dh, w.dl);
+    EpiSym es{w.sh, w.sl, nullptr, nullptr, s.mp, qs, 1.f / (sD * sc[i].x), 0.f, sS};
+    TRY(run<TileS>(g, s.batch, true, es, st));
+    // Q = b S + c (A S + S A)
+    g = base_args(s, s.mr, s.mr, s.mp, s.mp, s.mp, qs, qs);
+    pairs(g, p.ah, p.al, w.sh, w.sl);
+    pairs(g, w.sh, w.sl, p.ah, p.al);
+    EpiSym eq{w.qh, w.ql, w.sh, w.sl, s.mp, qs, (float)q.coef[3 * i + 2] / (sc[i].A * sS), (float)q.coef[3 * i + 1] / sS, sQ};
+    TRY(run<TileS>(g, s.batch, true, eq, st));
+    // D <- |D| (a D + B D + Q X)
+    g = base_args(s, s.m, s.nc, s.mp, s.mp, s.mp, qs, ts);
+    pairs(g, p.bh, p.bl, w.th, w.tl);
+    pairs(g, w.qh, w.ql, p.th, p.tl);
+    EpiCarry e{w.carry, s.np, s.m * s.np, 1.f / (sc[i].B * sD), (float)q.coef[3 * i], w.norm};
+    TRY(run<TileS>(g, s.batch, false, e, st));
+  }
+  // dG
+  SumArgs sa{};
+  sa.x = q.g;
+  sa.y = Mat{w.carry, s.np, 1, s.m * s.np};
+  sa.brs = s.n;
+  sa.outer = s.m;
+  sa.inner = s.n;
+  sa.part = w.part;
+  TRY(launch_sums<1>(q.src, sa, nb, s.batch, st));
+  const long long total = (long long)s.m * s.n;
+  const unsigned gx = (unsigned)((total + 1023) / 1024 > 4096 ? 4096 : (total + 1023) / 1024);
+  const dim3 grid(gx, s.batch);
+#define GO(SRC)                                                                                                            \
+  hipLaunchKernelGGL(grad_out_kernel<SRC>, grid, dim3(256), 0, st, q.g, w.carry, s.np, s.m * s.np, s.m, s.n, w.part, nb,  \
+                     sv.norm, (float)q.eps, q.out, q.ors, q.ocs, q.obs, q.dtype)
+  if (q.src == SRC_F32) GO(SRC_F32);
+  else if (q.src == SRC_F16) GO(SRC_F16);
+  else if (q.src == SRC_BF16) GO(SRC_BF16);
+  else GO(SRC_C64);
+#undef GO
+  return hipGetLastError();
+}
+
+int src_of(int dtype) {
+  return dtype == TCMI_F32 ? SRC_F32 : dtype == TCMI_F16 ? SRC_F16 : dtype == TCMI_BF16 ? SRC_BF16 : dtype == TCMI_C64 ? SRC_C64 : -1;
+}
+
+bool sizes_ok(int rows, int cols, int batch, int steps, int dtype) {
+  return rows >= 1 && cols >= 1 && batch >= 1 && batch <= 65535 && rows <= (1 << 24) && cols <= (1 << 24) && steps >= 1 &&
+         steps <= TCMI_NS_MAX_STEPS && src_of(dtype) >= 0;
+}
+
+// a matrix with its shorter axis as rows
+Mat oriented(const void* p, long long rs, long long cs, long long bs, bool flip) { return flip ? Mat{p, cs, rs, bs} : Mat{p, rs, cs, bs}; }
+
+}  // namespace orth
+}  // namespace tcmi
+
+using namespace tcmi::orth;
+
+extern "C" {
+
+long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full, int dtype, int what) {
+  if (!sizes_ok(rows, cols, batch, steps, dtype) || what < 0 || what > 3) return -1;
+  const Shape s = shape_of(rows, cols, batch, dtype);
+  Arena a{nullptr};
+  if (what == TCMI_NS_WORK) take_work(a, s, full != 0, false);
+  else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true, true);
+  else if (what == TCMI_NS_SAVED) take_saved(a, s, steps);
+  else take_grad(a, s);
+  return a.used;
+}
+
+int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long g_bs, void* out, int rows, int cols, int batch,
+                       int steps, const double* coef_host, double eps, int full, void* saved, long long saved_bytes, void* work,
+                       long long work_bytes, int dtype, void* stream) {
+  if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !out || !coef_host || !work || !(eps >= 0) || (saved && !full))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: bad argument");
+  const Shape s = shape_of(rows, cols, batch, dtype);
+  Arena aw{(char*)work}, av{(char*)saved};
+  Work w = take_work(aw, s, full != 0, saved != nullptr);
+  Saved sv{};
+  if (saved) sv = take_saved(av, s, steps);
+  if (aw.used > work_bytes || (saved && av.used > saved_bytes) || ((uintptr_t)work & 255) || ((uintptr_t)saved & 255))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: workspace too small or not 256-byte aligned");
+  Scales sc[TCMI_NS_MAX_STEPS];
+  if (!scales_of(steps, coef_host, sc))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: these coefficients let a singular value grow past 64");
+  Problem q{};
+  q.g = oriented(g, g_rs, g_cs, g_bs, s.flip);
+  q.out = out;
+  q.ors = s.flip ? 1 : cols;
+  q.ocs = s.flip ? cols : 1;
+  q.obs = (long long)rows * cols;
+  q.src = src_of(dtype);
+  q.dtype = dtype;
+  q.steps = steps;
+  q.coef = coef_host;
+  q.eps = eps;
+  q.full = full != 0;
+  const hipError_t e = forward(s, q, sc, w, saved ? &sv : nullptr, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
+}
+
+int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long long g_bs, const void* dout, long long d_rs,
+                            long long d_cs, long long d_bs, void* dg, int rows, int cols, int batch, int steps,
+                            const double* coef_host, double eps, const void* saved, long long saved_bytes, void* work,
+                            long long work_bytes, int dtype, void* stream) {
+  if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !dout || !dg || !coef_host || !saved || !work || !(eps >= 0))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: bad argument");
+  const Shape s = shape_of(rows, cols, batch, dtype);
+  Arena aw{(char*)work}, av{(char*)const_cast<void*>(saved)};
+  GradWork w = take_grad(aw, s);
+  const Saved sv = take_saved(av, s, steps);
+  if (aw.used > work_bytes || av.used > saved_bytes || ((uintptr_t)work & 255) || ((uintptr_t)saved & 255))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: workspace too small or not 256-byte aligned");
+  Scales sc[TCMI_NS_MAX_STEPS];
+  if (!scales_of(steps, coef_host, sc))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: these coefficients let a singular value grow past 64");
+  Problem q{};
+  q.g = oriented(g, g_rs, g_cs, g_bs, s.flip);
+  q.out = dg;
+  q.ors = s.flip ? 1 : cols;
+  q.ocs = s.flip ? cols : 1;
+  q.obs = (long long)rows * cols;
+  q.src = src_of(dtype);
+  q.dtype = dtype;
+  q.steps = steps;
+  q.coef = coef_host;
+  q.eps = eps;
+  q.full = true;
+  const hipError_t e = backward(s, q, oriented(dout, d_rs, d_cs, d_bs, s.flip), sc, w, sv, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
+}
+
+int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, const void* grad, long long g_rs, long long g_cs,
+                   long long g_bs, float* buf, long long b_rs, long long b_cs, long long b_bs, int rows, int cols, int batch,
+                   double momentum, int nesterov, double keep, double rate, int steps, const double* coef_host, double eps,
+                   int full, void* work, long long work_bytes, int dtype, void* stream) {
+  if (!sizes_ok(rows, cols, batch, steps, dtype) || dtype == TCMI_C64 || !param || !grad || !buf || !coef_host || !work || !(eps >= 0) ||
+      !(momentum >= 0) || !(momentum < 1))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: bad argument");
+  const Shape s = shape_of(rows, cols, batch, dtype);
+  Arena aw{(char*)work};
+  Work w = take_work(aw, s, full != 0, false);
+  if (aw.used > work_bytes || ((uintptr_t)work & 255))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: workspace too small or not 256-byte aligned");
+  Scales sc[TCMI_NS_MAX_STEPS];
+  if (!scales_of(steps, coef_host, sc))
+    return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: these coefficients let a singular value grow past 64");
+  Problem q{};
+  q.g = oriented(grad, g_rs, g_cs, g_bs, s.flip);
+  q.out = param;
+  q.ors = s.flip ? p_cs : p_rs;
+  q.ocs = s.flip ? p_rs : p_cs;
+  q.obs = p_bs;
+  q.src = src_of(dtype);
+  q.dtype = dtype;
+  q.steps = steps;
+  q.coef = coef_host;
+  q.eps = eps;
+  q.full = full != 0;
+  q.buf = buf;
+  q.brs = s.flip ? b_cs : b_rs;
+  q.bcs = s.flip ? b_rs : b_cs;
+  q.bbs = b_bs;
+  q.rest = (float)(1.0 - momentum);
+  q.nesterov = nesterov;
+  q.keep = (float)keep;
+  q.rate = (float)rate;
+  const hipError_t e = forward(s, q, sc, w, nullptr, reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
+}
+
+}  // extern "C"

@@ -350,6 +350,133 @@ def rq(mat):
     return _h(r).contiguous(), _h(q).contiguous()
 
 
+# ----------------------------------------------------------------------------- Newton-Schulz orthogonalisation
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _train_code(t):
+    """dtype code of the training operators; what they do not take is refused by name"""
+    import torch
+
+    codes = {torch.float32: _lib.TCMI_F32, torch.float16: _lib.TCMI_F16, torch.bfloat16: _lib.TCMI_BF16,
+             torch.complex64: _lib.TCMI_C64}
+    if t.dtype not in codes:
+        raise TypeError(f"needs float32, bfloat16, float16 or complex64, got {t.dtype}")
+    return codes[t.dtype]
+
+
+def _need_gpu(what, *ts):
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.TcmiError(f"{what}: tensors must live on the GPU (no CPU fallback)")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on different devices ({dev} and {t.device})")
+        dev = t.device
+
+
+def _ns_coefficients(steps, coefficients, eps):
+    """(steps, 3 * steps float64 values as a tuple): one triple for every step, or one triple per step"""
+    import math
+
+    if isinstance(steps, bool) or int(steps) != steps or not 1 <= steps <= _lib.NS_MAX_STEPS:
+        raise ValueError(f"steps must be 1 .. {_lib.NS_MAX_STEPS}, got {steps!r}")
+    steps = int(steps)
+    c = list(coefficients)
+    rows = [c] * steps if len(c) == 3 and not any(hasattr(x, "__len__") for x in c) else c
+    if len(rows) != steps or any(not hasattr(r, "__len__") or len(r) != 3 for r in rows):
+        raise ValueError("coefficients: one triple (a, b, c), or one triple for each of the steps")
+    flat = tuple(float(x) for r in rows for x in r)
+    if not all(math.isfinite(x) for x in flat):
+        raise ValueError("coefficients must be finite")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"eps must be finite and not negative, got {eps!r}")
+    return steps, flat
+
+
+def _host_doubles(flat):
+    import ctypes
+
+    return (ctypes.c_double * len(flat))(*flat)
+
+
+def _as_batch(t):
+    """[batch, rows, cols] of a tensor with at least two axes; strides of the matrices are kept where a view can"""
+    lead = 1
+    for k in t.shape[:-2]:
+        lead *= k
+    return t.resolve_conj().resolve_neg().reshape((lead,) + tuple(t.shape[-2:]))
+
+
+def newton_schulz(mat, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7):
+    """The matrices ``mat[..., :, :]`` pushed towards their orthogonal (complex: unitary) polar factor by Newton-Schulz
+    products, ``X = mat / (|mat|_F + eps)``, then ``steps`` times ``X <- a X + (b A + c A A) X`` with ``A = X X^H``.
+
+    ``coefficients``: one triple ``(a, b, c)``, or one per step.  The default drives every singular value into about
+    0.7 .. 1.2 in five steps (enough for an optimiser's update); ``(1.5, -0.5, 0)`` converges to the polar factor itself.
+    float32, bfloat16, float16, complex64; any strides; same shape and dtype out.  Differentiable once, including in
+    ``backend.value_and_grad`` / ``vmap``: unlike the gradient of :func:`svd_trunc` its gradient has no
+    ``1 / (s_i^2 - s_j^2)`` and holds at an isometry, where all singular values agree.  A zero matrix gives zero, a
+    non-finite entry makes its whole matrix NaN.  Coefficients that let singular values grow past 64 are refused.
+    The result is held to the accuracy of the dtype: bfloat16 runs one matrix product per product, the others (and
+    anything on the autograd tape) three on two-piece operands."""
+    import torch
+
+    if not torch.is_tensor(mat) or mat.dim() < 2:
+        raise ValueError("newton_schulz needs a tensor with at least two axes")
+    steps, flat = _ns_coefficients(steps, coefficients, eps)
+    _train_code(mat)
+    _need_gpu("newton_schulz", mat)
+    if _tracked(mat):
+        return _ad()["newton_schulz"](mat, steps, flat, float(eps))[0]
+    return _newton_schulz_raw(mat, steps, flat, float(eps), False)[0]
+
+
+def _newton_schulz_raw(mat, steps, flat, eps, saving):
+    import torch
+
+    code = _train_code(mat)
+    x = _as_batch(mat)
+    b, m, n = x.shape
+    out = torch.empty((b, m, n), dtype=mat.dtype, device=mat.device)
+    if out.numel() == 0:
+        return out.reshape(mat.shape), torch.empty(0, dtype=torch.uint8, device=mat.device)
+    full = int(saving or mat.dtype != torch.bfloat16)
+    L = _lib.lib()
+    nbytes = L.tcmi_ns_work_bytes(m, n, b, steps, full, code, _lib.NS_WORK_SAVING if saving else _lib.NS_WORK)
+    if nbytes < 0:
+        raise ValueError(f"newton_schulz: {b} matrices of {m} x {n} are out of range")
+    work = torch.empty(nbytes, dtype=torch.uint8, device=mat.device)
+    saved = torch.empty(L.tcmi_ns_work_bytes(m, n, b, steps, 1, code, _lib.NS_SAVED) if saving else 0, dtype=torch.uint8,
+                        device=mat.device)
+    with torch.cuda.device(mat.device):
+        _lib.check(L.tcmi_newton_schulz(x.data_ptr(), x.stride(1), x.stride(2), x.stride(0), out.data_ptr(), m, n, b, steps,
+                                        _host_doubles(flat), eps, full, saved.data_ptr() if saving else None, saved.numel(),
+                                        work.data_ptr(), work.numel(), code, _stream(mat)), "tcmi_newton_schulz")
+    return out.reshape(mat.shape), saved
+
+
+def _newton_schulz_grad_raw(mat, saved, dout, steps, flat, eps):
+    import torch
+
+    code = _train_code(mat)
+    x, d = _as_batch(mat), _as_batch(dout.to(mat.dtype))
+    b, m, n = x.shape
+    out = torch.empty((b, m, n), dtype=mat.dtype, device=mat.device)
+    if out.numel() == 0:
+        return out.reshape(mat.shape)
+    L = _lib.lib()
+    work = torch.empty(L.tcmi_ns_work_bytes(m, n, b, steps, 1, code, _lib.NS_WORK_GRAD), dtype=torch.uint8, device=mat.device)
+    with torch.cuda.device(mat.device):
+        _lib.check(L.tcmi_newton_schulz_grad(x.data_ptr(), x.stride(1), x.stride(2), x.stride(0), d.data_ptr(), d.stride(1),
+                                             d.stride(2), d.stride(0), out.data_ptr(), m, n, b, steps, _host_doubles(flat), eps,
+                                             saved.data_ptr(), saved.numel(), work.data_ptr(), work.numel(), code, _stream(mat)),
+                   "tcmi_newton_schulz_grad")
+    return out.reshape(mat.shape)
+
+
 # ----------------------------------------------------------------------------- reverse mode
 # The MPS path under ``backend.value_and_grad`` (reference tests/test_mpscircuit.py:437-497).  Forward
 # passes are the same kernels; the backward rules below are written in terms of ``matmul`` (so every
@@ -565,9 +692,59 @@ def _ad():
                 return torch.stack([_qr_backward(q[i], r[i], gq[i], gr[i]) for i in range(q.shape[0])])
             return _qr_backward(q, r, gq, gr)
 
+    class NewtonSchulz(torch.autograd.Function):
+        """(result, what the gradient needs as one block of bytes for the whole batch)"""
+
+        generate_vmap_rule = False
+
+        @staticmethod
+        def forward(mat, steps, flat, eps):
+            return _newton_schulz_raw(mat, steps, flat, eps, True)
+
+        @staticmethod
+        def vmap(info, in_dims, mat, steps, flat, eps):
+            out, saved = NewtonSchulz.apply(mat.movedim(in_dims[0], 0), steps, flat, eps)
+            return (out, saved), (0, None)
+
+        @staticmethod
+        def setup_context(ctx, inputs, output):
+            mat, ctx.steps, ctx.flat, ctx.eps = inputs
+            ctx.mark_non_differentiable(output[1])
+            ctx.save_for_backward(mat, output[1])
+
+        @staticmethod
+        def backward(ctx, dout, _):
+            mat, saved = ctx.saved_tensors
+            return NewtonSchulzGrad.apply(mat, saved, dout, ctx.steps, ctx.flat, ctx.eps), None, None, None
+
+    class NewtonSchulzGrad(torch.autograd.Function):
+        generate_vmap_rule = False
+
+        @staticmethod
+        def forward(mat, saved, dout, steps, flat, eps):
+            return _newton_schulz_grad_raw(mat, saved, dout, steps, flat, eps)
+
+        @staticmethod
+        def vmap(info, in_dims, mat, saved, dout, steps, flat, eps):
+            dm, _, dd = in_dims[:3]
+            if dm is None:                   # one matrix, many cotangents: `saved` belongs to the one matrix
+                outs = [NewtonSchulzGrad.apply(mat, saved, dout.select(dd, i), steps, flat, eps) for i in range(info.batch_size)]
+                return torch.stack(outs), 0
+            mat = mat.movedim(dm, 0)
+            dout = dout.movedim(dd, 0) if dd is not None else dout.expand(mat.shape)
+            return NewtonSchulzGrad.apply(mat, saved, dout, steps, flat, eps), 0
+
+        @staticmethod
+        def setup_context(ctx, inputs, output):
+            pass
+
+        @staticmethod
+        def backward(ctx, *_):
+            raise NotImplementedError("newton_schulz is differentiable once")
+
     # the decompositions' saved tensors are their own outputs: under torch.func they arrive wrapped, and
     # the rules above only use torch ops and ``matmul`` on them
-    _AD.update(matmul=Matmul.apply, svd=Svd.apply, qr=Qr.apply)
+    _AD.update(matmul=Matmul.apply, svd=Svd.apply, qr=Qr.apply, newton_schulz=NewtonSchulz.apply)
     return _AD
 
 
