@@ -338,6 +338,293 @@ __global__ __launch_bounds__(256) void grad_out_kernel(Mat gm, const float* d, l
   }
 }
 
+// ------------------------------------------------------------------------------------------- matrices that fit one CU
+// One workgroup per matrix, everything in LDS, f32 matrix instructions (exact products): one launch instead of four per
+// step.  Taken when a step's operands fit 160 KB of LDS.  Bound by the latency of the chain load -> norm -> 3 products a
+// step -> store: five steps of a 24 x 28 matrix are 15 dependent products.
+// Fragments: of 16 consecutive k, lane group g = lane >> 4 takes k = 4 g .. 4 g + 3 (the sum does not care which lane holds
+// which k), so a row operand is one 16-byte LDS read and a column operand four 4-byte reads; with rows 4 (mod 8) floats
+// apart neither has bank conflicts.
+struct SmallShape {
+  int m, n, cx, R, C, R16, C16, ldx, lda;
+};
+
+__host__ __device__ inline SmallShape small_shape(int m, int n, int cx) {
+  SmallShape s;
+  s.m = m;
+  s.n = n;
+  s.cx = cx;
+  s.R = cx * m;
+  s.C = cx * n;
+  s.R16 = (s.R + 15) & ~15;
+  s.C16 = (s.C + 15) & ~15;
+  s.ldx = s.C16 + 4;
+  s.lda = s.R16 + 4;
+  return s;
+}
+
+constexpr int SMALL_THREADS = 512, SMALL_WAVES = 8, SMALL_TILES = 8;        // 16 x 16 tiles per wave in the update
+
+struct SmallArgs {
+  Mat src, dy;
+  int m, n, cx, steps, flat;               // flat: 1 when the source is contiguous along n
+  float coef[3 * TCMI_NS_MAX_STEPS];
+  float eps;
+  float* buf;
+  long long brs, bcs, bbs;
+  float rest;
+  int nesterov;
+  void* out;
+  long long ors, ocs, obs;
+  int dtype, update;
+  float keep, rate;
+  float* saved;                            // [batch][steps][m][C] iterates, then the norm: [batch] (null: not kept)
+  float* norm;
+};
+
+__device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+  return c;
+}
+
+// sum_k p[i][k] q[j][k] for one 16 x 16 tile; lane holds rows 4 (lane >> 4) + r, column lane & 15
+__device__ __forceinline__ f32x4 rows_rows(const float* p, const float* q, int ld, int K, f32x4 c) {
+  const int at = (threadIdx.x & 15) * ld + 4 * ((threadIdx.x & 63) >> 4);
+  for (int k = 0; k < K; k += 16)
+    c = mfma4(*reinterpret_cast<const f32x4*>(p + at + k), *reinterpret_cast<const f32x4*>(q + at + k), c);
+  return c;
+}
+
+// sum_k p[i][k] x[k][j]
+__device__ __forceinline__ f32x4 rows_cols(const float* p, int ldp, const float* x, int ldx, int K, f32x4 c) {
+  const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  for (int k = 0; k < K; k += 16) {
+    const float* xx = x + (k + 4 * g) * ldx + l;
+    c = mfma4(*reinterpret_cast<const f32x4*>(p + l * ldp + 4 * g + k), f32x4{xx[0], xx[ldx], xx[2 * ldx], xx[3 * ldx]}, c);
+  }
+  return c;
+}
+
+// f(i0, j0) for the tiles on and below the diagonal, dealt to the waves
+template <class F>
+__device__ __forceinline__ void lower_tiles(int R16, F f) {
+  const int wave = threadIdx.x >> 6, t = R16 / 16;
+  int k = 0;
+  for (int i = 0; i < t; ++i)
+    for (int j = 0; j <= i; ++j, ++k)
+      if (k % SMALL_WAVES == wave) f(i * 16, j * 16);
+}
+
+__device__ __forceinline__ void put_both(float* a, int lda, int i0, int j0, f32x4 v) {
+  const int j = j0 + (threadIdx.x & 15), i = i0 + 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) a[(i + r) * lda + j] = v[r];
+  *reinterpret_cast<f32x4*>(a + j * lda + i) = v;
+}
+
+__device__ __forceinline__ f32x4 get_tile(const float* a, int ld, int i0, int j0) {
+  const float* p = a + (i0 + 4 * ((threadIdx.x & 63) >> 4)) * ld + j0 + (threadIdx.x & 15);
+  return f32x4{p[0], p[ld], p[2 * ld], p[3 * ld]};
+}
+
+__device__ __forceinline__ double small_sum(double v, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int k = 0; k < SMALL_WAVES; ++k) v += red[k];
+  return v;
+}
+
+__device__ __forceinline__ void embed(float* x, int ldx, const SmallShape& s, int i, int j, float2 v) {
+  x[i * ldx + j] = v.x;
+  if (s.cx == 2) {
+    x[i * ldx + j + s.n] = v.y;
+    x[(i + s.m) * ldx + j] = -v.y;
+    x[(i + s.m) * ldx + j + s.n] = v.x;
+  }
+}
+
+// element k of an m x n matrix, consecutive k along its contiguous axis
+__device__ __forceinline__ void place(int k, int m, int n, int flat, int& i, int& j) {
+  if (flat) {
+    i = k / n;
+    j = k - i * n;
+  } else {
+    j = k / m;
+    i = k - j * m;
+  }
+}
+
+__device__ __forceinline__ void gram(const float* X, float* A, const SmallShape& s) {
+  lower_tiles(s.R16, [&](int i0, int j0) {
+    put_both(A, s.lda, i0, j0, rows_rows(X + i0 * s.ldx, X + j0 * s.ldx, s.ldx, s.C16, f32x4{0.f, 0.f, 0.f, 0.f}));
+  });
+}
+
+__device__ __forceinline__ void poly(const float* A, float* Bm, const SmallShape& s, float b, float c) {
+  lower_tiles(s.R16, [&](int i0, int j0) {
+    const f32x4 v = rows_rows(A + i0 * s.lda, A + j0 * s.lda, s.lda, s.R16, f32x4{0.f, 0.f, 0.f, 0.f});
+    const f32x4 a = get_tile(A, s.lda, i0, j0);
+    f32x4 o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = fmaf(c, v[r], b * a[r]);
+    put_both(Bm, s.lda, i0, j0, o);
+  });
+}
+
+// X <- a X + B X (+ Q Y): all waves finish reading before any writes
+template <bool TWO>
+__device__ __forceinline__ void update(float* X, const float* Bm, const float* Q, const float* Y, const SmallShape& s, float a) {
+  const int wave = threadIdx.x >> 6, tc = s.C16 / 16, tiles = tc * (s.R16 / 16);
+  f32x4 res[SMALL_TILES];
+#pragma unroll
+  for (int u = 0; u < SMALL_TILES; ++u) {
+    const int t = wave + u * SMALL_WAVES;
+    if (t < tiles) {
+      const int i0 = t / tc * 16, j0 = t % tc * 16;
+      f32x4 v = rows_cols(Bm + i0 * s.lda, s.lda, X + j0, s.ldx, s.R16, f32x4{0.f, 0.f, 0.f, 0.f});
+      if (TWO) v = rows_cols(Q + i0 * s.lda, s.lda, Y + j0, s.ldx, s.R16, v);
+      const f32x4 x = get_tile(X, s.ldx, i0, j0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) res[u][r] = fmaf(a, x[r], v[r]);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < SMALL_TILES; ++u) {
+    const int t = wave + u * SMALL_WAVES;
+    if (t < tiles) {
+      float* p = X + (t / tc * 16 + 4 * ((threadIdx.x & 63) >> 4)) * s.ldx + t % tc * 16 + (threadIdx.x & 15);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[r * s.ldx] = res[u][r];
+    }
+  }
+  __syncthreads();
+}
+
+template <int SRC>
+__global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float mem[];
+  __shared__ double red[SMALL_WAVES];
+  const SmallShape s = small_shape(a.m, a.n, a.cx);
+  float *X = mem, *A = X + s.R16 * s.ldx, *Bm = A + s.R16 * s.lda;
+  const long long bz = blockIdx.x;
+  for (int k = threadIdx.x; k < s.R16 * s.ldx; k += SMALL_THREADS) X[k] = 0.f;
+  __syncthreads();
+  double sum = 0.0;
+  for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
+    int i, j;
+    place(k, s.m, s.n, a.flat, i, j);
+    float2 v = fetch<SRC>(a.src.p, bz * a.src.bs + i * a.src.rs + j * a.src.cs);
+    if (a.buf) {
+      float* m = a.buf + bz * a.bbs + i * a.brs + j * a.bcs;
+      const float nv = fmaf(a.rest, v.x - m[0], m[0]);
+      m[0] = nv;
+      v.x = direction(v.x, nv, a.rest, a.nesterov);
+    }
+    sum += (double)v.x * v.x + (double)v.y * v.y;
+    embed(X, s.ldx, s, i, j, v);
+  }
+  const double nrm = sqrt(small_sum(sum, red)), full = nrm + (double)a.eps;
+  if (a.norm && threadIdx.x == 0) a.norm[bz] = (float)nrm;
+  const float inv = full == 0.0 ? 0.f : (float)(1.0 / full);
+  for (int k = threadIdx.x; k < s.R16 * s.ldx; k += SMALL_THREADS) X[k] *= inv;
+  __syncthreads();
+  for (int t = 0; t < a.steps; ++t) {
+    if (a.saved) {
+      float* w = a.saved + (bz * a.steps + t) * s.m * s.C;
+      for (int k = threadIdx.x; k < s.m * s.C; k += SMALL_THREADS) w[k] = X[k / s.C * s.ldx + k % s.C];
+    }
+    gram(X, A, s);
+    __syncthreads();
+    poly(A, Bm, s, a.coef[3 * t + 1], a.coef[3 * t + 2]);
+    __syncthreads();
+    update<false>(X, Bm, nullptr, nullptr, s, a.coef[3 * t]);
+  }
+  for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
+    int i, j;
+    place(k, s.m, s.n, a.ocs <= a.ors, i, j);
+    const float x = X[i * s.ldx + j];
+    const long long at = bz * a.obs + i * a.ors + j * a.ocs;
+    if (SRC == SRC_C64) {
+      ((float2*)a.out)[at] = make_float2(x, X[i * s.ldx + j + s.n]);
+    } else if (a.update) {
+      const float old = SRC == SRC_F32 ? ((float*)a.out)[at] : SRC == SRC_F16 ? (float)((f16*)a.out)[at] : (float)((__bf16*)a.out)[at];
+      put(a.out, a.dtype, at, fmaf(a.rate, x, a.keep * old));
+    } else {
+      put(a.out, a.dtype, at, x);
+    }
+  }
+}
+
+template <int SRC>
+__global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float mem[];
+  __shared__ double red[SMALL_WAVES];
+  const SmallShape s = small_shape(a.m, a.n, a.cx);
+  const int xs = s.R16 * s.ldx, as = s.R16 * s.lda;
+  float *X = mem, *D = X + xs, *A = D + xs, *Bm = A + as, *S = Bm + as, *Q = S + as;
+  const long long bz = blockIdx.x;
+  for (int k = threadIdx.x; k < 2 * xs; k += SMALL_THREADS) X[k] = 0.f;
+  __syncthreads();
+  for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
+    int i, j;
+    place(k, s.m, s.n, a.dy.cs <= a.dy.rs, i, j);
+    embed(D, s.ldx, s, i, j, fetch<SRC>(a.dy.p, bz * a.dy.bs + i * a.dy.rs + j * a.dy.cs));
+  }
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  for (int t = a.steps - 1; t >= 0; --t) {
+    const float *w = a.saved + (bz * a.steps + t) * s.m * s.C, b = a.coef[3 * t + 1], c = a.coef[3 * t + 2];
+    for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
+      const int i = k / s.n, j = k % s.n;
+      embed(X, s.ldx, s, i, j, make_float2(w[i * s.C + j], s.cx == 2 ? w[i * s.C + j + s.n] : 0.f));
+    }
+    __syncthreads();
+    gram(X, A, s);
+    lower_tiles(s.R16, [&](int i0, int j0) {
+      f32x4 v = rows_rows(D + i0 * s.ldx, X + j0 * s.ldx, s.ldx, s.C16, zero);
+      put_both(S, s.lda, i0, j0, rows_rows(X + i0 * s.ldx, D + j0 * s.ldx, s.ldx, s.C16, v));
+    });
+    __syncthreads();
+    poly(A, Bm, s, b, c);
+    lower_tiles(s.R16, [&](int i0, int j0) {
+      f32x4 v = rows_rows(A + i0 * s.lda, S + j0 * s.lda, s.lda, s.R16, zero);
+      v = rows_rows(S + i0 * s.lda, A + j0 * s.lda, s.lda, s.R16, v);
+      const f32x4 g = get_tile(S, s.lda, i0, j0);
+      f32x4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = fmaf(c, v[r], b * g[r]);
+      put_both(Q, s.lda, i0, j0, o);
+    });
+    __syncthreads();
+    update<true>(D, Bm, Q, X, s, a.coef[3 * t]);
+  }
+  double sum = 0.0;
+  for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
+    int i, j;
+    place(k, s.m, s.n, a.flat, i, j);
+    const float2 g = fetch<SRC>(a.src.p, bz * a.src.bs + i * a.src.rs + j * a.src.cs);
+    sum += (double)g.x * D[i * s.ldx + j];
+    if (SRC == SRC_C64) sum += (double)g.y * D[i * s.ldx + j + s.n];
+  }
+  const double inner = small_sum(sum, red), nr = a.norm[bz], full = nr + (double)a.eps;
+  const float f1 = full == 0.0 ? 0.f : (float)(1.0 / full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * full * nr));
+  for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
+    int i, j;
+    place(k, s.m, s.n, a.flat, i, j);
+    const float2 g = fetch<SRC>(a.src.p, bz * a.src.bs + i * a.src.rs + j * a.src.cs);
+    const long long at = bz * a.obs + i * a.ors + j * a.ocs;
+    const float x = D[i * s.ldx + j] * f1 - g.x * f2;
+    if (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2(x, D[i * s.ldx + j + s.n] * f1 - g.y * f2);
+    else put(a.out, a.dtype, at, x);
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------- host side
 using TileS = Tile<128, 128, 2, 2>;
 
@@ -589,6 +876,47 @@ Args base_args(const Shape& s, int M, int N, long long K, long long lda, long lo
   return g;
 }
 
+constexpr int SMALL_LDS = 156 * 1024;        // of 160 KB: the reductions take a little
+
+// bytes of LDS of the one-workgroup form; 0: it does not fit
+int small_bytes(const Shape& s, bool grad) {
+  if (s.mr > 512 || s.nc > 4096) return 0;
+  const SmallShape q = small_shape(s.m, s.n, s.cx);
+  if ((q.R16 / 16) * (q.C16 / 16) > SMALL_WAVES * SMALL_TILES) return 0;
+  const long long b = 4ll * ((grad ? 2 : 1) * q.R16 * q.ldx + (grad ? 4 : 2) * q.R16 * q.lda);
+  return b <= SMALL_LDS ? (int)b : 0;
+}
+
+// the saved block of the one-workgroup form: norms, then the iterates
+struct SmallSaved {
+  float *norm, *x;
+};
+
+SmallSaved take_small(Arena& w, const Shape& s, int steps) {
+  SmallSaved v;
+  v.norm = w.take<float>(s.batch);
+  v.x = w.take<float>((long long)s.batch * steps * s.m * s.nc);
+  return v;
+}
+
+template <int SRC, bool GRAD>
+hipError_t small_launch(const SmallArgs& a, int bytes, int batch, hipStream_t st) {
+  const void* f = GRAD ? reinterpret_cast<const void*>(small_grad_kernel<SRC>) : reinterpret_cast<const void*>(small_kernel<SRC>);
+  const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS);
+  if (e != hipSuccess) return e;
+  if (GRAD) hipLaunchKernelGGL(small_grad_kernel<SRC>, dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
+  else hipLaunchKernelGGL(small_kernel<SRC>, dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
+  return hipGetLastError();
+}
+
+template <bool GRAD>
+hipError_t small_by_type(int src, const SmallArgs& a, int bytes, int batch, hipStream_t st) {
+  if (src == SRC_F32) return small_launch<SRC_F32, GRAD>(a, bytes, batch, st);
+  if (src == SRC_F16) return small_launch<SRC_F16, GRAD>(a, bytes, batch, st);
+  if (src == SRC_BF16) return small_launch<SRC_BF16, GRAD>(a, bytes, batch, st);
+  return small_launch<SRC_C64, GRAD>(a, bytes, batch, st);
+}
+
 #define TRY(x)                                   \
   do {                                           \
     const hipError_t e_ = (x);                   \
@@ -626,6 +954,33 @@ struct Problem {
   float rest, keep, rate;
   int nesterov;
 };
+
+SmallArgs small_args(const Shape& s, const Problem& q) {
+  SmallArgs a{};
+  a.src = q.g;
+  a.m = s.m;
+  a.n = s.n;
+  a.cx = s.cx;
+  a.steps = q.steps;
+  a.flat = q.g.cs <= q.g.rs;
+  for (int i = 0; i < 3 * q.steps; ++i) a.coef[i] = (float)q.coef[i];
+  a.eps = (float)q.eps;
+  a.buf = q.buf;
+  a.brs = q.brs;
+  a.bcs = q.bcs;
+  a.bbs = q.bbs;
+  a.rest = q.rest;
+  a.nesterov = q.nesterov;
+  a.out = q.out;
+  a.ors = q.ors;
+  a.ocs = q.ocs;
+  a.obs = q.obs;
+  a.dtype = q.dtype;
+  a.update = q.buf != nullptr;
+  a.keep = q.keep;
+  a.rate = q.rate;
+  return a;
+}
 
 hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
   const int nb = sum_blocks(s);
@@ -813,6 +1168,11 @@ long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full,
   if (!sizes_ok(rows, cols, batch, steps, dtype) || what < 0 || what > 3) return -1;
   const Shape s = shape_of(rows, cols, batch, dtype);
   Arena a{nullptr};
+  if (small_bytes(s, what == TCMI_NS_SAVED || what == TCMI_NS_WORK_GRAD || what == TCMI_NS_WORK_SAVING)) {
+    if (what == TCMI_NS_SAVED) take_small(a, s, steps);
+    else a.take<char>(1);
+    return a.used;
+  }
   if (what == TCMI_NS_WORK) take_work(a, s, full != 0, false);
   else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true, true);
   else if (what == TCMI_NS_SAVED) take_saved(a, s, steps);
@@ -826,10 +1186,14 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
   if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !out || !coef_host || !work || !(eps >= 0) || (saved && !full))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype);
+  const int small = small_bytes(s, saved != nullptr);
   Arena aw{(char*)work}, av{(char*)saved};
-  Work w = take_work(aw, s, full != 0, saved != nullptr);
+  Work w{};
   Saved sv{};
-  if (saved) sv = take_saved(av, s, steps);
+  SmallSaved ss{};
+  if (!small) w = take_work(aw, s, full != 0, saved != nullptr);
+  if (saved && small) ss = take_small(av, s, steps);
+  if (saved && !small) sv = take_saved(av, s, steps);
   if (aw.used > work_bytes || (saved && av.used > saved_bytes) || ((uintptr_t)work & 255) || ((uintptr_t)saved & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: workspace too small or not 256-byte aligned");
   Scales sc[TCMI_NS_MAX_STEPS];
@@ -847,7 +1211,15 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
   q.coef = coef_host;
   q.eps = eps;
   q.full = full != 0;
-  const hipError_t e = forward(s, q, sc, w, saved ? &sv : nullptr, reinterpret_cast<hipStream_t>(stream));
+  hipError_t e;
+  if (small) {
+    SmallArgs a = small_args(s, q);
+    a.saved = ss.x;
+    a.norm = ss.norm;
+    e = small_by_type<false>(q.src, a, small, batch, reinterpret_cast<hipStream_t>(stream));
+  } else {
+    e = forward(s, q, sc, w, saved ? &sv : nullptr, reinterpret_cast<hipStream_t>(stream));
+  }
   return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
 }
 
@@ -859,8 +1231,16 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype);
   Arena aw{(char*)work}, av{(char*)const_cast<void*>(saved)};
-  GradWork w = take_grad(aw, s);
-  const Saved sv = take_saved(av, s, steps);
+  const int small = small_bytes(s, true);
+  GradWork w{};
+  Saved sv{};
+  SmallSaved ss{};
+  if (small) {
+    ss = take_small(av, s, steps);
+  } else {
+    w = take_grad(aw, s);
+    sv = take_saved(av, s, steps);
+  }
   if (aw.used > work_bytes || av.used > saved_bytes || ((uintptr_t)work & 255) || ((uintptr_t)saved & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: workspace too small or not 256-byte aligned");
   Scales sc[TCMI_NS_MAX_STEPS];
@@ -878,7 +1258,16 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
   q.coef = coef_host;
   q.eps = eps;
   q.full = true;
-  const hipError_t e = backward(s, q, oriented(dout, d_rs, d_cs, d_bs, s.flip), sc, w, sv, reinterpret_cast<hipStream_t>(stream));
+  hipError_t e;
+  if (small) {
+    SmallArgs a = small_args(s, q);
+    a.dy = oriented(dout, d_rs, d_cs, d_bs, s.flip);
+    a.saved = ss.x;
+    a.norm = ss.norm;
+    e = small_by_type<true>(q.src, a, small, batch, reinterpret_cast<hipStream_t>(stream));
+  } else {
+    e = backward(s, q, oriented(dout, d_rs, d_cs, d_bs, s.flip), sc, w, sv, reinterpret_cast<hipStream_t>(stream));
+  }
   return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
 }
 
@@ -890,8 +1279,10 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
       !(momentum >= 0) || !(momentum < 1))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype);
+  const int small = small_bytes(s, false);
   Arena aw{(char*)work};
-  Work w = take_work(aw, s, full != 0, false);
+  Work w{};
+  if (!small) w = take_work(aw, s, full != 0, false);
   if (aw.used > work_bytes || ((uintptr_t)work & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: workspace too small or not 256-byte aligned");
   Scales sc[TCMI_NS_MAX_STEPS];
@@ -917,7 +1308,8 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
   q.nesterov = nesterov;
   q.keep = (float)keep;
   q.rate = (float)rate;
-  const hipError_t e = forward(s, q, sc, w, nullptr, reinterpret_cast<hipStream_t>(stream));
+  const hipError_t e = small ? small_by_type<false>(q.src, small_args(s, q), small, batch, reinterpret_cast<hipStream_t>(stream))
+                             : forward(s, q, sc, w, nullptr, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
 }
 

@@ -34,7 +34,7 @@ def test_abi_refuses_before_a_launch():
     lib = _lib.lib()
     co = linalg._host_doubles(linalg.NS_COEFFICIENTS * 5)
     p = 1 << 20
-    args = (p, 4, 1, 16, p, 4, 4, 1, 5, co, 1e-7, 1, None, 0, p, 1 << 40, _lib.TCMI_F32, None)
+    args = (p, 400, 1, 160000, p, 400, 400, 1, 5, co, 1e-7, 1, None, 0, p, 1 << 40, _lib.TCMI_F32, None)
 
     def changed(**kw):
         a = list(args)
