@@ -49,14 +49,13 @@ __device__ __forceinline__ float scale_of(float top) {
   return ldexpf(1.f, k > 100 ? 100 : k < -100 ? -100 : k);
 }
 
-// Rows of an operand, k padded to 64.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per
-// row, whose inverse goes to inv[row].  One wave per row, the second read comes from the cache.
+// Rows of an operand, k padded.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per row, whose
+// inverse goes to inv[row].  One wave per row, the second read comes from the cache.
 template <int DT>
-__global__ __launch_bounds__(256) void rows_kernel(const void* src, long long rs, int rows, int cols, int colsp, void* hi, f16* lo,
-                                                   float* inv) {
+__global__ __launch_bounds__(256) void rows_kernel(const void* src, long long rs, int rows, int cols, int colsp, void* out, float* inv) {
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= rows) return;
-  const long long in = row * rs, out = (long long)row * colsp;
+  const long long in = row * rs;
   if constexpr (DT == TCMI_F32) {
     const float* p = (const float*)src + in;
     float top = 0.f;
@@ -64,16 +63,18 @@ __global__ __launch_bounds__(256) void rows_kernel(const void* src, long long rs
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const float s = scale_of(top);
+    f16* q = (f16*)out + (long long)row * 2 * colsp;
     for (int c = lane; c < colsp; c += 64) {
       f16 h, l;
       two_pieces(c < cols ? p[c] * s : 0.f, h, l);
-      ((f16*)hi)[out + c] = h;
-      lo[out + c] = l;
+      q[kpos<2>(c)] = h;
+      q[kpos<2>(c) + 32] = l;
     }
     if (lane == 0) inv[row] = 1.f / s;
   } else {
     const unsigned short* p = (const unsigned short*)src + in;
-    for (int c = lane; c < colsp; c += 64) ((unsigned short*)hi)[out + c] = c < cols ? p[c] : 0;
+    unsigned short* q = (unsigned short*)out + (long long)row * colsp;
+    for (int c = lane; c < colsp; c += 64) q[c] = c < cols ? p[c] : 0;
   }
 }
 
@@ -104,11 +105,12 @@ __global__ __launch_bounds__(256) void top_kernel(const void* src, long long rs,
   if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// out[c][row] = src[row][c] * r[row] * scale as f16 pieces, rows padded to 64 with zeros.  A zero factor gives zero
+// out[c][row] = src[row][c] * r[row] * scale as f16 pieces (two for f32), rows padded with zeros.  A zero factor gives zero
 // whatever the row holds.
 template <int DT>
 __global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs, int rows, int cols, const float* r,
-                                                   const float* part, int nparts, f16* hi, f16* lo, long long ldt, float* inv) {
+                                                   const float* part, int nparts, f16* out, int rowsp, float* inv) {
+  constexpr int P = DT == TCMI_F32 ? 2 : 1;
   __shared__ float tile[64][65];
   __shared__ float red[4];
   const int tid = threadIdx.x, u = tid & 63, w = tid >> 6;
@@ -135,11 +137,12 @@ __global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs
 #pragma unroll 4
   for (int k = w; k < 64; k += 4) {
     const int c = c0 + k, row = r0 + u;
-    if (c < cols) {                                  // the grid covers the padded rows exactly
+    if (c < cols && row < rowsp) {
       f16 h, l;
       two_pieces(tile[u][k], h, l);
-      hi[c * ldt + row] = h;
-      if (lo) lo[c * ldt + row] = l;
+      f16* q = out + (long long)c * P * rowsp + kpos<P>(row);
+      q[0] = h;
+      if (P == 2) q[32] = l;
     }
   }
 }
@@ -177,12 +180,13 @@ __device__ __forceinline__ void logits(const Logits& q, const Args& g, int m0, i
 
 // forward: per row the tile's maximum and sum of exponentials, and the target's logit where it lies in the tile
 struct EpiLse {
+  static constexpr bool WHOLE = true;
   Logits q;
   float2* part;                  // [T][tiles of classes]
   float* target;                 // [T]
   const long long* y;
   template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int, bool, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
+  __device__ void tile(const Args& g, int m0, int n0, int, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
     logits<T>(q, g, m0, n0, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
     float2* stat = reinterpret_cast<float2*>(lds);                    // [WN][BM]
@@ -230,7 +234,7 @@ struct EpiLse {
 };
 
 // joins the tiles of a row: one wave per row
-__global__ __launch_bounds__(256) void join_kernel(const float2* part, int tiles, const float* target, const long long* y,
+__global__ __launch_bounds__(256) void rowstat_kernel(const float2* part, int tiles, const float* target, const long long* y,
                                                    long long ignore, int T, int V, float* lse, float* loss) {
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (t >= T) return;
@@ -289,16 +293,18 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* loss, const lo
 }
 
 // backward: P as f16 pieces, row-major for dh and transposed for dw, zero in the padding and in ignored rows
+template <int P>
 struct EpiProb {
+  static constexpr bool WHOLE = true;
   Logits q;
   const float* lse;
   const long long* y;
   long long ignore;
   int V;
-  f16 *hi, *lo, *thi, *tlo;
-  long long ld, ldt;             // padded classes of the piece, padded rows
+  f16 *p, *pt;                   // [T][P * vp], [classes][P * tp]
+  int vp, tp;                    // padded classes of the piece, padded rows
   template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+  __device__ void tile(const Args& g, int m0, int n0, int, char*, f32x4 (&acc)[T::MI][T::NI]) const {
     logits<T>(q, g, m0, n0, acc);
     each<T>(m0, n0, acc, [&](int row, int col, f32x4 x) {
       const bool in = row < g.M;
@@ -308,27 +314,25 @@ struct EpiProb {
       f16x4 vh, vl;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float p = 0.f;
+        float v = 0.f;
         if (keep && col + r < g.N) {
-          p = __expf(x[r] - l);
-          if (col + r + q.v0 == yt) p -= 1.f;
-          if (bad) p = NAN;
+          v = __expf(x[r] - l);
+          if (col + r + q.v0 == yt) v -= 1.f;
+          if (bad) v = NAN;
         }
         f16 a, b;
-        two_pieces(p * PSCALE, a, b);
+        two_pieces(v * PSCALE, a, b);
         vh[r] = a;
         vl[r] = b;
       }
-      if (in && col < ld) {
-        *reinterpret_cast<f16x4*>(hi + row * ld + col) = vh;
-        if (lo) *reinterpret_cast<f16x4*>(lo + row * ld + col) = vl;
-      }
-      if (row < ldt) {
+      if (in && col < vp) store_four<P>(p + (long long)row * P * vp, col, vh, vl);
+      if (row < tp) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           if (col + r < g.N) {
-            thi[(col + r) * ldt + row] = vh[r];
-            if (tlo) tlo[(col + r) * ldt + row] = vl[r];
+            f16* o = pt + (long long)(col + r) * P * tp + kpos<P>(row);
+            o[0] = vh[r];
+            if (P == 2) o[32] = vl[r];
           }
       }
     });
@@ -337,39 +341,38 @@ struct EpiProb {
 
 // a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor
 struct EpiGrad {
+  static constexpr bool WHOLE = false;
   const float* inv;              // inverse of the other operand's scale, on the device
   float* sum;                    // f32 [rows][N] (null: only one piece)
   int first, last;
   const float* r;                // null: 1
   void* out;
   int dtype;
-  template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+  __device__ __forceinline__ void four(const Args& g, int, bool, int row, int col, f32x4 v) const {
+    if (row >= g.M) return;
     const float al = *inv * (1.f / PSCALE);
-    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
-      if (row >= g.M) return;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (col + k >= g.N) continue;
-        const long long at = (long long)row * g.N + col + k;
-        float x = al * v[k];
-        if (!first) x += sum[at];
-        if (!last) sum[at] = x;
-        else put(out, dtype, at, r ? (r[row] == 0.f ? 0.f : x * r[row]) : x);
-      }
-    });
+    for (int k = 0; k < 4; ++k) {
+      if (col + k >= g.N) continue;
+      const long long at = (long long)row * g.N + col + k;
+      float x = al * v[k];
+      if (!first) x += sum[at];
+      if (!last) sum[at] = x;
+      else put(out, dtype, at, r ? (r[row] == 0.f ? 0.f : x * r[row]) : x);
+    }
   }
 };
 
 // db_v = sum_t P[t][v] r_t from the transposed pieces: one wave per class
-__global__ __launch_bounds__(256) void bias_kernel(const f16* hi, const f16* lo, long long ldt, const float* r, int T, int vc, void* out,
-                                                   int dtype, int v0) {
+template <int P>
+__global__ __launch_bounds__(256) void bias_kernel(const f16* pt, int tp, const float* r, int T, int vc, void* out, int dtype, int v0) {
   const int v = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (v >= vc) return;
+  const f16* q = pt + (long long)v * P * tp;
   float s = 0.f;
   for (int t = lane; t < T; t += 64) {
-    float p = (float)hi[v * ldt + t];
-    if (lo) p += (float)lo[v * ldt + t];
+    float p = (float)q[kpos<P>(t)];
+    if (P == 2) p += (float)q[kpos<P>(t) + 32];
     s = fmaf(p, r[t], s);
   }
 #pragma unroll
@@ -378,8 +381,6 @@ __global__ __launch_bounds__(256) void bias_kernel(const f16* hi, const f16* lo,
 }
 
 // ---------------------------------------------------------------------------------------------------------- host side
-using TileL = Tile<128, 128, 2, 2>;
-
 struct Arena {
   char* base;
   long long used = 0;
@@ -393,29 +394,28 @@ struct Arena {
 
 struct Shape {
   int T, D, V, dtype;
+  int P;                         // pieces per operand: 2 for f32
   int dp, tp;                    // padded features, padded rows
-  bool split;                    // f32: two pieces
   bool h_direct, w_direct;       // the operand is read where it lies
 };
 
 struct Rows {                    // the forward operands when they are not read in place
-  void *h, *w;
-  f16 *hl, *wl;
+  f16 *h, *w;
   float *hs, *ws;
 };
 
 Rows take_rows(Arena& a, const Shape& s) {
   Rows r{};
-  if (!s.h_direct) r.h = a.take<f16>((long long)s.T * s.dp);
-  if (!s.w_direct) r.w = a.take<f16>((long long)s.V * s.dp);
-  if (s.split) {
-    r.hl = a.take<f16>((long long)s.T * s.dp);
-    r.wl = a.take<f16>((long long)s.V * s.dp);
+  if (!s.h_direct) r.h = a.take<f16>((long long)s.T * s.P * s.dp);
+  if (!s.w_direct) r.w = a.take<f16>((long long)s.V * s.P * s.dp);
+  if (s.P == 2) {
     r.hs = a.take<float>(s.T);
     r.ws = a.take<float>(s.V);
   }
   return r;
 }
+
+using LseTile = Mid;
 
 struct FwdWork {
   Rows rows;
@@ -426,14 +426,14 @@ struct FwdWork {
 FwdWork take_fwd(Arena& a, const Shape& s) {
   FwdWork w{};
   w.rows = take_rows(a, s);
-  w.part = a.take<float2>((long long)s.T * ((s.V + TileL::BN - 1) / TileL::BN));
+  w.part = a.take<float2>((long long)s.T * ((s.V + LseTile::BN - 1) / LseTile::BN));
   w.target = a.take<float>(s.T);
   return w;
 }
 
 // classes per piece of the backward: P and its transpose take at most about 1 GiB, pieces of equal size
 int piece_of(const Shape& s) {
-  const long long per = (long long)(s.T + s.tp) * 2 * (s.split ? 2 : 1);
+  const long long per = (long long)(s.T + s.tp) * 2 * s.P;
   long long most = (1ll << 30) / per / 256 * 256;
   if (most < 1024) most = 1024;
   const long long pieces = (s.V + most - 1) / most;
@@ -443,13 +443,13 @@ int piece_of(const Shape& s) {
 
 struct BwdWork {
   Rows rows;
-  float *r, *parth, *partw, *invh, *invw, *sum;
-  f16 *ph, *pl, *qh, *ql, *th, *tl, *wh, *wl;      // P, P^T, h^T, w^T of the piece
+  float *r, *parth, *partw, *invh, *invw, *sum, *split;
+  f16 *p, *pt, *ht, *wt;                           // P, P^T, h^T, w^T of the piece
 };
 
 BwdWork take_bwd(Arena& a, const Shape& s) {
   BwdWork w{};
-  const long long vc = piece_of(s), vp = (vc + 63) & ~63ll;
+  const long long vc = piece_of(s), vp = kpad(vc, s.P);
   w.rows = take_rows(a, s);
   w.r = a.take<float>(s.T);
   w.parth = a.take<float>(PARTS);
@@ -457,16 +457,11 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
   w.invh = a.take<float>(1);
   w.invw = a.take<float>(1);
   w.sum = vc < s.V ? a.take<float>((long long)s.T * s.D) : nullptr;
-  w.ph = a.take<f16>(s.T * vp);
-  w.qh = a.take<f16>(vc * s.tp);
-  w.th = a.take<f16>((long long)s.D * s.tp);
-  w.wh = a.take<f16>(s.D * vp);
-  if (s.split) {
-    w.pl = a.take<f16>(s.T * vp);
-    w.ql = a.take<f16>(vc * s.tp);
-    w.tl = a.take<f16>((long long)s.D * s.tp);
-    w.wl = a.take<f16>(s.D * vp);
-  }
+  w.split = a.take<float>(PART_BYTES / 4);
+  w.p = a.take<f16>(s.T * vp * s.P);
+  w.pt = a.take<f16>(vc * s.tp * s.P);
+  w.ht = a.take<f16>((long long)s.D * s.tp * s.P);
+  w.wt = a.take<f16>(s.D * vp * s.P);
   return w;
 }
 
@@ -483,24 +478,19 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
     else hipLaunchKernelGGL(K<TCMI_BF16>, __VA_ARGS__);                                            \
   } while (0)
 
-template <class Epi>
-hipError_t run(Args& g, int dtype, const Epi& e, hipStream_t st) {
-  unsigned blocks;
-  if (!plan<TileL>(g, 1, false, &blocks)) return hipErrorInvalidValue;
-  if (dtype == TCMI_BF16) hipLaunchKernelGGL((product_kernel<bf16x8, TileL, Epi>), dim3(blocks), dim3(TileL::THREADS), 0, st, g, e);
-  else hipLaunchKernelGGL((product_kernel<f16x8, TileL, Epi>), dim3(blocks), dim3(TileL::THREADS), 0, st, g, e);
-  return hipGetLastError();
+template <int P, class Epi>
+hipError_t run(const Args& g, const Epi& e, hipStream_t st) {
+  if constexpr (Epi::WHOLE) return launch<f16x8, P, LseTile>(g, false, e, st);
+  else return launch_best<f16x8, P>(g, false, e, st);
 }
 
-void pairs(Args& g, const void* ah, const void* al, const void* bh, const void* bl) {
-  auto add = [&](const void* a, const void* b) {
-    g.a[g.nseg] = a;
-    g.b[g.nseg] = b;
-    ++g.nseg;
-  };
-  add(ah, bh);
-  if (bl) add(ah, bl);
-  if (al) add(al, bh);
+// the logits' product: 16-bit heads in their own type
+template <int P, class Epi>
+hipError_t run_logits(const Args& g, int dtype, const Epi& e, hipStream_t st) {
+  if constexpr (P == 1) {
+    if (dtype == TCMI_BF16) return launch<bf16x8, 1, LseTile>(g, false, e, st);
+  }
+  return run<P>(g, e, st);
 }
 
 struct In {
@@ -512,11 +502,11 @@ struct In {
 
 hipError_t operands(const Shape& s, const In& in, const Rows& r, hipStream_t st) {
   if (!s.h_direct) {
-    BY_TYPE(s.dtype, rows_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, s.dp, r.h, r.hl, r.hs);
+    BY_TYPE(s.dtype, rows_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, s.dp, r.h, r.hs);
     TRY(hipGetLastError());
   }
   if (!s.w_direct) {
-    BY_TYPE(s.dtype, rows_kernel, dim3((s.V + 3) / 4), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, s.dp, r.w, r.wl, r.ws);
+    BY_TYPE(s.dtype, rows_kernel, dim3((s.V + 3) / 4), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, s.dp, r.w, r.ws);
     TRY(hipGetLastError());
   }
   return hipSuccess;
@@ -527,22 +517,24 @@ Args logit_args(const Shape& s, const In& in, const Rows& r, int v0, int vc) {
   Args g{};
   g.M = s.T;
   g.N = vc;
-  g.K = s.dp;
-  g.lda = s.h_direct ? in.hrs : s.dp;
-  g.ldb = s.w_direct ? in.wrs : s.dp;
-  const void* h = s.h_direct ? in.h : r.h;
-  const f16* w = (const f16*)(s.w_direct ? in.w : r.w) + v0 * g.ldb;
-  pairs(g, h, r.hl, w, r.wl ? r.wl + v0 * g.ldb : nullptr);
+  g.K = s.P * s.dp;
+  g.lda = s.h_direct ? in.hrs : s.P * s.dp;
+  g.ldb = s.w_direct ? in.wrs : s.P * s.dp;
+  g.batch = 1;
+  g.nseg = 1;
+  g.a[0] = s.h_direct ? in.h : r.h;
+  g.b[0] = (const f16*)(s.w_direct ? in.w : r.w) + v0 * g.ldb;
   return g;
 }
 
+template <int P>
 hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, float* loss, float* total, float* count, int mean,
                    hipStream_t st) {
   TRY(operands(s, in, w.rows, st));
-  Args g = logit_args(s, in, w.rows, 0, s.V);
-  EpiLse e{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y};
-  TRY(run(g, s.dtype, e, st));
-  hipLaunchKernelGGL(join_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, w.part, g.tn, w.target, in.y, in.ignore, s.T, s.V, lse, loss);
+  const Args g = logit_args(s, in, w.rows, 0, s.V);
+  TRY(run_logits<P>(g, s.dtype, EpiLse{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
+  const int tiles = (s.V + LseTile::BN - 1) / LseTile::BN;
+  hipLaunchKernelGGL(rowstat_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, w.part, tiles, w.target, in.y, in.ignore, s.T, s.V, lse, loss);
   TRY(hipGetLastError());
   if (total) {
     hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, in.y, in.ignore, s.T, mean, total, count);
@@ -551,6 +543,7 @@ hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, f
   return hipSuccess;
 }
 
+template <int P>
 hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float* lse, const float* dloss, int per_row, const float* count,
                     void* dh, void* dw, void* db, hipStream_t st) {
   TRY(operands(s, in, w.rows, st));
@@ -562,8 +555,8 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
     const int nb = blocks(s.T);
     BY_TYPE(s.dtype, top_kernel, dim3(nb), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, w.r, w.parth);
     TRY(hipGetLastError());
-    BY_TYPE(s.dtype, turn_kernel, dim3(s.tp / 64, (s.D + 63) / 64), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, w.r, w.parth, nb, w.th,
-            w.tl, (long long)s.tp, w.invh);
+    BY_TYPE(s.dtype, turn_kernel, dim3((s.tp + 63) / 64, (s.D + 63) / 64), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, w.r, w.parth, nb,
+            w.ht, s.tp, w.invh);
     TRY(hipGetLastError());
   }
   const int nbw = blocks(s.V);
@@ -573,37 +566,35 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
   }
   const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
   for (int v0 = 0; v0 < s.V; v0 += vc) {
-    const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (n + 63) & ~63;
-    Args g = logit_args(s, in, w.rows, v0, n);
-    EpiProb e{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.ph, w.pl, w.qh, w.ql, np, s.tp};
-    TRY(run(g, s.dtype, e, st));
+    const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P);
+    TRY(run_logits<P>(logit_args(s, in, w.rows, v0, n), s.dtype,
+                      EpiProb<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.p, w.pt, np, s.tp}, st));
+    Args d{};
+    d.N = s.D;
+    d.batch = 1;
+    d.nseg = 1;
+    d.part = w.split;
     if (dh) {
-      BY_TYPE(s.dtype, turn_kernel, dim3(np / 64, (s.D + 63) / 64), dim3(256), 0, st, (const char*)in.w + v0 * in.wrs * size, in.wrs, n,
-              s.D, none, w.partw, nbw, w.wh, w.wl, (long long)np, w.invw);
+      BY_TYPE(s.dtype, turn_kernel, dim3((np + 63) / 64, (s.D + 63) / 64), dim3(256), 0, st, (const char*)in.w + v0 * in.wrs * size, in.wrs,
+              n, s.D, none, w.partw, nbw, w.wt, np, w.invw);
       TRY(hipGetLastError());
-      Args d{};
       d.M = s.T;
-      d.N = s.D;
-      d.K = np;
-      d.lda = np;
-      d.ldb = np;
-      pairs(d, w.ph, w.pl, w.wh, w.wl);
-      EpiGrad eh{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype};
-      TRY(run(d, TCMI_F16, eh, st));
+      d.K = P * np;
+      d.lda = d.ldb = d.K;
+      d.a[0] = w.p;
+      d.b[0] = w.wt;
+      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype}, st));
     }
     if (dw) {
-      Args d{};
       d.M = n;
-      d.N = s.D;
-      d.K = s.tp;
-      d.lda = s.tp;
-      d.ldb = s.tp;
-      pairs(d, w.qh, w.ql, w.th, w.tl);
-      EpiGrad ew{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype};
-      TRY(run(d, TCMI_F16, ew, st));
+      d.K = P * s.tp;
+      d.lda = d.ldb = d.K;
+      d.a[0] = w.pt;
+      d.b[0] = w.ht;
+      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype}, st));
     }
     if (db) {
-      hipLaunchKernelGGL(bias_kernel, dim3((n + 3) / 4), dim3(256), 0, st, w.qh, w.ql, (long long)s.tp, w.r, s.T, n, db, s.dtype, v0);
+      hipLaunchKernelGGL(bias_kernel<P>, dim3((n + 3) / 4), dim3(256), 0, st, w.pt, s.tp, w.r, s.T, n, db, s.dtype, v0);
       TRY(hipGetLastError());
     }
   }
@@ -626,9 +617,9 @@ Shape shape_of(int T, int D, int V, int dtype, bool h_direct, bool w_direct) {
   s.D = D;
   s.V = V;
   s.dtype = dtype;
-  s.dp = (D + 63) & ~63;
-  s.tp = (T + 63) & ~63;
-  s.split = dtype == TCMI_F32;
+  s.P = dtype == TCMI_F32 ? 2 : 1;
+  s.dp = (int)kpad(D, s.P);
+  s.tp = (int)kpad(T, s.P);
   s.h_direct = h_direct;
   s.w_direct = w_direct;
   return s;
@@ -663,7 +654,7 @@ int tcmi_linear_cross_entropy(const void* h, long long h_rs, const void* w, long
   if (a.used > work_bytes || ((uintptr_t)work & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy: workspace too small or not 256-byte aligned");
   const In in{h, w, bias, h_rs, w_rs, target, ignore_index};
-  const hipError_t e = forward(s, in, k, lse, loss, total, count, mean, reinterpret_cast<hipStream_t>(stream));
+  const hipError_t e = (s.P == 2 ? forward<2> : forward<1>)(s, in, k, lse, loss, total, count, mean, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
 }
 
@@ -680,7 +671,7 @@ int tcmi_linear_cross_entropy_grad(const void* h, long long h_rs, const void* w,
   if (a.used > work_bytes || ((uintptr_t)work & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy_grad: workspace too small or not 256-byte aligned");
   const In in{h, w, bias, h_rs, w_rs, target, ignore_index};
-  const hipError_t e = backward(s, in, k, lse, dloss, per_row, count, dh, dw, db, reinterpret_cast<hipStream_t>(stream));
+  const hipError_t e = (s.P == 2 ? backward<2> : backward<1>)(s, in, k, lse, dloss, per_row, count, dh, dw, db, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
 }
 

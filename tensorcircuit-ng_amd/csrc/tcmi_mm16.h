@@ -1,13 +1,14 @@
 // Matrix core of the training operators: C[m][n] = sum_s sum_k A_s[m][k] B_s[n][k] on the f16 / bf16 matrix pipe with f32
-// accumulators, up to six pairs ("segments") of k-contiguous operands per product, and an epilogue functor per use.
+// accumulators, up to two pairs ("segments") of k-contiguous operands per product (P D + Q X), and an epilogue functor per use.
 //
-// Segments carry the precision: an f32 operand x is held as two f16 pieces x = hi + lo (11 + 11 significand bits), and
-// x y ~= hi hi' + hi lo' + lo hi' is three segments of one accumulation; what is dropped is below 2^-22 |x y|, the size of
-// an f32 rounding.  Sums of several products (P D + Q X) are segments too.
+// P pieces per operand carry the precision.  P = 1: the f16 / bf16 values.  P = 2: an f32 value x is held as two f16 pieces,
+// x = hi + lo (11 + 11 significand bits), and x y ~= hi hi' + hi lo' + lo hi': three matrix products per fragment pair; what is
+// dropped is below 2^-22 |x y|.  The pieces lie interleaved, 32 hi then 32 lo of the same 32 k, so that both forms have
+// the same 128-byte k step in memory and in LDS and differ only in which fragments meet.
 //
-// Operand contract (checked by the callers on the host): rows are k-contiguous and 16-byte aligned, K is a multiple of
-// 64 with everything beyond the true length zero, row indices past the end are clamped (never read outside), and the
-// epilogue masks what the clamped rows produce.
+// Operand contract (checked by the callers on the host): rows are k-contiguous and 16-byte aligned, K (stored values a row)
+// is a multiple of 64 with everything beyond the true length zero, row indices past the end are clamped (never read
+// outside), and the epilogue masks what the clamped rows produce.
 #ifndef TCMI_MM16_H
 #define TCMI_MM16_H
 
@@ -23,19 +24,27 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int MAX_SEG = 6;
-
 struct Args {
-  const void* a[MAX_SEG];
-  const void* b[MAX_SEG];
+  const void* a[2];
+  const void* b[2];
   int nseg;
-  int M, N, K;                 // K a multiple of 64
+  int M, N, K;                 // K: stored values of a row, a multiple of 64
   long long lda, ldb;          // elements between rows
   long long sa, sb;            // elements between batch members
   int tm, tn;                  // tiles per matrix
   int tri;                     // 1: C is symmetric, only tiles with row tile >= column tile are computed
   int tiles;                   // tiles per batch member (tm * tn, or the triangle)
+  int batch;
+  int split;                   // > 1: the k steps are dealt to `split` workgroups, whose sums join_kernel adds
+  float* part;                 // [split][batch * tiles][BM * BN]
 };
+
+// where logical k lies in a row of P pieces (the low piece 32 further), and the padded length of a row
+template <int P>
+__host__ __device__ constexpr long long kpos(long long k) {
+  return P == 1 ? k : ((k >> 5) << 6) + (k & 31);
+}
+__host__ __device__ constexpr long long kpad(long long k, int P) { return P == 1 ? (k + 63) & ~63ll : (k + 31) & ~31ll; }
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -44,21 +53,15 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// Which tile a workgroup computes.  Workgroups go to the eight XCDs in turn; renumbered so that each XCD (its own L2) gets
-// one contiguous range, in bands of 8 row tiles, whose operand rows it then reads from its L2.
-__device__ __forceinline__ void tile_of(const Args& g, int& ti, int& tj, int& bz) {
-  const unsigned total = gridDim.x, id = blockIdx.x;
-  const unsigned q = total >> 3, r = total & 7, x = id & 7;
-  const unsigned w = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
-  bz = (int)(w / (unsigned)g.tiles);
-  const unsigned t = w % (unsigned)g.tiles;
+// tile t of a batch member
+__device__ __forceinline__ void tile_at(const Args& g, unsigned t, int& ti, int& tj) {
   if (g.tri) {
     unsigned i = (unsigned)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
     while (i * (i + 1) / 2 > t) --i;
     while ((i + 1) * (i + 2) / 2 <= t) ++i;
     ti = (int)i;
     tj = (int)(t - i * (i + 1) / 2);
-  } else {
+  } else {                                          // bands of 8 row tiles: their operand rows stay in an L2
     const unsigned band = t / (8u * g.tn), in = t % (8u * g.tn);
     const unsigned rows = min(8u, (unsigned)g.tm - band * 8u);
     ti = (int)(band * 8u + in % rows);
@@ -66,24 +69,35 @@ __device__ __forceinline__ void tile_of(const Args& g, int& ti, int& tj, int& bz
   }
 }
 
-template <int BM_, int BN_, int WM_, int WN_>
+// Workgroups go to the eight XCDs in turn; renumbered so that each XCD (its own L2) gets one contiguous range.
+__device__ __forceinline__ unsigned unit_of() {
+  const unsigned total = gridDim.x, id = blockIdx.x;
+  const unsigned q = total >> 3, r = total & 7, x = id & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
+}
+
+template <int BM_, int BN_, int WM_, int WN_, int PER_CU_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PER_CU = PER_CU_;
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
-  static constexpr int STAGE = (BM + BN) * 128;            // bytes of one 64-deep k step of both operands
+  static constexpr int STAGE = (BM + BN) * 128;            // bytes of one k step of both operands
+  static constexpr int LDS = 2 * STAGE;
 };
 
 using LdsPtr = __attribute__((address_space(3))) void*;
 
-// One product tile.  `acc[mi][ni]` holds C[row][col .. col + 3] with row = m0 + wm * BM / WM + 16 mi + (lane & 15) and
-// col = n0 + wn * BN / WN + 16 ni + 4 (lane >> 4): the B fragment is the first MFMA operand, so a lane ends with four
-// neighbouring columns of one row.
-// LDS: a row's 64 k values are eight 16-byte chunks; chunk c of row r lies at position c ^ (r & 7), which spreads the 16
-// rows a fragment read touches over all banks.  Global -> LDS goes without registers (buffer_load ... lds), two stages.
 #ifdef __HIP_DEVICE_COMPILE__          // the host pass does not know the buffer resource type
-template <class V, class T>
-__device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, char* lds, f32x4 (&acc)[T::MI][T::NI]) {
+// The k steps [s0, s1) of one product tile.  `acc[i][j]` holds C[row][col .. col + 3] with
+// row = m0 + (wm MI + i) 16 + (lane & 15) and col = n0 + (wn NI + j) 16 + 4 (lane >> 4): the B fragment is the first
+// matrix operand, so a lane ends with four neighbouring columns of one row.
+//
+// LDS: a row's k step is eight 16-byte chunks; chunk c of row r lies at position c ^ (r & 7), which spreads the 16 rows of a
+// fragment read over all banks.  Global -> LDS goes without registers (buffer_load ... lds) into two stages; fragments go
+// LDS -> registers half a step ahead of the matrix instructions that use them.  One barrier a step: when every wave has its
+// stage in registers and its loads of the next stage have landed, the stage is free for the loads of the step after.
+template <class V, int P, class T>
+__device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, int s0, int s1, char* lds, f32x4 (&acc)[T::MI][T::NI]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / T::WN, wn = wave % T::WN;
   constexpr int LA = T::BM / 8 / T::WAVES, LB = T::BN / 8 / T::WAVES;      // loads per wave: 8 rows of 128 bytes each
@@ -102,8 +116,8 @@ __device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, c
   }
   const long long offa = ((long long)bz * g.sa + (long long)m0 * g.lda) * 2;
   const long long offb = ((long long)bz * g.sb + (long long)n0 * g.ldb) * 2;
-  const int ksteps = g.K >> 6, steps = ksteps * g.nseg;
-  int ls = 0, lk = 0;                                                   // segment and k step of the next load
+  const int ksteps = g.K >> 6;
+  int ls = s0 / ksteps, lk = s0 % ksteps;                               // segment and k step of the next load
 
   auto load = [&](int stage) {
     char* base = lds + stage * T::STAGE;
@@ -122,50 +136,58 @@ __device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, c
     }
   };
 
-  load(0);
-  for (int s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);                 // this wave's loads of step s are in LDS, its reads of step s - 1 done
-    __syncthreads();
-    if (s + 1 < steps) load((s + 1) & 1);
-    const char* pa = lds + (s & 1) * T::STAGE + (wm * T::MI * 16) * 128;
-    const char* pb = lds + (s & 1) * T::STAGE + (T::BM + wn * T::NI * 16) * 128;
-    const int r = lane & 15;
+  const int r = lane & 15;
+  const int at[2] = {(((lane >> 4)) ^ (r & 7)) * 16 + r * 128, ((4 + (lane >> 4)) ^ (r & 7)) * 16 + r * 128};
+  const char* pa = lds + (wm * T::MI * 16) * 128;
+  const char* pb = lds + (T::BM + wn * T::NI * 16) * 128;
+  auto read_a = [&](V (&f)[T::MI], int stage, int half) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = ((k * 4 + (lane >> 4)) ^ (r & 7)) * 16 + r * 128;
-      V fa[T::MI], fb[T::NI];
+    for (int i = 0; i < T::MI; ++i) f[i] = *reinterpret_cast<const V*>(pa + stage * T::STAGE + i * 2048 + at[half]);
+  };
+  auto read_b = [&](V (&f)[T::NI], int stage, int half) {
 #pragma unroll
-      for (int i = 0; i < T::MI; ++i) fa[i] = *reinterpret_cast<const V*>(pa + i * 2048 + c);
+    for (int i = 0; i < T::NI; ++i) f[i] = *reinterpret_cast<const V*>(pb + stage * T::STAGE + i * 2048 + at[half]);
+  };
+  auto multiply = [&](const V (&fa)[T::MI], const V (&fb)[T::NI]) {
 #pragma unroll
-      for (int i = 0; i < T::NI; ++i) fb[i] = *reinterpret_cast<const V*>(pb + i * 2048 + c);
+    for (int i = 0; i < T::MI; ++i)
 #pragma unroll
-      for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < T::NI; ++j) acc[i][j] = mfma(fb[j], fa[i], acc[i][j]);
+      for (int j = 0; j < T::NI; ++j) acc[i][j] = mfma(fb[j], fa[i], acc[i][j]);
+  };
+  V a0[T::MI], a1[T::MI], b0[T::NI], b1[T::NI], b2[T::NI];
+  // one k step: b holds the first half's B fragments, bn receives the next step's
+  auto step = [&](int s, V (&b)[T::NI], V (&bn)[T::NI]) {
+    const int stage = (s - s0) & 1;
+    read_b(b1, stage, 1);
+    read_a(a1, stage, 1);
+    multiply(a0, b);
+    if constexpr (P == 2) multiply(a0, b1);
+    if (s + 1 < s1) {
+      __builtin_amdgcn_s_waitcnt(0);               // this stage is in registers, the next one has landed
+      __syncthreads();
+      if (s + 2 < s1) load(stage);
+      read_b(bn, stage ^ 1, 0);
+      read_a(a0, stage ^ 1, 0);
     }
+    if constexpr (P == 1) multiply(a1, b1);
+    else multiply(a1, b);
+  };
+
+  load(0);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (s0 + 1 < s1) load(1);
+  read_b(b0, 0, 0);
+  read_a(a0, 0, 0);
+  for (int s = s0; s < s1; s += 2) {
+    step(s, b0, P == 1 ? b0 : b2);
+    if (s + 1 < s1) step(s + 1, P == 1 ? b0 : b2, b0);
   }
 }
-
 #endif
 
-// Epi: __device__ void tile(const Args&, int m0, int n0, int bz, bool mirror, char* lds, f32x4 (&acc)[MI][NI])
-template <class V, class T, class Epi>
-__global__ __launch_bounds__(T::THREADS) void product_kernel(Args g, Epi e) {
-#ifdef __HIP_DEVICE_COMPILE__
-  __shared__ __attribute__((aligned(128))) char lds[2 * T::STAGE];
-  int ti, tj, bz;
-  tile_of(g, ti, tj, bz);
-  f32x4 acc[T::MI][T::NI];
-#pragma unroll
-  for (int i = 0; i < T::MI; ++i)
-#pragma unroll
-    for (int j = 0; j < T::NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  product<V, T>(g, ti * T::BM, tj * T::BN, bz, lds, acc);
-  e.template tile<T>(g, ti * T::BM, tj * T::BN, bz, g.tri && ti != tj, lds, acc);
-#endif
-}
-
-// calls f(row, col, value) for the lane's accumulators, four neighbouring columns a call
+// An epilogue works on whole tiles (WHOLE: void tile<T>(g, m0, n0, bz, lds, acc)) or on four neighbouring columns of a row
+// at a time (void four(g, bz, mirror, row, col, v); the product may then be split along k).
 template <class T, class F>
 __device__ __forceinline__ void each(int m0, int n0, const f32x4 (&acc)[T::MI][T::NI], F f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -177,22 +199,127 @@ __device__ __forceinline__ void each(int m0, int n0, const f32x4 (&acc)[T::MI][T
       f(m0 + wm * T::MI * 16 + i * 16 + (lane & 15), n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4), acc[i][j]);
 }
 
+template <class V, int P, class T, class Epi>
+__global__ __launch_bounds__(T::THREADS, T::PER_CU * T::WAVES / 4) void product_kernel(Args g, Epi e) {
+#ifdef __HIP_DEVICE_COMPILE__
+  extern __shared__ __attribute__((aligned(128))) char lds[];
+  const unsigned w = unit_of(), per = (unsigned)(g.tiles * g.batch), u = w % per, sp = w / per;
+  const int bz = (int)(u / (unsigned)g.tiles);
+  int ti, tj;
+  tile_at(g, u % (unsigned)g.tiles, ti, tj);
+  const int m0 = ti * T::BM, n0 = tj * T::BN, steps = (g.K >> 6) * g.nseg;
+  const int s0 = (int)((long long)steps * sp / g.split), s1 = (int)((long long)steps * (sp + 1) / g.split);
+  f32x4 acc[T::MI][T::NI];
+#pragma unroll
+  for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  product<V, P, T>(g, m0, n0, bz, s0, s1, lds, acc);
+  if constexpr (Epi::WHOLE) {
+    e.template tile<T>(g, m0, n0, bz, lds, acc);
+  } else {
+    if (g.split > 1) {
+      f32x4* p = reinterpret_cast<f32x4*>(g.part) + (long long)w * (T::BM * T::BN / 4) + threadIdx.x;
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < T::NI; ++j) p[(i * T::NI + j) * T::THREADS] = acc[i][j];
+      return;
+    }
+    const bool mirror = g.tri && ti != tj;
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) { e.four(g, bz, mirror, row, col, v); });
+  }
+#endif
+}
+
+// adds the parts of a split product in a fixed order and applies the epilogue: one workgroup per fragment column of a tile
+template <class T, class Epi>
+__global__ __launch_bounds__(T::THREADS) void join_kernel(Args g, Epi e) {
+  constexpr unsigned F = T::MI * T::NI;
+  const unsigned u = blockIdx.x / F, f = blockIdx.x % F, per = (unsigned)(g.tiles * g.batch);
+  const int bz = (int)(u / (unsigned)g.tiles);
+  int ti, tj;
+  tile_at(g, u % (unsigned)g.tiles, ti, tj);
+  const f32x4* p = reinterpret_cast<const f32x4*>(g.part) + (long long)u * (T::BM * T::BN / 4) + f * T::THREADS + threadIdx.x;
+  const long long step = (long long)per * (T::BM * T::BN / 4);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < g.split; ++k) v += p[k * step];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = ti * T::BM + (wave / T::WN) * T::MI * 16 + (int)(f / T::NI) * 16 + (lane & 15);
+  const int col = tj * T::BN + (wave % T::WN) * T::NI * 16 + (int)(f % T::NI) * 16 + 4 * (lane >> 4);
+  e.four(g, bz, g.tri && ti != tj, row, col, v);
+}
+
 __device__ __forceinline__ void two_pieces(float x, f16& hi, f16& lo) {
   hi = (f16)x;
   lo = (f16)(x - (float)hi);
 }
 
-// host side: tile counts and launch
+// four neighbouring values, stored as P pieces at logical column col (a multiple of 4)
+template <int P>
+__device__ __forceinline__ void store_four(f16* row, int col, const f16x4& hi, const f16x4& lo) {
+  f16* p = row + kpos<P>(col);
+  *reinterpret_cast<f16x4*>(p) = hi;
+  if (P == 2) *reinterpret_cast<f16x4*>(p + 32) = lo;
+}
+
+// ---- host side ----
+using Big = Tile<256, 256, 2, 2, 1>;
+using Mid = Tile<128, 128, 2, 2, 2>;
+using Slim = Tile<128, 64, 4, 1, 2>;
+
+constexpr long long PART_BYTES = 512ll * 128 * 128 * 4;       // workspace of a split product
+
 template <class T>
-inline bool plan(Args& g, int batch, bool tri, unsigned* blocks) {
+inline long long tile_count(const Args& g, bool tri) {
+  const long long tm = (g.M + T::BM - 1) / T::BM, tn = (g.N + T::BN - 1) / T::BN;
+  return (tri ? tm * (tm + 1) / 2 : tm * tn) * g.batch;
+}
+
+template <class V, int P, class T, class Epi>
+hipError_t launch(Args g, bool tri, const Epi& e, hipStream_t st) {
   g.tm = (g.M + T::BM - 1) / T::BM;
   g.tn = (g.N + T::BN - 1) / T::BN;
   g.tri = tri ? 1 : 0;
-  const long long tiles = tri ? (long long)g.tm * (g.tm + 1) / 2 : (long long)g.tm * g.tn;
-  if (tiles * batch >= (1ll << 31) || tiles < 1) return false;
+  const long long tiles = tri ? (long long)g.tm * (g.tm + 1) / 2 : (long long)g.tm * g.tn, units = tiles * g.batch;
+  if (units < 1 || units >= (1ll << 24) || g.K < 64 || (g.K & 63) || g.nseg < 1) return hipErrorInvalidValue;
   g.tiles = (int)tiles;
-  *blocks = (unsigned)(tiles * batch);
-  return true;
+  g.split = 1;
+  if constexpr (!Epi::WHOLE) {
+    // too few tiles for the card's workgroups: deal the k steps out too, at least 8 to each
+    const long long slots = 256ll * T::PER_CU, steps = (long long)(g.K / 64) * g.nseg;
+    if (g.part && units * 4 < slots * 3) {
+      long long s = slots / units;
+      s = s < steps / 8 ? s : steps / 8;
+      const long long room = PART_BYTES / (units * T::BM * T::BN * 4);
+      s = s < room ? s : room;
+      if (s > 1) g.split = (int)s;
+    }
+  }
+  static bool raised = false;                                 // the attribute belongs to the function, not to a call
+  if (!raised) {
+    const hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<V, P, T, Epi>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+    if (r != hipSuccess) return r;
+    raised = true;
+  }
+  hipLaunchKernelGGL((product_kernel<V, P, T, Epi>), dim3((unsigned)(units * g.split)), dim3(T::THREADS), T::LDS, st, g, e);
+  hipError_t r = hipGetLastError();
+  if constexpr (!Epi::WHOLE) {
+    if (r == hipSuccess && g.split > 1) {
+      hipLaunchKernelGGL((join_kernel<T, Epi>), dim3((unsigned)(units * T::MI * T::NI)), dim3(T::THREADS), 0, st, g, e);
+      r = hipGetLastError();
+    }
+  }
+  return r;
+}
+
+// tile by the shape of the result
+template <class V, int P, class Epi>
+hipError_t launch_best(const Args& g, bool tri, const Epi& e, hipStream_t st) {
+  if (!tri && g.N <= 64) return launch<V, P, Slim>(g, tri, e, st);
+  return launch<V, P, Mid>(g, tri, e, st);
 }
 
 }  // namespace mm16

@@ -104,8 +104,8 @@ __global__ __launch_bounds__(256) void sums_kernel(SumArgs a) {
 }
 
 // Operand layout: a 64 x 64 tile of the source becomes f16 pieces, row-major and transposed (both k-contiguous for the
-// products that read them), zero beyond the matrix up to the next multiple of 64, and the f32 carry.  Bound by its
-// writes.  norm: the tile is divided by (sqrt(sum of part) + eps); every workgroup adds the partial sums itself.
+// products that read them), zero beyond the matrix up to the padded length, and the f32 carry.  Bound by its writes.
+// part: the tile is divided by (sqrt(sum of part) + eps); every workgroup adds the partial sums itself.
 struct PackArgs {
   Mat src;
   int m, n, tx, ty, fast_rows;             // logical size, tiles, 1: the source is contiguous along rows
@@ -117,7 +117,7 @@ struct PackArgs {
   long long brs, bcs, bbs;
   float rest;
   int nesterov;
-  f16 *hi, *lo, *thi, *tlo;                // lo, tlo null: one piece
+  f16 *x, *t;                              // X [mr][ld], X^T [nc][ldt]
   long long ld, os, ldt, ts;               // row strides and batch strides
   float* carry;                            // f32 [m][ldc] (null: none); complex: im at column n + j
   int carry_raw;                           // 1: the carry is not divided by the norm
@@ -125,11 +125,11 @@ struct PackArgs {
   int embed;                               // complex as a real matrix of twice the size
 };
 
-template <int SRC>
+template <int SRC, int P>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
-  __shared__ float tr[64][65], tim[SRC == SRC_C64 || SRC == SRC_PLANAR ? 64 : 1][65];
-  __shared__ double red[4];
   constexpr bool MAYBE_COMPLEX = SRC == SRC_C64 || SRC == SRC_PLANAR;
+  __shared__ float tr[64][65], tim[MAYBE_COMPLEX ? 64 : 1][65];
+  __shared__ double red[4];
   const unsigned tiles = (unsigned)a.tx * a.ty;
   const int bz = blockIdx.x / tiles, t = blockIdx.x % tiles, i0 = (t / a.tx) * 64, j0 = (t % a.tx) * 64;
   float inv = 1.f;
@@ -159,14 +159,13 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
   __syncthreads();
   const float cinv = a.carry_raw ? 1.f : inv;
   const bool twice = MAYBE_COMPLEX && a.embed;
-  const int mrows = twice ? a.m : (a.m + 63) & ~63, ncols = twice ? a.n : (a.n + 63) & ~63;
-  f16 *hi = a.hi + (long long)bz * a.os, *lo = a.lo ? a.lo + (long long)bz * a.os : nullptr;
-  f16 *thi = a.thi + (long long)bz * a.ts, *tlo = a.tlo ? a.tlo + (long long)bz * a.ts : nullptr;
-  auto store = [&](f16* ph, f16* pl, long long at, float x) {
+  const int mrows = twice ? a.m : (int)kpad(a.m, P), ncols = twice ? a.n : (int)kpad(a.n, P);
+  f16 *px = a.x + (long long)bz * a.os, *pt = a.t + (long long)bz * a.ts;
+  auto store = [&](f16* row, int k, float x) {
     f16 h, l;
     two_pieces(x * inv * a.scale, h, l);
-    ph[at] = h;
-    if (pl) pl[at] = l;
+    row[kpos<P>(k)] = h;
+    if (P == 2) row[kpos<P>(k) + 32] = l;
   };
 #pragma unroll 4
   for (int k = w; k < 64; k += 4) {
@@ -174,13 +173,13 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
       const int i = i0 + k, j = j0 + u;
       if (i < a.m && j < ncols) {
         const float re = tr[k][u];
-        store(hi, lo, i * a.ld + j, re);
+        store(px + i * a.ld, j, re);
         if (a.carry && j < a.n) a.carry[(long long)bz * a.cbs + i * a.ldc + j] = re * cinv;
         if (twice) {
           const float im = tim[MAYBE_COMPLEX ? k : 0][u];
-          store(hi, lo, i * a.ld + j + a.n, im);
-          store(hi, lo, (long long)(i + a.m) * a.ld + j, -im);
-          store(hi, lo, (long long)(i + a.m) * a.ld + j + a.n, re);
+          store(px + i * a.ld, j + a.n, im);
+          store(px + (i + a.m) * a.ld, j, -im);
+          store(px + (i + a.m) * a.ld, j + a.n, re);
           if (a.carry) a.carry[(long long)bz * a.cbs + i * a.ldc + j + a.n] = im * cinv;
         }
       }
@@ -189,12 +188,12 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
       const int i = i0 + u, j = j0 + k;
       if (j < a.n && i < mrows) {
         const float re = tr[u][k];
-        store(thi, tlo, j * a.ldt + i, re);
+        store(pt + j * a.ldt, i, re);
         if (twice) {
           const float im = tim[MAYBE_COMPLEX ? u : 0][k];
-          store(thi, tlo, (long long)(j + a.n) * a.ldt + i, im);
-          store(thi, tlo, j * a.ldt + i + a.m, -im);
-          store(thi, tlo, (long long)(j + a.n) * a.ldt + i + a.m, re);
+          store(pt + (j + a.n) * a.ldt, i, im);
+          store(pt + j * a.ldt, i + a.m, -im);
+          store(pt + (j + a.n) * a.ldt, i + a.m, re);
         }
       }
     }
@@ -205,79 +204,74 @@ __global__ __launch_bounds__(256) void clear_kernel(uint4* p, long long n) {
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = make_uint4(0, 0, 0, 0);
 }
 
-// A symmetric result as f16 pieces: value = alpha acc + beta (src hi + src lo), stored times `scale`; the tile below the
-// diagonal also writes its mirror image.  Columns up to the padded width get zeros.
+// A symmetric result as f16 pieces: value = alpha acc + beta src, stored times `scale`; a tile below the diagonal also
+// writes its mirror image.  Columns up to the padded width get zeros.
+template <int P>
 struct EpiSym {
-  f16 *hi, *lo;
-  const f16 *shi, *slo;
+  static constexpr bool WHOLE = false;
+  f16* out;
+  const f16* src;
   long long ld, bs;
   float alpha, beta, scale;
-  template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int bz, bool mirror, char*, f32x4 (&acc)[T::MI][T::NI]) const {
-    const int wide = (g.M + 63) & ~63;
-    f16 *h = hi + bz * bs, *l = lo ? lo + bz * bs : nullptr;
-    const f16 *sh = shi ? shi + bz * bs : nullptr, *sl = slo ? slo + bz * bs : nullptr;
-    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
-      f16x4 vh, vl, s4 = {}, t4 = {};
-      if (sh && row < g.M && col < wide) {
-        s4 = *reinterpret_cast<const f16x4*>(sh + (long long)row * ld + col);
-        if (sl) t4 = *reinterpret_cast<const f16x4*>(sl + (long long)row * ld + col);
-      }
+  __device__ __forceinline__ void four(const Args& g, int bz, bool mirror, int row, int col, f32x4 v) const {
+    const int wide = (int)kpad(g.M, P);
+    const bool in = row < g.M && col < wide;
+    f16* o = out + bz * bs;
+    f16x4 s4 = {}, t4 = {}, vh, vl;
+    if (src && in) {
+      const f16* s = src + bz * bs + row * ld + kpos<P>(col);
+      s4 = *reinterpret_cast<const f16x4*>(s);
+      if (P == 2) t4 = *reinterpret_cast<const f16x4*>(s + 32);
+    }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = v[r] * alpha;
-        if (sh) x += beta * ((float)s4[r] + (float)t4[r]);
-        x = row < g.M && col + r < g.M ? x * scale : 0.f;
-        f16 a, b;
-        two_pieces(x, a, b);
-        vh[r] = a;
-        vl[r] = b;
-      }
-      if (row < g.M && col < wide) {
-        *reinterpret_cast<f16x4*>(h + (long long)row * ld + col) = vh;
-        if (l) *reinterpret_cast<f16x4*>(l + (long long)row * ld + col) = vl;
-      }
-      if (mirror && row < wide) {
+    for (int r = 0; r < 4; ++r) {
+      float x = fmaf(v[r], alpha, beta * ((float)s4[r] + (float)t4[r]));
+      x = row < g.M && col + r < g.M ? x * scale : 0.f;
+      f16 a, b;
+      two_pieces(x, a, b);
+      vh[r] = a;
+      vl[r] = b;
+    }
+    if (in) store_four<P>(o + row * ld, col, vh, vl);
+    if (mirror && row < wide) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (col + r < g.M) {
-            h[(long long)(col + r) * ld + row] = vh[r];
-            if (l) l[(long long)(col + r) * ld + row] = vl[r];
-          }
-      }
-    });
+      for (int r = 0; r < 4; ++r)
+        if (col + r < g.M) {
+          f16* p = o + (col + r) * ld + kpos<P>(row);
+          p[0] = vh[r];
+          if (P == 2) p[32] = vl[r];
+        }
+    }
   }
 };
 
 // carry <- beta carry + alpha acc (f32, in place: a thread reads and writes the same element)
 struct EpiCarry {
+  static constexpr bool WHOLE = false;
   float* carry;
   long long ld, bs;
   float alpha, beta;
   const float* dev;              // [batch] further factor of acc held on the device (null: none)
-  template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int bz, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+  __device__ __forceinline__ void four(const Args& g, int bz, bool, int row, int col, f32x4 v) const {
+    if (row >= g.M) return;
     const float al = dev ? alpha * dev[bz] : alpha;
-    float* c = carry + bz * bs;
-    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
-      if (row >= g.M) return;
-      float* p = c + (long long)row * ld + col;
-      if (col + 3 < g.N) {
-        f32x4 x = *reinterpret_cast<f32x4*>(p);
+    float* p = carry + bz * bs + row * ld + col;
+    if (col + 3 < g.N) {
+      f32x4 x = *reinterpret_cast<f32x4*>(p);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = fmaf(al, v[r], beta * x[r]);
-        *reinterpret_cast<f32x4*>(p) = x;
-      } else {
+      for (int r = 0; r < 4; ++r) x[r] = fmaf(al, v[r], beta * x[r]);
+      *reinterpret_cast<f32x4*>(p) = x;
+    } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (col + r < g.N) p[r] = fmaf(al, v[r], beta * p[r]);
-      }
-    });
+      for (int r = 0; r < 4; ++r)
+        if (col + r < g.N) p[r] = fmaf(al, v[r], beta * p[r]);
+    }
   }
 };
 
 // the last step: x = beta carry + alpha acc goes to the caller's matrix (out = x) or into a weight (out = keep out + rate x)
 struct EpiOut {
+  static constexpr bool WHOLE = false;
   const float* carry;
   long long ld, bs;
   float alpha, beta;
@@ -286,29 +280,27 @@ struct EpiOut {
   int dtype, n;                  // n: columns; complex: columns of the imaginary part start there
   int update;
   float keep, rate;
-  template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int bz, bool, char*, f32x4 (&acc)[T::MI][T::NI]) const {
-    const float* c = carry + bz * bs;
-    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
+  __device__ __forceinline__ void four(const Args& g, int bz, bool, int row, int col, f32x4 v) const {
+    if (row >= g.M) return;
+    const float* c = carry + bz * bs + row * ld;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = col + r;
-        if (row >= g.M || j >= g.N) continue;
-        const float x = fmaf(alpha, v[r], beta * c[(long long)row * ld + j]);
-        if (dtype == TCMI_C64) {
-          const int im = j >= n;
-          ((float*)out)[2 * (bz * os + row * rs + (j - im * n) * cs) + im] = x;
+    for (int r = 0; r < 4; ++r) {
+      const int j = col + r;
+      if (j >= g.N) continue;
+      const float x = fmaf(alpha, v[r], beta * c[j]);
+      if (dtype == TCMI_C64) {
+        const int im = j >= n;
+        ((float*)out)[2 * (bz * os + row * rs + (j - im * n) * cs) + im] = x;
+      } else {
+        const long long at = bz * os + row * rs + j * cs;
+        if (update) {
+          const float old = dtype == TCMI_F32 ? ((float*)out)[at] : dtype == TCMI_F16 ? (float)((f16*)out)[at] : (float)((__bf16*)out)[at];
+          put(out, dtype, at, fmaf(rate, x, keep * old));
         } else {
-          const long long at = bz * os + row * rs + j * cs;
-          if (update) {
-            const float old = dtype == TCMI_F32 ? ((float*)out)[at] : dtype == TCMI_F16 ? (float)((f16*)out)[at] : (float)((__bf16*)out)[at];
-            put(out, dtype, at, fmaf(rate, x, keep * old));
-          } else {
-            put(out, dtype, at, x);
-          }
+          put(out, dtype, at, x);
         }
       }
-    });
+    }
   }
 };
 
@@ -626,18 +618,18 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
 }
 
 // ---------------------------------------------------------------------------------------------------------- host side
-using TileS = Tile<128, 128, 2, 2>;
-
 struct Shape {
   int m, n;                       // min, max of the caller's two dimensions
   bool flip;                      // the caller's matrix is taller than wide: X is its transpose
   int cx;                         // 2 for complex
   int mr, nc;                     // size of the (embedded) real matrix
-  long long mp, np;               // padded to 64
+  int P;                          // pieces per operand
+  long long mp, np;               // stored row lengths over mr and nc: padded, times the pieces
+  long long ldc;                  // f32 rows of the carry
   int batch;
 };
 
-Shape shape_of(int rows, int cols, int batch, int dtype) {
+Shape shape_of(int rows, int cols, int batch, int dtype, bool full) {
   Shape s;
   s.flip = rows > cols;
   s.m = s.flip ? cols : rows;
@@ -645,8 +637,10 @@ Shape shape_of(int rows, int cols, int batch, int dtype) {
   s.cx = dtype == TCMI_C64 ? 2 : 1;
   s.mr = s.cx * s.m;
   s.nc = s.cx * s.n;
-  s.mp = (s.mr + 63ll) & ~63ll;
-  s.np = (s.nc + 63ll) & ~63ll;
+  s.P = full ? 2 : 1;
+  s.mp = s.P * kpad(s.mr, s.P);
+  s.np = s.P * kpad(s.nc, s.P);
+  s.ldc = (s.nc + 3ll) & ~3ll;
   s.batch = batch;
   return s;
 }
@@ -663,22 +657,15 @@ struct Arena {                    // hands out 256-byte aligned pieces of a call
 };
 
 struct Pieces {                   // one step's operands
-  f16 *xh, *xl, *th, *tl, *ah, *al, *bh, *bl;
+  f16 *x, *t, *a, *b;
 };
 
-Pieces take_pieces(Arena& w, const Shape& s, bool full) {
-  Pieces p{};
-  const long long x = s.mr * s.np * s.batch, t = s.nc * s.mp * s.batch, q = s.mr * s.mp * s.batch;
-  p.xh = w.take<f16>(x);
-  p.th = w.take<f16>(t);
-  p.ah = w.take<f16>(q);
-  p.bh = w.take<f16>(q);
-  if (full) {
-    p.xl = w.take<f16>(x);
-    p.tl = w.take<f16>(t);
-    p.al = w.take<f16>(q);
-    p.bl = w.take<f16>(q);
-  }
+Pieces take_pieces(Arena& w, const Shape& s) {
+  Pieces p;
+  p.x = w.take<f16>(s.mr * s.np * s.batch);
+  p.t = w.take<f16>(s.nc * s.mp * s.batch);
+  p.a = w.take<f16>(s.mr * s.mp * s.batch);
+  p.b = w.take<f16>(s.mr * s.mp * s.batch);
   return p;
 }
 
@@ -686,17 +673,17 @@ constexpr int MAX_PART = 256;
 
 struct Work {
   double* part;
-  float* norm;
-  float* carry;
+  float *norm, *carry, *split;
   Pieces p;
 };
 
-Work take_work(Arena& w, const Shape& s, bool full, bool saved) {
+Work take_work(Arena& w, const Shape& s, bool saved) {
   Work k{};
   k.part = w.take<double>((long long)s.batch * MAX_PART);
   k.norm = w.take<float>(s.batch);
-  k.carry = w.take<float>(s.m * s.np * s.batch);
-  if (!saved) k.p = take_pieces(w, s, full);
+  k.carry = w.take<float>(s.m * s.ldc * s.batch);
+  k.split = w.take<float>(PART_BYTES / 4);
+  if (!saved) k.p = take_pieces(w, s);
   return k;
 }
 
@@ -708,31 +695,26 @@ struct Saved {
 Saved take_saved(Arena& w, const Shape& s, int steps) {
   Saved v{};
   v.norm = w.take<float>(s.batch);
-  for (int i = 0; i < steps; ++i) v.p[i] = take_pieces(w, s, true);
+  for (int i = 0; i < steps; ++i) v.p[i] = take_pieces(w, s);
   return v;
 }
 
 struct GradWork {
   double* part;
-  float* norm;
-  float* carry;
-  f16 *dh, *dl, *th, *tl, *sh, *sl, *qh, *ql;
+  float *norm, *carry, *split;
+  f16 *d, *t, *s, *q;
 };
 
 GradWork take_grad(Arena& w, const Shape& s) {
   GradWork k{};
   k.part = w.take<double>((long long)s.batch * MAX_PART);
   k.norm = w.take<float>(s.batch);
-  k.carry = w.take<float>(s.m * s.np * s.batch);
-  const long long x = s.mr * s.np * s.batch, t = s.nc * s.mp * s.batch, q = s.mr * s.mp * s.batch;
-  k.dh = w.take<f16>(x);
-  k.dl = w.take<f16>(x);
-  k.th = w.take<f16>(t);
-  k.tl = w.take<f16>(t);
-  k.sh = w.take<f16>(q);
-  k.sl = w.take<f16>(q);
-  k.qh = w.take<f16>(q);
-  k.ql = w.take<f16>(q);
+  k.carry = w.take<float>(s.m * s.ldc * s.batch);
+  k.split = w.take<float>(PART_BYTES / 4);
+  k.d = w.take<f16>(s.mr * s.np * s.batch);
+  k.t = w.take<f16>(s.nc * s.mp * s.batch);
+  k.s = w.take<f16>(s.mr * s.mp * s.batch);
+  k.q = w.take<f16>(s.mr * s.mp * s.batch);
   return k;
 }
 
@@ -789,24 +771,9 @@ bool scales_of(int steps, const double* coef, Scales* out) {
   return s * SLACK <= MAX_S;
 }
 
-template <class T, class Epi>
-hipError_t run(Args& g, int batch, bool tri, const Epi& e, hipStream_t st) {
-  unsigned blocks;
-  if (!plan<T>(g, batch, tri, &blocks)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((product_kernel<f16x8, T, Epi>), dim3(blocks), dim3(T::THREADS), 0, st, g, e);
-  return hipGetLastError();
-}
-
-// segments of (ah + al)(bh + bl)^T without al bl; a null low piece drops its products
-void pairs(Args& g, const f16* ah, const f16* al, const f16* bh, const f16* bl) {
-  auto add = [&](const f16* a, const f16* b) {
-    g.a[g.nseg] = a;
-    g.b[g.nseg] = b;
-    ++g.nseg;
-  };
-  add(ah, bh);
-  if (bl) add(ah, bl);
-  if (al) add(al, bh);
+template <int P, class Epi>
+hipError_t run(const Args& g, bool tri, const Epi& e, hipStream_t st) {
+  return launch_best<f16x8, P>(g, tri, e, st);
 }
 
 int sum_blocks(const Shape& s) {
@@ -833,6 +800,7 @@ hipError_t launch_sums(int src, SumArgs a, int blocks, int batch, hipStream_t st
   return hipGetLastError();
 }
 
+template <int P>
 hipError_t launch_pack(int src, PackArgs a, const Shape& s, hipStream_t st) {
   a.m = s.m;
   a.n = s.n;
@@ -844,16 +812,16 @@ hipError_t launch_pack(int src, PackArgs a, const Shape& s, hipStream_t st) {
   a.os = s.mr * s.np;
   a.ldt = s.mp;
   a.ts = s.nc * s.mp;
-  a.ldc = s.np;
-  a.cbs = s.m * s.np;
+  a.ldc = s.ldc;
+  a.cbs = s.m * s.ldc;
   const long long blocks = (long long)a.tx * a.ty * s.batch;
   if (blocks >= (1ll << 31)) return hipErrorInvalidValue;
   const dim3 grid((unsigned)blocks);
-  if (src == SRC_F32) hipLaunchKernelGGL(pack_kernel<SRC_F32>, grid, dim3(256), 0, st, a);
-  else if (src == SRC_F16) hipLaunchKernelGGL(pack_kernel<SRC_F16>, grid, dim3(256), 0, st, a);
-  else if (src == SRC_BF16) hipLaunchKernelGGL(pack_kernel<SRC_BF16>, grid, dim3(256), 0, st, a);
-  else if (src == SRC_C64) hipLaunchKernelGGL(pack_kernel<SRC_C64>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(pack_kernel<SRC_PLANAR>, grid, dim3(256), 0, st, a);
+  if (src == SRC_F32) hipLaunchKernelGGL((pack_kernel<SRC_F32, P>), grid, dim3(256), 0, st, a);
+  else if (src == SRC_F16) hipLaunchKernelGGL((pack_kernel<SRC_F16, P>), grid, dim3(256), 0, st, a);
+  else if (src == SRC_BF16) hipLaunchKernelGGL((pack_kernel<SRC_BF16, P>), grid, dim3(256), 0, st, a);
+  else if (src == SRC_C64) hipLaunchKernelGGL((pack_kernel<SRC_C64, P>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((pack_kernel<SRC_PLANAR, P>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -864,16 +832,23 @@ hipError_t clear(void* p, long long bytes, hipStream_t st) {
   return hipGetLastError();
 }
 
-Args base_args(const Shape& s, int M, int N, long long K, long long lda, long long ldb, long long sa, long long sb) {
+Args base_args(const Shape& s, float* split, int M, int N, long long K, long long ld, long long sa, long long sb) {
   Args g{};
   g.M = M;
   g.N = N;
   g.K = (int)K;
-  g.lda = lda;
-  g.ldb = ldb;
+  g.lda = g.ldb = ld;
   g.sa = sa;
   g.sb = sb;
+  g.batch = s.batch;
+  g.part = split;
   return g;
+}
+
+void pair(Args& g, const f16* a, const f16* b) {
+  g.a[g.nseg] = a;
+  g.b[g.nseg] = b;
+  ++g.nseg;
 }
 
 constexpr int SMALL_LDS = 156 * 1024;        // of 160 KB: the reductions take a little
@@ -924,20 +899,18 @@ hipError_t small_by_type(int src, const SmallArgs& a, int bytes, int batch, hipS
   } while (0)
 
 // A, B and the update of one step from the pieces of X; the update's epilogue is the caller's
-template <class Epi>
-hipError_t ns_step(const Shape& s, const Pieces& p, const Scales& c, const double* co, bool full, const Epi& last, hipStream_t st) {
+template <int P, class Epi>
+hipError_t ns_step(const Shape& s, const Pieces& p, const Scales& c, const double* co, float* split, const Epi& last, hipStream_t st) {
   const long long xs = s.mr * s.np, ts = s.nc * s.mp, qs = s.mr * s.mp;
-  Args g = base_args(s, s.mr, s.mr, s.np, s.np, s.np, xs, xs);
-  pairs(g, p.xh, p.xl, p.xh, p.xl);
-  EpiSym ea{p.ah, full ? p.al : nullptr, nullptr, nullptr, s.mp, qs, 1.f / (c.x * c.x), 0.f, c.A};
-  TRY(run<TileS>(g, s.batch, true, ea, st));
-  g = base_args(s, s.mr, s.mr, s.mp, s.mp, s.mp, qs, qs);
-  pairs(g, p.ah, p.al, p.ah, p.al);
-  EpiSym eb{p.bh, full ? p.bl : nullptr, p.ah, p.al, s.mp, qs, (float)co[2] / (c.A * c.A), (float)co[1] / c.A, c.B};
-  TRY(run<TileS>(g, s.batch, true, eb, st));
-  g = base_args(s, s.m, s.nc, s.mp, s.mp, s.mp, qs, ts);
-  pairs(g, p.bh, p.bl, p.th, p.tl);
-  return run<TileS>(g, s.batch, false, last, st);
+  Args g = base_args(s, split, s.mr, s.mr, s.np, s.np, xs, xs);
+  pair(g, p.x, p.x);
+  TRY(run<P>(g, true, EpiSym<P>{p.a, nullptr, s.mp, qs, 1.f / (c.x * c.x), 0.f, c.A}, st));
+  g = base_args(s, split, s.mr, s.mr, s.mp, s.mp, qs, qs);
+  pair(g, p.a, p.a);
+  TRY(run<P>(g, true, EpiSym<P>{p.b, p.a, s.mp, qs, (float)co[2] / (c.A * c.A), (float)co[1] / c.A, c.B}, st));
+  g = base_args(s, split, s.m, s.nc, s.mp, s.mp, qs, ts);
+  pair(g, p.b, p.t);
+  return run<P>(g, false, last, st);
 }
 
 struct Problem {
@@ -947,7 +920,6 @@ struct Problem {
   int src, dtype, steps;
   const double* coef;
   double eps;
-  bool full;
   // optimiser step
   float* buf;
   long long brs, bcs, bbs;
@@ -982,6 +954,9 @@ SmallArgs small_args(const Shape& s, const Problem& q) {
   return a;
 }
 
+bool padded(const Shape& s) { return s.cx == 2 && (s.mp != s.P * s.mr || s.np != s.P * s.nc); }
+
+template <int P>
 hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
   const int nb = sum_blocks(s);
   SumArgs sa{};
@@ -1002,20 +977,14 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
   }
   for (int i = 0; i < q.steps; ++i) {
     const Pieces& p = sv ? sv->p[i] : w.p;
-    if (s.cx == 2 && (s.mp != s.mr || s.np != s.nc) && (sv || i == 0)) {     // the doubled matrix's padding
-      TRY(clear(p.xh, s.mr * s.np * s.batch * 2, st));
-      TRY(clear(p.th, s.nc * s.mp * s.batch * 2, st));
-      if (q.full) {
-        TRY(clear(p.xl, s.mr * s.np * s.batch * 2, st));
-        TRY(clear(p.tl, s.nc * s.mp * s.batch * 2, st));
-      }
+    if (padded(s) && (sv || i == 0)) {               // the doubled matrix's padding
+      TRY(clear(p.x, s.mr * s.np * s.batch * 2, st));
+      TRY(clear(p.t, s.nc * s.mp * s.batch * 2, st));
     }
     PackArgs a{};
     a.scale = sc[i].x;
-    a.hi = p.xh;
-    a.lo = p.xl;
-    a.thi = p.th;
-    a.tlo = p.tl;
+    a.x = p.x;
+    a.t = p.t;
     if (i == 0) {
       a.src = q.g;
       a.part = w.part;
@@ -1029,31 +998,33 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
       a.bbs = q.bbs;
       a.rest = q.rest;
       a.nesterov = q.nesterov;
-      TRY(launch_pack(q.src, a, s, st));
+      TRY(launch_pack<P>(q.src, a, s, st));
     } else {
-      a.src = Mat{w.carry, s.np, 1, s.m * s.np};
-      TRY(launch_pack(SRC_PLANAR, a, s, st));
+      a.src = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
+      TRY(launch_pack<P>(SRC_PLANAR, a, s, st));
     }
     const float alpha = 1.f / (sc[i].B * sc[i].x), beta = (float)q.coef[3 * i];
     if (i + 1 < q.steps) {
-      EpiCarry e{w.carry, s.np, s.m * s.np, alpha, beta, nullptr};
-      TRY(ns_step(s, p, sc[i], q.coef + 3 * i, q.full, e, st));
+      EpiCarry e{w.carry, s.ldc, s.m * s.ldc, alpha, beta, nullptr};
+      TRY(ns_step<P>(s, p, sc[i], q.coef + 3 * i, w.split, e, st));
     } else {
-      EpiOut e{w.carry, s.np, s.m * s.np, alpha, beta, q.out, q.ors, q.ocs, q.obs, q.dtype, s.n, q.buf != nullptr, q.keep, q.rate};
-      TRY(ns_step(s, p, sc[i], q.coef + 3 * i, q.full, e, st));
+      EpiOut e{w.carry, s.ldc, s.m * s.ldc, alpha, beta, q.out, q.ors, q.ocs, q.obs, q.dtype, s.n, q.buf != nullptr, q.keep, q.rate};
+      TRY(ns_step<P>(s, p, sc[i], q.coef + 3 * i, w.split, e, st));
     }
   }
   return hipSuccess;
 }
 
+hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
+  return s.P == 2 ? forward<2>(s, q, sc, w, sv, st) : forward<1>(s, q, sc, w, sv, st);
+}
+
 hipError_t backward(const Shape& s, const Problem& q, const Mat& dy, const Scales* sc, GradWork& w, const Saved& sv, hipStream_t st) {
   const long long xs = s.mr * s.np, ts = s.nc * s.mp, qs = s.mr * s.mp;
   const int nb = sum_blocks(s);
-  if (s.cx == 2 && (s.mp != s.mr || s.np != s.nc)) {
-    TRY(clear(w.dh, xs * s.batch * 2, st));
-    TRY(clear(w.dl, xs * s.batch * 2, st));
-    TRY(clear(w.th, ts * s.batch * 2, st));
-    TRY(clear(w.tl, ts * s.batch * 2, st));
+  if (padded(s)) {
+    TRY(clear(w.d, xs * s.batch * 2, st));
+    TRY(clear(w.t, ts * s.batch * 2, st));
   }
   double bound[TCMI_NS_MAX_STEPS];
   double sig = 1.0;
@@ -1082,7 +1053,7 @@ hipError_t backward(const Shape& s, const Problem& q, const Mat& dy, const Scale
       sa.inner = s.n;
       TRY(launch_sums<0>(q.src, sa, nb, s.batch, st));
     } else {
-      sa.x = Mat{w.carry, s.np, 1, s.m * s.np};
+      sa.x = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
       sa.inner = s.nc;
       TRY(launch_sums<0>(SRC_F32, sa, nb, s.batch, st));
     }
@@ -1091,41 +1062,36 @@ hipError_t backward(const Shape& s, const Problem& q, const Mat& dy, const Scale
     a.npart = nb;
     a.norm_out = w.norm;
     a.scale = sD;
-    a.hi = w.dh;
-    a.lo = w.dl;
-    a.thi = w.th;
-    a.tlo = w.tl;
+    a.x = w.d;
+    a.t = w.t;
     if (first) {
       a.src = dy;
       a.carry = w.carry;
       a.carry_raw = 1;                               // D itself; only its pieces are divided, the epilogue multiplies
     } else {
-      a.src = Mat{w.carry, s.np, 1, s.m * s.np};
+      a.src = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
     }
-    TRY(launch_pack(first ? q.src : SRC_PLANAR, a, s, st));
+    TRY(launch_pack<2>(first ? q.src : SRC_PLANAR, a, s, st));
     // S = D X^T + X D^T
-    Args g = base_args(s, s.mr, s.mr, s.np, s.np, s.np, xs, xs);
-    pairs(g, w.dh, w.dl, p.xh, p.xl);
-    pairs(g, p.xh, p.xl, w.dh, w.dl);
-    EpiSym es{w.sh, w.sl, nullptr, nullptr, s.mp, qs, 1.f / (sD * sc[i].x), 0.f, sS};
-    TRY(run<TileS>(g, s.batch, true, es, st));
+    Args g = base_args(s, w.split, s.mr, s.mr, s.np, s.np, xs, xs);
+    pair(g, w.d, p.x);
+    pair(g, p.x, w.d);
+    TRY(run<2>(g, true, EpiSym<2>{w.s, nullptr, s.mp, qs, 1.f / (sD * sc[i].x), 0.f, sS}, st));
     // Q = b S + c (A S + S A)
-    g = base_args(s, s.mr, s.mr, s.mp, s.mp, s.mp, qs, qs);
-    pairs(g, p.ah, p.al, w.sh, w.sl);
-    pairs(g, w.sh, w.sl, p.ah, p.al);
-    EpiSym eq{w.qh, w.ql, w.sh, w.sl, s.mp, qs, (float)q.coef[3 * i + 2] / (sc[i].A * sS), (float)q.coef[3 * i + 1] / sS, sQ};
-    TRY(run<TileS>(g, s.batch, true, eq, st));
-    // D <- |D| (a D + B D + Q X)
-    g = base_args(s, s.m, s.nc, s.mp, s.mp, s.mp, qs, ts);
-    pairs(g, p.bh, p.bl, w.th, w.tl);
-    pairs(g, w.qh, w.ql, p.th, p.tl);
-    EpiCarry e{w.carry, s.np, s.m * s.np, 1.f / (sc[i].B * sD), (float)q.coef[3 * i], w.norm};
-    TRY(run<TileS>(g, s.batch, false, e, st));
+    g = base_args(s, w.split, s.mr, s.mr, s.mp, s.mp, qs, qs);
+    pair(g, p.a, w.s);
+    pair(g, w.s, p.a);
+    TRY(run<2>(g, true, EpiSym<2>{w.q, w.s, s.mp, qs, (float)q.coef[3 * i + 2] / (sc[i].A * sS), (float)q.coef[3 * i + 1] / sS, sQ}, st));
+    // D <- a D + |D| (B D + Q X) / |D|
+    g = base_args(s, w.split, s.m, s.nc, s.mp, s.mp, qs, ts);
+    pair(g, p.b, w.t);
+    pair(g, w.q, p.t);
+    TRY(run<2>(g, false, EpiCarry{w.carry, s.ldc, s.m * s.ldc, 1.f / (sc[i].B * sD), (float)q.coef[3 * i], w.norm}, st));
   }
   // dG
   SumArgs sa{};
   sa.x = q.g;
-  sa.y = Mat{w.carry, s.np, 1, s.m * s.np};
+  sa.y = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
   sa.brs = s.n;
   sa.outer = s.m;
   sa.inner = s.n;
@@ -1135,7 +1101,7 @@ hipError_t backward(const Shape& s, const Problem& q, const Mat& dy, const Scale
   const unsigned gx = (unsigned)((total + 1023) / 1024 > 4096 ? 4096 : (total + 1023) / 1024);
   const dim3 grid(gx, s.batch);
 #define GO(SRC)                                                                                                            \
-  hipLaunchKernelGGL(grad_out_kernel<SRC>, grid, dim3(256), 0, st, q.g, w.carry, s.np, s.m * s.np, s.m, s.n, w.part, nb,  \
+  hipLaunchKernelGGL(grad_out_kernel<SRC>, grid, dim3(256), 0, st, q.g, w.carry, s.ldc, s.m * s.ldc, s.m, s.n, w.part, nb, \
                      sv.norm, (float)q.eps, q.out, q.ors, q.ocs, q.obs, q.dtype)
   if (q.src == SRC_F32) GO(SRC_F32);
   else if (q.src == SRC_F16) GO(SRC_F16);
@@ -1166,15 +1132,15 @@ extern "C" {
 
 long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full, int dtype, int what) {
   if (!sizes_ok(rows, cols, batch, steps, dtype) || what < 0 || what > 3) return -1;
-  const Shape s = shape_of(rows, cols, batch, dtype);
+  const Shape s = shape_of(rows, cols, batch, dtype, full != 0 || what != TCMI_NS_WORK);
   Arena a{nullptr};
   if (small_bytes(s, what == TCMI_NS_SAVED || what == TCMI_NS_WORK_GRAD || what == TCMI_NS_WORK_SAVING)) {
     if (what == TCMI_NS_SAVED) take_small(a, s, steps);
     else a.take<char>(1);
     return a.used;
   }
-  if (what == TCMI_NS_WORK) take_work(a, s, full != 0, false);
-  else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true, true);
+  if (what == TCMI_NS_WORK) take_work(a, s, false);
+  else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true);
   else if (what == TCMI_NS_SAVED) take_saved(a, s, steps);
   else take_grad(a, s);
   return a.used;
@@ -1185,13 +1151,13 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
                        long long work_bytes, int dtype, void* stream) {
   if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !out || !coef_host || !work || !(eps >= 0) || (saved && !full))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: bad argument");
-  const Shape s = shape_of(rows, cols, batch, dtype);
+  const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
   const int small = small_bytes(s, saved != nullptr);
   Arena aw{(char*)work}, av{(char*)saved};
   Work w{};
   Saved sv{};
   SmallSaved ss{};
-  if (!small) w = take_work(aw, s, full != 0, saved != nullptr);
+  if (!small) w = take_work(aw, s, saved != nullptr);
   if (saved && small) ss = take_small(av, s, steps);
   if (saved && !small) sv = take_saved(av, s, steps);
   if (aw.used > work_bytes || (saved && av.used > saved_bytes) || ((uintptr_t)work & 255) || ((uintptr_t)saved & 255))
@@ -1210,7 +1176,6 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
   q.steps = steps;
   q.coef = coef_host;
   q.eps = eps;
-  q.full = full != 0;
   hipError_t e;
   if (small) {
     SmallArgs a = small_args(s, q);
@@ -1229,7 +1194,7 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
                             long long work_bytes, int dtype, void* stream) {
   if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !dout || !dg || !coef_host || !saved || !work || !(eps >= 0))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: bad argument");
-  const Shape s = shape_of(rows, cols, batch, dtype);
+  const Shape s = shape_of(rows, cols, batch, dtype, true);
   Arena aw{(char*)work}, av{(char*)const_cast<void*>(saved)};
   const int small = small_bytes(s, true);
   GradWork w{};
@@ -1257,7 +1222,6 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
   q.steps = steps;
   q.coef = coef_host;
   q.eps = eps;
-  q.full = true;
   hipError_t e;
   if (small) {
     SmallArgs a = small_args(s, q);
@@ -1278,11 +1242,11 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
   if (!sizes_ok(rows, cols, batch, steps, dtype) || dtype == TCMI_C64 || !param || !grad || !buf || !coef_host || !work || !(eps >= 0) ||
       !(momentum >= 0) || !(momentum < 1))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: bad argument");
-  const Shape s = shape_of(rows, cols, batch, dtype);
+  const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
   const int small = small_bytes(s, false);
   Arena aw{(char*)work};
   Work w{};
-  if (!small) w = take_work(aw, s, full != 0, false);
+  if (!small) w = take_work(aw, s, false);
   if (aw.used > work_bytes || ((uintptr_t)work & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: workspace too small or not 256-byte aligned");
   Scales sc[TCMI_NS_MAX_STEPS];
@@ -1299,7 +1263,6 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
   q.steps = steps;
   q.coef = coef_host;
   q.eps = eps;
-  q.full = full != 0;
   q.buf = buf;
   q.brs = s.flip ? b_cs : b_rs;
   q.bcs = s.flip ? b_rs : b_cs;
