@@ -415,8 +415,6 @@ Rows take_rows(Arena& a, const Shape& s) {
   return r;
 }
 
-using LseTile = Mid;
-
 struct FwdWork {
   Rows rows;
   float2* part;
@@ -426,7 +424,7 @@ struct FwdWork {
 FwdWork take_fwd(Arena& a, const Shape& s) {
   FwdWork w{};
   w.rows = take_rows(a, s);
-  w.part = a.take<float2>((long long)s.T * ((s.V + LseTile::BN - 1) / LseTile::BN));
+  w.part = a.take<float2>((long long)s.T * ((s.V + 63) / 64));          // the narrowest tile of classes is 64 wide
   w.target = a.take<float>(s.T);
   return w;
 }
@@ -479,16 +477,15 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
   } while (0)
 
 template <int P, class Epi>
-hipError_t run(const Args& g, const Epi& e, hipStream_t st) {
-  if constexpr (Epi::WHOLE) return launch<f16x8, P, LseTile>(g, false, e, st);
-  else return launch_best<f16x8, P>(g, false, e, st);
+hipError_t run(Args& g, const Epi& e, hipStream_t st) {
+  return launch_best<f16x8, P>(g, false, e, st);
 }
 
 // the logits' product: 16-bit heads in their own type
 template <int P, class Epi>
-hipError_t run_logits(const Args& g, int dtype, const Epi& e, hipStream_t st) {
+hipError_t run_logits(Args& g, int dtype, const Epi& e, hipStream_t st) {
   if constexpr (P == 1) {
-    if (dtype == TCMI_BF16) return launch<bf16x8, 1, LseTile>(g, false, e, st);
+    if (dtype == TCMI_BF16) return launch_best<bf16x8, 1>(g, false, e, st);
   }
   return run<P>(g, e, st);
 }
@@ -531,9 +528,9 @@ template <int P>
 hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, float* loss, float* total, float* count, int mean,
                    hipStream_t st) {
   TRY(operands(s, in, w.rows, st));
-  const Args g = logit_args(s, in, w.rows, 0, s.V);
+  Args g = logit_args(s, in, w.rows, 0, s.V);
   TRY(run_logits<P>(g, s.dtype, EpiLse{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
-  const int tiles = (s.V + LseTile::BN - 1) / LseTile::BN;
+  const int tiles = g.tn;
   hipLaunchKernelGGL(rowstat_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, w.part, tiles, w.target, in.y, in.ignore, s.T, s.V, lse, loss);
   TRY(hipGetLastError());
   if (total) {
@@ -567,7 +564,8 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
   const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
   for (int v0 = 0; v0 < s.V; v0 += vc) {
     const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P);
-    TRY(run_logits<P>(logit_args(s, in, w.rows, v0, n), s.dtype,
+    Args g = logit_args(s, in, w.rows, v0, n);
+    TRY(run_logits<P>(g, s.dtype,
                       EpiProb<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.p, w.pt, np, s.tp}, st));
     Args d{};
     d.N = s.D;

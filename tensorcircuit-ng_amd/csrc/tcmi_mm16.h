@@ -265,7 +265,7 @@ __device__ __forceinline__ void store_four(f16* row, int col, const f16x4& hi, c
 }
 
 // ---- host side ----
-using Big = Tile<256, 256, 2, 2, 1>;
+using Big = Tile<256, 256, 2, 4, 1>;
 using Mid = Tile<128, 128, 2, 2, 2>;
 using Slim = Tile<128, 64, 4, 1, 2>;
 
@@ -278,7 +278,7 @@ inline long long tile_count(const Args& g, bool tri) {
 }
 
 template <class V, int P, class T, class Epi>
-hipError_t launch(Args g, bool tri, const Epi& e, hipStream_t st) {
+hipError_t launch(Args& g, bool tri, const Epi& e, hipStream_t st) {
   g.tm = (g.M + T::BM - 1) / T::BM;
   g.tn = (g.N + T::BN - 1) / T::BN;
   g.tri = tri ? 1 : 0;
@@ -317,8 +317,11 @@ hipError_t launch(Args g, bool tri, const Epi& e, hipStream_t st) {
 
 // tile by the shape of the result
 template <class V, int P, class Epi>
-hipError_t launch_best(const Args& g, bool tri, const Epi& e, hipStream_t st) {
+hipError_t launch_best(Args& g, bool tri, const Epi& e, hipStream_t st) {
   if (!tri && g.N <= 64) return launch<V, P, Slim>(g, tri, e, st);
+  if constexpr (P == 1) {
+    if (tile_count<Big>(g, tri) >= (tri ? 120 : 192)) return launch<V, P, Big>(g, tri, e, st);
+  }
   return launch<V, P, Mid>(g, tri, e, st);
 }
 

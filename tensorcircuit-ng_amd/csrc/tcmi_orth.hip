@@ -772,7 +772,7 @@ bool scales_of(int steps, const double* coef, Scales* out) {
 }
 
 template <int P, class Epi>
-hipError_t run(const Args& g, bool tri, const Epi& e, hipStream_t st) {
+hipError_t run(Args& g, bool tri, const Epi& e, hipStream_t st) {
   return launch_best<f16x8, P>(g, tri, e, st);
 }
 
