@@ -24,7 +24,7 @@ namespace lce {
 using namespace mm16;
 
 constexpr float PSCALE = 16384.f;            // P lies in [-1, 1]
-constexpr int PARTS = 256;
+constexpr int PARTS = 1024;                   // partial maxima of an operand
 
 template <int DT>
 __device__ __forceinline__ float fetch(const void* p, long long at) {
@@ -41,6 +41,28 @@ __device__ __forceinline__ void put(void* p, int dt, long long at, float v) {
   else ((__bf16*)p)[at] = (__bf16)v;
 }
 
+// four neighbouring elements; vec: the address is aligned for one load
+template <int DT>
+__device__ __forceinline__ f32x4 fetch4(const void* p, long long at, bool vec) {
+  if (vec) {
+    if constexpr (DT == TCMI_F32) return *reinterpret_cast<const f32x4*>((const float*)p + at);
+    else if constexpr (DT == TCMI_F16) return __builtin_convertvector(*reinterpret_cast<const f16x4*>((const f16*)p + at), f32x4);
+    else return __builtin_convertvector(*reinterpret_cast<const bf16x4*>((const __bf16*)p + at), f32x4);
+  }
+  return f32x4{fetch<DT>(p, at), fetch<DT>(p, at + 1), fetch<DT>(p, at + 2), fetch<DT>(p, at + 3)};
+}
+
+// four elements from column c of a row of `cols`, zero behind its end
+template <int DT>
+__device__ __forceinline__ f32x4 fetch_row4(const void* p, long long row, int c, int cols, bool vec) {
+  if (c + 3 < cols) return fetch4<DT>(p, row + c, vec);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    if (c + k < cols) v[k] = fetch<DT>(p, row + c + k);
+  return v;
+}
+
 // power of two that brings `top` into [2^14, 2^15); 1 for zero and for what is not finite
 __device__ __forceinline__ float scale_of(float top) {
   const unsigned e = __float_as_uint(top) >> 23;
@@ -52,29 +74,49 @@ __device__ __forceinline__ float scale_of(float top) {
 // Rows of an operand, k padded.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per row, whose
 // inverse goes to inv[row].  One wave per row, the second read comes from the cache.
 template <int DT>
-__global__ __launch_bounds__(256) void rows_kernel(const void* src, long long rs, int rows, int cols, int colsp, void* out, float* inv) {
+__global__ __launch_bounds__(256) void rows_kernel(const void* src, long long rs, int rows, int cols, int colsp, int vec, void* out,
+                                                   float* inv) {
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= rows) return;
   const long long in = row * rs;
   if constexpr (DT == TCMI_F32) {
-    const float* p = (const float*)src + in;
     float top = 0.f;
-    for (int c = lane; c < cols; c += 64) top = fmaxf(top, fabsf(p[c]));
+    for (int c = 4 * lane; c < cols; c += 256) {
+      const f32x4 v = fetch_row4<DT>(src, in, c, cols, vec);
+      top = fmaxf(fmaxf(fmaxf(top, fabsf(v[0])), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     const float s = scale_of(top);
     f16* q = (f16*)out + (long long)row * 2 * colsp;
-    for (int c = lane; c < colsp; c += 64) {
-      f16 h, l;
-      two_pieces(c < cols ? p[c] * s : 0.f, h, l);
-      q[kpos<2>(c)] = h;
-      q[kpos<2>(c) + 32] = l;
+    for (int c = 4 * lane; c < colsp; c += 256) {
+      const f32x4 v = fetch_row4<DT>(src, in, c, cols, vec);
+      f16x4 hi, lo;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f16 h, l;
+        two_pieces(v[k] * s, h, l);
+        hi[k] = h;
+        lo[k] = l;
+      }
+      store_four<2>(q, c, hi, lo);
     }
     if (lane == 0) inv[row] = 1.f / s;
   } else {
     const unsigned short* p = (const unsigned short*)src + in;
     unsigned short* q = (unsigned short*)out + (long long)row * colsp;
-    for (int c = lane; c < colsp; c += 64) q[c] = c < cols ? p[c] : 0;
+    typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+    for (int c = 4 * lane; c < colsp; c += 256) {
+      u16x4 v = {0, 0, 0, 0};
+      if (vec && c + 3 < cols) {
+        v = *reinterpret_cast<const u16x4*>(p + c);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c + k < cols) v[k] = p[c + k];
+      }
+      *reinterpret_cast<u16x4*>(q + c) = v;
+    }
   }
 }
 
@@ -87,16 +129,23 @@ __global__ __launch_bounds__(256) void factor_kernel(const long long* y, long lo
   r[t] = y[t] == ignore ? 0.f : g;
 }
 
-// partial maxima of |x| (times a row factor; rows whose factor is zero do not count)
+// partial maxima of |x| (times a row factor; rows whose factor is zero do not count); one wave per row, bound by its reads
 template <int DT>
-__global__ __launch_bounds__(256) void top_kernel(const void* src, long long rs, int rows, int cols, const float* r, float* part) {
+__global__ __launch_bounds__(256) void top_kernel(const void* src, long long rs, int rows, int cols, int vec, const float* r, float* part) {
   __shared__ float red[4];
   float top = 0.f;
   const int lane = threadIdx.x & 63;
   for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4) {
     const float f = r ? fabsf(r[row]) : 1.f;
     if (f == 0.f) continue;
-    for (int c = lane; c < cols; c += 64) top = fmaxf(top, fabsf(fetch<DT>(src, row * rs + c)) * f);
+    const long long at = row * rs;
+    float t = 0.f;
+#pragma unroll 4
+    for (int c = 4 * lane; c < cols; c += 256) {
+      const f32x4 v = fetch_row4<DT>(src, at, c, cols, vec);
+      t = fmaxf(fmaxf(fmaxf(t, fabsf(v[0])), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    }
+    top = fmaxf(top, t * f);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -106,43 +155,48 @@ __global__ __launch_bounds__(256) void top_kernel(const void* src, long long rs,
 }
 
 // out[c][row] = src[row][c] * r[row] * scale as f16 pieces (two for f32), rows padded with zeros.  A zero factor gives zero
-// whatever the row holds.
+// whatever the row holds.  64 x 64 tiles through LDS, four elements a thread on both sides.
 template <int DT>
-__global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs, int rows, int cols, const float* r,
+__global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs, int rows, int cols, int vec, const float* r,
                                                    const float* part, int nparts, f16* out, int rowsp, float* inv) {
   constexpr int P = DT == TCMI_F32 ? 2 : 1;
   __shared__ float tile[64][65];
   __shared__ float red[4];
-  const int tid = threadIdx.x, u = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x;
   float top = 0.f;
   for (int k = tid; k < nparts; k += 256) top = fmaxf(top, part[k]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (u == 0) red[w] = top;
+  if ((tid & 63) == 0) red[tid >> 6] = top;
   __syncthreads();
   const float s = scale_of(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, u = (tid & 15) * 4, w = tid >> 4;
   if (r0 == 0 && c0 == 0 && tid == 0) *inv = 1.f / s;
-#pragma unroll 4
-  for (int k = w; k < 64; k += 4) {
-    const int row = r0 + k, c = c0 + u;
-    float x = 0.f;
-    if (row < rows && c < cols) {
+#pragma unroll
+  for (int k = w; k < 64; k += 16) {
+    const int row = r0 + k;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (row < rows) {
       const float f = r ? r[row] : 1.f;
-      if (f != 0.f) x = fetch<DT>(src, row * rs + c) * f * s;
+      if (f != 0.f) v = fetch_row4<DT>(src, row * rs, c0 + u, cols, vec) * f * s;
     }
-    tile[k][u] = x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) tile[k][u + e] = v[e];
   }
   __syncthreads();
-#pragma unroll 4
-  for (int k = w; k < 64; k += 4) {
+#pragma unroll
+  for (int k = w; k < 64; k += 16) {
     const int c = c0 + k, row = r0 + u;
     if (c < cols && row < rowsp) {
-      f16 h, l;
-      two_pieces(tile[u][k], h, l);
-      f16* q = out + (long long)c * P * rowsp + kpos<P>(row);
-      q[0] = h;
-      if (P == 2) q[32] = l;
+      f16x4 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f16 h, l;
+        two_pieces(tile[u + e][k], h, l);
+        hi[e] = h;
+        lo[e] = l;
+      }
+      store_four<P>(out + (long long)c * P * rowsp, row, hi, lo);
     }
   }
 }
@@ -363,17 +417,20 @@ struct EpiGrad {
   }
 };
 
-// db_v = sum_t P[t][v] r_t from the transposed pieces: one wave per class
+// db_v = sum_t P[t][v] r_t from the transposed pieces (zero behind the last row): one wave per class
 template <int P>
 __global__ __launch_bounds__(256) void bias_kernel(const f16* pt, int tp, const float* r, int T, int vc, void* out, int dtype, int v0) {
   const int v = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (v >= vc) return;
   const f16* q = pt + (long long)v * P * tp;
   float s = 0.f;
-  for (int t = lane; t < T; t += 64) {
-    float p = (float)q[kpos<P>(t)];
-    if (P == 2) p += (float)q[kpos<P>(t) + 32];
-    s = fmaf(p, r[t], s);
+  for (int t = 4 * lane; t < tp; t += 256) {
+    const f16x4 hi = *reinterpret_cast<const f16x4*>(q + kpos<P>(t));
+    f32x4 p = __builtin_convertvector(hi, f32x4);
+    if (P == 2) p += __builtin_convertvector(*reinterpret_cast<const f16x4*>(q + kpos<P>(t) + 32), f32x4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (t + e < T) s = fmaf(p[e], r[t + e], s);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
@@ -490,6 +547,9 @@ hipError_t run_logits(Args& g, int dtype, const Epi& e, hipStream_t st) {
   return run<P>(g, e, st);
 }
 
+// whether rows can be read four elements at a time
+int vec4(const void* p, long long rs, int dtype) { return rs % 4 == 0 && ((uintptr_t)p & (dtype == TCMI_F32 ? 15 : 7)) == 0; }
+
 struct In {
   const void *h, *w, *bias;
   long long hrs, wrs;
@@ -499,11 +559,13 @@ struct In {
 
 hipError_t operands(const Shape& s, const In& in, const Rows& r, hipStream_t st) {
   if (!s.h_direct) {
-    BY_TYPE(s.dtype, rows_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, s.dp, r.h, r.hs);
+    BY_TYPE(s.dtype, rows_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, s.dp,
+            vec4(in.h, in.hrs, s.dtype), r.h, r.hs);
     TRY(hipGetLastError());
   }
   if (!s.w_direct) {
-    BY_TYPE(s.dtype, rows_kernel, dim3((s.V + 3) / 4), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, s.dp, r.w, r.ws);
+    BY_TYPE(s.dtype, rows_kernel, dim3((s.V + 3) / 4), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, s.dp,
+            vec4(in.w, in.wrs, s.dtype), r.w, r.ws);
     TRY(hipGetLastError());
   }
   return hipSuccess;
@@ -550,15 +612,15 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
   const float* none = nullptr;
   if (dw) {
     const int nb = blocks(s.T);
-    BY_TYPE(s.dtype, top_kernel, dim3(nb), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, w.r, w.parth);
+    BY_TYPE(s.dtype, top_kernel, dim3(nb), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, vec4(in.h, in.hrs, s.dtype), w.r, w.parth);
     TRY(hipGetLastError());
-    BY_TYPE(s.dtype, turn_kernel, dim3((s.tp + 63) / 64, (s.D + 63) / 64), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, w.r, w.parth, nb,
-            w.ht, s.tp, w.invh);
+    BY_TYPE(s.dtype, turn_kernel, dim3((s.tp + 63) / 64, (s.D + 63) / 64), dim3(256), 0, st, in.h, in.hrs, s.T, s.D,
+            vec4(in.h, in.hrs, s.dtype), w.r, w.parth, nb, w.ht, s.tp, w.invh);
     TRY(hipGetLastError());
   }
   const int nbw = blocks(s.V);
   if (dh) {
-    BY_TYPE(s.dtype, top_kernel, dim3(nbw), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, none, w.partw);
+    BY_TYPE(s.dtype, top_kernel, dim3(nbw), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, vec4(in.w, in.wrs, s.dtype), none, w.partw);
     TRY(hipGetLastError());
   }
   const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
@@ -574,7 +636,7 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
     d.part = w.split;
     if (dh) {
       BY_TYPE(s.dtype, turn_kernel, dim3((np + 63) / 64, (s.D + 63) / 64), dim3(256), 0, st, (const char*)in.w + v0 * in.wrs * size, in.wrs,
-              n, s.D, none, w.partw, nbw, w.wt, np, w.invw);
+              n, s.D, vec4(in.w, in.wrs, s.dtype), none, w.partw, nbw, w.wt, np, w.invw);
       TRY(hipGetLastError());
       d.M = s.T;
       d.K = P * np;

@@ -42,6 +42,14 @@ __device__ __forceinline__ float2 fetch(const void* p, long long at) {
   return make_float2(0.f, 0.f);
 }
 
+// four neighbours, the address aligned for one load
+template <int SRC>
+__device__ __forceinline__ f32x4 fetch4(const void* p, long long at) {
+  if constexpr (SRC == SRC_F16) return __builtin_convertvector(*reinterpret_cast<const f16x4*>((const f16*)p + at), f32x4);
+  else if constexpr (SRC == SRC_BF16) return __builtin_convertvector(*reinterpret_cast<const bf16x4*>((const __bf16*)p + at), f32x4);
+  else return *reinterpret_cast<const f32x4*>((const float*)p + at);
+}
+
 __device__ __forceinline__ void put(void* p, int dtype, long long at, float v) {
   if (dtype == TCMI_F32) ((float*)p)[at] = v;
   else if (dtype == TCMI_F16) ((f16*)p)[at] = (f16)v;
@@ -63,7 +71,7 @@ __device__ __forceinline__ double block_sum(double v, double* red) {        // 2
 // result does not depend on the order of the workgroups.  lanes: threads along the contiguous axis.
 struct SumArgs {
   Mat x, y;
-  int outer, inner, lanes;
+  int outer, inner, lanes, vec;            // vec: four neighbours can be read (and the momentum updated) at once
   double* part;               // [batch][gridDim.x]
   float* buf;                 // MODE 2: momentum, strides below
   long long brs, bcs, bbs;
@@ -77,28 +85,58 @@ __device__ __forceinline__ float direction(float g, float v, float rest, int nes
 }
 
 template <int SRC, int MODE>
+__device__ __forceinline__ double sums_one(const SumArgs& a, long long o, int i, long long bx, long long by) {
+  const float2 v = fetch<SRC>(a.x.p, bx + o * a.x.rs + i * a.x.cs);
+  if constexpr (MODE == 1) {              // y: planar f32 D, imaginary parts brs further on
+    const float* d = (const float*)a.y.p + by + o * a.y.rs + i * a.y.cs;
+    double s = (double)v.x * d[0];
+    if constexpr (SRC == SRC_C64) s += (double)v.y * d[a.brs];
+    return s;
+  } else if constexpr (MODE == 2) {
+    float* m = a.buf + by + o * a.brs + i * a.bcs;
+    const float nv = fmaf(a.rest, v.x - m[0], m[0]);
+    m[0] = nv;
+    const float u = direction(v.x, nv, a.rest, a.nesterov);
+    return (double)u * u;
+  } else {
+    return (double)v.x * v.x + (double)v.y * v.y;
+  }
+}
+
+template <int SRC, int MODE>
 __global__ __launch_bounds__(256) void sums_kernel(SumArgs a) {
   __shared__ double red[4];
   const int per = 256 / a.lanes, r0 = threadIdx.x / a.lanes, c0 = threadIdx.x % a.lanes;
-  const long long bx = (long long)blockIdx.y * a.x.bs;
+  const long long bx = (long long)blockIdx.y * a.x.bs, by = (long long)blockIdx.y * (MODE == 2 ? a.bbs : a.y.bs);
   double s = 0.0;
-  for (int o = blockIdx.x * per + r0; o < a.outer; o += gridDim.x * per)
-    for (int i = c0; i < a.inner; i += a.lanes) {
-      const float2 v = fetch<SRC>(a.x.p, bx + o * a.x.rs + i * a.x.cs);
-      if constexpr (MODE == 1) {          // x: caller's G (complex: planar D holds re at i, im further on, see y strides)
-        const float* d = (const float*)a.y.p + (long long)blockIdx.y * a.y.bs + o * a.y.rs + i * a.y.cs;
-        s += (double)v.x * d[0];
-        if constexpr (SRC == SRC_C64) s += (double)v.y * d[a.brs];
-      } else if constexpr (MODE == 2) {
-        float* m = a.buf + (long long)blockIdx.y * a.bbs + o * a.brs + i * a.bcs;
-        const float nv = fmaf(a.rest, v.x - m[0], m[0]);
-        m[0] = nv;
-        const float u = direction(v.x, nv, a.rest, a.nesterov);
-        s += (double)u * u;
-      } else {
-        s += (double)v.x * v.x + (double)v.y * v.y;
+  for (long long o = blockIdx.x * per + r0; o < a.outer; o += gridDim.x * per) {
+    int i = c0;
+    if constexpr (SRC != SRC_C64 && MODE != 1) {
+      if (a.vec) {                        // four neighbours a thread; f32 sums of four squares would overflow, so f64 at once
+        i = 4 * c0;
+#pragma unroll 2
+        for (; i + 3 < a.inner; i += 4 * a.lanes) {
+          const f32x4 v = fetch4<SRC>(a.x.p, bx + o * a.x.rs + i);
+          f32x4 u = v;
+          if constexpr (MODE == 2) {
+            f32x4* m = reinterpret_cast<f32x4*>(a.buf + by + o * a.brs + i);
+            f32x4 w = *m;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[k] = fmaf(a.rest, v[k] - w[k], w[k]);
+              u[k] = direction(v[k], w[k], a.rest, a.nesterov);
+            }
+            *m = w;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s += (double)u[k] * u[k];
+        }
+        for (const int e = min(i + 4, a.inner); i < e; ++i) s += sums_one<SRC, MODE>(a, o, i, bx, by);
+        continue;
       }
     }
+    for (; i < a.inner; i += a.lanes) s += sums_one<SRC, MODE>(a, o, i, bx, by);
+  }
   s = block_sum(s, red);
   if (threadIdx.x == 0) a.part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
@@ -108,7 +146,7 @@ __global__ __launch_bounds__(256) void sums_kernel(SumArgs a) {
 // part: the tile is divided by (sqrt(sum of part) + eps); every workgroup adds the partial sums itself.
 struct PackArgs {
   Mat src;
-  int m, n, tx, ty, fast_rows;             // logical size, tiles, 1: the source is contiguous along rows
+  int m, n, tx, ty, fast_rows, vec;        // logical size, tiles, 1: the source is contiguous along its columns; vec: four at once
   const double* part;
   int npart;
   float eps, scale;                        // pieces = value * scale
@@ -141,59 +179,114 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const double d = nrm + (double)a.eps;
     inv = d == 0.0 ? 0.f : (float)(1.0 / d);
   }
+  // 16 threads along an axis, four elements each, 16 lines at a time
   const long long base = (long long)bz * a.src.bs;
-  const int u = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int k = w; k < 64; k += 4) {
-    const int il = a.fast_rows ? u : k, jl = a.fast_rows ? k : u, i = i0 + il, j = j0 + jl;
-    float2 v = make_float2(0.f, 0.f);
-    if (i < a.m && j < a.n) {
-      const long long at = base + i * a.src.rs + j * a.src.cs;
-      v = fetch<SRC>(a.src.p, at);
-      if (SRC == SRC_PLANAR && a.embed) v.y = ((const float*)a.src.p)[at + a.n];
-      if (a.buf) v.x = direction(v.x, a.buf[(long long)bz * a.bbs + i * a.brs + j * a.bcs], a.rest, a.nesterov);
+  const int u = (threadIdx.x & 15) * 4, w = threadIdx.x >> 4;
+  const int flen = a.fast_rows ? a.m : a.n;
+#pragma unroll
+  for (int k = w; k < 64; k += 16) {
+    const int line = (a.fast_rows ? j0 : i0) + k, f0 = (a.fast_rows ? i0 : j0) + u;
+    const long long ls = a.fast_rows ? a.src.cs : a.src.rs, fs = a.fast_rows ? a.src.rs : a.src.cs;
+    f32x4 re = {0.f, 0.f, 0.f, 0.f}, im = {0.f, 0.f, 0.f, 0.f};
+    if (line < (a.fast_rows ? a.n : a.m)) {
+      const long long at = base + line * ls + f0 * fs;
+      if (SRC != SRC_C64 && a.vec && f0 + 3 < flen) {
+        re = fetch4<SRC>(a.src.p, at);
+        if (SRC == SRC_PLANAR && a.embed) {
+          const float* q = (const float*)a.src.p + at + a.n;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) im[e] = q[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (f0 + e < flen) {
+            const float2 v = fetch<SRC>(a.src.p, at + e * fs);
+            re[e] = v.x;
+            im[e] = SRC == SRC_PLANAR && a.embed ? ((const float*)a.src.p)[at + e * fs + a.n] : v.y;
+          }
+      }
+      if (a.buf) {
+        const long long bt = (long long)bz * a.bbs + (a.fast_rows ? line * a.bcs + f0 * a.brs : line * a.brs + f0 * a.bcs);
+        const long long bf = a.fast_rows ? a.brs : a.bcs;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (f0 + e < flen) re[e] = direction(re[e], a.buf[bt + e * bf], a.rest, a.nesterov);
+      }
     }
-    tr[il][jl] = v.x;
-    if (MAYBE_COMPLEX) tim[MAYBE_COMPLEX ? il : 0][jl] = v.y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int il = a.fast_rows ? u + e : k, jl = a.fast_rows ? k : u + e;
+      tr[il][jl] = re[e];
+      if (MAYBE_COMPLEX) tim[MAYBE_COMPLEX ? il : 0][jl] = im[e];
+    }
   }
   __syncthreads();
-  const float cinv = a.carry_raw ? 1.f : inv;
+  const float cinv = a.carry_raw ? 1.f : inv, xs = inv * a.scale;
   const bool twice = MAYBE_COMPLEX && a.embed;
   const int mrows = twice ? a.m : (int)kpad(a.m, P), ncols = twice ? a.n : (int)kpad(a.n, P);
   f16 *px = a.x + (long long)bz * a.os, *pt = a.t + (long long)bz * a.ts;
-  auto store = [&](f16* row, int k, float x) {
-    f16 h, l;
-    two_pieces(x * inv * a.scale, h, l);
-    row[kpos<P>(k)] = h;
-    if (P == 2) row[kpos<P>(k) + 32] = l;
+  // four values at k .. k + 3 of a row, as far as `len` reaches (`len` - k in 1 .. 4)
+  auto store = [&](f16* row, int k, int len, f32x4 v) {
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f16 h, l;
+      two_pieces(v[e] * xs, h, l);
+      hi[e] = h;
+      lo[e] = l;
+    }
+    if (k + 3 < len && (k & 3) == 0) {
+      store_four<P>(row, k, hi, lo);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k + e < len) {
+          row[kpos<P>(k + e)] = hi[e];
+          if (P == 2) row[kpos<P>(k + e) + 32] = lo[e];
+        }
+    }
   };
-#pragma unroll 4
-  for (int k = w; k < 64; k += 4) {
-    {                                      // rows of X: lanes along j
+  auto carry = [&](float* q, int left, f32x4 v) {
+    if (left > 3 && ((uintptr_t)q & 15) == 0) {
+      *reinterpret_cast<f32x4*>(q) = v * cinv;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) q[e] = v[e] * cinv;
+    }
+  };
+#pragma unroll
+  for (int k = w; k < 64; k += 16) {
+    {                                      // rows of X
       const int i = i0 + k, j = j0 + u;
       if (i < a.m && j < ncols) {
-        const float re = tr[k][u];
-        store(px + i * a.ld, j, re);
-        if (a.carry && j < a.n) a.carry[(long long)bz * a.cbs + i * a.ldc + j] = re * cinv;
+        const f32x4 re = {tr[k][u], tr[k][u + 1], tr[k][u + 2], tr[k][u + 3]};
+        store(px + i * a.ld, j, ncols, re);
+        float* c = a.carry ? a.carry + (long long)bz * a.cbs + i * a.ldc + j : nullptr;
+        if (c && j < a.n) carry(c, a.n - j, re);
         if (twice) {
-          const float im = tim[MAYBE_COMPLEX ? k : 0][u];
-          store(px + i * a.ld, j + a.n, im);
-          store(px + (i + a.m) * a.ld, j, -im);
-          store(px + (i + a.m) * a.ld, j + a.n, re);
-          if (a.carry) a.carry[(long long)bz * a.cbs + i * a.ldc + j + a.n] = im * cinv;
+          const int q = MAYBE_COMPLEX ? k : 0;
+          const f32x4 im = {tim[q][u], tim[q][u + 1], tim[q][u + 2], tim[q][u + 3]};
+          store(px + i * a.ld, j + a.n, 2 * a.n, im);
+          store(px + (i + a.m) * a.ld, j, a.n, -im);
+          store(px + (i + a.m) * a.ld, j + a.n, 2 * a.n, re);
+          if (c) carry(c + a.n, a.n - j, im);
         }
       }
     }
-    {                                      // rows of X^T: lanes along i
+    {                                      // rows of X^T
       const int i = i0 + u, j = j0 + k;
       if (j < a.n && i < mrows) {
-        const float re = tr[u][k];
-        store(pt + j * a.ldt, i, re);
+        const f32x4 re = {tr[u][k], tr[u + 1][k], tr[u + 2][k], tr[u + 3][k]};
+        store(pt + j * a.ldt, i, mrows, re);
         if (twice) {
-          const float im = tim[MAYBE_COMPLEX ? u : 0][k];
-          store(pt + (j + a.n) * a.ldt, i, im);
-          store(pt + j * a.ldt, i + a.m, -im);
-          store(pt + (j + a.n) * a.ldt, i + a.m, re);
+          const f32x4 im = MAYBE_COMPLEX ? f32x4{tim[MAYBE_COMPLEX ? u : 0][k], tim[MAYBE_COMPLEX ? u + 1 : 0][k],
+                                                 tim[MAYBE_COMPLEX ? u + 2 : 0][k], tim[MAYBE_COMPLEX ? u + 3 : 0][k]}
+                                         : re;
+          store(pt + (j + a.n) * a.ldt, i, a.m, im);
+          store(pt + j * a.ldt, i + a.m, 2 * a.m, -im);
+          store(pt + (j + a.n) * a.ldt, i + a.m, 2 * a.m, re);
         }
       }
     }
@@ -669,7 +762,7 @@ Pieces take_pieces(Arena& w, const Shape& s) {
   return p;
 }
 
-constexpr int MAX_PART = 256;
+constexpr int MAX_PART = 1024;
 
 struct Work {
   double* part;
@@ -777,9 +870,14 @@ hipError_t run(Args& g, bool tri, const Epi& e, hipStream_t st) {
 }
 
 int sum_blocks(const Shape& s) {
-  long long n = (long long)s.m * s.n / 2048;
-  const int cap = s.batch >= 64 ? 16 : s.batch >= 8 ? 64 : MAX_PART;
+  long long n = (long long)s.m * s.n / 4096;
+  const int cap = s.batch >= 64 ? 16 : s.batch >= 8 ? 64 : s.batch > 1 ? 256 : MAX_PART;
   return (int)(n < 1 ? 1 : n > cap ? cap : n);
+}
+
+// whether four neighbours along the contiguous axis (stride cs) form one aligned load
+bool aligned4(const void* p, long long rs, long long cs, long long bs, int size) {
+  return cs == 1 && rs % 4 == 0 && bs % 4 == 0 && ((uintptr_t)p & (4 * size - 1)) == 0;
 }
 
 template <int MODE>
@@ -791,7 +889,10 @@ hipError_t launch_sums(int src, SumArgs a, int blocks, int batch, hipStream_t st
     if (MODE == 2) { t = a.brs; a.brs = a.bcs; a.bcs = t; }
     const int o = a.outer; a.outer = a.inner; a.inner = o;
   }
-  a.lanes = a.inner > 128 ? 256 : a.inner > 64 ? 128 : a.inner > 32 ? 64 : 32;
+  a.vec = src != SRC_C64 && aligned4(a.x.p, a.x.rs, a.x.cs, a.x.bs, src == SRC_F32 ? 4 : 2) &&
+          (MODE != 2 || aligned4(a.buf, a.brs, a.bcs, a.bbs, 4));
+  const int wide = a.vec ? (a.inner + 3) / 4 : a.inner;
+  a.lanes = wide > 128 ? 256 : wide > 64 ? 128 : wide > 32 ? 64 : wide > 16 ? 32 : 16;
   const dim3 grid(blocks, batch);
   if (src == SRC_F32) hipLaunchKernelGGL((sums_kernel<SRC_F32, MODE>), grid, dim3(256), 0, st, a);
   else if (src == SRC_F16) hipLaunchKernelGGL((sums_kernel<SRC_F16, MODE>), grid, dim3(256), 0, st, a);
@@ -808,6 +909,8 @@ hipError_t launch_pack(int src, PackArgs a, const Shape& s, hipStream_t st) {
   a.ty = (s.m + 63) / 64;
   a.embed = s.cx == 2;
   a.fast_rows = a.src.rs < a.src.cs;
+  a.vec = src != SRC_C64 && aligned4(a.src.p, a.fast_rows ? a.src.cs : a.src.rs, a.fast_rows ? a.src.rs : a.src.cs, a.src.bs,
+                                     src == SRC_F32 || src == SRC_PLANAR ? 4 : 2);
   a.ld = s.np;
   a.os = s.mr * s.np;
   a.ldt = s.mp;
