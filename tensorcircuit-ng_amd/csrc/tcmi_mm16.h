@@ -14,6 +14,7 @@
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 namespace tcmi {
 namespace mm16 {
@@ -77,16 +78,26 @@ __device__ __forceinline__ unsigned unit_of() {
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (id >> 3);
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int PER_CU_>
+template <int BM_, int BN_, int WM_, int WN_, int PER_CU_, int STAGES_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, PER_CU = PER_CU_;
   static constexpr int WAVES = WM * WN, THREADS = WAVES * 64;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
   static constexpr int STAGE = (BM + BN) * 128;            // bytes of one k step of both operands
-  static constexpr int LDS = 2 * STAGE;
+  static constexpr int STAGES = STAGES_, LDS = STAGES * STAGE;
+  static constexpr int LOADS = (BM + BN) / 8 / WAVES;      // loads of a wave per step
+  static_assert((STAGES - 1) * LOADS < 64, "vmcnt holds 6 bits");
+  static constexpr int YOUNG = (STAGES - 2) * LOADS;       // loads that may still be under way in the middle of a step
 };
 
 using LdsPtr = __attribute__((address_space(3))) void*;
+
+// Waits until all but this wave's YOUNG youngest loads have landed in LDS and none of its LDS reads is under way, then for the
+// other waves; no memory operation moves across (the compiler's own barrier would wait for every load).
+template <int YOUNG>
+__device__ __forceinline__ void wait_and_meet() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(YOUNG) : "memory");
+}
 
 #ifdef __HIP_DEVICE_COMPILE__          // the host pass does not know the buffer resource type
 // The k steps [s0, s1) of one product tile.  `acc[i][j]` holds C[row][col .. col + 3] with
@@ -96,7 +107,7 @@ using LdsPtr = __attribute__((address_space(3))) void*;
 // LDS: a row's k step is eight 16-byte chunks; chunk c of row r lies at position c ^ (r & 7), which spreads the 16 rows of a
 // fragment read over all banks.  Global -> LDS goes without registers (buffer_load ... lds) into two stages; fragments go
 // LDS -> registers half a step ahead of the matrix instructions that use them.  One barrier a step: when every wave has its
-// stage in registers and its loads of the next stage have landed, the stage is free for the loads of the step after.
+// stage in registers and its loads of the next stage have landed, the stage is free for the loads STAGES steps on.
 template <class V, int P, class T>
 __device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, int s0, int s1, char* lds, f32x4 (&acc)[T::MI][T::NI]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -131,10 +142,9 @@ __device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, i
 #pragma unroll
     for (int j = 0; j < LB; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (LdsPtr)(base + T::BM * 128 + (j * T::WAVES + wave) * 1024), 16, vb[j], so, 0, 0);
-    if (++lk == ksteps) {
-      lk = 0;
-      ++ls;
-    }
+    const int wrap = lk + 1 == ksteps;
+    lk = wrap ? 0 : lk + 1;
+    ls += wrap;
   };
 
   const int r = lane & 15;
@@ -156,33 +166,52 @@ __device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, i
       for (int j = 0; j < T::NI; ++j) acc[i][j] = mfma(fb[j], fa[i], acc[i][j]);
   };
   V a0[T::MI], a1[T::MI], b0[T::NI], b1[T::NI], b2[T::NI];
-  // one k step: b holds the first half's B fragments, bn receives the next step's
-  auto step = [&](int s, V (&b)[T::NI], V (&bn)[T::NI]) {
-    const int stage = (s - s0) & 1;
+  // One k step: b holds the first half's B fragments, bn receives the next step's.  MORE: a next step exists, FILL: so does the
+  // one whose loads take this stage (constants: no branches in the loop).
+  int stage = 0;
+  auto step = [&](auto more, auto fill, V (&b)[T::NI], V (&bn)[T::NI]) {
+    const int next = stage + 1 == T::STAGES ? 0 : stage + 1;
     read_b(b1, stage, 1);
     read_a(a1, stage, 1);
     multiply(a0, b);
     if constexpr (P == 2) multiply(a0, b1);
-    if (s + 1 < s1) {
-      __builtin_amdgcn_s_waitcnt(0);               // this stage is in registers, the next one has landed
-      __syncthreads();
-      if (s + 2 < s1) load(stage);
-      read_b(bn, stage ^ 1, 0);
-      read_a(a0, stage ^ 1, 0);
+    if constexpr (more) {
+      // this stage is in registers, the next one has landed (near the end, where fewer loads are under way: all have)
+      wait_and_meet<fill ? T::YOUNG : 0>();
+      if constexpr (fill) load(stage);
+      read_b(bn, next, 0);
+      read_a(a0, next, 0);
     }
     if constexpr (P == 1) multiply(a1, b1);
     else multiply(a1, b);
+    stage = next;
   };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
 
-  load(0);
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (s0 + 1 < s1) load(1);
+  for (int k = 0; k < T::STAGES && s0 + k < s1; ++k) load(k);
+  if (s0 + T::STAGES - 1 < s1) wait_and_meet<T::YOUNG + T::LOADS>();      // the first stage has landed
+  else wait_and_meet<0>();
   read_b(b0, 0, 0);
   read_a(a0, 0, 0);
-  for (int s = s0; s < s1; s += 2) {
-    step(s, b0, P == 1 ? b0 : b2);
-    if (s + 1 < s1) step(s + 1, P == 1 ? b0 : b2, b0);
+  int s = s0;
+  if constexpr (P == 1) {
+    for (; s + T::STAGES < s1; ++s) step(yes, yes, b0, b0);
+    for (; s + 1 < s1; ++s) step(yes, no, b0, b0);
+    step(no, no, b0, b0);
+  } else {
+    for (; s + T::STAGES + 1 < s1; s += 2) {
+      step(yes, yes, b0, b2);
+      step(yes, yes, b2, b0);
+    }
+    // at most STAGES + 1 steps left; the fragments change places with each
+    for (; s + 1 < s1; ++s) {
+      if (s + T::STAGES < s1) step(yes, yes, b0, b2);
+      else step(yes, no, b0, b2);
+#pragma unroll
+      for (int i = 0; i < T::NI; ++i) b0[i] = b2[i];
+    }
+    step(no, no, b0, b2);
   }
 }
 #endif
@@ -266,11 +295,32 @@ __device__ __forceinline__ void store_four(f16* row, int col, const f16x4& hi, c
 }
 
 // ---- host side ----
-using Big = Tile<256, 256, 2, 4, 1>;
-using Mid = Tile<128, 128, 2, 2, 2>;
-using Slim = Tile<128, 64, 4, 1, 2>;
+using Big = Tile<256, 256, 2, 4, 1, 2>;
+using Wide = Tile<192, 192, 2, 4, 1, 2>;
+using Mid = Tile<128, 128, 2, 2, 2, 2>;
+using Slim = Tile<128, 64, 4, 1, 2, 2>;
+using Tiny = Tile<64, 64, 2, 2, 4, 2>;
 
 constexpr long long PART_BYTES = 512ll * 128 * 128 * 4;       // workspace of a split product
+
+// Which tile, and into how many parts along k.  Time of one k step of one round in microseconds, by the workgroups that share a
+// CU, measured on products of 1000 .. 8192 rows (one / two pieces):
+//   256 x 256   1.8                    one workgroup a CU; 1120 - 1180 TFLOP/s when the card is full
+//   192 x 192   1.19                   one; 253 tiles of a 4096 x 4096 symmetric result: 76 us (256: 107, 128: 100)
+//   128 x 128   0.72 / 0.73, two 1.02 / 1.2          1080 TFLOP/s; two pieces 446 (1340 on the pipe)
+//   128 x 64    0.60, two 0.69 / 0.71                results up to 64 columns
+//   64 x 64     0.38 / 0.48, two 0.56 / 0.58, three 0.68 / 0.70, four 0.79 / 0.80
+// A product whose tiles do not fill the card takes smaller tiles (1000 x 1537 x 1000, two pieces: 18 us, 128 x 128: 27) or
+// is split along k; its parts cost a second launch (4 us) and one write and one read of themselves (4 TB/s).
+template <class T, int P>
+inline double step_us(int per_cu) {
+  const double one = P == 1;
+  if (T::BM == 256) return 1.8;
+  if (T::BM == 192) return 1.19;
+  if (T::BM == 128 && T::BN == 128) return per_cu == 1 ? (one ? 0.72 : 0.73) : (one ? 1.02 : 1.2);
+  if (T::BM == 128) return per_cu == 1 ? 0.60 : (one ? 0.69 : 0.71);
+  return per_cu == 1 ? (one ? 0.38 : 0.48) : per_cu == 2 ? (one ? 0.56 : 0.58) : per_cu == 3 ? (one ? 0.68 : 0.70) : (one ? 0.79 : 0.80);
+}
 
 template <class T>
 inline long long tile_count(const Args& g, bool tri) {
@@ -278,26 +328,33 @@ inline long long tile_count(const Args& g, bool tri) {
   return (tri ? tm * (tm + 1) / 2 : tm * tn) * g.batch;
 }
 
+// the cheapest split of a product over tiles T, and its time
+template <class T, int P>
+inline double cost_of(const Args& g, bool tri, bool may_split, int* split) {
+  const long long units = tile_count<T>(g, tri), steps = (long long)(g.K / 64) * g.nseg;
+  double best = 1e30;
+  for (const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (s > 1 && (!may_split || steps < 4 * s || units * s * T::BM * T::BN * 4 > PART_BYTES)) break;
+    const long long u = units * s, round = 256 * T::PER_CU, rest = u % round, k = (steps + s - 1) / s;
+    double t = k * ((u / round) * step_us<T, P>(T::PER_CU) + (rest ? step_us<T, P>((int)((rest + 255) / 256)) : 0.0));
+    if (s > 1) t += 4.0 + u * T::BM * T::BN * 8.0 / 4e6;
+    if (t < best) {
+      best = t;
+      *split = s;
+    }
+  }
+  return best;
+}
+
 template <class V, int P, class T, class Epi>
-hipError_t launch(Args& g, bool tri, const Epi& e, hipStream_t st) {
+hipError_t launch(Args& g, bool tri, int split, const Epi& e, hipStream_t st) {
   g.tm = (g.M + T::BM - 1) / T::BM;
   g.tn = (g.N + T::BN - 1) / T::BN;
   g.tri = tri ? 1 : 0;
   const long long tiles = tri ? (long long)g.tm * (g.tm + 1) / 2 : (long long)g.tm * g.tn, units = tiles * g.batch;
   if (units < 1 || units >= (1ll << 24) || g.K < 64 || (g.K & 63) || g.nseg < 1) return hipErrorInvalidValue;
   g.tiles = (int)tiles;
-  g.split = 1;
-  if constexpr (!Epi::WHOLE) {
-    // too few tiles for the card's workgroups: deal the k steps out too, at least 8 to each
-    const long long slots = 256ll * T::PER_CU, steps = (long long)(g.K / 64) * g.nseg;
-    if (g.part && units * 4 < slots * 3) {
-      long long s = slots / units;
-      s = s < steps / 8 ? s : steps / 8;
-      const long long room = PART_BYTES / (units * T::BM * T::BN * 4);
-      s = s < room ? s : room;
-      if (s > 1) g.split = (int)s;
-    }
-  }
+  g.split = split;
   static bool raised = false;                                 // the attribute belongs to the function, not to a call
   if (!raised) {
     const hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<V, P, T, Epi>),
@@ -316,14 +373,20 @@ hipError_t launch(Args& g, bool tri, const Epi& e, hipStream_t st) {
   return r;
 }
 
-// tile by the shape of the result
 template <class V, int P, class Epi>
 hipError_t launch_best(Args& g, bool tri, const Epi& e, hipStream_t st) {
-  if (!tri && g.N <= 64) return launch<V, P, Slim>(g, tri, e, st);
+  const bool may = !Epi::WHOLE && g.part;
+  int split[5] = {1, 1, 1, 1, 1};
+  const double big = P == 1 ? cost_of<Big, P>(g, tri, may, split) : 1e30, wide = P == 1 ? cost_of<Wide, P>(g, tri, may, split + 1) : 1e30,
+               mid = cost_of<Mid, P>(g, tri, may, split + 2), slim = tri ? 1e30 : cost_of<Slim, P>(g, tri, may, split + 3),
+               tiny = cost_of<Tiny, P>(g, tri, may, split + 4);
   if constexpr (P == 1) {
-    if (tile_count<Big>(g, tri) >= (tri ? 120 : 192)) return launch<V, P, Big>(g, tri, e, st);
+    if (big <= wide && big <= mid && big <= slim && big <= tiny) return launch<V, P, Big>(g, tri, split[0], e, st);
+    if (wide <= mid && wide <= slim && wide <= tiny) return launch<V, P, Wide>(g, tri, split[1], e, st);
   }
-  return launch<V, P, Mid>(g, tri, e, st);
+  if (mid <= slim && mid <= tiny) return launch<V, P, Mid>(g, tri, split[2], e, st);
+  if (slim <= tiny) return launch<V, P, Slim>(g, tri, split[3], e, st);
+  return launch<V, P, Tiny>(g, tri, split[4], e, st);
 }
 
 }  // namespace mm16
