@@ -71,114 +71,139 @@ __device__ __forceinline__ float scale_of(float top) {
   return ldexpf(1.f, k > 100 ? 100 : k < -100 ? -100 : k);
 }
 
-// Rows of an operand, k padded.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per row, whose
-// inverse goes to inv[row].  One wave per row, the second read comes from the cache.
-template <int DT>
-__global__ __launch_bounds__(256) void rows_kernel(const void* src, long long rs, int rows, int cols, int colsp, int vec, void* out,
-                                                   float* inv) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  const long long in = row * rs;
-  if constexpr (DT == TCMI_F32) {
-    float top = 0.f;
-    for (int c = 4 * lane; c < cols; c += 256) {
-      const f32x4 v = fetch_row4<DT>(src, in, c, cols, vec);
-      top = fmaxf(fmaxf(fmaxf(top, fabsf(v[0])), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float s = scale_of(top);
-    f16* q = (f16*)out + (long long)row * 2 * colsp;
-    for (int c = 4 * lane; c < colsp; c += 256) {
-      const f32x4 v = fetch_row4<DT>(src, in, c, cols, vec);
-      f16x4 hi, lo;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f16 h, l;
-        two_pieces(v[k] * s, h, l);
-        hi[k] = h;
-        lo[k] = l;
-      }
-      store_four<2>(q, c, hi, lo);
-    }
-    if (lane == 0) inv[row] = 1.f / s;
-  } else {
-    const unsigned short* p = (const unsigned short*)src + in;
-    unsigned short* q = (unsigned short*)out + (long long)row * colsp;
-    typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
-    for (int c = 4 * lane; c < colsp; c += 256) {
-      u16x4 v = {0, 0, 0, 0};
-      if (vec && c + 3 < cols) {
-        v = *reinterpret_cast<const u16x4*>(p + c);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (c + k < cols) v[k] = p[c + k];
-      }
-      *reinterpret_cast<u16x4*>(q + c) = v;
-    }
-  }
-}
+// One pass over the rows of h and of w, a wave per row, bound by its reads (and writes, where a copy is made):
+//   out   the row with k padded.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per row, whose
+//         inverse goes to inv[row] (the second read of the row comes from the cache).
+//   r     h only: the factor of row t in the gradients, from its target and dloss.
+//   part  partial maxima of |x| (h: times |r|, and |r| itself; rows whose factor is zero do not count).
+struct Operand {
+  const void* src;
+  long long rs;
+  int rows, cols, colsp, vec, blocks;
+  f16* out;
+  float *inv, *part;
+};
 
-// r_t: the factor of row t in the gradients
-__global__ __launch_bounds__(256) void factor_kernel(const long long* y, long long ignore, const float* dloss, int per_row,
-                                                     const float* count, int T, float* r) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= T) return;
-  const float g = per_row ? dloss[t] : count ? dloss[0] / count[0] : dloss[0];
-  r[t] = y[t] == ignore ? 0.f : g;
-}
+struct Prep {
+  Operand h, w;
+  const long long* y;
+  long long ignore;
+  const float *dloss, *count;
+  int per_row;
+  float* r;                      // null: no factors (forward)
+};
 
-// partial maxima of |x| (times a row factor; rows whose factor is zero do not count); one wave per row, bound by its reads
 template <int DT>
-__global__ __launch_bounds__(256) void top_kernel(const void* src, long long rs, int rows, int cols, int vec, const float* r, float* part) {
+__global__ __launch_bounds__(256) void prep_kernel(Prep a) {
   __shared__ float red[4];
+  const bool is_h = (int)blockIdx.x < a.h.blocks;
+  const Operand& o = is_h ? a.h : a.w;
+  const int block = is_h ? blockIdx.x : blockIdx.x - a.h.blocks, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   float top = 0.f;
-  const int lane = threadIdx.x & 63;
-  for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4) {
-    const float f = r ? fabsf(r[row]) : 1.f;
-    if (f == 0.f) continue;
-    const long long at = row * rs;
-    float t = 0.f;
-#pragma unroll 4
-    for (int c = 4 * lane; c < cols; c += 256) {
-      const f32x4 v = fetch_row4<DT>(src, at, c, cols, vec);
-      t = fmaxf(fmaxf(fmaxf(t, fabsf(v[0])), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+  for (int row = block * 4 + wave; row < o.rows; row += o.blocks * 4) {
+    const long long in = row * o.rs;
+    float f = 1.f;
+    if (is_h && a.r) {
+      f = a.per_row ? a.dloss[row] : a.count ? a.dloss[0] / a.count[0] : a.dloss[0];
+      if (a.y[row] == a.ignore) f = 0.f;
+      if (lane == 0) a.r[row] = f;
     }
-    top = fmaxf(top, t * f);
-  }
+    float t = 0.f;
+    if ((o.part && f != 0.f) || (o.out && DT == TCMI_F32)) {
+#pragma unroll 4
+      for (int c = 4 * lane; c < o.cols; c += 256) {
+        const f32x4 v = fetch_row4<DT>(o.src, in, c, o.cols, o.vec);
+        t = fmaxf(fmaxf(fmaxf(t, fabsf(v[0])), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+      }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (lane == 0) red[threadIdx.x >> 6] = top;
+      for (int k = 32; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor(t, k));
+      if (f != 0.f) top = fmaxf(top, (is_h && a.r ? fmaxf(t, 1.f) : t) * fabsf(f));
+    }
+    if (!o.out) continue;
+    if constexpr (DT == TCMI_F32) {
+      const float s = scale_of(t);
+      f16* q = o.out + (long long)row * 2 * o.colsp;
+      for (int c = 4 * lane; c < o.colsp; c += 256) {
+        const f32x4 v = fetch_row4<DT>(o.src, in, c, o.cols, o.vec);
+        f16x4 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          f16 h, l;
+          two_pieces(v[k] * s, h, l);
+          hi[k] = h;
+          lo[k] = l;
+        }
+        store_four<2>(q, c, hi, lo);
+      }
+      if (lane == 0) o.inv[row] = 1.f / s;
+    } else {
+      typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+      const unsigned short* p = (const unsigned short*)o.src + in;
+      unsigned short* q = (unsigned short*)o.out + (long long)row * o.colsp;
+      for (int c = 4 * lane; c < o.colsp; c += 256) {
+        u16x4 v = {0, 0, 0, 0};
+        if (o.vec && c + 3 < o.cols) {
+          v = *reinterpret_cast<const u16x4*>(p + c);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (c + k < o.cols) v[k] = p[c + k];
+        }
+        *reinterpret_cast<u16x4*>(q + c) = v;
+      }
+    }
+  }
+  if (!o.part) return;
+  if (lane == 0) red[wave] = top;
   __syncthreads();
-  if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if (threadIdx.x == 0) o.part[block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
 // out[c][row] = src[row][c] * r[row] * scale as f16 pieces (two for f32), rows padded with zeros.  A zero factor gives zero
-// whatever the row holds.  64 x 64 tiles through LDS, four elements a thread on both sides.
+// whatever the row holds.  ones: behind the last column one more, the factors themselves (their product with P is the
+// bias's gradient).  64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
+struct Turn {
+  const void* src;
+  long long rs;
+  int rows, cols, rowsp, vec, ones, tx, tiles;
+  const float *r, *part;
+  int nparts;
+  f16* out;
+  float* inv;
+};
+
 template <int DT>
-__global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs, int rows, int cols, int vec, const float* r,
-                                                   const float* part, int nparts, f16* out, int rowsp, float* inv) {
+__global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
   constexpr int P = DT == TCMI_F32 ? 2 : 1;
   __shared__ float tile[64][65];
   __shared__ float red[4];
-  const int tid = threadIdx.x;
+  const bool first = (int)blockIdx.x < x.tiles;
+  const Turn& a = first ? x : y;
+  const int tid = threadIdx.x, block = first ? blockIdx.x : blockIdx.x - x.tiles;
   float top = 0.f;
-  for (int k = tid; k < nparts; k += 256) top = fmaxf(top, part[k]);
+  for (int k = tid; k < a.nparts; k += 256) top = fmaxf(top, a.part[k]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   if ((tid & 63) == 0) red[tid >> 6] = top;
   __syncthreads();
   const float s = scale_of(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, u = (tid & 15) * 4, w = tid >> 4;
-  if (r0 == 0 && c0 == 0 && tid == 0) *inv = 1.f / s;
+  const int r0 = block % a.tx * 64, c0 = block / a.tx * 64, u = (tid & 15) * 4, w = tid >> 4;
+  if (block == 0 && tid == 0) *a.inv = 1.f / s;
 #pragma unroll
   for (int k = w; k < 64; k += 16) {
     const int row = r0 + k;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (row < rows) {
-      const float f = r ? r[row] : 1.f;
-      if (f != 0.f) v = fetch_row4<DT>(src, row * rs, c0 + u, cols, vec) * f * s;
+    if (row < a.rows) {
+      const float f = a.r ? a.r[row] : 1.f;
+      if (f != 0.f) {
+        v = fetch_row4<DT>(a.src, row * a.rs, c0 + u, a.cols, a.vec);
+        if (a.ones) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c0 + u + e == a.cols) v[e] = 1.f;
+        }
+        v = v * f * s;
+      }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) tile[k][u + e] = v[e];
@@ -187,7 +212,7 @@ __global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs
 #pragma unroll
   for (int k = w; k < 64; k += 16) {
     const int c = c0 + k, row = r0 + u;
-    if (c < cols && row < rowsp) {
+    if (c < a.cols + a.ones && row < a.rowsp) {
       f16x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -196,7 +221,7 @@ __global__ __launch_bounds__(256) void turn_kernel(const void* src, long long rs
         hi[e] = h;
         lo[e] = l;
       }
-      store_four<P>(out + (long long)c * P * rowsp, row, hi, lo);
+      store_four<P>(a.out + (long long)c * P * a.rowsp, row, hi, lo);
     }
   }
 }
@@ -287,11 +312,10 @@ struct EpiLse {
   }
 };
 
-// joins the tiles of a row: one wave per row
-__global__ __launch_bounds__(256) void rowstat_kernel(const float2* part, int tiles, const float* target, const long long* y,
-                                                   long long ignore, int T, int V, float* lse, float* loss) {
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (t >= T) return;
+// the loss of row t from its tiles' statistics, by one wave
+__device__ __forceinline__ float row_loss(const float2* part, int tiles, const float* target, const long long* y, long long ignore, int t,
+                                          int V, float* lse) {
+  const int lane = threadIdx.x & 63;
   const float2* p = part + (long long)t * tiles;
   float top = -INFINITY, bad = 0.f;
   for (int k = lane; k < tiles; k += 64) {
@@ -305,25 +329,16 @@ __global__ __launch_bounds__(256) void rowstat_kernel(const float2* part, int ti
   for (int k = lane; k < tiles; k += 64) sum += p[k].x == -INFINITY ? 0.f : p[k].y * expf(p[k].x - at);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if (lane == 0) {
-    const float l = at + logf(sum);
-    lse[t] = l;
-    const long long yt = y[t];
-    loss[t] = yt == ignore ? 0.f : yt < 0 || yt >= V ? NAN : l - target[t];
-  }
+  const float l = at + logf(sum);
+  if (lane == 0) lse[t] = l;
+  const long long yt = y[t];
+  return yt == ignore ? 0.f : yt < 0 || yt >= V ? NAN : l - target[t];
 }
 
-// sum or mean over the rows that count, in f64 and a fixed order
-__global__ __launch_bounds__(1024) void total_kernel(const float* loss, const long long* y, long long ignore, int T, int mean,
-                                                     float* out, float* count) {
+// sum or mean over the rows that count, in f64 and a fixed order; 16 waves
+__device__ __forceinline__ void total_of(double s, int c, int mean, float* out, float* count) {
   __shared__ double rs[16];
   __shared__ int rc[16];
-  double s = 0.0;
-  int c = 0;
-  for (int t = threadIdx.x; t < T; t += 1024) {
-    s += loss[t];
-    c += y[t] != ignore;
-  }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     s += __shfl_xor(s, o);
@@ -344,6 +359,42 @@ __global__ __launch_bounds__(1024) void total_kernel(const float* loss, const lo
     *count = (float)c;
     *out = (float)(mean ? s / c : s);                // no row counts: 0 / 0
   }
+}
+
+__global__ __launch_bounds__(256) void rowstat_kernel(const float2* part, int tiles, const float* target, const long long* y,
+                                                      long long ignore, int T, int V, float* lse, float* loss) {
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= T) return;
+  const float x = row_loss(part, tiles, target, y, ignore, t, V, lse);
+  if ((threadIdx.x & 63) == 0) loss[t] = x;
+}
+
+__global__ __launch_bounds__(1024) void total_kernel(const float* loss, const long long* y, long long ignore, int T, int mean, float* out,
+                                                     float* count) {
+  double s = 0.0;
+  int c = 0;
+  for (int t = threadIdx.x; t < T; t += 1024) {
+    s += loss[t];
+    c += y[t] != ignore;
+  }
+  total_of(s, c, mean, out, count);
+}
+
+// both in one workgroup, where there is little to read
+__global__ __launch_bounds__(1024) void rowstat_total_kernel(const float2* part, int tiles, const float* target, const long long* y,
+                                                             long long ignore, int T, int V, float* lse, float* loss, int mean, float* out,
+                                                             float* count) {
+  double s = 0.0;
+  int c = 0;
+  for (int t = threadIdx.x >> 6; t < T; t += 16) {
+    const float x = row_loss(part, tiles, target, y, ignore, t, V, lse);
+    if ((threadIdx.x & 63) == 0) {
+      loss[t] = x;
+      s += x;
+      c += y[t] != ignore;
+    }
+  }
+  total_of(s, c, mean, out, count);
 }
 
 // backward: P as f16 pieces, row-major for dh and transposed for dw, zero in the padding and in ignored rows
@@ -393,26 +444,32 @@ struct EpiProb {
   }
 };
 
-// a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor
+// a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor;
+// a column behind the last one is the bias's gradient
 struct EpiGrad {
   static constexpr bool WHOLE = false;
   const float* inv;              // inverse of the other operand's scale, on the device
-  float* sum;                    // f32 [rows][N] (null: only one piece)
+  float* sum;                    // f32 [rows][cols] (null: only one piece)
   int first, last;
   const float* r;                // null: 1
   void* out;
-  int dtype;
+  int dtype, cols;
+  void* db;
   __device__ __forceinline__ void four(const Args& g, int, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
     const float al = *inv * (1.f / PSCALE);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (col + k >= g.N) continue;
-      const long long at = (long long)row * g.N + col + k;
       float x = al * v[k];
+      if (col + k == cols) {
+        put(db, dtype, row, x);
+        continue;
+      }
+      const long long at = (long long)row * cols + col + k;
       if (!first) x += sum[at];
       if (!last) sum[at] = x;
-      else put(out, dtype, at, r ? (r[row] == 0.f ? 0.f : x * r[row]) : x);
+      else if (out) put(out, dtype, at, r ? (r[row] == 0.f ? 0.f : x * r[row]) : x);
     }
   }
 };
@@ -515,7 +572,7 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
   w.split = a.take<float>(PART_BYTES / 4);
   w.p = a.take<f16>(s.T * vp * s.P);
   w.pt = a.take<f16>(vc * s.tp * s.P);
-  w.ht = a.take<f16>((long long)s.D * s.tp * s.P);
+  w.ht = a.take<f16>((long long)(s.D + 1) * s.tp * s.P);
   w.wt = a.take<f16>(s.D * vp * s.P);
   return w;
 }
@@ -524,13 +581,6 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
   do {                                           \
     const hipError_t e_ = (x);                   \
     if (e_ != hipSuccess) return e_;             \
-  } while (0)
-
-#define BY_TYPE(dt, K, ...)                                                                        \
-  do {                                                                                             \
-    if ((dt) == TCMI_F32) hipLaunchKernelGGL(K<TCMI_F32>, __VA_ARGS__);                            \
-    else if ((dt) == TCMI_F16) hipLaunchKernelGGL(K<TCMI_F16>, __VA_ARGS__);                       \
-    else hipLaunchKernelGGL(K<TCMI_BF16>, __VA_ARGS__);                                            \
   } while (0)
 
 template <int P, class Epi>
@@ -557,18 +607,39 @@ struct In {
   long long ignore;
 };
 
-hipError_t operands(const Shape& s, const In& in, const Rows& r, hipStream_t st) {
-  if (!s.h_direct) {
-    BY_TYPE(s.dtype, rows_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, s.dp,
-            vec4(in.h, in.hrs, s.dtype), r.h, r.hs);
-    TRY(hipGetLastError());
-  }
-  if (!s.w_direct) {
-    BY_TYPE(s.dtype, rows_kernel, dim3((s.V + 3) / 4), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, s.dp,
-            vec4(in.w, in.wrs, s.dtype), r.w, r.ws);
-    TRY(hipGetLastError());
-  }
-  return hipSuccess;
+// the pass over the operands: what the logits' product cannot read in place, and for the backward the factors and maxima
+hipError_t prepare(const Shape& s, const In& in, const Rows& rows, Prep a, hipStream_t st) {
+  auto one = [&](Operand& o, const void* src, long long rs, int n, f16* out, float* inv) {
+    o.src = src;
+    o.rs = rs;
+    o.rows = n;
+    o.cols = s.D;
+    o.colsp = s.dp;
+    o.vec = vec4(src, rs, s.dtype);
+    o.out = out;
+    o.inv = inv;
+    const bool work = out || o.part || (&o == &a.h && a.r);
+    o.blocks = !work ? 0 : n / 4 < 1 ? 1 : n / 4 > PARTS ? PARTS : n / 4;
+  };
+  one(a.h, in.h, in.hrs, s.T, rows.h, rows.hs);
+  one(a.w, in.w, in.wrs, s.V, rows.w, rows.ws);
+  const int blocks = a.h.blocks + a.w.blocks;
+  if (!blocks) return hipSuccess;
+  if (s.dtype == TCMI_F32) hipLaunchKernelGGL(prep_kernel<TCMI_F32>, dim3(blocks), dim3(256), 0, st, a);
+  else if (s.dtype == TCMI_F16) hipLaunchKernelGGL(prep_kernel<TCMI_F16>, dim3(blocks), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(prep_kernel<TCMI_BF16>, dim3(blocks), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+int parts_of(int rows) { return rows / 4 < 1 ? 1 : rows / 4 > PARTS ? PARTS : rows / 4; }
+
+hipError_t turn(const Shape& s, const Turn& x, const Turn& y, hipStream_t st) {
+  const int blocks = x.tiles + y.tiles;
+  if (!blocks) return hipSuccess;
+  if (s.dtype == TCMI_F32) hipLaunchKernelGGL(turn_kernel<TCMI_F32>, dim3(blocks), dim3(256), 0, st, x, y);
+  else if (s.dtype == TCMI_F16) hipLaunchKernelGGL(turn_kernel<TCMI_F16>, dim3(blocks), dim3(256), 0, st, x, y);
+  else hipLaunchKernelGGL(turn_kernel<TCMI_BF16>, dim3(blocks), dim3(256), 0, st, x, y);
+  return hipGetLastError();
 }
 
 // the logits' product for the classes [v0, v0 + vc)
@@ -589,10 +660,15 @@ Args logit_args(const Shape& s, const In& in, const Rows& r, int v0, int vc) {
 template <int P>
 hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, float* loss, float* total, float* count, int mean,
                    hipStream_t st) {
-  TRY(operands(s, in, w.rows, st));
+  TRY(prepare(s, in, w.rows, Prep{}, st));
   Args g = logit_args(s, in, w.rows, 0, s.V);
   TRY(run_logits<P>(g, s.dtype, EpiLse{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
   const int tiles = g.tn;
+  if (total && (long long)s.T * tiles <= 8192) {       // 64 KB of statistics
+    hipLaunchKernelGGL(rowstat_total_kernel, dim3(1), dim3(1024), 0, st, w.part, tiles, w.target, in.y, in.ignore, s.T, s.V, lse, loss, mean,
+                       total, count);
+    return hipGetLastError();
+  }
   hipLaunchKernelGGL(rowstat_kernel, dim3((s.T + 3) / 4), dim3(256), 0, st, w.part, tiles, w.target, in.y, in.ignore, s.T, s.V, lse, loss);
   TRY(hipGetLastError());
   if (total) {
@@ -605,55 +681,59 @@ hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, f
 template <int P>
 hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float* lse, const float* dloss, int per_row, const float* count,
                     void* dh, void* dw, void* db, hipStream_t st) {
-  TRY(operands(s, in, w.rows, st));
-  hipLaunchKernelGGL(factor_kernel, dim3((s.T + 255) / 256), dim3(256), 0, st, in.y, in.ignore, dloss, per_row, count, s.T, w.r);
-  TRY(hipGetLastError());
-  auto blocks = [](int rows) { return rows / 4 < 1 ? 1 : rows / 4 > PARTS ? PARTS : rows / 4; };
-  const float* none = nullptr;
-  if (dw) {
-    const int nb = blocks(s.T);
-    BY_TYPE(s.dtype, top_kernel, dim3(nb), dim3(256), 0, st, in.h, in.hrs, s.T, s.D, vec4(in.h, in.hrs, s.dtype), w.r, w.parth);
-    TRY(hipGetLastError());
-    BY_TYPE(s.dtype, turn_kernel, dim3((s.tp + 63) / 64, (s.D + 63) / 64), dim3(256), 0, st, in.h, in.hrs, s.T, s.D,
-            vec4(in.h, in.hrs, s.dtype), w.r, w.parth, nb, w.ht, s.tp, w.invh);
-    TRY(hipGetLastError());
-  }
-  const int nbw = blocks(s.V);
-  if (dh) {
-    BY_TYPE(s.dtype, top_kernel, dim3(nbw), dim3(256), 0, st, in.w, in.wrs, s.V, s.D, vec4(in.w, in.wrs, s.dtype), none, w.partw);
-    TRY(hipGetLastError());
-  }
+  // the bias's gradient as one more column of h^T costs nothing where the columns do not fill their tiles
+  const int ones = db && s.D % 64 != 0, want_dw = dw || ones;
+  Prep a{};
+  a.y = in.y;
+  a.ignore = in.ignore;
+  a.dloss = dloss;
+  a.count = count;
+  a.per_row = per_row;
+  a.r = w.r;
+  if (want_dw) a.h.part = w.parth;
+  if (dh) a.w.part = w.partw;
+  TRY(prepare(s, in, w.rows, a, st));
   const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
   for (int v0 = 0; v0 < s.V; v0 += vc) {
     const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P);
+    Turn th{}, tw{};
+    if (want_dw && v0 == 0) {
+      th = Turn{in.h, in.hrs, s.T, s.D, s.tp, vec4(in.h, in.hrs, s.dtype), ones, (s.tp + 63) / 64, 0, w.r, w.parth, parts_of(s.T), w.ht, w.invh};
+      th.tiles = th.tx * ((s.D + ones + 63) / 64);
+    }
+    if (dh) {
+      tw = Turn{(const char*)in.w + v0 * in.wrs * size, in.wrs, n, s.D, np, vec4(in.w, in.wrs, s.dtype), 0, (np + 63) / 64, 0, nullptr,
+                w.partw, parts_of(s.V), w.wt, w.invw};
+      tw.tiles = tw.tx * ((s.D + 63) / 64);
+    }
+    TRY(turn(s, th, tw, st));
     Args g = logit_args(s, in, w.rows, v0, n);
     TRY(run_logits<P>(g, s.dtype,
                       EpiProb<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.p, w.pt, np, s.tp}, st));
     Args d{};
-    d.N = s.D;
     d.batch = 1;
     d.nseg = 1;
     d.part = w.split;
     if (dh) {
-      BY_TYPE(s.dtype, turn_kernel, dim3((np + 63) / 64, (s.D + 63) / 64), dim3(256), 0, st, (const char*)in.w + v0 * in.wrs * size, in.wrs,
-              n, s.D, vec4(in.w, in.wrs, s.dtype), none, w.partw, nbw, w.wt, np, w.invw);
-      TRY(hipGetLastError());
       d.M = s.T;
+      d.N = s.D;
       d.K = P * np;
       d.lda = d.ldb = d.K;
       d.a[0] = w.p;
       d.b[0] = w.wt;
-      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype}, st));
+      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr}, st));
     }
-    if (dw) {
+    if (want_dw) {
       d.M = n;
+      d.N = s.D + ones;
       d.K = P * s.tp;
       d.lda = d.ldb = d.K;
       d.a[0] = w.pt;
       d.b[0] = w.ht;
-      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype}, st));
+      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, dw ? (char*)dw + (long long)v0 * s.D * size : nullptr, s.dtype, s.D,
+                            ones ? (char*)db + (long long)v0 * size : nullptr}, st));
     }
-    if (db) {
+    if (db && !ones) {
       hipLaunchKernelGGL(bias_kernel<P>, dim3((n + 3) / 4), dim3(256), 0, st, w.pt, s.tp, w.r, s.T, n, db, s.dtype, v0);
       TRY(hipGetLastError());
     }

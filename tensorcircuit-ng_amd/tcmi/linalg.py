@@ -396,6 +396,15 @@ def _ns_coefficients(steps, coefficients, eps):
     return steps, flat
 
 
+def _on(device):
+    """the tensors' device as the current one (nothing to do when it is)"""
+    import contextlib
+
+    import torch
+
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _host_doubles(flat):
     import ctypes
 
@@ -451,7 +460,7 @@ def _newton_schulz_raw(mat, steps, flat, eps, saving):
     work = torch.empty(nbytes, dtype=torch.uint8, device=mat.device)
     saved = torch.empty(L.tcmi_ns_work_bytes(m, n, b, steps, 1, code, _lib.NS_SAVED) if saving else 0, dtype=torch.uint8,
                         device=mat.device)
-    with torch.cuda.device(mat.device):
+    with _on(mat.device):
         _lib.check(L.tcmi_newton_schulz(x.data_ptr(), x.stride(1), x.stride(2), x.stride(0), out.data_ptr(), m, n, b, steps,
                                         _host_doubles(flat), eps, full, saved.data_ptr() if saving else None, saved.numel(),
                                         work.data_ptr(), work.numel(), code, _stream(mat)), "tcmi_newton_schulz")
@@ -469,7 +478,7 @@ def _newton_schulz_grad_raw(mat, saved, dout, steps, flat, eps):
         return out.reshape(mat.shape)
     L = _lib.lib()
     work = torch.empty(L.tcmi_ns_work_bytes(m, n, b, steps, 1, code, _lib.NS_WORK_GRAD), dtype=torch.uint8, device=mat.device)
-    with torch.cuda.device(mat.device):
+    with _on(mat.device):
         _lib.check(L.tcmi_newton_schulz_grad(x.data_ptr(), x.stride(1), x.stride(2), x.stride(0), d.data_ptr(), d.stride(1),
                                              d.stride(2), d.stride(0), out.data_ptr(), m, n, b, steps, _host_doubles(flat), eps,
                                              saved.data_ptr(), saved.numel(), work.data_ptr(), work.numel(), code, _stream(mat)),

@@ -48,52 +48,51 @@ _REDUCTIONS = ("none", "sum", "mean")
 
 
 def _lce_raw(h, w, target, bias, ignore_index, reduction):
-    """(loss, lse, count): h [T, D], w [V, D], target [T]; loss is per row for reduction "none" """
+    """(loss, stat): h [T, D], w [V, D], target [T]; loss is per row for reduction "none".  stat, what the gradient needs: the
+    rows' log sums, how many rows count, and (not "none") the rows' losses"""
     t, d = h.shape
     v = w.shape[0]
     code = linalg._train_code(h)
-    dev = h.device
-    lse = torch.empty(t, dtype=torch.float32, device=dev)
-    rows = torch.empty(t, dtype=torch.float32, device=dev)
-    total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-    count = torch.empty((), dtype=torch.float32, device=dev)
+    per_row = reduction == "none"
+    loss = torch.empty(t if per_row else (), dtype=torch.float32, device=h.device)
+    stat = torch.empty(t + 1 if per_row else 2 * t + 1, dtype=torch.float32, device=h.device)
     if t == 0:
-        if total is not None:
-            total.fill_(math.nan if reduction == "mean" else 0.0)
-        return (rows if total is None else total), lse, count.zero_()
+        if not per_row:
+            loss.fill_(math.nan if reduction == "mean" else 0.0)
+        return loss, stat.zero_()
     L = _lib.lib()
-    nbytes = L.tcmi_lce_work_bytes(h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), t, d, v, code, 0)
+    hp, hs, wp, ws, lse = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), stat.data_ptr()
+    nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, 0)
     if nbytes < 0:
         raise ValueError(f"linear_cross_entropy: {t} rows, {d} features, {v} classes are out of range")
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    work = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+    with linalg._on(h.device):
         _lib.check(L.tcmi_linear_cross_entropy(
-            h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), None if bias is None else bias.data_ptr(), target.data_ptr(),
-            ignore_index, t, d, v, lse.data_ptr(), rows.data_ptr(), None if total is None else total.data_ptr(),
-            count.data_ptr(), int(reduction == "mean"), work.data_ptr(), work.numel(), code, linalg._stream(h)),
-            "tcmi_linear_cross_entropy")
-    return (rows if total is None else total), lse, count
+            hp, hs, wp, ws, None if bias is None else bias.data_ptr(), target.data_ptr(), ignore_index, t, d, v, lse,
+            loss.data_ptr() if per_row else lse + 4 * (t + 1), None if per_row else loss.data_ptr(), lse + 4 * t,
+            int(reduction == "mean"), work.data_ptr(), nbytes, code, linalg._stream(h)), "tcmi_linear_cross_entropy")
+    return loss, stat
 
 
-def _lce_grad_raw(h, w, target, bias, lse, count, dloss, ignore_index, reduction, need):
+def _lce_grad_raw(h, w, target, bias, stat, dloss, ignore_index, reduction, need):
     t, d = h.shape
     v = w.shape[0]
     dev = h.device
-    outs = [torch.empty_like(x, memory_format=torch.contiguous_format) if n else None for x, n in zip((h, w, bias), need)]
+    outs = [torch.empty(x.shape, dtype=x.dtype, device=dev) if n else None for x, n in zip((h, w, bias), need)]
     if t == 0:
         return tuple(torch.empty(0, device=dev) if o is None else o.zero_() for o in outs)
     code = linalg._train_code(h)
     dloss = dloss.to(torch.float32).contiguous()
     L = _lib.lib()
-    nbytes = L.tcmi_lce_work_bytes(h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), t, d, v, code, 1)
+    hp, hs, wp, ws, lse = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), stat.data_ptr()
+    nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, 1)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     ptrs = [None if o is None else o.data_ptr() for o in outs]
-    with torch.cuda.device(dev):
+    with linalg._on(dev):
         _lib.check(L.tcmi_linear_cross_entropy_grad(
-            h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), None if bias is None else bias.data_ptr(), target.data_ptr(),
-            ignore_index, t, d, v, lse.data_ptr(), dloss.data_ptr(), int(reduction == "none"),
-            count.data_ptr() if reduction == "mean" else None, *ptrs, work.data_ptr(), work.numel(), code, linalg._stream(h)),
-            "tcmi_linear_cross_entropy_grad")
+            hp, hs, wp, ws, None if bias is None else bias.data_ptr(), target.data_ptr(), ignore_index, t, d, v, lse,
+            dloss.data_ptr(), int(reduction == "none"), lse + 4 * t if reduction == "mean" else None, *ptrs, work.data_ptr(),
+            nbytes, code, linalg._stream(h)), "tcmi_linear_cross_entropy_grad")
     return tuple(torch.empty(0, device=dev) if o is None else o for o in outs)
 
 
@@ -117,14 +116,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def setup_context(ctx, inputs, output):
         h, w, target, bias, ctx.ignore_index, ctx.reduction = inputs
-        ctx.mark_non_differentiable(output[1], output[2])
-        ctx.save_for_backward(h, w, target, bias, output[1], output[2])
+        ctx.mark_non_differentiable(output[1])
+        ctx.save_for_backward(h, w, target, bias, output[1])
 
     @staticmethod
-    def backward(ctx, dloss, *_):
-        h, w, target, bias, lse, count = ctx.saved_tensors
+    def backward(ctx, dloss, _):
+        h, w, target, bias, stat = ctx.saved_tensors
         need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3] and bias is not None)
-        dh, dw, db = _LinearCrossEntropyGrad.apply(h, w, target, bias, lse, count, dloss, ctx.ignore_index, ctx.reduction, need)
+        dh, dw, db = _LinearCrossEntropyGrad.apply(h, w, target, bias, stat, dloss, ctx.ignore_index, ctx.reduction, need)
         return dh if need[0] else None, dw if need[1] else None, None, db if need[2] else None, None, None
 
 
@@ -132,12 +131,12 @@ class _LinearCrossEntropyGrad(torch.autograd.Function):
     generate_vmap_rule = False
 
     @staticmethod
-    def forward(h, w, target, bias, lse, count, dloss, ignore_index, reduction, need):
-        return _lce_grad_raw(h, w, target, bias, lse, count, dloss, ignore_index, reduction, need)
+    def forward(h, w, target, bias, stat, dloss, ignore_index, reduction, need):
+        return _lce_grad_raw(h, w, target, bias, stat, dloss, ignore_index, reduction, need)
 
     @staticmethod
     def vmap(info, in_dims, *args):
-        return _vmap_loop(_LinearCrossEntropyGrad.apply, info, in_dims[:7] + (None,) * 3, args)
+        return _vmap_loop(_LinearCrossEntropyGrad.apply, info, in_dims[:6] + (None,) * 3, args)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
@@ -268,7 +267,7 @@ def muon_step(param: Tensor, grad: Tensor, momentum_buffer: Tensor, lr: float = 
             raise ValueError(f"muon_step: {b} matrices of {m} x {n} are out of range")
         work = torch.empty(nbytes, dtype=torch.uint8, device=p.device)
         r = 0.2 * math.sqrt(max(m, n)) if adjust_lr_fn == "match_rms_adamw" else math.sqrt(max(1.0, m / n))
-        with torch.cuda.device(p.device):
+        with linalg._on(p.device):
             _lib.check(L.tcmi_muon_step(
                 p.data_ptr(), p.stride(1), p.stride(2), p.stride(0), g.data_ptr(), g.stride(1), g.stride(2), g.stride(0),
                 v.data_ptr(), v.stride(1), v.stride(2), v.stride(0), m, n, b, float(momentum), int(bool(nesterov)),
