@@ -260,6 +260,8 @@ __device__ __forceinline__ void logits(const Logits& q, const Args& g, int m0, i
 // forward: per row the tile's maximum and sum of exponentials, and the target's logit where it lies in the tile
 struct EpiLse {
   static constexpr bool WHOLE = true;
+  template <class T>
+  static constexpr int lds() { return T::WN * T::BM * 8; }
   Logits q;
   float2* part;                  // [T][tiles of classes]
   float* target;                 // [T]
@@ -408,9 +410,18 @@ struct EpiProb {
   int V;
   f16 *p, *pt;                   // [T][P * vp], [classes][P * tp]
   int vp, tp;                    // padded classes of the piece, padded rows
+  // the transposed tile, its rows 8 elements longer than the tile: 16-byte aligned, no bank conflicts
   template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int, char*, f32x4 (&acc)[T::MI][T::NI]) const {
+  static constexpr int line() { return T::BM + 8; }
+  template <class T>
+  static constexpr int lds() { return P * T::BN * line<T>() * 2; }
+  // P goes out from the registers, eight bytes a lane; P^T through LDS, sixteen (from the registers it would be two: 1021 x
+  // 28 x 16384 f32 took 50 us)
+  template <class T>
+  __device__ void tile(const Args& g, int m0, int n0, int, char* lds_bytes, f32x4 (&acc)[T::MI][T::NI]) const {
+    f16* lt = reinterpret_cast<f16*>(lds_bytes);
     logits<T>(q, g, m0, n0, acc);
+    __syncthreads();
     each<T>(m0, n0, acc, [&](int row, int col, f32x4 x) {
       const bool in = row < g.M;
       const long long yt = in ? y[row] : ignore;
@@ -431,16 +442,21 @@ struct EpiProb {
         vl[r] = b;
       }
       if (in && col < vp) store_four<P>(p + (long long)row * P * vp, col, vh, vl);
-      if (row < tp) {
+      f16* o = lt + (col - n0) * line<T>() + row - m0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (col + r < g.N) {
-            f16* o = pt + (long long)(col + r) * P * tp + kpos<P>(row);
-            o[0] = vh[r];
-            if (P == 2) o[32] = vl[r];
-          }
+      for (int r = 0; r < 4; ++r) {
+        o[r * line<T>()] = vh[r];
+        if (P == 2) o[(T::BN + r) * line<T>()] = vl[r];
       }
     });
+    __syncthreads();
+    for (int k = threadIdx.x; k < T::BN * (T::BM / 8); k += T::THREADS) {
+      const int c = k / (T::BM / 8), rl = k % (T::BM / 8) * 8, row = m0 + rl;
+      if (n0 + c >= g.N || row >= tp) continue;
+      f16* o = pt + (long long)(n0 + c) * P * tp + kpos<P>(row);
+      *reinterpret_cast<f16x8*>(o) = *reinterpret_cast<const f16x8*>(lt + c * line<T>() + rl);
+      if (P == 2) *reinterpret_cast<f16x8*>(o + 32) = *reinterpret_cast<const f16x8*>(lt + (T::BN + c) * line<T>() + rl);
+    }
   }
 };
 

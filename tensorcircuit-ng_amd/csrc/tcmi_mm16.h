@@ -216,7 +216,7 @@ __device__ __forceinline__ void product(const Args& g, int m0, int n0, int bz, i
 }
 #endif
 
-// An epilogue works on whole tiles (WHOLE: void tile<T>(g, m0, n0, bz, lds, acc)) or on four neighbouring columns of a row
+// An epilogue works on whole tiles (WHOLE: void tile<T>(g, m0, n0, bz, lds, acc), with lds<T>() bytes of LDS) or on four neighbouring columns of a row
 // at a time (void four(g, bz, mirror, row, col, v); the product may then be split along k).
 template <class T, class F>
 __device__ __forceinline__ void each(int m0, int n0, const f32x4 (&acc)[T::MI][T::NI], F f) {
@@ -355,14 +355,16 @@ hipError_t launch(Args& g, bool tri, int split, const Epi& e, hipStream_t st) {
   if (units < 1 || units >= (1ll << 24) || g.K < 64 || (g.K & 63) || g.nseg < 1) return hipErrorInvalidValue;
   g.tiles = (int)tiles;
   g.split = split;
+  int lds = T::LDS;
+  if constexpr (Epi::WHOLE) lds = lds > Epi::template lds<T>() ? lds : Epi::template lds<T>();
   static bool raised = false;                                 // the attribute belongs to the function, not to a call
   if (!raised) {
     const hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<V, P, T, Epi>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS);
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (r != hipSuccess) return r;
     raised = true;
   }
-  hipLaunchKernelGGL((product_kernel<V, P, T, Epi>), dim3((unsigned)(units * g.split)), dim3(T::THREADS), T::LDS, st, g, e);
+  hipLaunchKernelGGL((product_kernel<V, P, T, Epi>), dim3((unsigned)(units * g.split)), dim3(T::THREADS), lds, st, g, e);
   hipError_t r = hipGetLastError();
   if constexpr (!Epi::WHOLE) {
     if (r == hipSuccess && g.split > 1) {

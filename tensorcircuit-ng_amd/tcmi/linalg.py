@@ -439,7 +439,9 @@ def newton_schulz(mat, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float 
     _train_code(mat)
     _need_gpu("newton_schulz", mat)
     if _tracked(mat):
-        return _ad()["newton_schulz"](mat, steps, flat, float(eps))[0]
+        if torch._C._are_functorch_transforms_active():
+            return _ad()["newton_schulz"](mat, steps, flat, float(eps))[0]
+        return _ad()["newton_schulz_eager"](mat, steps, flat, float(eps))
     return _newton_schulz_raw(mat, steps, flat, float(eps), False)[0]
 
 
@@ -726,6 +728,21 @@ def _ad():
             mat, saved = ctx.saved_tensors
             return NewtonSchulzGrad.apply(mat, saved, dout, ctx.steps, ctx.flat, ctx.eps), None, None, None
 
+    class NewtonSchulzEager(torch.autograd.Function):
+        """the same outside torch.func, whose calling convention costs two signature look-ups a call (60 us)"""
+
+        @staticmethod
+        def forward(ctx, mat, steps, flat, eps):
+            out, saved = _newton_schulz_raw(mat, steps, flat, eps, True)
+            ctx.steps, ctx.flat, ctx.eps = steps, flat, eps
+            ctx.save_for_backward(mat, saved)
+            return out
+
+        @staticmethod
+        def backward(ctx, dout):
+            grad = NewtonSchulzGrad.apply if torch.is_grad_enabled() else _newton_schulz_grad_raw
+            return grad(*ctx.saved_tensors, dout, ctx.steps, ctx.flat, ctx.eps), None, None, None
+
     class NewtonSchulzGrad(torch.autograd.Function):
         generate_vmap_rule = False
 
@@ -753,7 +770,8 @@ def _ad():
 
     # the decompositions' saved tensors are their own outputs: under torch.func they arrive wrapped, and
     # the rules above only use torch ops and ``matmul`` on them
-    _AD.update(matmul=Matmul.apply, svd=Svd.apply, qr=Qr.apply, newton_schulz=NewtonSchulz.apply)
+    _AD.update(matmul=Matmul.apply, svd=Svd.apply, qr=Qr.apply, newton_schulz=NewtonSchulz.apply,
+               newton_schulz_eager=NewtonSchulzEager.apply)
     return _AD
 
 

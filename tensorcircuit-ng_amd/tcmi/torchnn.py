@@ -102,6 +102,25 @@ def _vmap_loop(fn, info, in_dims, args):
     return tuple(torch.stack([o[k] for o in outs]) for k in range(len(outs[0]))), tuple(0 for _ in outs[0])
 
 
+class _LinearCrossEntropyEager(torch.autograd.Function):
+    """the same outside torch.func, whose calling convention costs two signature look-ups a call (60 us)"""
+
+    @staticmethod
+    def forward(ctx, h, w, target, bias, ignore_index, reduction):
+        loss, stat = _lce_raw(h, w, target, bias, ignore_index, reduction)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        ctx.save_for_backward(h, w, target, bias, stat)
+        return loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        h, w, target, bias, stat = ctx.saved_tensors
+        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[3])
+        grad = _LinearCrossEntropyGrad.apply if torch.is_grad_enabled() else _lce_grad_raw
+        dh, dw, db = grad(h, w, target, bias, stat, dloss, ctx.ignore_index, ctx.reduction, need)
+        return dh if need[0] else None, dw if need[1] else None, None, db if need[2] else None, None, None
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     generate_vmap_rule = False
 
@@ -185,7 +204,12 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, target: Tensor, bias: Op
     b = None if bias is None else bias.contiguous()
     y = target.reshape(-1).contiguous()
     args = (h, w, y, b, int(ignore_index), reduction)
-    loss = (_LinearCrossEntropy.apply if linalg._tracked(h, w, b, y) else _lce_raw)(*args)[0]
+    if not linalg._tracked(h, w, b, y):
+        loss = _lce_raw(*args)[0]
+    elif torch._C._are_functorch_transforms_active():
+        loss = _LinearCrossEntropy.apply(*args)[0]
+    else:
+        loss = _LinearCrossEntropyEager.apply(*args)
     return loss.reshape(target.shape) if reduction == "none" else loss
 
 
