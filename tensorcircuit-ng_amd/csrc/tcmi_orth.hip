@@ -710,6 +710,409 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
   }
 }
 
+// ------------------------------------------------------------------------------- few rows, long columns: two reads of G
+// Every X of the iteration is a polynomial M of A_0 = X_0 X_0^H times X_0, so for a short side up to 64 (embedded) the steps
+// run on m x m matrices alone: one pass forms G G^H, one workgroup iterates
+//     P = a + b A + c A A,  M <- P M,  A <- P A P
+// and a second pass writes M G.  A_k is no longer formed from X_k: an error of A_0 in a direction of small singular
+// value grows by a^2 a step, 2e4 in five, so everything m x m is f64 (G G^H too: its products are exact, its sums f64).
+// The gradient alike: D_k = U_k dY + V_k X_0 with U <- P U, V <- P V + Q M,
+//     T = (U dY X_0^H + V A_0) M,  S = T + T^H,  Q = b S + c (A S + S A),
+// from one pass for dY G^H and one for U dY + V G.  Bound by the reads of G for long sides, by the chain of small f64
+// products (17 forward, 55 for the gradient) for short ones.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+
+constexpr int THIN_R = 64, THIN_GRAD_R = 32, THIN_COLS = 64, THIN_MAX_PART = 128;
+
+struct ThinArgs {
+  Mat g, dy;                     // rows = the short side
+  int m, n, cx, steps, flat, dflat, chunks, parts;
+  double coef[3 * TCMI_NS_MAX_STEPS];
+  double eps;
+  float* buf;
+  long long brs, bcs, bbs;
+  float rest;
+  int nesterov;
+  void* out;
+  long long ors, ocs, obs;
+  int dtype, update, oflat;
+  float keep, rate;
+  double* part;                  // [batch][parts][R16 R16]
+  double* norm;                  // [batch]
+  double* a0;                    // [batch][R16 R16], kept for the gradient (null: not kept)
+  double* steps_mem;             // gradient: [batch][steps][3][R16 R16] P, M, A
+  float *m1, *m2;                // [batch][R16 R16]: out = m1 G, or m1 dY + m2 G
+};
+
+__device__ __forceinline__ f64x4 mfma64(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+
+// loads columns [j0, j0 + 64) of a matrix into LDS rows of ld floats, embedded, zero outside
+template <int SRC, bool BUF>
+__device__ __forceinline__ void thin_load(float* x, int ld, const ThinArgs& a, const Mat& src, int flat, long long bz, int j0, bool momentum) {
+  const int R16 = (a.cx * a.m + 15) & ~15;
+  for (int k = threadIdx.x; k < R16 * ld; k += 256) x[k] = 0.f;
+  __syncthreads();
+  const int cols = min(THIN_COLS, a.n - j0);
+  for (int k = threadIdx.x; k < a.m * THIN_COLS; k += 256) {
+    int i, j;
+    if (flat) {
+      i = k / THIN_COLS;
+      j = k % THIN_COLS;
+    } else {
+      j = k / a.m;
+      i = k - j * a.m;
+    }
+    if (j >= cols) continue;
+    float2 v = fetch<SRC>(src.p, bz * src.bs + i * src.rs + (long long)(j0 + j) * src.cs);
+    if (BUF && a.buf) {
+      float* m = a.buf + bz * a.bbs + i * a.brs + (long long)(j0 + j) * a.bcs;
+      float nv = m[0];
+      if (momentum) {
+        nv = fmaf(a.rest, v.x - nv, nv);
+        m[0] = nv;
+      }
+      v.x = direction(v.x, nv, a.rest, a.nesterov);
+    }
+    x[i * ld + j] = v.x;
+    if (a.cx == 2) {
+      x[i * ld + j + THIN_COLS] = v.y;
+      x[(i + a.m) * ld + j] = -v.y;
+      x[(i + a.m) * ld + j + THIN_COLS] = v.x;
+    }
+  }
+  __syncthreads();
+}
+
+// partial sums of G G^H (lower tiles), or of G dY^H (all tiles)
+template <int SRC, bool GRAD>
+__global__ __launch_bounds__(256) void thin_gram_kernel(ThinArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float mem[];
+  const int R16 = (a.cx * a.m + 15) & ~15, w = a.cx * THIN_COLS, ld = w + 4, tr = R16 / 16;
+  const long long bz = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+  float *X = mem, *D = mem + R16 * ld;
+  f64x4 acc[4] = {};
+  for (int c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+    thin_load<SRC, !GRAD>(X, ld, a, a.g, a.flat, bz, c * THIN_COLS, true);
+    if (GRAD) thin_load<SRC, false>(D, ld, a, a.dy, a.dflat, bz, c * THIN_COLS, false);
+    int t = 0, u = 0;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const int i = q / 4, j = q % 4;
+      if (i >= tr || j >= tr || (!GRAD && j > i)) continue;
+      if (t++ % 4 != wave) continue;
+      const float* p = X + (i * 16 + l) * ld + 4 * g;
+      const float* s = (GRAD ? D : X) + (j * 16 + l) * ld + 4 * g;
+      f64x4 v = u == 0 ? acc[0] : u == 1 ? acc[1] : u == 2 ? acc[2] : acc[3];
+      for (int k = 0; k < w; k += 16) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(p + k), y = *reinterpret_cast<const f32x4*>(s + k);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v = mfma64((double)x[r], (double)y[r], v);
+      }
+      if (u == 0) acc[0] = v;
+      else if (u == 1) acc[1] = v;
+      else if (u == 2) acc[2] = v;
+      else acc[3] = v;
+      ++u;
+    }
+    __syncthreads();
+  }
+  double* out = a.part + (bz * gridDim.x + blockIdx.x) * R16 * R16;
+  int t = 0, u = 0;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const int i = q / 4, j = q % 4;
+    if (i >= tr || j >= tr || (!GRAD && j > i)) continue;
+    if (t++ % 4 != wave) continue;
+    const f64x4 v = u == 0 ? acc[0] : u == 1 ? acc[1] : u == 2 ? acc[2] : acc[3];
+    ++u;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = i * 16 + g + 4 * r, col = j * 16 + l;
+      out[row * R16 + col] = v[r];
+      if (!GRAD && i != j) out[col * R16 + row] = v[r];
+    }
+  }
+}
+
+constexpr int THIN_THREADS = 512;
+
+// c += sum_k p[i][k] q[j][k], rows ld doubles apart
+__device__ __forceinline__ f64x4 rows64(const double* p, const double* q, int ld, int R16, f64x4 c) {
+  const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  p += l * ld + 2 * g;
+  q += l * ld + 2 * g;
+  for (int k = 0; k < R16; k += 8) {
+    const f64x2 x = *reinterpret_cast<const f64x2*>(p + k), y = *reinterpret_cast<const f64x2*>(q + k);
+    c = mfma64(x[0], y[0], c);
+    c = mfma64(x[1], y[1], c);
+  }
+  return c;
+}
+
+// f(i0, j0) for the tiles dealt to the waves; LOWER: on and below the diagonal
+template <bool LOWER, class F>
+__device__ __forceinline__ void tiles64(int R16, F f) {
+  const int wave = threadIdx.x >> 6, t = R16 / 16;
+  int k = 0;
+  for (int i = 0; i < t; ++i)
+    for (int j = 0; j < (LOWER ? i + 1 : t); ++j, ++k)
+      if (k % (THIN_THREADS / 64) == wave) f(i * 16, j * 16);
+}
+
+template <class F>
+__device__ __forceinline__ void cells64(int i0, int j0, f64x4 v, F f) {        // f(row, col, value) of a tile's four cells
+  const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) f(i0 + g + 4 * r, j0 + l, v[r]);
+}
+
+// out = sym(p q) for commuting symmetric p, q: lower tiles, written twice
+__device__ __forceinline__ void sym64(const double* p, const double* q, double* out, int ld, int R16) {
+  tiles64<true>(R16, [&](int i0, int j0) {
+    cells64(i0, j0, rows64(p + i0 * ld, q + j0 * ld, ld, R16, f64x4{0, 0, 0, 0}), [&](int i, int j, double x) {
+      out[i * ld + j] = x;
+      out[j * ld + i] = x;
+    });
+  });
+}
+
+__device__ __forceinline__ void poly64(const double* A, double* P, int ld, int R16, double a, double b, double c) {
+  tiles64<true>(R16, [&](int i0, int j0) {
+    cells64(i0, j0, rows64(A + i0 * ld, A + j0 * ld, ld, R16, f64x4{0, 0, 0, 0}), [&](int i, int j, double x) {
+      x = c * x + b * A[i * ld + j] + (i == j ? a : 0.0);
+      P[i * ld + j] = x;
+      P[j * ld + i] = x;
+    });
+  });
+}
+
+// the iteration on m x m matrices; STEPS: P, M (before the step) and A of every step go to memory for the gradient
+template <bool STEPS>
+__device__ __forceinline__ void thin_iterate(const ThinArgs& a, double* A, double* P, double* M, double* T, int ld, int R16, long long bz) {
+  for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) M[k / R16 * ld + k % R16] = k / R16 == k % R16 ? 1.0 : 0.0;
+  for (int t = 0; t < a.steps; ++t) {
+    __syncthreads();
+    poly64(A, P, ld, R16, a.coef[3 * t], a.coef[3 * t + 1], a.coef[3 * t + 2]);
+    __syncthreads();
+    if (STEPS) {
+      double* w = a.steps_mem + (bz * a.steps + t) * 3 * R16 * R16;
+      for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) {
+        const int at = k / R16 * ld + k % R16;
+        w[k] = P[at];
+        w[R16 * R16 + k] = M[at];
+        w[2 * R16 * R16 + k] = A[at];
+      }
+      if (t + 1 == a.steps) break;
+    }
+    sym64(P, M, T, ld, R16);
+    __syncthreads();
+    double* x = M;
+    M = T;
+    T = x;
+    if (t + 1 < a.steps) {
+      sym64(P, A, T, ld, R16);
+      __syncthreads();
+      sym64(P, T, A, ld, R16);
+    }
+  }
+  __syncthreads();
+  if (!STEPS) {
+    const double n = a.norm[bz] + a.eps, inv = n == 0.0 ? 0.0 : 1.0 / n;
+    for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) a.m1[bz * R16 * R16 + k] = (float)(M[k / R16 * ld + k % R16] * inv);
+  }
+}
+
+// sum of the parts of a pass, in a fixed order
+__device__ __forceinline__ double part_sum(const ThinArgs& a, long long bz, int R16, int k) {
+  double s = 0.0;
+  const double* p = a.part + bz * a.parts * R16 * R16 + k;
+#pragma unroll 4
+  for (int i = 0; i < a.parts; ++i) s += p[(long long)i * R16 * R16];
+  return s;
+}
+
+__global__ __launch_bounds__(THIN_THREADS) void thin_poly_kernel(ThinArgs a) {
+  extern __shared__ __attribute__((aligned(16))) double mem64[];
+  __shared__ double nrm;
+  const int R = a.cx * a.m, R16 = (R + 15) & ~15, ld = R16 + 2, sz = R16 * ld;
+  const long long bz = blockIdx.x;
+  double *A = mem64, *P = A + sz, *M = P + sz, *T = M + sz;
+  for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) A[k / R16 * ld + k % R16] = part_sum(a, bz, R16, k);
+  __syncthreads();
+  if (threadIdx.x < 64) {                     // |G|^2 is the trace (of the upper block)
+    double s = threadIdx.x < a.m ? A[threadIdx.x * ld + threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (threadIdx.x == 0) {
+      nrm = sqrt(s);
+      a.norm[bz] = nrm;
+    }
+  }
+  __syncthreads();
+  const double n = nrm + a.eps, inv = n == 0.0 ? 0.0 : 1.0 / (n * n);
+  for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) {
+    double& x = A[k / R16 * ld + k % R16];
+    x *= inv;
+    if (a.a0) a.a0[bz * R16 * R16 + k] = x;
+  }
+  thin_iterate<false>(a, A, P, M, T, ld, R16, bz);
+}
+
+__global__ __launch_bounds__(THIN_THREADS) void thin_grad_poly_kernel(ThinArgs a) {
+  extern __shared__ __attribute__((aligned(16))) double mem64[];
+  __shared__ double tr;
+  const int R = a.cx * a.m, R16 = (R + 15) & ~15, ld = R16 + 2, sz = R16 * ld, q2 = R16 * R16;
+  const long long bz = blockIdx.x;
+  double *A0 = mem64, *Wt = A0 + sz, *U = Wt + sz, *V = U + sz, *Vt = V + sz, *P = Vt + sz, *M = P + sz, *A = M + sz, *Z = A + sz, *S = Z + sz,
+         *Q = S + sz;
+  const double nr = a.norm[bz], n = nr + a.eps, inv = n == 0.0 ? 0.0 : 1.0 / n;
+  for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
+    const int i = k / R16, j = k % R16, at = i * ld + j;
+    A0[at] = A[at] = a.a0[bz * q2 + k];
+    Wt[at] = part_sum(a, bz, R16, k) * inv;        // G dY^H / N = (dY X_0^H)^H
+    U[at] = i == j ? 1.0 : 0.0;
+    V[at] = Vt[at] = 0.0;
+  }
+  __syncthreads();
+  thin_iterate<true>(a, A, P, M, Z, ld, R16, bz);
+  const f64x4 zero = {0, 0, 0, 0};
+  for (int t = a.steps - 1; t >= 0; --t) {
+    const double* w = a.steps_mem + (bz * a.steps + t) * 3 * q2;
+    const double b = a.coef[3 * t + 1], c = a.coef[3 * t + 2];
+    __syncthreads();
+    for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
+      const int at = k / R16 * ld + k % R16;
+      P[at] = w[k];
+      M[at] = w[q2 + k];
+      A[at] = w[2 * q2 + k];
+    }
+    __syncthreads();
+    tiles64<false>(R16, [&](int i0, int j0) {      // Z = U W + V A_0
+      f64x4 v = rows64(U + i0 * ld, Wt + j0 * ld, ld, R16, zero);
+      v = rows64(V + i0 * ld, A0 + j0 * ld, ld, R16, v);
+      cells64(i0, j0, v, [&](int i, int j, double x) { Z[i * ld + j] = x; });
+    });
+    __syncthreads();
+    tiles64<false>(R16, [&](int i0, int j0) {      // Q holds T = Z M for the moment
+      cells64(i0, j0, rows64(Z + i0 * ld, M + j0 * ld, ld, R16, zero), [&](int i, int j, double x) { Q[i * ld + j] = x; });
+    });
+    __syncthreads();
+    for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
+      const int i = k / R16, j = k % R16;
+      S[i * ld + j] = Q[i * ld + j] + Q[j * ld + i];
+    }
+    __syncthreads();
+    tiles64<true>(R16, [&](int i0, int j0) {       // Q = b S + c (A S + S A)
+      f64x4 v = rows64(A + i0 * ld, S + j0 * ld, ld, R16, zero);
+      v = rows64(S + i0 * ld, A + j0 * ld, ld, R16, v);
+      cells64(i0, j0, v, [&](int i, int j, double x) {
+        x = c * x + b * S[i * ld + j];
+        Q[i * ld + j] = x;
+        Q[j * ld + i] = x;
+      });
+    });
+    __syncthreads();
+    sym64(P, U, Z, ld, R16);                       // U <- P U
+    tiles64<false>(R16, [&](int i0, int j0) {      // V <- P V + Q M, kept with its transpose
+      f64x4 v = rows64(P + i0 * ld, Vt + j0 * ld, ld, R16, zero);
+      v = rows64(Q + i0 * ld, M + j0 * ld, ld, R16, v);
+      cells64(i0, j0, v, [&](int i, int j, double x) { S[i * ld + j] = x; });
+    });
+    __syncthreads();
+    for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
+      const int i = k / R16, j = k % R16;
+      V[i * ld + j] = S[i * ld + j];
+      Vt[j * ld + i] = S[i * ld + j];
+      U[i * ld + j] = Z[i * ld + j];
+    }
+  }
+  __syncthreads();
+  // <D, X_0> = trace of U W + V A_0 (half of the embedded one)
+  double s = 0.0;
+  for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
+    const int i = k / R16, j = k % R16;
+    s += U[i * ld + j] * Wt[i * ld + j] + V[i * ld + j] * A0[i * ld + j];
+  }
+  __shared__ double red[THIN_THREADS / 64];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int k = 0; k < THIN_THREADS / 64; ++k) s += red[k];
+    tr = s / a.cx;
+  }
+  __syncthreads();
+  // dG = D / N - G <D, G> / (N^2 |G|), D = U dY + V G / N, <D, G> = N <D, X_0>
+  const double f = nr == 0.0 ? 0.0 : tr * inv / nr;
+  for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
+    const int i = k / R16, j = k % R16;
+    a.m1[bz * q2 + k] = (float)(U[i * ld + j] * inv);
+    a.m2[bz * q2 + k] = (float)(V[i * ld + j] * inv * inv - (i == j ? f : 0.0));
+  }
+}
+
+// out = m1 G, or m1 dY + m2 G, 64 columns a workgroup
+template <int SRC, bool GRAD>
+__global__ __launch_bounds__(256) void thin_apply_kernel(ThinArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float mem[];
+  const int R16 = (a.cx * a.m + 15) & ~15, M16 = (a.m + 15) & ~15, w = a.cx * THIN_COLS, ld = w + 4, ldm = R16 + 4;
+  const long long bz = blockIdx.y;
+  const int j0 = blockIdx.x * THIN_COLS, wave = threadIdx.x >> 6, tc = w / 16, tiles = tc * (M16 / 16);
+  float *X = mem, *M1 = X + R16 * ld, *D = M1 + R16 * ldm, *M2 = D + R16 * ld;
+  for (int k = threadIdx.x; k < R16 * R16; k += 256) {
+    M1[k / R16 * ldm + k % R16] = a.m1[bz * R16 * R16 + k];
+    if (GRAD) M2[k / R16 * ldm + k % R16] = a.m2[bz * R16 * R16 + k];
+  }
+  thin_load<SRC, !GRAD>(X, ld, a, a.g, a.flat, bz, j0, false);
+  if (GRAD) thin_load<SRC, false>(D, ld, a, a.dy, a.dflat, bz, j0, false);
+  f32x4 res[8];                                    // at most 64 x 128 results: 32 tiles, 8 a wave
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int t = wave + u * 4;
+    if (t >= tiles) continue;
+    const int i0 = t / tc * 16, c0 = t % tc * 16;
+    f32x4 v = rows_cols((GRAD ? M2 : M1) + i0 * ldm, ldm, X + c0, ld, R16, f32x4{0.f, 0.f, 0.f, 0.f});
+    if (GRAD) v = rows_cols(M1 + i0 * ldm, ldm, D + c0, ld, R16, v);
+    res[u] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int t = wave + u * 4;
+    if (t >= tiles) continue;
+    float* p = X + (t / tc * 16 + 4 * ((threadIdx.x & 63) >> 4)) * ld + t % tc * 16 + (threadIdx.x & 15);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r * ld] = res[u][r];
+  }
+  __syncthreads();
+  const int cols = min(THIN_COLS, a.n - j0);
+  for (int k = threadIdx.x; k < a.m * THIN_COLS; k += 256) {
+    int i, j;
+    if (a.oflat) {
+      i = k / THIN_COLS;
+      j = k % THIN_COLS;
+    } else {
+      j = k / a.m;
+      i = k - j * a.m;
+    }
+    if (j >= cols) continue;
+    const float x = X[i * ld + j];
+    const long long at = bz * a.obs + i * a.ors + (long long)(j0 + j) * a.ocs;
+    if (SRC == SRC_C64) {
+      ((float2*)a.out)[at] = make_float2(x, X[i * ld + j + THIN_COLS]);
+    } else if (!GRAD && a.update) {
+      const float old = SRC == SRC_F32 ? ((float*)a.out)[at] : SRC == SRC_F16 ? (float)((f16*)a.out)[at] : (float)((__bf16*)a.out)[at];
+      put(a.out, a.dtype, at, fmaf(a.rate, x, a.keep * old));
+    } else {
+      put(a.out, a.dtype, at, x);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------- host side
 struct Shape {
   int m, n;                       // min, max of the caller's two dimensions
@@ -1118,6 +1521,121 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
   return hipSuccess;
 }
 
+// ---- few rows, long columns
+bool thin_fits(const Shape& s, bool grad) { return s.mr <= (grad ? THIN_GRAD_R : THIN_R); }
+
+int thin_r16(const Shape& s) { return (s.mr + 15) & ~15; }
+
+int thin_chunks(const Shape& s) { return (s.n + THIN_COLS - 1) / THIN_COLS; }
+
+// workgroups of a pass over the columns: enough for the card, few enough that one workgroup adds their sums quickly
+int thin_parts(const Shape& s) {
+  const int r = thin_r16(s);
+  int most = r <= 16 ? THIN_MAX_PART : r <= 32 ? 64 : 32;
+  const int room = (512 + s.batch - 1) / s.batch, c = thin_chunks(s);
+  if (most > room) most = room < 4 ? 4 : room;
+  return c < most ? c : most;
+}
+
+struct ThinWork {
+  double *part, *norm, *steps;
+  float *m1, *m2;
+};
+
+ThinWork take_thin(Arena& w, const Shape& s, bool grad, int steps) {
+  ThinWork k{};
+  const long long q = (long long)thin_r16(s) * thin_r16(s) * s.batch;
+  k.part = w.take<double>(q * thin_parts(s));
+  k.norm = w.take<double>(s.batch);
+  k.m1 = w.take<float>(q);
+  if (grad) {
+    k.m2 = w.take<float>(q);
+    k.steps = w.take<double>(3 * q * steps);
+  }
+  return k;
+}
+
+struct ThinSaved {
+  double *norm, *a0;
+};
+
+ThinSaved take_thin_saved(Arena& w, const Shape& s) {
+  ThinSaved v;
+  v.norm = w.take<double>(s.batch);
+  v.a0 = w.take<double>((long long)thin_r16(s) * thin_r16(s) * s.batch);
+  return v;
+}
+
+ThinArgs thin_args(const Shape& s, const Problem& q, const ThinWork& w) {
+  ThinArgs a{};
+  a.g = q.g;
+  a.m = s.m;
+  a.n = s.n;
+  a.cx = s.cx;
+  a.steps = q.steps;
+  a.flat = q.g.cs <= q.g.rs;
+  a.oflat = q.ocs <= q.ors;
+  a.chunks = thin_chunks(s);
+  a.parts = thin_parts(s);
+  for (int i = 0; i < 3 * q.steps; ++i) a.coef[i] = q.coef[i];
+  a.eps = q.eps;
+  a.buf = q.buf;
+  a.brs = q.brs;
+  a.bcs = q.bcs;
+  a.bbs = q.bbs;
+  a.rest = q.rest;
+  a.nesterov = q.nesterov;
+  a.out = q.out;
+  a.ors = q.ors;
+  a.ocs = q.ocs;
+  a.obs = q.obs;
+  a.dtype = q.dtype;
+  a.update = q.buf != nullptr;
+  a.keep = q.keep;
+  a.rate = q.rate;
+  a.part = w.part;
+  a.norm = w.norm;
+  a.m1 = w.m1;
+  a.m2 = w.m2;
+  a.steps_mem = w.steps;
+  return a;
+}
+
+template <int SRC, bool GRAD>
+hipError_t thin_launch(const Shape& s, const ThinArgs& a, hipStream_t st) {
+  const int r = thin_r16(s), ld = s.cx * THIN_COLS + 4, gram = (GRAD ? 2 : 1) * r * ld * 4, apply = (GRAD ? 2 : 1) * r * (ld + r + 4) * 4,
+            poly = (GRAD ? 11 : 4) * r * (r + 2) * 8;
+  static bool raised = false;
+  if (!raised) {
+    const int most = THIN_R * (2 * THIN_COLS + 4) * 4 + THIN_R * (THIN_R + 4) * 4;
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(thin_gram_kernel<SRC, GRAD>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == hipSuccess)
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(thin_apply_kernel<SRC, GRAD>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == hipSuccess)
+      e = hipFuncSetAttribute(GRAD ? reinterpret_cast<const void*>(thin_grad_poly_kernel) : reinterpret_cast<const void*>(thin_poly_kernel),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS);
+    if (e != hipSuccess) return e;
+    raised = true;
+  }
+  hipLaunchKernelGGL((thin_gram_kernel<SRC, GRAD>), dim3(a.parts, s.batch), dim3(256), gram, st, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if (GRAD) hipLaunchKernelGGL(thin_grad_poly_kernel, dim3(s.batch), dim3(THIN_THREADS), poly, st, a);
+  else hipLaunchKernelGGL(thin_poly_kernel, dim3(s.batch), dim3(THIN_THREADS), poly, st, a);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((thin_apply_kernel<SRC, GRAD>), dim3(a.chunks, s.batch), dim3(256), apply, st, a);
+  return hipGetLastError();
+}
+
+template <bool GRAD>
+hipError_t thin(const Shape& s, int src, const ThinArgs& a, hipStream_t st) {
+  if (src == SRC_F32) return thin_launch<SRC_F32, GRAD>(s, a, st);
+  if (src == SRC_F16) return thin_launch<SRC_F16, GRAD>(s, a, st);
+  if (src == SRC_BF16) return thin_launch<SRC_BF16, GRAD>(s, a, st);
+  return thin_launch<SRC_C64, GRAD>(s, a, st);
+}
+
 hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
   return s.P == 2 ? forward<2>(s, q, sc, w, sv, st) : forward<1>(s, q, sc, w, sv, st);
 }
@@ -1242,6 +1760,11 @@ long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full,
     else a.take<char>(1);
     return a.used;
   }
+  if (thin_fits(s, what != TCMI_NS_WORK)) {
+    if (what == TCMI_NS_SAVED) take_thin_saved(a, s);
+    else take_thin(a, s, what == TCMI_NS_WORK_GRAD, steps);
+    return a.used;
+  }
   if (what == TCMI_NS_WORK) take_work(a, s, false);
   else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true);
   else if (what == TCMI_NS_SAVED) take_saved(a, s, steps);
@@ -1255,14 +1778,24 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
   if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !out || !coef_host || !work || !(eps >= 0) || (saved && !full))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
+  // three forms: one workgroup per matrix; two passes around m x m matrices; a sequence of large products
   const int small = small_bytes(s, saved != nullptr);
+  const bool narrow = !small && thin_fits(s, saved != nullptr);
   Arena aw{(char*)work}, av{(char*)saved};
   Work w{};
   Saved sv{};
   SmallSaved ss{};
-  if (!small) w = take_work(aw, s, saved != nullptr);
-  if (saved && small) ss = take_small(av, s, steps);
-  if (saved && !small) sv = take_saved(av, s, steps);
+  ThinWork tw{};
+  ThinSaved ts{};
+  if (small) {
+    if (saved) ss = take_small(av, s, steps);
+  } else if (narrow) {
+    tw = take_thin(aw, s, false, steps);
+    if (saved) ts = take_thin_saved(av, s);
+  } else {
+    w = take_work(aw, s, saved != nullptr);
+    if (saved) sv = take_saved(av, s, steps);
+  }
   if (aw.used > work_bytes || (saved && av.used > saved_bytes) || ((uintptr_t)work & 255) || ((uintptr_t)saved & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: workspace too small or not 256-byte aligned");
   Scales sc[TCMI_NS_MAX_STEPS];
@@ -1285,6 +1818,11 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
     a.saved = ss.x;
     a.norm = ss.norm;
     e = small_by_type<false>(q.src, a, small, batch, reinterpret_cast<hipStream_t>(stream));
+  } else if (narrow) {
+    ThinArgs a = thin_args(s, q, tw);
+    a.a0 = ts.a0;
+    if (saved) a.norm = ts.norm;
+    e = thin<false>(s, q.src, a, reinterpret_cast<hipStream_t>(stream));
   } else {
     e = forward(s, q, sc, w, saved ? &sv : nullptr, reinterpret_cast<hipStream_t>(stream));
   }
@@ -1300,11 +1838,17 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
   const Shape s = shape_of(rows, cols, batch, dtype, true);
   Arena aw{(char*)work}, av{(char*)const_cast<void*>(saved)};
   const int small = small_bytes(s, true);
+  const bool narrow = !small && thin_fits(s, true);
   GradWork w{};
   Saved sv{};
   SmallSaved ss{};
+  ThinWork tw{};
+  ThinSaved ts{};
   if (small) {
     ss = take_small(av, s, steps);
+  } else if (narrow) {
+    tw = take_thin(aw, s, true, steps);
+    ts = take_thin_saved(av, s);
   } else {
     w = take_grad(aw, s);
     sv = take_saved(av, s, steps);
@@ -1332,6 +1876,13 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
     a.saved = ss.x;
     a.norm = ss.norm;
     e = small_by_type<true>(q.src, a, small, batch, reinterpret_cast<hipStream_t>(stream));
+  } else if (narrow) {
+    ThinArgs a = thin_args(s, q, tw);
+    a.dy = oriented(dout, d_rs, d_cs, d_bs, s.flip);
+    a.dflat = a.dy.cs <= a.dy.rs;
+    a.a0 = ts.a0;
+    a.norm = ts.norm;
+    e = thin<true>(s, q.src, a, reinterpret_cast<hipStream_t>(stream));
   } else {
     e = backward(s, q, oriented(dout, d_rs, d_cs, d_bs, s.flip), sc, w, sv, reinterpret_cast<hipStream_t>(stream));
   }
@@ -1347,9 +1898,12 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
   const int small = small_bytes(s, false);
+  const bool narrow = !small && thin_fits(s, false);
   Arena aw{(char*)work};
   Work w{};
-  if (!small) w = take_work(aw, s, false);
+  ThinWork tw{};
+  if (narrow) tw = take_thin(aw, s, false, steps);
+  else if (!small) w = take_work(aw, s, false);
   if (aw.used > work_bytes || ((uintptr_t)work & 255))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: workspace too small or not 256-byte aligned");
   Scales sc[TCMI_NS_MAX_STEPS];
@@ -1374,8 +1928,9 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
   q.nesterov = nesterov;
   q.keep = (float)keep;
   q.rate = (float)rate;
-  const hipError_t e = small ? small_by_type<false>(q.src, small_args(s, q), small, batch, reinterpret_cast<hipStream_t>(stream))
-                             : forward(s, q, sc, w, nullptr, reinterpret_cast<hipStream_t>(stream));
+  const hipError_t e = small    ? small_by_type<false>(q.src, small_args(s, q), small, batch, reinterpret_cast<hipStream_t>(stream))
+                       : narrow ? thin<false>(s, q.src, thin_args(s, q, tw), reinterpret_cast<hipStream_t>(stream))
+                                : forward(s, q, sc, w, nullptr, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
 }
 

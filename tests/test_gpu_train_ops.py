@@ -57,7 +57,8 @@ def _ns_tol(dtype, steps=5):
     return f32 + HALF_STEP[dtype] + (3 * steps * 2.2 * 2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
 
 
-SHAPES = [(1, 1), (1, 7), (9, 1), (3, 3), (24, 28), (63, 65), (64, 64), (65, 130), (130, 65), (128, 256), (200, 129), (129, 511)]
+SHAPES = [(1, 1), (1, 7), (9, 1), (3, 3), (24, 28), (63, 65), (64, 64), (65, 130), (130, 65), (128, 256), (200, 129), (129, 511),
+          (1, 3000), (7, 1500), (2000, 16), (40, 900), (33, 1100), (64, 777)]
 DTYPES = [torch.float32, torch.float16, torch.bfloat16, torch.complex64]
 
 
@@ -110,7 +111,7 @@ def test_newton_schulz_converges_to_the_polar_factor():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.complex64])
-@pytest.mark.parametrize("shape", [(20, 30), (150, 140)])
+@pytest.mark.parametrize("shape", [(20, 30), (10, 1500), (150, 140)])
 def test_newton_schulz_special_values(shape, dtype):
     from tcmi import linalg
 
@@ -141,7 +142,8 @@ def _ns_grad_tol(x, dy, want, dtype, eps=1e-7):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (24, 28), (64, 64), (130, 65), (129, 200)])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (9, 1), (24, 28), (64, 64), (130, 65), (129, 200),
+                                   (1, 3000), (7, 1500), (2000, 16), (31, 700), (1100, 40)])
 def test_newton_schulz_grad(shape, dtype):
     from tcmi import linalg
 
@@ -415,7 +417,7 @@ def _muon64(p, g, v, lr, wd, mu, nesterov, r, coef=DEFAULT, eps=1e-7):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("shape", [(24, 28), (1, 5), (200, 70), (70, 200), (3, 40, 30), (2, 2, 130, 64)])
+@pytest.mark.parametrize("shape", [(24, 28), (1, 5), (9, 2000), (1500, 60), (200, 70), (70, 200), (3, 40, 30), (2, 2, 130, 64)])
 def test_muon_step(shape, dtype):
     from tcmi import torchnn
 
