@@ -396,7 +396,7 @@ int tcmi_comm_destroy(void* comm);
  * Newton-Schulz orthogonalisation: N = |G|_F + eps, X = G / N, then `steps` times A = X X^H, X <- a X + (b A + c A A) X with
  * (a, b, c) = coef_host[3 i .. 3 i + 2] (host memory, float64).  g: [batch] matrices of rows x cols with element strides
  * rs / cs / bs; out: contiguous, same dtype (TCMI_F32, TCMI_F16, TCMI_BF16 or TCMI_C64).  full = 1: two f16 pieces per
- * operand (f32 accuracy), 0: one (results of bf16 accuracy).  saved (full only, may be NULL): what the gradient needs.
+ * operand (f32 accuracy), 0: one (TCMI_BF16 only).  saved (full only, may be NULL): what the gradient needs.
  * Coefficients that let a singular value grow past 64 are refused.  Workspaces: tcmi_ns_work_bytes(.., what) bytes,
  * 256-byte aligned, contents undefined; nothing is kept in them between calls.  A matrix with a non-finite entry gives NaN.
  * No counterpart in the reference, whose orthogonal factors come from its backends' svd / qr

@@ -259,7 +259,7 @@ __device__ __forceinline__ void logits(const Logits& q, const Args& g, int m0, i
 
 // forward: per row the tile's maximum and sum of exponentials, and the target's logit where it lies in the tile
 struct EpiLse {
-  static constexpr bool WHOLE = true;
+  static constexpr bool TILE = true, FOUR = false;
   template <class T>
   static constexpr int lds() { return T::WN * T::BM * 8; }
   Logits q;
@@ -267,7 +267,7 @@ struct EpiLse {
   float* target;                 // [T]
   const long long* y;
   template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
+  __device__ void tile(const Args& g, int m0, int n0, int, bool, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
     logits<T>(q, g, m0, n0, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
     float2* stat = reinterpret_cast<float2*>(lds);                    // [WN][BM]
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(1024) void rowstat_total_kernel(const float2* part,
 // backward: P as f16 pieces, row-major for dh and transposed for dw, zero in the padding and in ignored rows
 template <int P>
 struct EpiProb {
-  static constexpr bool WHOLE = true;
+  static constexpr bool TILE = true, FOUR = false;
   Logits q;
   const float* lse;
   const long long* y;
@@ -410,16 +410,13 @@ struct EpiProb {
   int V;
   f16 *p, *pt;                   // [T][P * vp], [classes][P * tp]
   int vp, tp;                    // padded classes of the piece, padded rows
-  // the transposed tile, its rows 8 elements longer than the tile: 16-byte aligned, no bank conflicts
   template <class T>
-  static constexpr int line() { return T::BM + 8; }
-  template <class T>
-  static constexpr int lds() { return P * T::BN * line<T>() * 2; }
+  static constexpr int lds() { return Transposed<T, P>::BYTES; }
   // P goes out from the registers, eight bytes a lane; P^T through LDS, sixteen (from the registers it would be two: 1021 x
   // 28 x 16384 f32 took 50 us)
   template <class T>
-  __device__ void tile(const Args& g, int m0, int n0, int, char* lds_bytes, f32x4 (&acc)[T::MI][T::NI]) const {
-    f16* lt = reinterpret_cast<f16*>(lds_bytes);
+  __device__ void tile(const Args& g, int m0, int n0, int, bool, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
+    const Transposed<T, P> turned{reinterpret_cast<f16*>(lds)};
     logits<T>(q, g, m0, n0, acc);
     __syncthreads();
     each<T>(m0, n0, acc, [&](int row, int col, f32x4 x) {
@@ -442,28 +439,17 @@ struct EpiProb {
         vl[r] = b;
       }
       if (in && col < vp) store_four<P>(p + (long long)row * P * vp, col, vh, vl);
-      f16* o = lt + (col - n0) * line<T>() + row - m0;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        o[r * line<T>()] = vh[r];
-        if (P == 2) o[(T::BN + r) * line<T>()] = vl[r];
-      }
+      turned.stage(row - m0, col - n0, vh, vl);
     });
     __syncthreads();
-    for (int k = threadIdx.x; k < T::BN * (T::BM / 8); k += T::THREADS) {
-      const int c = k / (T::BM / 8), rl = k % (T::BM / 8) * 8, row = m0 + rl;
-      if (n0 + c >= g.N || row >= tp) continue;
-      f16* o = pt + (long long)(n0 + c) * P * tp + kpos<P>(row);
-      *reinterpret_cast<f16x8*>(o) = *reinterpret_cast<const f16x8*>(lt + c * line<T>() + rl);
-      if (P == 2) *reinterpret_cast<f16x8*>(o + 32) = *reinterpret_cast<const f16x8*>(lt + (T::BN + c) * line<T>() + rl);
-    }
+    turned.flush(pt, (long long)P * tp, n0, g.N, m0, tp);
   }
 };
 
 // a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor;
 // a column behind the last one is the bias's gradient
 struct EpiGrad {
-  static constexpr bool WHOLE = false;
+  static constexpr bool TILE = false, FOUR = true;
   const float* inv;              // inverse of the other operand's scale, on the device
   float* sum;                    // f32 [rows][cols] (null: only one piece)
   int first, last;

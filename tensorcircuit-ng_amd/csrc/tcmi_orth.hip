@@ -298,23 +298,24 @@ __global__ __launch_bounds__(256) void clear_kernel(uint4* p, long long n) {
 }
 
 // A symmetric result as f16 pieces: value = alpha acc + beta src, stored times `scale`; a tile below the diagonal also
-// writes its mirror image.  Columns up to the padded width get zeros.
+// writes its mirror image (through LDS where the product is not split: two bytes a lane took 15 us of 85 at 4096 x 4096).
+// Columns up to the padded width get zeros.
 template <int P>
 struct EpiSym {
-  static constexpr bool WHOLE = false;
+  static constexpr bool TILE = true, FOUR = true;
   f16* out;
   const f16* src;
   long long ld, bs;
   float alpha, beta, scale;
-  __device__ __forceinline__ void four(const Args& g, int bz, bool mirror, int row, int col, f32x4 v) const {
-    const int wide = (int)kpad(g.M, P);
+  template <class T>
+  static constexpr int lds() { return Transposed<T, P>::BYTES; }
+  __device__ __forceinline__ void put_row(const Args& g, int bz, int wide, int row, int col, f32x4 v, f16x4& vh, f16x4& vl) const {
     const bool in = row < g.M && col < wide;
-    f16* o = out + bz * bs;
-    f16x4 s4 = {}, t4 = {}, vh, vl;
+    const long long at = bz * bs + row * ld + kpos<P>(col);
+    f16x4 s4 = {}, t4 = {};
     if (src && in) {
-      const f16* s = src + bz * bs + row * ld + kpos<P>(col);
-      s4 = *reinterpret_cast<const f16x4*>(s);
-      if (P == 2) t4 = *reinterpret_cast<const f16x4*>(s + 32);
+      s4 = *reinterpret_cast<const f16x4*>(src + at);
+      if (P == 2) t4 = *reinterpret_cast<const f16x4*>(src + at + 32);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -325,22 +326,44 @@ struct EpiSym {
       vh[r] = a;
       vl[r] = b;
     }
-    if (in) store_four<P>(o + row * ld, col, vh, vl);
+    if (in) {
+      *reinterpret_cast<f16x4*>(out + at) = vh;
+      if (P == 2) *reinterpret_cast<f16x4*>(out + at + 32) = vl;
+    }
+  }
+  __device__ __forceinline__ void four(const Args& g, int bz, bool mirror, int row, int col, f32x4 v) const {
+    const int wide = (int)kpad(g.M, P);
+    f16x4 vh, vl;
+    put_row(g, bz, wide, row, col, v, vh, vl);
     if (mirror && row < wide) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         if (col + r < g.M) {
-          f16* p = o + (col + r) * ld + kpos<P>(row);
+          f16* p = out + bz * bs + (col + r) * ld + kpos<P>(row);
           p[0] = vh[r];
           if (P == 2) p[32] = vl[r];
         }
     }
   }
+  template <class T>
+  __device__ __forceinline__ void tile(const Args& g, int m0, int n0, int bz, bool mirror, char* mem, f32x4 (&acc)[T::MI][T::NI]) const {
+    const int wide = (int)kpad(g.M, P);
+    const Transposed<T, P> turned{reinterpret_cast<f16*>(mem)};
+    __syncthreads();
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
+      f16x4 vh, vl;
+      put_row(g, bz, wide, row, col, v, vh, vl);
+      if (mirror) turned.stage(row - m0, col - n0, vh, vl);
+    });
+    if (!mirror) return;
+    __syncthreads();
+    turned.flush(out + bz * bs, ld, n0, g.M, m0, wide);
+  }
 };
 
 // carry <- beta carry + alpha acc (f32, in place: a thread reads and writes the same element)
 struct EpiCarry {
-  static constexpr bool WHOLE = false;
+  static constexpr bool TILE = false, FOUR = true;
   float* carry;
   long long ld, bs;
   float alpha, beta;
@@ -362,38 +385,73 @@ struct EpiCarry {
   }
 };
 
-// the last step: x = beta carry + alpha acc goes to the caller's matrix (out = x) or into a weight (out = keep out + rate x)
+// The last step: x = beta X + alpha acc goes to the caller's matrix (out = x) or into a weight (out = keep out + rate x).
+// P = 0: X is the f32 carry.  P > 0: the product is the transposed one, T B, so that a matrix taller than wide is written along
+// its rows too, and X comes from T's pieces (one piece, 2^-11 of X in the last step, is below what one-piece products cost).
+template <int P, int DT>
 struct EpiOut {
-  static constexpr bool WHOLE = false;
-  const float* carry;
+  static constexpr bool TILE = false, FOUR = true;
+  const void* src;               // f32 carry, or T
   long long ld, bs;
   float alpha, beta;
   void* out;
   long long rs, cs, os;
-  int dtype, n;                  // n: columns; complex: columns of the imaginary part start there
+  int n;                         // columns; complex: columns of the imaginary part start there
   int update;
   float keep, rate;
+  int vec;                       // rows contiguous and aligned for four elements
+  __device__ __forceinline__ float old_x(long long row, int j) const {
+    if constexpr (P == 0) return ((const float*)src)[row + j];
+    const f16* p = (const f16*)src + row + kpos<P>(j);
+    return P == 2 ? (float)p[0] + (float)p[32] : (float)p[0];
+  }
   __device__ __forceinline__ void four(const Args& g, int bz, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
-    const float* c = carry + bz * bs + row * ld;
+    const long long line = bz * bs + row * ld;
+    if (DT != TCMI_C64 && vec && col + 3 < g.N) {                    // four neighbours of a row-major matrix at once
+      f32x4 x;
+      if constexpr (P == 0) {
+        x = *reinterpret_cast<const f32x4*>((const float*)src + line + col);
+      } else {
+        const f16* p = (const f16*)src + line + kpos<P>(col);
+        x = __builtin_convertvector(*reinterpret_cast<const f16x4*>(p), f32x4);
+        if (P == 2) x += __builtin_convertvector(*reinterpret_cast<const f16x4*>(p + 32), f32x4);
+      }
+      const long long at = bz * os + row * rs + col;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = fmaf(alpha, v[r], beta * x[r]);
+      if constexpr (DT == TCMI_F32) out4<f32x4>((float*)out + at, x);
+      else if constexpr (DT == TCMI_F16) out4<f16x4>((f16*)out + at, x);
+      else if constexpr (DT == TCMI_BF16) out4<bf16x4>((__bf16*)out + at, x);
+      return;
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int j = col + r;
       if (j >= g.N) continue;
-      const float x = fmaf(alpha, v[r], beta * c[j]);
-      if (dtype == TCMI_C64) {
+      const float x = fmaf(alpha, v[r], beta * old_x(line, j));
+      if constexpr (DT == TCMI_C64) {
         const int im = j >= n;
         ((float*)out)[2 * (bz * os + row * rs + (j - im * n) * cs) + im] = x;
       } else {
         const long long at = bz * os + row * rs + j * cs;
         if (update) {
-          const float old = dtype == TCMI_F32 ? ((float*)out)[at] : dtype == TCMI_F16 ? (float)((f16*)out)[at] : (float)((__bf16*)out)[at];
-          put(out, dtype, at, fmaf(rate, x, keep * old));
+          const float old = DT == TCMI_F32 ? ((float*)out)[at] : DT == TCMI_F16 ? (float)((f16*)out)[at] : (float)((__bf16*)out)[at];
+          put(out, DT, at, fmaf(rate, x, keep * old));
         } else {
-          put(out, dtype, at, x);
+          put(out, DT, at, x);
         }
       }
     }
+  }
+  template <class V4, class E>
+  __device__ __forceinline__ void out4(E* p, f32x4 x) const {
+    if (update) {
+      const f32x4 old = __builtin_convertvector(*reinterpret_cast<const V4*>(p), f32x4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = fmaf(rate, x[r], keep * old[r]);
+    }
+    *reinterpret_cast<V4*>(p) = __builtin_convertvector(x, V4);
   }
 };
 
@@ -1404,19 +1462,16 @@ hipError_t small_by_type(int src, const SmallArgs& a, int bytes, int batch, hipS
     if (e_ != hipSuccess) return e_;             \
   } while (0)
 
-// A, B and the update of one step from the pieces of X; the update's epilogue is the caller's
-template <int P, class Epi>
-hipError_t ns_step(const Shape& s, const Pieces& p, const Scales& c, const double* co, float* split, const Epi& last, hipStream_t st) {
-  const long long xs = s.mr * s.np, ts = s.nc * s.mp, qs = s.mr * s.mp;
+// A, B of one step from the pieces of X
+template <int P>
+hipError_t ns_factor(const Shape& s, const Pieces& p, const Scales& c, const double* co, float* split, hipStream_t st) {
+  const long long xs = s.mr * s.np, qs = s.mr * s.mp;
   Args g = base_args(s, split, s.mr, s.mr, s.np, s.np, xs, xs);
   pair(g, p.x, p.x);
   TRY(run<P>(g, true, EpiSym<P>{p.a, nullptr, s.mp, qs, 1.f / (c.x * c.x), 0.f, c.A}, st));
   g = base_args(s, split, s.mr, s.mr, s.mp, s.mp, qs, qs);
   pair(g, p.a, p.a);
-  TRY(run<P>(g, true, EpiSym<P>{p.b, p.a, s.mp, qs, (float)co[2] / (c.A * c.A), (float)co[1] / c.A, c.B}, st));
-  g = base_args(s, split, s.m, s.nc, s.mp, s.mp, qs, ts);
-  pair(g, p.b, p.t);
-  return run<P>(g, false, last, st);
+  return run<P>(g, true, EpiSym<P>{p.b, p.a, s.mp, qs, (float)co[2] / (c.A * c.A), (float)co[1] / c.A, c.B}, st);
 }
 
 struct Problem {
@@ -1509,14 +1564,39 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
       a.src = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
       TRY(launch_pack<P>(SRC_PLANAR, a, s, st));
     }
+    TRY(ns_factor<P>(s, p, sc[i], q.coef + 3 * i, w.split, st));
     const float alpha = 1.f / (sc[i].B * sc[i].x), beta = (float)q.coef[3 * i];
+    const long long ts = s.nc * s.mp, qs = s.mr * s.mp, cs = s.m * s.ldc;
     if (i + 1 < q.steps) {
-      EpiCarry e{w.carry, s.ldc, s.m * s.ldc, alpha, beta, nullptr};
-      TRY(ns_step<P>(s, p, sc[i], q.coef + 3 * i, w.split, e, st));
-    } else {
-      EpiOut e{w.carry, s.ldc, s.m * s.ldc, alpha, beta, q.out, q.ors, q.ocs, q.obs, q.dtype, s.n, q.buf != nullptr, q.keep, q.rate};
-      TRY(ns_step<P>(s, p, sc[i], q.coef + 3 * i, w.split, e, st));
+      Args g = base_args(s, w.split, s.m, s.nc, s.mp, s.mp, qs, ts);
+      pair(g, p.b, p.t);
+      TRY(run<P>(g, false, EpiCarry{w.carry, s.ldc, cs, alpha, beta, nullptr}, st));
+      continue;
     }
+    const int size = q.dtype == TCMI_F32 ? 4 : 2, up = q.buf != nullptr;
+    hipError_t e = hipSuccess;
+#define LAST(DT)                                                                                                              \
+  if (q.dtype == DT) {                                                                                                        \
+    if (s.flip && DT != TCMI_C64) {                                                                                           \
+      Args g = base_args(s, w.split, s.nc, s.m, s.mp, s.mp, ts, qs);                                                          \
+      pair(g, p.t, p.b);                                                                                                      \
+      e = run<P>(g, false, EpiOut<P, DT>{p.t, s.mp, ts, alpha, beta / sc[i].x, q.out, q.ocs, q.ors, q.obs, s.n, up, q.keep, q.rate, \
+                                         aligned4(q.out, q.ocs, q.ors, q.obs, size)}, st);                                    \
+    } else {                                                                                                                  \
+      Args g = base_args(s, w.split, s.m, s.nc, s.mp, s.mp, qs, ts);                                                          \
+      pair(g, p.b, p.t);                                                                                                      \
+      e = run<P>(g, false, EpiOut<0, DT>{w.carry, s.ldc, cs, alpha, beta, q.out, q.ors, q.ocs, q.obs, s.n, up, q.keep, q.rate, \
+                                         aligned4(q.out, q.ors, q.ocs, q.obs, size)}, st);                                    \
+    }                                                                                                                         \
+  }
+    LAST(TCMI_BF16)
+    if constexpr (P == 2) {                          // one piece serves bf16 results only
+      LAST(TCMI_F32)
+      LAST(TCMI_F16)
+      LAST(TCMI_C64)
+    }
+#undef LAST
+    TRY(e);
   }
   return hipSuccess;
 }
@@ -1775,7 +1855,8 @@ long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full,
 int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long g_bs, void* out, int rows, int cols, int batch,
                        int steps, const double* coef_host, double eps, int full, void* saved, long long saved_bytes, void* work,
                        long long work_bytes, int dtype, void* stream) {
-  if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !out || !coef_host || !work || !(eps >= 0) || (saved && !full))
+  if (!sizes_ok(rows, cols, batch, steps, dtype) || !g || !out || !coef_host || !work || !(eps >= 0) || (saved && !full) ||
+      (!full && dtype != TCMI_BF16))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
   // three forms: one workgroup per matrix; two passes around m x m matrices; a sequence of large products
@@ -1894,7 +1975,7 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
                    double momentum, int nesterov, double keep, double rate, int steps, const double* coef_host, double eps,
                    int full, void* work, long long work_bytes, int dtype, void* stream) {
   if (!sizes_ok(rows, cols, batch, steps, dtype) || dtype == TCMI_C64 || !param || !grad || !buf || !coef_host || !work || !(eps >= 0) ||
-      !(momentum >= 0) || !(momentum < 1))
+      !(momentum >= 0) || !(momentum < 1) || (!full && dtype != TCMI_BF16))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
   const int small = small_bytes(s, false);
