@@ -226,38 +226,65 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
   }
 }
 
-// logits of a tile: acc times the rows' scales plus the bias
+// logits of a tile: acc times the rows' scales (two pieces only) plus the bias
 struct Logits {
-  const float *hs, *ws;          // f32: inverse scales of the rows of h and of w (null: 1)
+  const float *hs, *ws;          // f32: inverse scales of the rows of h and of w
   const void* bias;              // null: none
   int dtype;
   int v0;                        // first class of the piece
 };
 
-template <class T>
+template <int P, class T>
 __device__ __forceinline__ void logits(const Logits& q, const Args& g, int m0, int n0, f32x4 (&acc)[T::MI][T::NI]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+  if constexpr (P == 2) {
+    float rs[T::MI];
 #pragma unroll
-  for (int j = 0; j < T::NI; ++j) {
-    const int col = n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4);
-    f32x4 cs, cb;
+    for (int i = 0; i < T::MI; ++i) rs[i] = q.hs[min(m0 + wm * T::MI * 16 + i * 16 + (lane & 15), g.M - 1)];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int c = min(col + r, g.N - 1) + q.v0;
-      cs[r] = q.ws ? q.ws[c] : 1.f;
-      cb[r] = q.bias ? fetch_any(q.bias, q.dtype, c) : 0.f;
+    for (int j = 0; j < T::NI; ++j) {
+      const int col = n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float cs = q.ws[min(col + r, g.N - 1) + q.v0];
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i) acc[i][j][r] *= rs[i] * cs;
+      }
     }
+  }
+  if (q.bias) {
 #pragma unroll
-    for (int i = 0; i < T::MI; ++i) {
-      const int row = min(m0 + wm * T::MI * 16 + i * 16 + (lane & 15), g.M - 1);
-      const float rs = q.hs ? q.hs[row] : 1.f;
+    for (int j = 0; j < T::NI; ++j) {
+      const int col = n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(acc[i][j][r] * rs, cs[r], cb[r]);
+      for (int r = 0; r < 4; ++r) {
+        const float cb = fetch_any(q.bias, q.dtype, min(col + r, g.N - 1) + q.v0);
+#pragma unroll
+        for (int i = 0; i < T::MI; ++i) acc[i][j][r] += cb;
+      }
+    }
+  }
+  if (n0 + T::BN > g.N) {                            // the last tile of classes
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      const int col = n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (col + r >= g.N)
+#pragma unroll
+          for (int i = 0; i < T::MI; ++i) acc[i][j][r] = -INFINITY;
     }
   }
 }
 
+// where a row's target lies among the piece's columns; a column that does not exist if it is elsewhere
+__device__ __forceinline__ int local_target(long long y, int v0, int n) {
+  const long long k = y - v0;
+  return k >= 0 && k < n ? (int)k : -8;
+}
+
 // forward: per row the tile's maximum and sum of exponentials, and the target's logit where it lies in the tile
+template <int P>
 struct EpiLse {
   static constexpr bool TILE = true, FOUR = false;
   template <class T>
@@ -268,24 +295,22 @@ struct EpiLse {
   const long long* y;
   template <class T>
   __device__ void tile(const Args& g, int m0, int n0, int, bool, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
-    logits<T>(q, g, m0, n0, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+    const int c0 = n0 + wn * T::NI * 16 + 4 * (lane >> 4);
     float2* stat = reinterpret_cast<float2*>(lds);                    // [WN][BM]
+    logits<P, T>(q, g, m0, n0, acc);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) {
       const int rl = wm * T::MI * 16 + i * 16 + (lane & 15), row = m0 + rl;
-      const long long yt = row < g.M ? y[row] : -1;
+      const int yl = row < g.M ? local_target(y[row], 0, g.N) : -8;
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < T::NI; ++j) {
-        const int col = n0 + wn * T::NI * 16 + j * 16 + 4 * (lane >> 4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (col + r >= g.N) acc[i][j][r] = -INFINITY;
-          else if (col + r == yt) target[row] = acc[i][j][r];
-          top = fmaxf(top, acc[i][j][r]);
-        }
+        const f32x4 x = acc[i][j];
+        top = fmaxf(fmaxf(fmaxf(top, x[0]), x[1]), fmaxf(x[2], x[3]));
+        const int k = yl - c0 - 16 * j;
+        if ((unsigned)k < 4u) target[row] = k == 0 ? x[0] : k == 1 ? x[1] : k == 2 ? x[2] : x[3];
       }
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -417,30 +442,44 @@ struct EpiProb {
   template <class T>
   __device__ void tile(const Args& g, int m0, int n0, int, bool, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
     const Transposed<T, P> turned{reinterpret_cast<f16*>(lds)};
-    logits<T>(q, g, m0, n0, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+    const int cl = wn * T::NI * 16 + 4 * (lane >> 4);
+    logits<P, T>(q, g, m0, n0, acc);                 // -inf behind the last class: probability 0
     __syncthreads();
-    each<T>(m0, n0, acc, [&](int row, int col, f32x4 x) {
+#pragma unroll
+    for (int i = 0; i < T::MI; ++i) {
+      const int rl = wm * T::MI * 16 + i * 16 + (lane & 15), row = m0 + rl;
       const bool in = row < g.M;
       const long long yt = in ? y[row] : ignore;
-      const bool keep = in && yt != ignore, bad = keep && (yt < 0 || yt >= V);
-      const float l = keep ? lse[row] : 0.f;
-      f16x4 vh, vl;
+      const bool keep = in && yt != ignore;
+      // a target outside the classes poisons its row
+      const float l = !keep ? 0.f : yt < 0 || yt >= V ? NAN : lse[row];
+      const int yl = keep ? local_target(yt, q.v0, g.N) : -8;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = 0.f;
-        if (keep && col + r < g.N) {
-          v = __expf(x[r] - l);
-          if (col + r + q.v0 == yt) v -= 1.f;
-          if (bad) v = NAN;
+      for (int j = 0; j < T::NI; ++j) {
+        const f32x4 x = acc[i][j];
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = keep ? __expf(x[r] - l) * PSCALE : 0.f;        // whatever an ignored row holds
+        const int k = yl - n0 - cl - 16 * j;
+        if ((unsigned)k < 4u) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r == k) v[r] -= PSCALE;
         }
-        f16 a, b;
-        two_pieces(v * PSCALE, a, b);
-        vh[r] = a;
-        vl[r] = b;
+        f16x4 vh, vl;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f16 a, b;
+          two_pieces(v[r], a, b);
+          vh[r] = a;
+          vl[r] = b;
+        }
+        const int col = n0 + cl + 16 * j;
+        if (in && col < vp) store_four<P>(p + (long long)row * P * vp, col, vh, vl);
+        turned.stage(rl, cl + 16 * j, vh, vl);
       }
-      if (in && col < vp) store_four<P>(p + (long long)row * P * vp, col, vh, vl);
-      turned.stage(row - m0, col - n0, vh, vl);
-    });
+    }
     __syncthreads();
     turned.flush(pt, (long long)P * tp, n0, g.N, m0, tp);
   }
@@ -664,7 +703,7 @@ hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, f
                    hipStream_t st) {
   TRY(prepare(s, in, w.rows, Prep{}, st));
   Args g = logit_args(s, in, w.rows, 0, s.V);
-  TRY(run_logits<P>(g, s.dtype, EpiLse{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
+  TRY(run_logits<P>(g, s.dtype, EpiLse<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
   const int tiles = g.tn;
   if (total && (long long)s.T * tiles <= 8192) {       // 64 KB of statistics
     hipLaunchKernelGGL(rowstat_total_kernel, dim3(1), dim3(1024), 0, st, w.part, tiles, w.target, in.y, in.ignore, s.T, s.V, lse, loss, mean,
