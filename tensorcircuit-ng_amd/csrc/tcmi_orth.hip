@@ -385,6 +385,62 @@ struct EpiCarry {
   }
 };
 
+// A step's result as the next step's operands: x = beta carry + alpha acc stays in the carry and goes out as pieces, row-major
+// and (through LDS) transposed.  Real matrices; saves the pass that would read the carry again (27 us a step of 4096 x 4096).
+template <int P>
+struct EpiNext {
+  static constexpr bool TILE = true, FOUR = true;
+  float* carry;
+  long long ldc, cs;
+  float alpha, beta, scale;
+  f16 *x, *t;
+  long long ld, xs, ldt, ts;
+  template <class T>
+  static constexpr int lds() { return Transposed<T, P>::BYTES; }
+  __device__ __forceinline__ void put_row(const Args& g, int bz, int row, int col, f32x4 v, f16x4& vh, f16x4& vl) const {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (row < g.M && col < g.N) {                    // rows of the carry are padded to four columns
+      f32x4* c = reinterpret_cast<f32x4*>(carry + bz * cs + row * ldc + col);
+      const f32x4 old = *c;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = col + r < g.N ? fmaf(alpha, v[r], beta * old[r]) : 0.f;
+      *c = o;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      f16 a, b;
+      two_pieces(o[r] * scale, a, b);
+      vh[r] = a;
+      vl[r] = b;
+    }
+    if (row < g.M && col < (int)kpad(g.N, P)) store_four<P>(x + bz * xs + row * ld, col, vh, vl);
+  }
+  __device__ __forceinline__ void four(const Args& g, int bz, bool, int row, int col, f32x4 v) const {
+    f16x4 vh, vl;
+    put_row(g, bz, row, col, v, vh, vl);
+    if (row >= (int)kpad(g.M, P)) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (col + r < g.N) {
+        f16* o = t + bz * ts + (col + r) * ldt + kpos<P>(row);
+        o[0] = vh[r];
+        if (P == 2) o[32] = vl[r];
+      }
+  }
+  template <class T>
+  __device__ __forceinline__ void tile(const Args& g, int m0, int n0, int bz, bool, char* mem, f32x4 (&acc)[T::MI][T::NI]) const {
+    const Transposed<T, P> turned{reinterpret_cast<f16*>(mem)};
+    __syncthreads();
+    each<T>(m0, n0, acc, [&](int row, int col, f32x4 v) {
+      f16x4 vh, vl;
+      put_row(g, bz, row, col, v, vh, vl);
+      turned.stage(row - m0, col - n0, vh, vl);
+    });
+    __syncthreads();
+    turned.flush(t + bz * ts, ldt, n0, g.N, m0, (int)kpad(g.M, P));
+  }
+};
+
 // The last step: x = beta X + alpha acc goes to the caller's matrix (out = x) or into a weight (out = keep out + rate x).
 // P = 0: X is the f32 carry.  P > 0: the product is the transposed one, T B, so that a matrix taller than wide is written along
 // its rows too, and X comes from T's pieces (one piece, 2^-11 of X in the last step, is below what one-piece products cost).
@@ -1229,6 +1285,7 @@ struct Work {
   double* part;
   float *norm, *carry, *split;
   Pieces p;
+  f16* t2;                        // X^T changes places with this: a step's product reads one while it writes the other
 };
 
 Work take_work(Arena& w, const Shape& s, bool saved) {
@@ -1237,7 +1294,10 @@ Work take_work(Arena& w, const Shape& s, bool saved) {
   k.norm = w.take<float>(s.batch);
   k.carry = w.take<float>(s.m * s.ldc * s.batch);
   k.split = w.take<float>(PART_BYTES / 4);
-  if (!saved) k.p = take_pieces(w, s);
+  if (!saved) {
+    k.p = take_pieces(w, s);
+    if (s.cx == 1) k.t2 = w.take<f16>(s.nc * s.mp * s.batch);
+  }
   return k;
 }
 
@@ -1537,7 +1597,9 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
     TRY(launch_sums<0>(q.src, sa, nb, s.batch, st));
   }
   for (int i = 0; i < q.steps; ++i) {
-    const Pieces& p = sv ? sv->p[i] : w.p;
+    Pieces p = sv ? sv->p[i] : w.p;
+    if (!sv && s.cx == 1 && i % 2) p.t = w.t2;
+    const bool fused = i > 0 && s.cx == 1;           // the step before left this one's operands
     if (padded(s) && (sv || i == 0)) {               // the doubled matrix's padding
       TRY(clear(p.x, s.mr * s.np * s.batch * 2, st));
       TRY(clear(p.t, s.nc * s.mp * s.batch * 2, st));
@@ -1560,7 +1622,7 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
       a.rest = q.rest;
       a.nesterov = q.nesterov;
       TRY(launch_pack<P>(q.src, a, s, st));
-    } else {
+    } else if (!fused) {
       a.src = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
       TRY(launch_pack<P>(SRC_PLANAR, a, s, st));
     }
@@ -1570,7 +1632,13 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
     if (i + 1 < q.steps) {
       Args g = base_args(s, w.split, s.m, s.nc, s.mp, s.mp, qs, ts);
       pair(g, p.b, p.t);
-      TRY(run<P>(g, false, EpiCarry{w.carry, s.ldc, cs, alpha, beta, nullptr}, st));
+      if (s.cx == 1) {
+        const Pieces& n = sv ? sv->p[i + 1] : w.p;
+        f16* t = !sv && i % 2 == 0 ? w.t2 : n.t;
+        TRY(run<P>(g, false, EpiNext<P>{w.carry, s.ldc, cs, alpha, beta, sc[i + 1].x, n.x, t, s.np, s.mr * s.np, s.mp, ts}, st));
+      } else {
+        TRY(run<P>(g, false, EpiCarry{w.carry, s.ldc, cs, alpha, beta, nullptr}, st));
+      }
       continue;
     }
     const int size = q.dtype == TCMI_F32 ? 4 : 2, up = q.buf != nullptr;
