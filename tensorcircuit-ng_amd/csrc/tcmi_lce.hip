@@ -589,6 +589,7 @@ int piece_of(const Shape& s) {
   const long long per = (long long)(s.T + s.tp) * 2 * s.P;
   long long most = (1ll << 30) / per / 256 * 256;
   if (most < 1024) most = 1024;
+  if (most > (1 << 20)) most = 1 << 20;            // P's rows within the longest ones a product takes
   const long long pieces = (s.V + most - 1) / most;
   const long long c = ((s.V + pieces - 1) / pieces + 255) / 256 * 256;
   return (int)(c < s.V ? c : s.V);
@@ -783,13 +784,13 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
 }
 
 bool shape_ok(int T, int D, int V, int dtype) {
-  return T >= 1 && D >= 1 && V >= 1 && T <= (1 << 26) && D <= (1 << 20) && V <= (1 << 28) &&
+  return T >= 1 && D >= 1 && V >= 1 && T <= (1 << 21) && D <= (1 << 20) && V <= (1 << 28) &&
          (dtype == TCMI_F32 || dtype == TCMI_F16 || dtype == TCMI_BF16);
 }
 
 // an operand is read in place when its rows are whole k steps and 16-byte aligned
 bool direct(const void* p, long long rs, int D, int dtype) {
-  return dtype != TCMI_F32 && D % 64 == 0 && rs % 8 == 0 && rs < (1ll << 22) && ((uintptr_t)p & 15) == 0;
+  return dtype != TCMI_F32 && D % 64 == 0 && rs % 8 == 0 && rs <= MAX_ROW && ((uintptr_t)p & 15) == 0;
 }
 
 Shape shape_of(int T, int D, int V, int dtype, bool h_direct, bool w_direct) {

@@ -14,6 +14,8 @@
 
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
 #include <type_traits>
 
 namespace tcmi {
@@ -396,26 +398,36 @@ inline double cost_of(const Args& g, bool tri, bool may_split, int* split) {
   return best;
 }
 
+// Raises a kernel's limit of dynamic LDS, once per device (`done`: one bit each, up to 64; later devices every time).
+inline hipError_t raise_lds(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+  e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+constexpr long long MAX_ROW = 1ll << 22;       // elements between rows: 256 of them stay within 32-bit byte offsets
+
 template <class V, int P, class T, class Epi>
 hipError_t launch(Args& g, bool tri, int split, const Epi& e, hipStream_t st) {
   g.tm = (g.M + T::BM - 1) / T::BM;
   g.tn = (g.N + T::BN - 1) / T::BN;
   g.tri = tri ? 1 : 0;
   const long long tiles = tri ? (long long)g.tm * (g.tm + 1) / 2 : (long long)g.tm * g.tn, units = tiles * g.batch;
-  if (units < 1 || units >= (1ll << 24) || g.K < 64 || (g.K & 63) || g.nseg < 1) return hipErrorInvalidValue;
+  if (units < 1 || units >= (1ll << 24) || g.K < 64 || (g.K & 63) || g.nseg < 1 || g.lda > MAX_ROW || g.ldb > MAX_ROW) return hipErrorInvalidValue;
   g.tiles = (int)tiles;
   g.split = split;
   int lds = T::LDS;
   if constexpr (Epi::TILE) lds = lds > Epi::template lds<T>() ? lds : Epi::template lds<T>();
-  static bool raised = false;                                 // the attribute belongs to the function, not to a call
-  if (!raised) {
-    const hipError_t r = hipFuncSetAttribute(reinterpret_cast<const void*>(product_kernel<V, P, T, Epi>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (r != hipSuccess) return r;
-    raised = true;
-  }
+  static std::atomic<unsigned long long> done{0};
+  hipError_t r = raise_lds(reinterpret_cast<const void*>(product_kernel<V, P, T, Epi>), lds, done);
+  if (r != hipSuccess) return r;
   hipLaunchKernelGGL((product_kernel<V, P, T, Epi>), dim3((unsigned)(units * g.split)), dim3(T::THREADS), lds, st, g, e);
-  hipError_t r = hipGetLastError();
+  r = hipGetLastError();
   if constexpr (Epi::FOUR) {
     if (r == hipSuccess && g.split > 1) {
       hipLaunchKernelGGL((join_kernel<T, Epi>), dim3((unsigned)(units * T::MI * T::NI)), dim3(T::THREADS), 0, st, g, e);

@@ -1501,7 +1501,8 @@ SmallSaved take_small(Arena& w, const Shape& s, int steps) {
 template <int SRC, bool GRAD>
 hipError_t small_launch(const SmallArgs& a, int bytes, int batch, hipStream_t st) {
   const void* f = GRAD ? reinterpret_cast<const void*>(small_grad_kernel<SRC>) : reinterpret_cast<const void*>(small_kernel<SRC>);
-  const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS);
+  static std::atomic<unsigned long long> done{0};
+  const hipError_t e = raise_lds(f, SMALL_LDS, done);
   if (e != hipSuccess) return e;
   if (GRAD) hipLaunchKernelGGL(small_grad_kernel<SRC>, dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
   else hipLaunchKernelGGL(small_kernel<SRC>, dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
@@ -1753,20 +1754,15 @@ template <int SRC, bool GRAD>
 hipError_t thin_launch(const Shape& s, const ThinArgs& a, hipStream_t st) {
   const int r = thin_r16(s), ld = s.cx * THIN_COLS + 4, gram = (GRAD ? 2 : 1) * r * ld * 4, apply = (GRAD ? 2 : 1) * r * (ld + r + 4) * 4,
             poly = (GRAD ? 11 : 4) * r * (r + 2) * 8;
-  static bool raised = false;
-  if (!raised) {
-    const int most = THIN_R * (2 * THIN_COLS + 4) * 4 + THIN_R * (THIN_R + 4) * 4;
-    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(thin_gram_kernel<SRC, GRAD>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == hipSuccess)
-      e = hipFuncSetAttribute(reinterpret_cast<const void*>(thin_apply_kernel<SRC, GRAD>), hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == hipSuccess)
-      e = hipFuncSetAttribute(GRAD ? reinterpret_cast<const void*>(thin_grad_poly_kernel) : reinterpret_cast<const void*>(thin_poly_kernel),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, SMALL_LDS);
-    if (e != hipSuccess) return e;
-    raised = true;
-  }
+  static std::atomic<unsigned long long> done[3] = {};
+  const int most = THIN_R * (2 * THIN_COLS + 4) * 4 + THIN_R * (THIN_R + 4) * 4;
+  hipError_t e = raise_lds(reinterpret_cast<const void*>(thin_gram_kernel<SRC, GRAD>), most, done[0]);
+  if (e == hipSuccess) e = raise_lds(reinterpret_cast<const void*>(thin_apply_kernel<SRC, GRAD>), most, done[1]);
+  if (e == hipSuccess)
+    e = raise_lds(GRAD ? reinterpret_cast<const void*>(thin_grad_poly_kernel) : reinterpret_cast<const void*>(thin_poly_kernel), SMALL_LDS, done[2]);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL((thin_gram_kernel<SRC, GRAD>), dim3(a.parts, s.batch), dim3(256), gram, st, a);
-  hipError_t e = hipGetLastError();
+  e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (GRAD) hipLaunchKernelGGL(thin_grad_poly_kernel, dim3(s.batch), dim3(THIN_THREADS), poly, st, a);
   else hipLaunchKernelGGL(thin_poly_kernel, dim3(s.batch), dim3(THIN_THREADS), poly, st, a);
@@ -1889,6 +1885,9 @@ bool sizes_ok(int rows, int cols, int batch, int steps, int dtype) {
          steps <= TCMI_NS_MAX_STEPS && src_of(dtype) >= 0;
 }
 
+// the large form's rows have to stay within a product's offsets
+bool rows_ok(const Shape& s) { return s.np <= MAX_ROW && s.mp <= MAX_ROW; }
+
 // a matrix with its shorter axis as rows
 Mat oriented(const void* p, long long rs, long long cs, long long bs, bool flip) { return flip ? Mat{p, cs, rs, bs} : Mat{p, rs, cs, bs}; }
 
@@ -1913,6 +1912,7 @@ long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full,
     else take_thin(a, s, what == TCMI_NS_WORK_GRAD, steps);
     return a.used;
   }
+  if (!rows_ok(s)) return -1;
   if (what == TCMI_NS_WORK) take_work(a, s, false);
   else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true);
   else if (what == TCMI_NS_SAVED) take_saved(a, s, steps);
@@ -1942,6 +1942,7 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
     tw = take_thin(aw, s, false, steps);
     if (saved) ts = take_thin_saved(av, s);
   } else {
+    if (!rows_ok(s)) return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: a side is too long");
     w = take_work(aw, s, saved != nullptr);
     if (saved) sv = take_saved(av, s, steps);
   }
@@ -1999,6 +2000,7 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
     tw = take_thin(aw, s, true, steps);
     ts = take_thin_saved(av, s);
   } else {
+    if (!rows_ok(s)) return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: a side is too long");
     w = take_grad(aw, s);
     sv = take_saved(av, s, steps);
   }
@@ -2051,6 +2053,7 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
   Arena aw{(char*)work};
   Work w{};
   ThinWork tw{};
+  if (!small && !narrow && !rows_ok(s)) return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: a side is too long");
   if (narrow) tw = take_thin(aw, s, false, steps);
   else if (!small) w = take_work(aw, s, false);
   if (aw.used > work_bytes || ((uintptr_t)work & 255))

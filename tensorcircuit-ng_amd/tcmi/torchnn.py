@@ -176,7 +176,7 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, target: Tensor, bias: Op
     Rows whose target is ``ignore_index`` have loss 0 and contribute nothing to any gradient, whatever they hold; the mean
     over no rows is NaN (its gradients are zero).  Any other target outside ``0 .. classes - 1`` gives NaN, in the loss and
     in the gradients (checked where the targets live, nothing is read out of range).  Classes may be masked by a bias
-    of ``-inf``.  A non-finite float32 feature row gives NaN."""
+    of ``-inf``.  A non-finite feature or weight gives NaN.  float64 (``tc.set_dtype("complex128")``) is refused."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     if input.dim() < 1 or weight.dim() != 2 or input.shape[-1] != weight.shape[1]:
@@ -277,6 +277,8 @@ def muon_step(param: Tensor, grad: Tensor, momentum_buffer: Tensor, lr: float = 
     for name, x in (("param", param), ("momentum_buffer", momentum_buffer)):
         if torch._debug_has_internal_overlap(x) == 1:
             raise ValueError(f"muon_step: {name} has elements that share memory")
+    if momentum_buffer.numel() and momentum_buffer.data_ptr() in (param.data_ptr(), grad.data_ptr()):
+        raise ValueError("muon_step: momentum_buffer must not share memory with param or grad")
     linalg._need_gpu("muon_step", param, grad, momentum_buffer)
     if param.numel() == 0:
         return
@@ -344,5 +346,5 @@ class Muon(torch.optim.Optimizer):
                 state = self.state[p]
                 if "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
-                muon_step(p, p.grad, state["momentum_buffer"], **{k: v for k, v in group.items() if k != "params"})
+                muon_step(p, p.grad, state["momentum_buffer"], **{k: group[k] for k in self.defaults})   # not a scheduler's keys
         return loss

@@ -87,6 +87,42 @@ def test_newton_schulz_strides_and_batches(dtype):
         assert _rel(linalg.newton_schulz(dev.mH), _ns64(base.mH)) < _ns_tol(dtype)
 
 
+@pytest.mark.parametrize("dtype,shape", [
+    (torch.bfloat16, (700, 900)), (torch.bfloat16, (2300, 2100)), (torch.bfloat16, (3900, 4100)), (torch.bfloat16, (3, 70, 5000)),
+    (torch.float32, (1500, 1601)), (torch.float32, (8, 500, 300)), (torch.float32, (96, 4124)), (torch.float16, (1030, 260)),
+    (torch.complex64, (20, 130, 250)), (torch.complex64, (40, 3000))])
+def test_newton_schulz_larger(dtype, shape):
+    """sizes at which every tile shape, the split products and the two passes are chosen; the 64-bit formula on the GPU"""
+    from tcmi import linalg
+
+    x = _rand(98, *shape, dtype=dtype).cuda()
+    want = _ns64(x)
+    got = linalg.newton_schulz(x)
+    assert float((got.to(want.dtype) - want).norm() / want.norm()) < _ns_tol(dtype)
+    if dtype != torch.bfloat16 or shape[-1] < 1000:
+        dy = _rand(99, *shape, dtype=dtype).cuda()
+        leaf = x.clone().requires_grad_()
+        (g,) = torch.autograd.grad(linalg.newton_schulz(leaf), leaf, dy)
+        ref = _ns_grad64(x, dy)
+        for a, b, c, d in ((x, dy, g, ref),) if x.dim() == 2 else zip(x, dy, g, ref):
+            assert _rel(c, d.cpu()) < _ns_grad_tol(a, b, d, dtype)
+
+
+def test_newton_schulz_past_32_bits():
+    """more than 2^31 elements: the last matrix of a batch"""
+    from tcmi import linalg
+
+    x = torch.empty(41, 60, 900001, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(33)
+    for i in range(41):
+        x[i].normal_(generator=g)
+    got = linalg.newton_schulz(x)
+    for i in (0, 40):
+        want = _ns64(x[i])
+        assert float((got[i].double() - want).norm() / want.norm()) < _ns_tol(torch.float32)
+        assert float((got[i, -1, -1000:].double() - want[-1, -1000:]).norm() / want[-1, -1000:].norm()) < _ns_tol(torch.float32)
+
+
 def test_newton_schulz_low_rank_and_graded():
     """directions 1e-2 .. 1e-4 of the largest: the ones five steps amplify by up to 485"""
     from tcmi import linalg
@@ -406,6 +442,52 @@ def test_linear_cross_entropy_in_pieces():
     sizes = (torch.cat([p[2][0] for p in parts]), sum(p[2][1] for p in parts), sum(p[2][2] for p in parts))
     for g, r, s in zip(got, refs, sizes):
         assert float((g.cpu().double() * 70000 - r).norm()) < (rel + math.sqrt(70000) * 2.0 ** -22) * float(s.norm())
+
+
+@pytest.mark.parametrize("dtype,size", [
+    (torch.bfloat16, (2000, 300, 9000)), (torch.float32, (2000, 300, 9000)), (torch.float16, (700, 128, 40000)),
+    (torch.bfloat16, (4100, 640, 33001)), (torch.float32, (130, 65, 70000)), (torch.bfloat16, (2, 1111, 20000))])
+def test_linear_cross_entropy_larger(dtype, size):
+    """sizes at which every tile shape and the split products are chosen; the 64-bit formula on the GPU"""
+    from tcmi import torchnn
+
+    h, w, y, b = (t.cuda() for t in _ce_inputs(96, *size, dtype))
+    y[::11] = -100
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = torchnn.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction="sum")
+    got = torch.autograd.grad(loss, leaves)
+    want, grads, sizes = _ce64(h, w, y, b, -100, "sum")
+    logit, rel = _ce_tols(h[:512], w, dtype)
+    assert abs(float(loss.detach()) - float(want)) <= len(y) * (2 * logit + 2.0 ** -21) + 2.0 ** -22 * float(want)
+    for g, ref, sz in zip(got, grads, sizes):
+        slack = (rel + math.sqrt(max(size[0], size[2])) * 2.0 ** -22) * float(sz.norm()) + HALF_STEP[dtype] * float(ref.norm())
+        assert float((g.double() - ref).norm()) <= slack
+
+
+def test_linear_cross_entropy_past_32_bits():
+    """more than 2^31 weight elements: the last classes are read and written where they lie"""
+    from tcmi import torchnn
+
+    T, D, V = 5, 16384, 131272
+    g = torch.Generator(device="cuda").manual_seed(97)
+    w = torch.empty(V, D, dtype=torch.bfloat16, device="cuda")
+    for i in range(0, V, 8192):
+        w[i:i + 8192] = torch.randn(min(8192, V - i), D, device="cuda", generator=g) / 128
+    h = torch.randn(T, D, device="cuda", generator=g).bfloat16()
+    y = torch.tensor([V - 1, 0, V - 130, 65536, V - 2], device="cuda")
+    z = torch.cat([h.double() @ w[i:i + 8192].double().T for i in range(0, V, 8192)], 1)
+    want = torch.logsumexp(z, 1) - z.gather(1, y[:, None]).squeeze(1)
+    w.requires_grad_()
+    rows = torchnn.linear_cross_entropy(h, w, y, reduction="none")
+    top = float((h.double().abs() @ w[:8192].detach().double().abs().T).max()) * 1.5
+    assert float((rows.detach().double() - want).abs().max()) <= 2 * D * 2.0 ** -24 * top + 2.0 ** -21
+    (dw,) = torch.autograd.grad(rows.sum(), w)
+    p = torch.exp(z - torch.logsumexp(z, 1, keepdim=True))
+    p[torch.arange(T), y] -= 1.0
+    for rng in (slice(0, 64), slice(V - 200, V)):
+        ref, size = p[:, rng].T @ h.double(), p[:, rng].abs().T @ h.double().abs()
+        slack = (4 * D * 2.0 ** -24 * top + 2.0 ** -11 + 2.0 ** -20) * float(size.norm()) + 2.0 ** -8 * float(ref.norm())
+        assert float((dw[rng].double() - ref).norm()) <= slack
 
 
 # -------------------------------------------------------------------------------------------------------------- muon

@@ -120,3 +120,32 @@ def test_muon_state_survives_a_checkpoint():
     b.load_state_dict(a.state_dict())
     got = b.state[w]["momentum_buffer"]
     assert got.dtype == torch.float32 and bool((got == 1.0 + 2.0 ** -20).all())
+
+
+def test_muon_step_gets_its_own_options_only(monkeypatch):
+    """a learning-rate scheduler leaves keys of its own in the parameter groups"""
+    w = torch.nn.Parameter(torch.zeros(3, 4))
+    opt = torchnn.Muon([w], lr=0.5, ns_steps=3)
+    sched = torch.optim.lr_scheduler.StepLR(opt, step_size=1, gamma=0.1)
+    seen = []
+    monkeypatch.setattr(torchnn, "muon_step", lambda p, g, v, **kw: seen.append((v.dtype, kw)))
+    w.grad = torch.ones(3, 4)
+    opt.step()
+    sched.step()
+    opt.step()
+    assert [kw["lr"] for _, kw in seen] == [0.5, 0.05] and all(kw["ns_steps"] == 3 and "initial_lr" not in kw for _, kw in seen)
+    assert seen[0][0] == torch.float32
+
+
+def test_shared_memory_and_long_sides_are_refused():
+    p = torch.zeros(3, 4)
+    with pytest.raises(ValueError, match="share memory"):
+        torchnn.muon_step(p, torch.zeros(3, 4), p)
+    lib = _lib.lib()
+    f32 = _lib.TCMI_F32
+    assert lib.tcmi_ns_work_bytes(8, 1 << 24, 1, 5, 1, f32, 0) > 0            # few rows: any length
+    assert lib.tcmi_ns_work_bytes(200, 1 << 21, 1, 5, 1, f32, 0) > 0
+    assert lib.tcmi_ns_work_bytes(200, (1 << 21) + 1, 1, 5, 1, f32, 0) == -1  # 32-bit offsets of a product's rows
+    assert lib.tcmi_ns_work_bytes(200, (1 << 21) + 1, 1, 5, 0, _lib.TCMI_BF16, 0) > 0
+    assert lib.tcmi_lce_work_bytes(None, 64, None, 64, (1 << 21) + 1, 64, 100, f32, 0) == -1
+    assert lib.tcmi_lce_work_bytes(None, 64, None, 64, 1 << 21, 64, 100, f32, 0) > 0
