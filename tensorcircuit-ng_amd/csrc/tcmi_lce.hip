@@ -161,7 +161,8 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
 
 // out[c][row] = src[row][c] * r[row] * scale as f16 pieces (two for f32), rows padded with zeros.  A zero factor gives zero
 // whatever the row holds.  ones: behind the last column one more, the factors themselves (their product with P is the
-// bias's gradient).  64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
+// bias's gradient); 2 where all rows that count share one factor: its power of two only, which one piece holds exactly, the
+// epilogue multiplies the rest back (2^-11 of the factor would shift every entry the same way).  64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
 struct Turn {
   const void* src;
   long long rs;
@@ -171,6 +172,9 @@ struct Turn {
   f16* out;
   float* inv;
 };
+
+__device__ __forceinline__ float power_of(float f) { return __uint_as_float(__float_as_uint(f) & 0xff800000u); }
+__device__ __forceinline__ float mantissa_of(float f) { return __uint_as_float((__float_as_uint(f) & 0x007fffffu) | 0x3f800000u); }
 
 template <int DT>
 __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
@@ -200,9 +204,10 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
         if (a.ones) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (c0 + u + e == a.cols) v[e] = 1.f;
+            if (c0 + u + e == a.cols) v[e] = a.ones == 2 ? power_of(f) : f;
         }
-        v = v * f * s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (c0 + u + e == a.cols ? v[e] : v[e] * f) * s;
       }
     }
 #pragma unroll
@@ -212,7 +217,7 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
 #pragma unroll
   for (int k = w; k < 64; k += 16) {
     const int c = c0 + k, row = r0 + u;
-    if (c < a.cols + a.ones && row < a.rowsp) {
+    if (c < a.cols + (a.ones != 0) && row < a.rowsp) {
       f16x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -496,6 +501,7 @@ struct EpiGrad {
   void* out;
   int dtype, cols;
   void* db;
+  const float *dloss, *count;    // db: the factor all rows share, dloss (/ count), whose mantissa is still missing (null: none)
   __device__ __forceinline__ void four(const Args& g, int, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
     const float al = *inv * (1.f / PSCALE);
@@ -504,13 +510,14 @@ struct EpiGrad {
       if (col + k >= g.N) continue;
       float x = al * v[k];
       if (col + k == cols) {
+        if (dloss) x *= mantissa_of(count ? dloss[0] / count[0] : dloss[0]);
         put(db, dtype, row, x);
         continue;
       }
       const long long at = (long long)row * cols + col + k;
       if (!first) x += sum[at];
       if (!last) sum[at] = x;
-      else if (out) put(out, dtype, at, r ? (r[row] == 0.f ? 0.f : x * r[row]) : x);
+      else put(out, dtype, at, r ? (r[row] == 0.f ? 0.f : x * r[row]) : x);
     }
   }
 };
@@ -723,8 +730,9 @@ hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, f
 template <int P>
 hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float* lse, const float* dloss, int per_row, const float* count,
                     void* dh, void* dw, void* db, hipStream_t st) {
-  // the bias's gradient as one more column of h^T costs nothing where the columns do not fill their tiles
-  const int ones = db && s.D % 64 != 0, want_dw = dw || ones;
+  // The bias's gradient as one more column of h^T: free where the columns do not fill their tiles, and a further column of
+  // tiles still costs less than reading P^T again (1021 x 512 x 32768 f32: 29 us against 47).
+  const int ones = db && dw ? (per_row ? 1 : 2) : 0, more = ones != 0;
   Prep a{};
   a.y = in.y;
   a.ignore = in.ignore;
@@ -732,16 +740,16 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
   a.count = count;
   a.per_row = per_row;
   a.r = w.r;
-  if (want_dw) a.h.part = w.parth;
+  if (dw) a.h.part = w.parth;
   if (dh) a.w.part = w.partw;
   TRY(prepare(s, in, w.rows, a, st));
   const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
   for (int v0 = 0; v0 < s.V; v0 += vc) {
     const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P);
     Turn th{}, tw{};
-    if (want_dw && v0 == 0) {
+    if (dw && v0 == 0) {
       th = Turn{in.h, in.hrs, s.T, s.D, s.tp, vec4(in.h, in.hrs, s.dtype), ones, (s.tp + 63) / 64, 0, w.r, w.parth, parts_of(s.T), w.ht, w.invh};
-      th.tiles = th.tx * ((s.D + ones + 63) / 64);
+      th.tiles = th.tx * ((s.D + more + 63) / 64);
     }
     if (dh) {
       tw = Turn{(const char*)in.w + v0 * in.wrs * size, in.wrs, n, s.D, np, vec4(in.w, in.wrs, s.dtype), 0, (np + 63) / 64, 0, nullptr,
@@ -763,17 +771,17 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.lda = d.ldb = d.K;
       d.a[0] = w.p;
       d.b[0] = w.wt;
-      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr}, st));
+      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr, nullptr, nullptr}, st));
     }
-    if (want_dw) {
+    if (dw) {
       d.M = n;
-      d.N = s.D + ones;
+      d.N = s.D + more;
       d.K = P * s.tp;
       d.lda = d.ldb = d.K;
       d.a[0] = w.pt;
       d.b[0] = w.ht;
-      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, dw ? (char*)dw + (long long)v0 * s.D * size : nullptr, s.dtype, s.D,
-                            ones ? (char*)db + (long long)v0 * size : nullptr}, st));
+      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype, s.D,
+                            more ? (char*)db + (long long)v0 * size : nullptr, ones == 2 ? dloss : nullptr, count}, st));
     }
     if (db && !ones) {
       hipLaunchKernelGGL(bias_kernel<P>, dim3((n + 3) / 4), dim3(256), 0, st, w.pt, s.tp, w.r, s.T, n, db, s.dtype, v0);

@@ -423,7 +423,15 @@ def test_linear_cross_entropy_layouts(dtype):
         assert g.shape == ts[k].shape
         alls = [t.cuda().requires_grad_() for t in (h, w, b)]
         ref = torch.autograd.grad(torchnn.linear_cross_entropy(alls[0], alls[1], y.cuda(), alls[2]), alls)[k]
-        assert torch.equal(g, ref)
+        if k < 2:
+            assert torch.equal(g, ref)
+        else:
+            # The bias's gradient alone is summed by another kernel than with the weight's.  Either route: T products off by
+            # 2^-22 (the row factor in two pieces, or whole) and T f32 additions, 2^-24 each, of the terms |P r|; then one
+            # rounding to the type returned.
+            size = _ce64(h, w, y, b, -100, "mean")[2][2]
+            slack = 2 * (2.0 ** -22 + len(y) * 2.0 ** -24) * size + 2 * HALF_STEP[dtype] * ref.cpu().double().abs()
+            assert bool(((g - ref).cpu().double().abs() <= slack).all())
 
 
 def test_linear_cross_entropy_in_pieces():
