@@ -428,13 +428,17 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
 /* Softmax cross entropy of a linear head, logits never stored: h [tokens][features], w [classes][features] (row strides
  * h_rs, w_rs; features contiguous), bias [classes] or NULL, all of one dtype (TCMI_F32 / F16 / BF16); target int64.
  * Writes lse[tokens], loss[tokens] (f32; 0 for target == ignore_index, NaN for any other target outside [0, classes)) and,
- * with `total` given, the sum (mean = 0) or mean over the rows that count, and their number.
+ * with `total` given, the sum (mean = 0) or mean over the rows that count, and their number.  for_grad = 1: lse goes to
+ * tcmi_linear_cross_entropy_grad and is formed from the product that forms its logits (0: up to 16 rows read w once, uncopied).
  * No counterpart in the reference: it leaves classical heads to the host framework (tensorcircuit/torchnn.py). */
+#define TCMI_LCE_ALONE 0      /* tcmi_lce_work_bytes' `what`: tcmi_linear_cross_entropy with for_grad = 0 */
+#define TCMI_LCE_GRAD 1       /* tcmi_linear_cross_entropy_grad */
+#define TCMI_LCE_FOR_GRAD 2   /* tcmi_linear_cross_entropy with for_grad = 1 */
 long long tcmi_lce_work_bytes(const void* h, long long h_rs, const void* w, long long w_rs, int tokens, int features, int classes,
-                              int dtype, int backward_pass);
+                              int dtype, int what);
 int tcmi_linear_cross_entropy(const void* h, long long h_rs, const void* w, long long w_rs, const void* bias, const long long* target,
                               long long ignore_index, int tokens, int features, int classes, float* lse, float* loss, float* total,
-                              float* count, int mean, void* work, long long work_bytes, int dtype, void* stream);
+                              float* count, int mean, int for_grad, void* work, long long work_bytes, int dtype, void* stream);
 
 /* Its gradients (contiguous, dtype of the inputs; NULL: not wanted).  dloss: f32 [tokens] (per_row = 1) or one value,
  * divided by *count when count is given (mean).  lse from the forward call.  Ignored rows contribute nothing, whatever

@@ -344,6 +344,116 @@ struct EpiLse {
   }
 };
 
+// Up to 16 rows without a gradient (evaluating or serving single samples; before a gradient the logits of forward and
+// backward have to come from the same product, or exp(l - lse) - 1 of a certain row is their difference): w is read once, straight into the matrix instructions, whatever its
+// alignment, and no operand is copied.  A wave takes 32 classes at a time and keeps its rows' running maximum and sum of
+// exponentials; f32 heads use the f32 matrix instruction (exact products).  Bound by the read
+// of w: 10 x 3466 x 59851 bf16 124 us (3.3 TB/s; with copies and 128 x 128 tiles 436), 16 x 4096 x 65536 f32 256 us (4.2 TB/s; 707),
+// the same in bf16, which the tiles read in place, 130 us either way.
+constexpr int FEW_ROWS = 16, FEW_BLOCKS = 1024;
+
+template <int DT>
+struct FewArgs {
+  const void *h, *w, *bias;
+  long long hrs, wrs;
+  int T, D, V;
+  const long long* y;
+  float2* part;                  // [T][gridDim.x]
+  float* target;
+};
+
+// 16 bytes of a row from element c, zero behind its end; the row may start anywhere
+template <class V, class E>
+__device__ __forceinline__ V few_load(const E* row, int c, int cols) {
+  constexpr int N = 16 / sizeof(E);
+  V v;
+  if (c + N <= cols) {
+    __builtin_memcpy(&v, row + c, 16);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = c + k < cols ? row[c + k] : (E)0.f;
+  }
+  return v;
+}
+
+__device__ __forceinline__ f32x4 few_mul(f16x8 a, f16x8 b, f32x4 c) { return mfma(a, b, c); }
+__device__ __forceinline__ f32x4 few_mul(bf16x8 a, bf16x8 b, f32x4 c) { return mfma(a, b, c); }
+__device__ __forceinline__ f32x4 few_mul(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k], b[k], c, 0, 0, 0);
+  return c;
+}
+
+template <class V, class E, int DT>
+__global__ __launch_bounds__(256) void few_kernel(FewArgs<DT> a) {
+  constexpr int N = 16 / sizeof(E), K = 16 * N;      // elements of a load, of a pass of four loads
+  __shared__ float2 stat[4][FEW_ROWS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+  const E* h = (const E*)a.h + min(l, a.T - 1) * a.hrs;
+  const long long yt = l < a.T ? a.y[l] : -8;
+  float top = -INFINITY, sum = 0.f;
+  for (int v0 = (blockIdx.x * 4 + wave) * 32; v0 < a.V; v0 += gridDim.x * 128) {
+    const E* w0 = (const E*)a.w + (long long)min(v0 + l, a.V - 1) * a.wrs;
+    const E* w1 = (const E*)a.w + (long long)min(v0 + 16 + l, a.V - 1) * a.wrs;
+    f32x4 acc[2] = {};
+    for (int k = 0; k < a.D; k += K) {
+      V x[4], p[4], q[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = k + (4 * u + g) * N;            // the four lane groups read 64 neighbouring bytes of a row
+        p[u] = few_load<V, E>(w0, c, a.D);
+        q[u] = few_load<V, E>(w1, c, a.D);
+        x[u] = few_load<V, E>(h, c, a.D);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        acc[0] = few_mul(p[u], x[u], acc[0]);
+        acc[1] = few_mul(q[u], x[u], acc[1]);
+      }
+    }
+    // the lane holds classes v0 + 16 t + 4 g + r of row l
+    float most = top;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int v = v0 + 16 * t + 4 * g + r;
+        float x = acc[t][r];
+        if (a.bias) x += fetch<DT>(a.bias, min(v, a.V - 1));
+        if (v >= a.V) x = -INFINITY;
+        if (v == yt && v < a.V) a.target[l] = x;
+        acc[t][r] = x;
+        most = fmaxf(most, x);
+      }
+    const float at = most == -INFINITY ? 0.f : most;
+    sum *= __expf(top - at);                       // 0 while top is -inf
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += __expf(acc[t][r] - at);
+    top = most;
+  }
+  auto join = [&](float2 b) {
+    const float most = fmaxf(top, b.x), at = most == -INFINITY ? 0.f : most;
+    sum = sum * __expf(top - at) + b.y * __expf(b.x - at);
+    top = most;
+  };
+#pragma unroll
+  for (int o = 16; o < 64; o *= 2) {
+    const float2 b = make_float2(__shfl_xor(top, o), __shfl_xor(sum, o));
+    join(b);
+  }
+  if (lane < 16) stat[wave][l] = make_float2(top, sum);
+  __syncthreads();
+  if (threadIdx.x >= a.T) return;
+  float2 s = stat[0][threadIdx.x];
+  top = s.x;
+  sum = s.y;
+#pragma unroll
+  for (int k = 1; k < 4; ++k) join(stat[k][threadIdx.x]);
+  a.part[(long long)threadIdx.x * gridDim.x + blockIdx.x] = make_float2(top, sum);
+}
+
 // the loss of row t from its tiles' statistics, by one wave
 __device__ __forceinline__ float row_loss(const float2* part, int tiles, const float* target, const long long* y, long long ignore, int t,
                                           int V, float* lse) {
@@ -558,6 +668,7 @@ struct Shape {
   int T, D, V, dtype;
   int P;                         // pieces per operand: 2 for f32
   int dp, tp;                    // padded features, padded rows
+  bool few;                      // the forward of up to 16 rows without a gradient
   bool h_direct, w_direct;       // the operand is read where it lies
 };
 
@@ -583,9 +694,11 @@ struct FwdWork {
   float* target;
 };
 
+int few_blocks(const Shape& s) { return s.V >= 128 * FEW_BLOCKS ? FEW_BLOCKS : (s.V + 127) / 128; }
+
 FwdWork take_fwd(Arena& a, const Shape& s) {
   FwdWork w{};
-  w.rows = take_rows(a, s);
+  if (!s.few) w.rows = take_rows(a, s);
   w.part = a.take<float2>((long long)s.T * ((s.V + 63) / 64));          // the narrowest tile of classes is 64 wide
   w.target = a.take<float>(s.T);
   return w;
@@ -709,10 +822,33 @@ Args logit_args(const Shape& s, const In& in, const Rows& r, int v0, int vc) {
 template <int P>
 hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, float* loss, float* total, float* count, int mean,
                    hipStream_t st) {
-  TRY(prepare(s, in, w.rows, Prep{}, st));
-  Args g = logit_args(s, in, w.rows, 0, s.V);
-  TRY(run_logits<P>(g, s.dtype, EpiLse<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
-  const int tiles = g.tn;
+  int tiles;
+  if (s.few) {
+    tiles = few_blocks(s);
+    auto go = [&](auto kernel, auto args) {
+      args.h = in.h;
+      args.w = in.w;
+      args.bias = in.bias;
+      args.hrs = in.hrs;
+      args.wrs = in.wrs;
+      args.T = s.T;
+      args.D = s.D;
+      args.V = s.V;
+      args.y = in.y;
+      args.part = w.part;
+      args.target = w.target;
+      hipLaunchKernelGGL(kernel, dim3(tiles), dim3(256), 0, st, args);
+    };
+    if (s.dtype == TCMI_F32) go(few_kernel<f32x4, float, TCMI_F32>, FewArgs<TCMI_F32>{});
+    else if (s.dtype == TCMI_F16) go(few_kernel<f16x8, f16, TCMI_F16>, FewArgs<TCMI_F16>{});
+    else go(few_kernel<bf16x8, __bf16, TCMI_BF16>, FewArgs<TCMI_BF16>{});
+    TRY(hipGetLastError());
+  } else {
+    TRY(prepare(s, in, w.rows, Prep{}, st));
+    Args g = logit_args(s, in, w.rows, 0, s.V);
+    TRY(run_logits<P>(g, s.dtype, EpiLse<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
+    tiles = g.tn;
+  }
   if (total && (long long)s.T * tiles <= 8192) {       // 64 KB of statistics
     hipLaunchKernelGGL(rowstat_total_kernel, dim3(1), dim3(1024), 0, st, w.part, tiles, w.target, in.y, in.ignore, s.T, s.V, lse, loss, mean,
                        total, count);
@@ -801,8 +937,9 @@ bool direct(const void* p, long long rs, int D, int dtype) {
   return dtype != TCMI_F32 && D % 64 == 0 && rs % 8 == 0 && rs <= MAX_ROW && ((uintptr_t)p & 15) == 0;
 }
 
-Shape shape_of(int T, int D, int V, int dtype, bool h_direct, bool w_direct) {
+Shape shape_of(int T, int D, int V, int dtype, bool h_direct, bool w_direct, bool alone) {
   Shape s{};
+  s.few = alone && T <= FEW_ROWS;
   s.T = T;
   s.D = D;
   s.V = V;
@@ -823,22 +960,24 @@ using namespace tcmi::lce;
 extern "C" {
 
 long long tcmi_lce_work_bytes(const void* h, long long h_rs, const void* w, long long w_rs, int tokens, int features, int classes,
-                              int dtype, int backward_pass) {
-  if (!shape_ok(tokens, features, classes, dtype)) return -1;
-  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype));
+                              int dtype, int what) {
+  if (!shape_ok(tokens, features, classes, dtype) || what < 0 || what > 2) return -1;
+  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype),
+                           what == TCMI_LCE_ALONE);
   Arena a{nullptr};
-  if (backward_pass) take_bwd(a, s);
+  if (what == TCMI_LCE_GRAD) take_bwd(a, s);
   else take_fwd(a, s);
   return a.used;
 }
 
 int tcmi_linear_cross_entropy(const void* h, long long h_rs, const void* w, long long w_rs, const void* bias, const long long* target,
                               long long ignore_index, int tokens, int features, int classes, float* lse, float* loss, float* total,
-                              float* count, int mean, void* work, long long work_bytes, int dtype, void* stream) {
+                              float* count, int mean, int for_grad, void* work, long long work_bytes, int dtype, void* stream) {
   if (!shape_ok(tokens, features, classes, dtype) || !h || !w || !target || !lse || !loss || !work || (total && !count) || h_rs < features ||
       w_rs < features)
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy: bad argument");
-  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype));
+  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype),
+                           !for_grad);
   Arena a{(char*)work};
   const FwdWork k = take_fwd(a, s);
   if (a.used > work_bytes || ((uintptr_t)work & 255))
@@ -855,7 +994,7 @@ int tcmi_linear_cross_entropy_grad(const void* h, long long h_rs, const void* w,
   if (!shape_ok(tokens, features, classes, dtype) || !h || !w || !target || !lse || !dloss || !work || (!dh && !dw && !db) ||
       h_rs < features || w_rs < features)
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy_grad: bad argument");
-  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype));
+  const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype), false);
   Arena a{(char*)work};
   const BwdWork k = take_bwd(a, s);
   if (a.used > work_bytes || ((uintptr_t)work & 255))

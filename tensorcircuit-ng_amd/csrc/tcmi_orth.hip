@@ -833,7 +833,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
 // The gradient alike: D_k = U_k dY + V_k X_0 with U <- P U, V <- P V + Q M,
 //     T = (U dY X_0^H + V A_0) M,  S = T + T^H,  Q = b S + c (A S + S A),
 // from one pass for dY G^H and one for U dY + V G.  Bound by the reads of G for long sides, by the chain of small f64
-// products (17 forward, 55 for the gradient) for short ones.
+// products (17 forward, 55 for the gradient) for short ones.  33 x 1088 x 9 f32: 28 us a call (large form: 325); gradient of 38 x 14 x 5789
+// bf16: 157 us, most of it autograd's (3.0 ms).
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 

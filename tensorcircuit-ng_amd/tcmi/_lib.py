@@ -21,6 +21,8 @@ TCMI_BF16 = 5
 # tcmi_ns_work_bytes' last argument
 NS_MAX_STEPS = 16
 NS_WORK, NS_WORK_SAVING, NS_SAVED, NS_WORK_GRAD = range(4)
+# tcmi_lce_work_bytes' last argument
+LCE_ALONE, LCE_GRAD, LCE_FOR_GRAD = range(3)
 
 _lib = None
 
@@ -228,7 +230,7 @@ _SIGNATURES = {
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
-         ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p],
+         ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p],
     ),
     "tcmi_linear_cross_entropy_grad": (
         ctypes.c_int,

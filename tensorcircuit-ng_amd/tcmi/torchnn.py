@@ -47,7 +47,7 @@ TorchLayer = QuantumNet
 _REDUCTIONS = ("none", "sum", "mean")
 
 
-def _lce_raw(h, w, target, bias, ignore_index, reduction):
+def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
     """(loss, stat): h [T, D], w [V, D], target [T]; loss is per row for reduction "none".  stat, what the gradient needs: the
     rows' log sums, how many rows count, and (not "none") the rows' losses"""
     t, d = h.shape
@@ -62,7 +62,7 @@ def _lce_raw(h, w, target, bias, ignore_index, reduction):
         return loss, stat.zero_()
     L = _lib.lib()
     hp, hs, wp, ws, lse = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), stat.data_ptr()
-    nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, 0)
+    nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_FOR_GRAD if for_grad else _lib.LCE_ALONE)
     if nbytes < 0:
         raise ValueError(f"linear_cross_entropy: {t} rows, {d} features, {v} classes are out of range")
     work = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
@@ -70,7 +70,7 @@ def _lce_raw(h, w, target, bias, ignore_index, reduction):
         _lib.check(L.tcmi_linear_cross_entropy(
             hp, hs, wp, ws, None if bias is None else bias.data_ptr(), target.data_ptr(), ignore_index, t, d, v, lse,
             loss.data_ptr() if per_row else lse + 4 * (t + 1), None if per_row else loss.data_ptr(), lse + 4 * t,
-            int(reduction == "mean"), work.data_ptr(), nbytes, code, linalg._stream(h)), "tcmi_linear_cross_entropy")
+            int(reduction == "mean"), int(for_grad), work.data_ptr(), nbytes, code, linalg._stream(h)), "tcmi_linear_cross_entropy")
     return loss, stat
 
 
@@ -85,7 +85,7 @@ def _lce_grad_raw(h, w, target, bias, stat, dloss, ignore_index, reduction, need
     dloss = dloss.to(torch.float32).contiguous()
     L = _lib.lib()
     hp, hs, wp, ws, lse = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), stat.data_ptr()
-    nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, 1)
+    nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_GRAD)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     ptrs = [None if o is None else o.data_ptr() for o in outs]
     with linalg._on(dev):
@@ -107,7 +107,7 @@ class _LinearCrossEntropyEager(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, w, target, bias, ignore_index, reduction):
-        loss, stat = _lce_raw(h, w, target, bias, ignore_index, reduction)
+        loss, stat = _lce_raw(h, w, target, bias, ignore_index, reduction, True)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         ctx.save_for_backward(h, w, target, bias, stat)
         return loss
@@ -126,7 +126,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def forward(h, w, target, bias, ignore_index, reduction):
-        return _lce_raw(h, w, target, bias, ignore_index, reduction)
+        return _lce_raw(h, w, target, bias, ignore_index, reduction, True)
 
     @staticmethod
     def vmap(info, in_dims, *args):
@@ -205,7 +205,7 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, target: Tensor, bias: Op
     y = target.reshape(-1).contiguous()
     args = (h, w, y, b, int(ignore_index), reduction)
     if not linalg._tracked(h, w, b, y):
-        loss = _lce_raw(*args)[0]
+        loss = _lce_raw(*args, False)[0]
     elif torch._C._are_functorch_transforms_active():
         loss = _LinearCrossEntropy.apply(*args)[0]
     else:

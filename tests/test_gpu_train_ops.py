@@ -10,8 +10,9 @@ Tolerances (2-norms, derived from the number formats, not from runs):
 * its gradient: the same units (8 a step: six two-piece products and the carries), five steps, relative to what the
   cotangent could have grown to: 40 * 2^-22 * 3.45^5 |dY| / |D_0|.
 * linear_cross_entropy: a logit is off by (2^-21 + D 2^-24) sum |h||w| in f32, by D 2^-24 sum |h||w| from 16-bit operands (their
-  products are exact).  P then is off by twice that relatively plus 2^-21 (two pieces) or 2^-11 (one f16 piece), the sums by
-  sqrt(K) 2^-22; a gradient is held to that times |P| |w| (|P|^T |h|) plus half a step of the type it is returned in.
+  products are exact).  P then is off by twice that of the probability plus 2^-21 (two pieces) or 2^-11 (one f16 piece) of itself
+  plus half of f16's smallest step under its scale (_ce64), the sums by sqrt(K) 2^-22; a gradient is held to that times
+  |P| |w| (|P|^T |h|) plus half a step of the type it is returned in.
 """
 
 import math
@@ -267,10 +268,15 @@ def _ce64(h, w, y, b, ignore, reduction, dloss=None):
     d = torch.ones_like(rows) if dloss is None else dloss.double() * torch.ones_like(rows)
     r = torch.where(keep, d / n if reduction == "mean" else d, 0.0)
     p = torch.exp(z - lse[:, None])
+    # What the relative errors of P multiply: the probability itself where P = p - 1 is small against it (a logit off by e
+    # moves p - 1 by e p), and 2^-18, which times the smallest of them, 2^-21, is the 2^-39 that half of f16's smallest step,
+    # 2^-25, under the scale 2^14 may cost any entry.
+    q = p + 2.0 ** -18
     p[torch.arange(len(y)), yy] -= 1.0
+    q = torch.maximum(q, p.abs()) * r.abs()[:, None]
     p = p * r[:, None]
     hz = torch.where(keep[:, None], h, 0.0)
-    return loss, (p @ w, p.T @ hz, p.sum(0)), (p.abs() @ w.abs(), p.abs().T @ hz.abs(), p.abs().sum(0))
+    return loss, (p @ w, p.T @ hz, p.sum(0)), (q @ w.abs(), q.T @ hz.abs(), q.sum(0))
 
 
 def _ce_tols(h, w, dtype):
@@ -291,9 +297,11 @@ def _check_ce(h, w, y, b, dtype, reduction="mean", ignore=-100, dloss=None, keep
     assert loss.dtype == torch.float32 and loss.shape == want.shape
     n = 1 if reduction != "sum" else len(y)
     assert float((loss.detach().cpu().double() - want).abs().max()) <= n * (2 * logit + 2.0 ** -21) + 2.0 ** -22 * float(want.abs().max())
-    # without gradients the same kernels answer
+    # without gradients the same kernels answer, but up to 16 rows, which have their own
     plain = torchnn.linear_cross_entropy(h.cuda(), w.cuda(), y.cuda(), None if b is None else b.cuda(), ignore_index=ignore, reduction=reduction)
-    assert torch.equal(plain, loss.detach())
+    if len(y) > 16:
+        assert torch.equal(plain, loss.detach())
+    assert float((plain.cpu().double() - want).abs().max()) <= n * (2 * logit + 2.0 ** -21) + 2.0 ** -22 * float(want.abs().max())
     live = [t for t in leaves if t is not None]
     got = torch.autograd.grad(loss, live, None if dloss is None else dloss.cuda())
     K = max(w.shape[0], h.shape[0])
@@ -313,7 +321,7 @@ def _ce_inputs(seed, T, D, V, dtype, bias=True):
     return h, w, y, b
 
 
-CE_SIZES = [(1, 1, 1), (1, 3, 2), (5, 28, 4096), (64, 64, 128), (129, 100, 257), (33, 192, 1000), (300, 64, 129), (257, 320, 3001)]
+CE_SIZES = [(1, 1, 1), (1, 3, 2), (1, 700, 3001), (16, 257, 130), (17, 257, 130), (9, 96, 140000), (5, 28, 4096), (64, 64, 128), (129, 100, 257), (33, 192, 1000), (300, 64, 129), (257, 320, 3001)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])

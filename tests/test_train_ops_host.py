@@ -49,7 +49,7 @@ def test_abi_refuses_before_a_launch():
     assert changed(_9=linalg._host_doubles((30.0, 0.0, 0.0) * 5)) == -1 and b"past 64" in lib.tcmi_last_error()
     assert lib.tcmi_ns_work_bytes(4, 4, 1, 5, 1, _lib.TCMI_F32, 9) == -1
     assert lib.tcmi_lce_work_bytes(None, 4, None, 4, 0, 4, 4, _lib.TCMI_F32, 0) == -1
-    assert lib.tcmi_linear_cross_entropy(p, 3, p, 4, None, p, -100, 2, 4, 4, p, p, None, None, 0, p, 1 << 40, _lib.TCMI_F32, None) == -1
+    assert lib.tcmi_linear_cross_entropy(p, 3, p, 4, None, p, -100, 2, 4, 4, p, p, None, None, 0, 0, p, 1 << 40, _lib.TCMI_F32, None) == -1
     assert lib.tcmi_linear_cross_entropy_grad(p, 4, p, 4, None, p, -100, 2, 4, 4, p, p, 0, None, None, None, None, p, 1 << 40,
                                               _lib.TCMI_F32, None) == -1
 
