@@ -160,9 +160,11 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
 }
 
 // out[c][row] = src[row][c] * r[row] * scale as f16 pieces (two for f32), rows padded with zeros.  A zero factor gives zero
-// whatever the row holds.  ones: behind the last column one more, the factors themselves (their product with P is the
-// bias's gradient); 2 where all rows that count share one factor: its power of two only, which one piece holds exactly, the
-// epilogue multiplies the rest back (2^-11 of the factor would shift every entry the same way).  64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
+// whatever the row holds; an infinity anywhere else makes everything NaN (no scale would hold the rest beside it).
+// ones: behind the last column one more, the factors themselves (their product with P is the bias's gradient); 2 where all
+// rows that count share one factor: its power of two only, which one piece holds exactly, the epilogue multiplies the rest
+// back (2^-11 of the factor would shift every entry the same way).
+// 64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
 struct Turn {
   const void* src;
   long long rs;
@@ -174,7 +176,9 @@ struct Turn {
 };
 
 __device__ __forceinline__ float power_of(float f) { return __uint_as_float(__float_as_uint(f) & 0xff800000u); }
-__device__ __forceinline__ float mantissa_of(float f) { return __uint_as_float((__float_as_uint(f) & 0x007fffffu) | 0x3f800000u); }
+__device__ __forceinline__ float mantissa_of(float f) {
+  return f != f ? f : __uint_as_float((__float_as_uint(f) & 0x007fffffu) | 0x3f800000u);
+}
 
 template <int DT>
 __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
@@ -190,7 +194,8 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   if ((tid & 63) == 0) red[tid >> 6] = top;
   __syncthreads();
-  const float s = scale_of(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float s = top == INFINITY ? NAN : scale_of(top);
   const int r0 = block % a.tx * 64, c0 = block / a.tx * 64, u = (tid & 15) * 4, w = tid >> 4;
   if (block == 0 && tid == 0) *a.inv = 1.f / s;
 #pragma unroll
@@ -345,11 +350,11 @@ struct EpiLse {
 };
 
 // Up to 16 rows without a gradient (evaluating or serving single samples; before a gradient the logits of forward and
-// backward have to come from the same product, or exp(l - lse) - 1 of a certain row is their difference): w is read once, straight into the matrix instructions, whatever its
-// alignment, and no operand is copied.  A wave takes 32 classes at a time and keeps its rows' running maximum and sum of
-// exponentials; f32 heads use the f32 matrix instruction (exact products).  Bound by the read
-// of w: 10 x 3466 x 59851 bf16 124 us (3.3 TB/s; with copies and 128 x 128 tiles 436), 16 x 4096 x 65536 f32 256 us (4.2 TB/s; 707),
-// the same in bf16, which the tiles read in place, 130 us either way.
+// backward have to come from the same product, or exp(l - lse) - 1 of a certain row is their difference): w is read once,
+// straight into the matrix instructions, whatever its alignment, and no operand is copied.  A wave takes 32 classes at a time
+// and keeps its rows' running maximum and sum of exponentials; f32 heads use the f32 matrix instruction (exact products).
+// Bound by the read of w: 10 x 3466 x 59851 bf16 124 us (3.3 TB/s; with copies and 128 x 128 tiles 436), 16 x 4096 x 65536
+// f32 256 us (4.2 TB/s; 707), the same in bf16, which the tiles read in place, 130 us either way.
 constexpr int FEW_ROWS = 16, FEW_BLOCKS = 1024;
 
 template <int DT>
@@ -552,8 +557,8 @@ struct EpiProb {
   int vp, tp;                    // padded classes of the piece, padded rows
   template <class T>
   static constexpr int lds() { return Transposed<T, P>::BYTES; }
-  // P goes out from the registers, eight bytes a lane; P^T through LDS, sixteen (from the registers it would be two: 1021 x
-  // 28 x 16384 f32 took 50 us)
+  // P goes out from the registers, eight bytes a lane; P^T through LDS, sixteen (from the registers two, which alone took 50 us
+  // of 1021 x 28 x 16384 f32)
   template <class T>
   __device__ void tile(const Args& g, int m0, int n0, int, bool, char* lds, f32x4 (&acc)[T::MI][T::NI]) const {
     const Transposed<T, P> turned{reinterpret_cast<f16*>(lds)};

@@ -425,7 +425,7 @@ def newton_schulz(mat, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float 
 
     ``coefficients``: one triple ``(a, b, c)``, or one per step.  The default drives every singular value into about
     0.7 .. 1.2 in five steps (enough for an optimiser's update); ``(1.5, -0.5, 0)`` converges to the polar factor itself.
-    float32, bfloat16, float16, complex64; any strides; same shape and dtype out.  Differentiable once, including in
+    float32, bfloat16, float16, complex64; up to 65535 matrices; any strides; same shape and dtype out.  Differentiable once, including in
     ``backend.value_and_grad`` / ``vmap``: unlike the gradient of :func:`svd_trunc` its gradient has no
     ``1 / (s_i^2 - s_j^2)`` and holds at an isometry, where all singular values agree.  A zero matrix gives zero, a
     non-finite entry makes its whole matrix NaN.  Coefficients that let singular values grow past 64 are refused.

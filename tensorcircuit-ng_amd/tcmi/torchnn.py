@@ -47,6 +47,11 @@ TorchLayer = QuantumNet
 _REDUCTIONS = ("none", "sum", "mean")
 
 
+def _row_stride(x):
+    """elements between the rows of an operand; one row may carry any number there (an expanded one: 0)"""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
 def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
     """(loss, stat): h [T, D], w [V, D], target [T]; loss is per row for reduction "none".  stat, what the gradient needs: the
     rows' log sums, how many rows count, and (not "none") the rows' losses"""
@@ -61,7 +66,7 @@ def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
             loss.fill_(math.nan if reduction == "mean" else 0.0)
         return loss, stat.zero_()
     L = _lib.lib()
-    hp, hs, wp, ws, lse = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), stat.data_ptr()
+    hp, hs, wp, ws, lse = h.data_ptr(), _row_stride(h), w.data_ptr(), _row_stride(w), stat.data_ptr()
     nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_FOR_GRAD if for_grad else _lib.LCE_ALONE)
     if nbytes < 0:
         raise ValueError(f"linear_cross_entropy: {t} rows, {d} features, {v} classes are out of range")
@@ -84,7 +89,7 @@ def _lce_grad_raw(h, w, target, bias, stat, dloss, ignore_index, reduction, need
     code = linalg._train_code(h)
     dloss = dloss.to(torch.float32).contiguous()
     L = _lib.lib()
-    hp, hs, wp, ws, lse = h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0), stat.data_ptr()
+    hp, hs, wp, ws, lse = h.data_ptr(), _row_stride(h), w.data_ptr(), _row_stride(w), stat.data_ptr()
     nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_GRAD)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     ptrs = [None if o is None else o.data_ptr() for o in outs]
@@ -176,7 +181,12 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, target: Tensor, bias: Op
     Rows whose target is ``ignore_index`` have loss 0 and contribute nothing to any gradient, whatever they hold; the mean
     over no rows is NaN (its gradients are zero).  Any other target outside ``0 .. classes - 1`` gives NaN, in the loss and
     in the gradients (checked where the targets live, nothing is read out of range).  Classes may be masked by a bias
-    of ``-inf``.  A non-finite feature or weight gives NaN.  float64 (``tc.set_dtype("complex128")``) is refused."""
+    of ``-inf``.  A non-finite feature or weight of a row that counts gives NaN, or where the logits it makes are ``-inf`` a
+    class without probability and gradients of NaN.  float64 (``tc.set_dtype("complex128")``) is refused.
+
+    A training step may be captured into a graph (``torch.cuda.graph``).  As with any operator, let go of eager losses of the
+    same leaves first (torch ties a leaf's gradient to the stream of its oldest living graph), or capture
+    ``torch.autograd.grad`` instead of ``backward()``."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {_REDUCTIONS}, got {reduction!r}")
     if input.dim() < 1 or weight.dim() != 2 or input.shape[-1] != weight.shape[1]:
@@ -305,7 +315,8 @@ def muon_step(param: Tensor, grad: Tensor, momentum_buffer: Tensor, lr: float = 
 
 class Muon(torch.optim.Optimizer):
     """Optimiser of matrix-shaped parameters (:func:`muon_step` for each): ``QuantumNet``'s ``[layers, qubits]`` angles, the
-    weight of a classical head.  Vectors (biases) belong to another optimiser and are refused."""
+    weight of a classical head.  Vectors (biases) belong to another optimiser and are refused.  ``step`` may be captured into a
+    graph once every parameter has its momentum (after one eager step); the options of the captured step are fixed in it."""
 
     def __init__(self, params: Any, lr: float = 1e-3, weight_decay: float = 0.1, momentum: float = 0.95, nesterov: bool = True,
                  ns_coefficients: Any = linalg.NS_COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
@@ -345,6 +356,9 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("Muon: take one step before the capture (a captured first step would clear the "
+                                           "momentum on every replay)")
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 muon_step(p, p.grad, state["momentum_buffer"], **{k: group[k] for k in self.defaults})   # not a scheduler's keys
         return loss

@@ -442,6 +442,50 @@ def test_linear_cross_entropy_layouts(dtype):
             assert bool(((g - ref).cpu().double().abs() <= slack).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_cross_entropy_one_row_or_class_of_an_expanded_operand(dtype):
+    """one row cut from an expanded tensor carries stride 0, whether it is the input or the weight"""
+    from tcmi import torchnn
+
+    h, w, y, _ = _ce_inputs(94, 1, 64, 300, dtype, bias=False)
+    for grads in (False, True):
+        hd, wd = h.cuda().requires_grad_(grads), w.cuda().requires_grad_(grads)
+        want = torchnn.linear_cross_entropy(hd, wd, y.cuda())
+        row = hd[0].expand(4, 64)[:1]
+        assert row.stride(0) == 0
+        got = torchnn.linear_cross_entropy(row, wd, y.cuda())
+        assert torch.equal(got, want)
+        if grads:
+            for a, e in zip(torch.autograd.grad(got, (hd, wd)), torch.autograd.grad(want, (hd, wd))):
+                assert torch.equal(a, e)
+        # one class: the loss is log 1 and no gradient is left
+        only = wd[0].expand(4, 64)[:1]
+        loss = torchnn.linear_cross_entropy(hd, only, torch.zeros(1, dtype=torch.int64, device="cuda"))
+        assert float(loss) == 0.0
+        if grads:
+            for a in torch.autograd.grad(loss, (hd, wd)):
+                assert bool((a == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_cross_entropy_infinities_do_not_pass_for_numbers(dtype):
+    """a weight of -inf makes every gradient that it could enter NaN, never a number at a lost scale; so does a NaN loss factor"""
+    from tcmi import torchnn
+
+    h, w, y, b = _ce_inputs(95, 40, 30, 300, dtype)
+    h[:, 3] = h[:, 3].abs() + 0.5
+    w[5, 3] = -math.inf
+    y[y == 5] = 6
+    hd, wd, bd = (t.cuda().requires_grad_() for t in (h, w, b))
+    (dh,) = torch.autograd.grad(torchnn.linear_cross_entropy(hd, wd, y.cuda(), bd), hd)
+    assert bool(torch.isnan(dh).all())
+    for reduction, dloss in (("mean", torch.tensor(math.nan)), ("none", torch.full((40,), math.nan))):
+        hd, wd, bd = (t.cuda().requires_grad_() for t in (h, w.nan_to_num(neginf=0.0), b))
+        loss = torchnn.linear_cross_entropy(hd, wd, y.cuda(), bd, reduction=reduction)
+        for g in torch.autograd.grad(loss, (hd, wd, bd), dloss.cuda()):
+            assert bool(torch.isnan(g).all())
+
+
 def test_linear_cross_entropy_in_pieces():
     """enough rows that the classes are gone through in several pieces"""
     from tcmi import torchnn
@@ -545,6 +589,34 @@ def test_muon_strides():
     assert float((pd.cpu().double() - want).norm()) <= 0.02 * math.sqrt(50 / 40) * _ns_tol(torch.float32) * float(o.norm()) + 2.0 ** -22 * float(want.norm())
     assert bool((big[:, 1::2] == 0).all()) and torch.equal(vd[1::2].cpu(), v[1::2])
     assert float((vd[::2].cpu().double() - wv).norm()) <= 2.0 ** -22 * float(wv.norm())
+
+
+def test_muon_is_not_captured_before_its_first_step(monkeypatch):
+    """a captured first step would clear the momentum on every replay: refused (the capture is only pretended here)"""
+    from tcmi import torchnn
+
+    p = torch.nn.Parameter(_rand(133, 8, 6).cuda())
+    p.grad = _rand(134, 8, 6).cuda()
+    opt = torchnn.Muon([p])
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            opt.step()
+    assert not opt.state[p]
+    opt.step()
+    p.grad = _rand(135, 8, 6).cuda()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for rep in range(3):
+        twin = torch.nn.Parameter(p.detach().clone())
+        twin.grad = p.grad.clone()
+        other = torchnn.Muon([twin])
+        other.state[twin]["momentum_buffer"] = opt.state[p]["momentum_buffer"].clone()
+        other.step()
+        graph.replay()
+        assert torch.equal(p, twin) and torch.equal(opt.state[p]["momentum_buffer"], other.state[twin]["momentum_buffer"])
 
 
 # ---------------------------------------------------------------------------------------- graphs, streams, together
