@@ -539,8 +539,9 @@ __global__ __launch_bounds__(256) void grad_out_kernel(Mat gm, const float* d, l
 
 // ------------------------------------------------------------------------------------------- matrices that fit one CU
 // One workgroup per matrix, everything in LDS, f32 matrix instructions (exact products): one launch instead of four per
-// step.  Taken when a step's operands fit 160 KB of LDS.  Bound by the latency of the chain load -> norm -> 3 products a
-// step -> store: five steps of a 24 x 28 matrix are 15 dependent products.
+// step.  Taken when a step's operands fit 160 KB of LDS and the columns are few (small_bytes).  Bound by the latency of the chain
+// load -> norm -> 3 products a step -> store: five steps of a 24 x 28 matrix are 15 dependent products, 10.6 us of kernel
+// (with branches around all eight tiles a wave could have, and the tiles' places kept per lane: 14.3).
 // Fragments: of 16 consecutive k, lane group g = lane >> 4 takes k = 4 g .. 4 g + 3 (the sum does not care which lane holds
 // which k), so a row operand is one 16-byte LDS read and a column operand four 4-byte reads; with rows 4 (mod 8) floats
 // apart neither has bank conflicts.
@@ -562,7 +563,7 @@ __host__ __device__ inline SmallShape small_shape(int m, int n, int cx) {
   return s;
 }
 
-constexpr int SMALL_THREADS = 512, SMALL_WAVES = 8, SMALL_TILES = 8;        // 16 x 16 tiles per wave in the update
+constexpr int SMALL_THREADS = 512, SMALL_WAVES = 8, SMALL_TILES = 8;        // 16 x 16 tiles per wave in the update, at most
 
 struct SmallArgs {
   Mat src, dy;
@@ -590,29 +591,49 @@ __device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {
 // sum_k p[i][k] q[j][k] for one 16 x 16 tile; lane holds rows 4 (lane >> 4) + r, column lane & 15
 __device__ __forceinline__ f32x4 rows_rows(const float* p, const float* q, int ld, int K, f32x4 c) {
   const int at = (threadIdx.x & 15) * ld + 4 * ((threadIdx.x & 63) >> 4);
-  for (int k = 0; k < K; k += 16)
-    c = mfma4(*reinterpret_cast<const f32x4*>(p + at + k), *reinterpret_cast<const f32x4*>(q + at + k), c);
-  return c;
+  p += at;
+  q += at;
+  f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(q);
+  for (int k = 16; k < K; k += 16) {                 // the next reads go out before the products that wait for these
+    const f32x4 na = *reinterpret_cast<const f32x4*>(p + k), nb = *reinterpret_cast<const f32x4*>(q + k);
+    __builtin_amdgcn_sched_barrier(0);
+    c = mfma4(a, b, c);
+    a = na;
+    b = nb;
+  }
+  return mfma4(a, b, c);
 }
 
 // sum_k p[i][k] x[k][j]
 __device__ __forceinline__ f32x4 rows_cols(const float* p, int ldp, const float* x, int ldx, int K, f32x4 c) {
   const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-  for (int k = 0; k < K; k += 16) {
-    const float* xx = x + (k + 4 * g) * ldx + l;
-    c = mfma4(*reinterpret_cast<const f32x4*>(p + l * ldp + 4 * g + k), f32x4{xx[0], xx[ldx], xx[2 * ldx], xx[3 * ldx]}, c);
+  p += l * ldp + 4 * g;
+  x += 4 * g * ldx + l;
+  f32x4 a = *reinterpret_cast<const f32x4*>(p), b = {x[0], x[ldx], x[2 * ldx], x[3 * ldx]};
+  for (int k = 16; k < K; k += 16) {
+    x += 16 * ldx;
+    const f32x4 na = *reinterpret_cast<const f32x4*>(p + k), nb = {x[0], x[ldx], x[2 * ldx], x[3 * ldx]};
+    __builtin_amdgcn_sched_barrier(0);
+    c = mfma4(a, b, c);
+    a = na;
+    b = nb;
   }
-  return c;
+  return mfma4(a, b, c);
 }
+
+__device__ __forceinline__ int small_wave() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6); }
 
 // f(i0, j0) for the tiles on and below the diagonal, dealt to the waves
 template <class F>
 __device__ __forceinline__ void lower_tiles(int R16, F f) {
-  const int wave = threadIdx.x >> 6, t = R16 / 16;
-  int k = 0;
-  for (int i = 0; i < t; ++i)
-    for (int j = 0; j <= i; ++j, ++k)
-      if (k % SMALL_WAVES == wave) f(i * 16, j * 16);
+  const int t = R16 / 16;
+  int i = 0, j = small_wave();
+  while (true) {
+    while (j > i) j -= ++i;                          // a row of tiles holds one more than the one above
+    if (i >= t) return;
+    f(i * 16, j * 16);
+    j += SMALL_WAVES;
+  }
 }
 
 __device__ __forceinline__ void put_both(float* a, int lda, int i0, int j0, f32x4 v) {
@@ -667,8 +688,8 @@ __device__ __forceinline__ void gram(const float* X, float* A, const SmallShape&
 
 __device__ __forceinline__ void poly(const float* A, float* Bm, const SmallShape& s, float b, float c) {
   lower_tiles(s.R16, [&](int i0, int j0) {
-    const f32x4 v = rows_rows(A + i0 * s.lda, A + j0 * s.lda, s.lda, s.R16, f32x4{0.f, 0.f, 0.f, 0.f});
     const f32x4 a = get_tile(A, s.lda, i0, j0);
+    const f32x4 v = rows_rows(A + i0 * s.lda, A + j0 * s.lda, s.lda, s.R16, f32x4{0.f, 0.f, 0.f, 0.f});
     f32x4 o;
 #pragma unroll
     for (int r = 0; r < 4; ++r) o[r] = fmaf(c, v[r], b * a[r]);
@@ -677,25 +698,25 @@ __device__ __forceinline__ void poly(const float* A, float* Bm, const SmallShape
 }
 
 // X <- a X + B X (+ Q Y): all waves finish reading before any writes
-template <bool TWO>
+template <bool TWO, int SLOTS>
 __device__ __forceinline__ void update(float* X, const float* Bm, const float* Q, const float* Y, const SmallShape& s, float a) {
-  const int wave = threadIdx.x >> 6, tc = s.C16 / 16, tiles = tc * (s.R16 / 16);
-  f32x4 res[SMALL_TILES];
+  const int wave = small_wave(), tc = s.C16 / 16, tiles = tc * (s.R16 / 16);
+  f32x4 res[SLOTS];
 #pragma unroll
-  for (int u = 0; u < SMALL_TILES; ++u) {
+  for (int u = 0; u < SLOTS; ++u) {
     const int t = wave + u * SMALL_WAVES;
     if (t < tiles) {
       const int i0 = t / tc * 16, j0 = t % tc * 16;
+      const f32x4 x = get_tile(X, s.ldx, i0, j0);
       f32x4 v = rows_cols(Bm + i0 * s.lda, s.lda, X + j0, s.ldx, s.R16, f32x4{0.f, 0.f, 0.f, 0.f});
       if (TWO) v = rows_cols(Q + i0 * s.lda, s.lda, Y + j0, s.ldx, s.R16, v);
-      const f32x4 x = get_tile(X, s.ldx, i0, j0);
 #pragma unroll
       for (int r = 0; r < 4; ++r) res[u][r] = fmaf(a, x[r], v[r]);
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < SMALL_TILES; ++u) {
+  for (int u = 0; u < SLOTS; ++u) {
     const int t = wave + u * SMALL_WAVES;
     if (t < tiles) {
       float* p = X + (t / tc * 16 + 4 * ((threadIdx.x & 63) >> 4)) * s.ldx + t % tc * 16 + (threadIdx.x & 15);
@@ -706,7 +727,7 @@ __device__ __forceinline__ void update(float* X, const float* Bm, const float* Q
   __syncthreads();
 }
 
-template <int SRC>
+template <int SRC, int SLOTS>
 __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs a) {
   extern __shared__ __attribute__((aligned(16))) float mem[];
   __shared__ double red[SMALL_WAVES];
@@ -739,11 +760,12 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs a) {
       float* w = a.saved + (bz * a.steps + t) * s.m * s.C;
       for (int k = threadIdx.x; k < s.m * s.C; k += SMALL_THREADS) w[k] = X[k / s.C * s.ldx + k % s.C];
     }
+    const float ca = a.coef[3 * t], cb = a.coef[3 * t + 1], cc = a.coef[3 * t + 2];
     gram(X, A, s);
     __syncthreads();
-    poly(A, Bm, s, a.coef[3 * t + 1], a.coef[3 * t + 2]);
+    poly(A, Bm, s, cb, cc);
     __syncthreads();
-    update<false>(X, Bm, nullptr, nullptr, s, a.coef[3 * t]);
+    update<false, SLOTS>(X, Bm, nullptr, nullptr, s, ca);
   }
   for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
     int i, j;
@@ -761,7 +783,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs a) {
   }
 }
 
-template <int SRC>
+template <int SRC, int SLOTS>
 __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) {
   extern __shared__ __attribute__((aligned(16))) float mem[];
   __shared__ double red[SMALL_WAVES];
@@ -778,7 +800,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
   }
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   for (int t = a.steps - 1; t >= 0; --t) {
-    const float *w = a.saved + (bz * a.steps + t) * s.m * s.C, b = a.coef[3 * t + 1], c = a.coef[3 * t + 2];
+    const float *w = a.saved + (bz * a.steps + t) * s.m * s.C, ca = a.coef[3 * t], b = a.coef[3 * t + 1], c = a.coef[3 * t + 2];
     for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
       const int i = k / s.n, j = k % s.n;
       embed(X, s.ldx, s, i, j, make_float2(w[i * s.C + j], s.cx == 2 ? w[i * s.C + j + s.n] : 0.f));
@@ -801,7 +823,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
       put_both(Q, s.lda, i0, j0, o);
     });
     __syncthreads();
-    update<true>(D, Bm, Q, X, s, a.coef[3 * t]);
+    update<true, SLOTS>(D, Bm, Q, X, s, ca);
   }
   double sum = 0.0;
   for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
@@ -958,12 +980,17 @@ __device__ __forceinline__ f64x4 rows64(const double* p, const double* q, int ld
   const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
   p += l * ld + 2 * g;
   q += l * ld + 2 * g;
-  for (int k = 0; k < R16; k += 8) {
-    const f64x2 x = *reinterpret_cast<const f64x2*>(p + k), y = *reinterpret_cast<const f64x2*>(q + k);
+  f64x2 x = *reinterpret_cast<const f64x2*>(p), y = *reinterpret_cast<const f64x2*>(q);
+  for (int k = 8; k < R16; k += 8) {                 // the next reads go out before the products that wait for these
+    const f64x2 nx = *reinterpret_cast<const f64x2*>(p + k), ny = *reinterpret_cast<const f64x2*>(q + k);
+    __builtin_amdgcn_sched_barrier(0);
     c = mfma64(x[0], y[0], c);
     c = mfma64(x[1], y[1], c);
+    x = nx;
+    y = ny;
   }
-  return c;
+  c = mfma64(x[0], y[0], c);
+  return mfma64(x[1], y[1], c);
 }
 
 // f(i0, j0) for the tiles dealt to the waves; LOWER: on and below the diagonal
@@ -1478,9 +1505,17 @@ void pair(Args& g, const f16* a, const f16* b) {
 
 constexpr int SMALL_LDS = 156 * 1024;        // of 160 KB: the reductions take a little
 
-// bytes of LDS of the one-workgroup form; 0: it does not fit
+bool thin_fits(const Shape& s, bool grad) { return s.mr <= (grad ? THIN_GRAD_R : THIN_R); }
+
+// Where the two-pass form could take the matrix too, the one-workgroup form stops here: its time grows with the columns, the
+// other's chain of m x m products does not.  Result / gradient of one f32 matrix in us, one workgroup and two passes:
+// 8 x 192 17 / 33 and 20 / 37, 8 x 320 25 / 49 and 20 / 38, 24 x 192 29 / 54 and 31 / 66, 24 x 320 43 / 80 and 31 / 67,
+// 56 x 192 61 and 81, 56 x 320 80 and 80; 2000 x 8 x 300 101 / 252 and 97 / 200.
+constexpr int SMALL_COLS = 240;
+
+// bytes of LDS of the one-workgroup form; 0: it does not fit, or another is quicker
 int small_bytes(const Shape& s, bool grad) {
-  if (s.mr > 512 || s.nc > 4096) return 0;
+  if (s.mr > 512 || s.nc > 4096 || (thin_fits(s, grad) && s.nc > SMALL_COLS)) return 0;
   const SmallShape q = small_shape(s.m, s.n, s.cx);
   if ((q.R16 / 16) * (q.C16 / 16) > SMALL_WAVES * SMALL_TILES) return 0;
   const long long b = 4ll * ((grad ? 2 : 1) * q.R16 * q.ldx + (grad ? 4 : 2) * q.R16 * q.lda);
@@ -1499,23 +1534,33 @@ SmallSaved take_small(Arena& w, const Shape& s, int steps) {
   return v;
 }
 
-template <int SRC, bool GRAD>
+template <int SRC, bool GRAD, int SLOTS>
 hipError_t small_launch(const SmallArgs& a, int bytes, int batch, hipStream_t st) {
-  const void* f = GRAD ? reinterpret_cast<const void*>(small_grad_kernel<SRC>) : reinterpret_cast<const void*>(small_kernel<SRC>);
+  const void* f = GRAD ? reinterpret_cast<const void*>(small_grad_kernel<SRC, SLOTS>) : reinterpret_cast<const void*>(small_kernel<SRC, SLOTS>);
   static std::atomic<unsigned long long> done{0};
   const hipError_t e = raise_lds(f, SMALL_LDS, done);
   if (e != hipSuccess) return e;
-  if (GRAD) hipLaunchKernelGGL(small_grad_kernel<SRC>, dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
-  else hipLaunchKernelGGL(small_kernel<SRC>, dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
+  if (GRAD) hipLaunchKernelGGL((small_grad_kernel<SRC, SLOTS>), dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
+  else hipLaunchKernelGGL((small_kernel<SRC, SLOTS>), dim3(batch), dim3(SMALL_THREADS), bytes, st, a);
   return hipGetLastError();
+}
+
+// as many tiles a wave as the matrix needs: the branches around those that it lacks are what a step of a small one waits for
+template <int SRC, bool GRAD>
+hipError_t small_slots(const SmallArgs& a, int bytes, int batch, hipStream_t st) {
+  const SmallShape q = small_shape(a.m, a.n, a.cx);
+  const int tiles = (q.R16 / 16) * (q.C16 / 16);
+  if (tiles <= SMALL_WAVES) return small_launch<SRC, GRAD, 1>(a, bytes, batch, st);
+  if (tiles <= 2 * SMALL_WAVES) return small_launch<SRC, GRAD, 2>(a, bytes, batch, st);
+  return small_launch<SRC, GRAD, SMALL_TILES>(a, bytes, batch, st);
 }
 
 template <bool GRAD>
 hipError_t small_by_type(int src, const SmallArgs& a, int bytes, int batch, hipStream_t st) {
-  if (src == SRC_F32) return small_launch<SRC_F32, GRAD>(a, bytes, batch, st);
-  if (src == SRC_F16) return small_launch<SRC_F16, GRAD>(a, bytes, batch, st);
-  if (src == SRC_BF16) return small_launch<SRC_BF16, GRAD>(a, bytes, batch, st);
-  return small_launch<SRC_C64, GRAD>(a, bytes, batch, st);
+  if (src == SRC_F32) return small_slots<SRC_F32, GRAD>(a, bytes, batch, st);
+  if (src == SRC_F16) return small_slots<SRC_F16, GRAD>(a, bytes, batch, st);
+  if (src == SRC_BF16) return small_slots<SRC_BF16, GRAD>(a, bytes, batch, st);
+  return small_slots<SRC_C64, GRAD>(a, bytes, batch, st);
 }
 
 #define TRY(x)                                   \
@@ -1672,8 +1717,6 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
 }
 
 // ---- few rows, long columns
-bool thin_fits(const Shape& s, bool grad) { return s.mr <= (grad ? THIN_GRAD_R : THIN_R); }
-
 int thin_r16(const Shape& s) { return (s.mr + 15) & ~15; }
 
 int thin_chunks(const Shape& s) { return (s.n + THIN_COLS - 1) / THIN_COLS; }

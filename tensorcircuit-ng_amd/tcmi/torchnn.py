@@ -60,22 +60,30 @@ def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
     code = linalg._train_code(h)
     per_row = reduction == "none"
     loss = torch.empty(t if per_row else (), dtype=torch.float32, device=h.device)
-    stat = torch.empty(t + 1 if per_row else 2 * t + 1, dtype=torch.float32, device=h.device)
     if t == 0:
+        stat = torch.empty(1, dtype=torch.float32, device=h.device)
         if not per_row:
             loss.fill_(math.nan if reduction == "mean" else 0.0)
         return loss, stat.zero_()
     L = _lib.lib()
-    hp, hs, wp, ws, lse = h.data_ptr(), _row_stride(h), w.data_ptr(), _row_stride(w), stat.data_ptr()
+    hp, hs, wp, ws = h.data_ptr(), _row_stride(h), w.data_ptr(), _row_stride(w)
     nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_FOR_GRAD if for_grad else _lib.LCE_ALONE)
     if nbytes < 0:
         raise ValueError(f"linear_cross_entropy: {t} rows, {d} features, {v} classes are out of range")
-    work = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+    floats = t + 1 if per_row else 2 * t + 1
+    if for_grad:
+        stat = torch.empty(floats, dtype=torch.float32, device=h.device)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+        lse = stat.data_ptr()
+    else:                            # nobody needs them after the call: the workspace's tail
+        stat, work = None, torch.empty(nbytes + 4 * floats, dtype=torch.uint8, device=h.device)
+        lse = work.data_ptr() + nbytes
     with linalg._on(h.device):
         _lib.check(L.tcmi_linear_cross_entropy(
             hp, hs, wp, ws, None if bias is None else bias.data_ptr(), target.data_ptr(), ignore_index, t, d, v, lse,
             loss.data_ptr() if per_row else lse + 4 * (t + 1), None if per_row else loss.data_ptr(), lse + 4 * t,
-            int(reduction == "mean"), int(for_grad), work.data_ptr(), nbytes, code, linalg._stream(h)), "tcmi_linear_cross_entropy")
+            int(reduction == "mean"), int(for_grad), work.data_ptr(), nbytes, code, linalg._raw_stream(h.device)),
+            "tcmi_linear_cross_entropy")
     return loss, stat
 
 
@@ -97,7 +105,7 @@ def _lce_grad_raw(h, w, target, bias, stat, dloss, ignore_index, reduction, need
         _lib.check(L.tcmi_linear_cross_entropy_grad(
             hp, hs, wp, ws, None if bias is None else bias.data_ptr(), target.data_ptr(), ignore_index, t, d, v, lse,
             dloss.data_ptr(), int(reduction == "none"), lse + 4 * t if reduction == "mean" else None, *ptrs, work.data_ptr(),
-            nbytes, code, linalg._stream(h)), "tcmi_linear_cross_entropy_grad")
+            nbytes, code, linalg._raw_stream(dev)), "tcmi_linear_cross_entropy_grad")
     return tuple(torch.empty(0, device=dev) if o is None else o for o in outs)
 
 
@@ -206,13 +214,13 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, target: Tensor, bias: Op
     if target.dtype != torch.int64:
         raise TypeError(f"linear_cross_entropy: target must be int64, got {target.dtype}")
     linalg._need_gpu("linear_cross_entropy", input, weight, target, bias)
-    h = input.reshape(-1, input.shape[-1])
+    h = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])
     w = weight
     # features contiguous, rows apart (a broadcast or transposed operand is copied; autograd takes its gradient back)
     h = h if h.stride(1) == 1 and h.stride(0) >= h.shape[1] else h.contiguous()
     w = w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] else w.contiguous()
     b = None if bias is None else bias.contiguous()
-    y = target.reshape(-1).contiguous()
+    y = (target if target.dim() == 1 else target.reshape(-1)).contiguous()
     args = (h, w, y, b, int(ignore_index), reduction)
     if not linalg._tracked(h, w, b, y):
         loss = _lce_raw(*args, False)[0]
@@ -308,7 +316,7 @@ def muon_step(param: Tensor, grad: Tensor, momentum_buffer: Tensor, lr: float = 
                 p.data_ptr(), p.stride(1), p.stride(2), p.stride(0), g.data_ptr(), g.stride(1), g.stride(2), g.stride(0),
                 v.data_ptr(), v.stride(1), v.stride(2), v.stride(0), m, n, b, float(momentum), int(bool(nesterov)),
                 1.0 - float(lr) * float(weight_decay), -float(lr) * r, steps, linalg._host_doubles(flat), float(eps), full,
-                work.data_ptr(), work.numel(), code, linalg._stream(p)), "tcmi_muon_step")
+                work.data_ptr(), nbytes, code, linalg._raw_stream(p.device)), "tcmi_muon_step")
         torch.autograd.graph.increment_version(param)
         torch.autograd.graph.increment_version(momentum_buffer)
 

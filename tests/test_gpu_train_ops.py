@@ -199,6 +199,25 @@ def test_newton_schulz_grad(shape, dtype):
             assert _rel(got, want) < _ns_grad_tol(x, dy, want, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(8, 120), (8, 121), (240, 7), (13, 241), (17, 239), (16, 256), (32, 240), (241, 32), (60, 242)])
+def test_newton_schulz_where_its_forms_meet(shape, dtype):
+    """short sides around the number of columns at which one workgroup gives way to two passes, and both sides of every
+    number of tiles a wave holds"""
+    from tcmi import linalg
+
+    x, dy = _rand(30, 3, *shape, dtype=dtype), _rand(31, 3, *shape, dtype=dtype)
+    plain = linalg.newton_schulz(x.cuda())
+    leaf = x.cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf)
+    (got,) = torch.autograd.grad(out, leaf, dy.cuda())
+    for k in range(3):
+        want = _ns64(x[k])
+        assert _rel(plain[k], want) < _ns_tol(dtype) and _rel(out[k], want) < _ns_tol(dtype)
+        want = _ns_grad64(x[k], dy[k])
+        assert _rel(got[k], want) < _ns_grad_tol(x[k], dy[k], want, dtype)
+
+
 def test_newton_schulz_grad_against_differences():
     """and at an isometry, where the gradient of an SVD does not exist"""
     from tcmi import linalg
