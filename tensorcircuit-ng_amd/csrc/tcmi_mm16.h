@@ -344,6 +344,22 @@ struct Transposed {
       if (P == 2) *reinterpret_cast<f16x8*>(o + 32) = *reinterpret_cast<const f16x8*>(lds + (T::BN + c) * LINE + rl);
     }
   }
+  // the other half of a doubled complex matrix: row c of the transpose goes to row c + n (the real part, c < n), or negated to
+  // row c - n, `cols` columns further on (cols and n multiples of 16)
+  __device__ __forceinline__ void flush_twin(f16* base, long long ld, int n0, int rows, int m0, int cols, int n) const {
+    for (int k = threadIdx.x; k < T::BN * (T::BM / 8); k += T::THREADS) {
+      const int c = k / (T::BM / 8), rl = k % (T::BM / 8) * 8;
+      if (n0 + c >= rows || m0 + rl >= cols) continue;
+      const bool im = n0 + c >= n;
+      f16* o = base + (long long)(n0 + c + (im ? -n : n)) * ld + kpos<P>(m0 + rl + cols);
+      f16x8 v = *reinterpret_cast<const f16x8*>(lds + c * LINE + rl);
+      *reinterpret_cast<f16x8*>(o) = im ? -v : v;
+      if (P == 2) {
+        v = *reinterpret_cast<const f16x8*>(lds + (T::BN + c) * LINE + rl);
+        *reinterpret_cast<f16x8*>(o + 32) = im ? -v : v;
+      }
+    }
+  }
 };
 
 // ---- host side ----

@@ -141,6 +141,9 @@ __global__ __launch_bounds__(256) void sums_kernel(SumArgs a) {
   if (threadIdx.x == 0) a.part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
+// 1 / d as f32; 0 for 0, and finite for norms that only subnormal numbers have
+__device__ __forceinline__ float inverse(double d) { return d == 0.0 ? 0.f : d < 3e-39 ? 3e38f : (float)(1.0 / d); }
+
 // Operand layout: a 64 x 64 tile of the source becomes f16 pieces, row-major and transposed (both k-contiguous for the
 // products that read them), zero beyond the matrix up to the padded length, and the f32 carry.  Bound by its writes.
 // part: the tile is divided by (sqrt(sum of part) + eps); every workgroup adds the partial sums itself.
@@ -176,8 +179,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     for (int k = threadIdx.x; k < a.npart; k += 256) s += a.part[(long long)bz * a.npart + k];
     const double nrm = sqrt(block_sum(s, red));
     if (a.norm_out && t == 0 && threadIdx.x == 0) a.norm_out[bz] = (float)nrm;
-    const double d = nrm + (double)a.eps;
-    inv = d == 0.0 ? 0.f : (float)(1.0 / d);
+    inv = inverse(nrm + (double)a.eps);
   }
   // 16 threads along an axis, four elements each, 16 lines at a time
   const long long base = (long long)bz * a.src.bs;
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     }
   }
   __syncthreads();
-  const float cinv = a.carry_raw ? 1.f : inv, xs = inv * a.scale;
+  const float cinv = a.carry_raw ? 1.f : inv;
   const bool twice = MAYBE_COMPLEX && a.embed;
   const int mrows = twice ? a.m : (int)kpad(a.m, P), ncols = twice ? a.n : (int)kpad(a.n, P);
   f16 *px = a.x + (long long)bz * a.os, *pt = a.t + (long long)bz * a.ts;
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       f16 h, l;
-      two_pieces(v[e] * xs, h, l);
+      two_pieces(v[e] * inv * a.scale, h, l);
       hi[e] = h;
       lo[e] = l;
     }
@@ -386,7 +388,9 @@ struct EpiCarry {
 };
 
 // A step's result as the next step's operands: x = beta carry + alpha acc stays in the carry and goes out as pieces, row-major
-// and (through LDS) transposed.  Real matrices; saves the pass that would read the carry again (27 us a step of 4096 x 4096).
+// and (through LDS) transposed.  Saves the pass that would read the carry again (27 us a step of 4096 x 4096).  Complex
+// matrices (n > 0: columns of the imaginary part start there) need sides that are multiples of 16: the product forms the
+// upper half [Re, Im], and the lower one [-Im, Re] is written beside it.
 template <int P>
 struct EpiNext {
   static constexpr bool TILE = true, FOUR = true;
@@ -395,8 +399,11 @@ struct EpiNext {
   float alpha, beta, scale;
   f16 *x, *t;
   long long ld, xs, ldt, ts;
+  int n;
   template <class T>
   static constexpr int lds() { return Transposed<T, P>::BYTES; }
+  // rows of X^T that hold values or their padding
+  __device__ __forceinline__ int tall(const Args& g) const { return n ? g.M : (int)kpad(g.M, P); }
   __device__ __forceinline__ void put_row(const Args& g, int bz, int row, int col, f32x4 v, f16x4& vh, f16x4& vl) const {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     if (row < g.M && col < g.N) {                    // rows of the carry are padded to four columns
@@ -413,18 +420,31 @@ struct EpiNext {
       vh[r] = a;
       vl[r] = b;
     }
-    if (row < g.M && col < (int)kpad(g.N, P)) store_four<P>(x + bz * xs + row * ld, col, vh, vl);
+    if (row < g.M && col < (int)kpad(g.N, P)) {
+      f16* o = x + bz * xs + row * ld;
+      store_four<P>(o, col, vh, vl);
+      if (n) {
+        if (col < n) store_four<P>(o + g.M * ld, col + n, vh, vl);
+        else store_four<P>(o + g.M * ld, col - n, -vh, -vl);
+      }
+    }
   }
   __device__ __forceinline__ void four(const Args& g, int bz, bool, int row, int col, f32x4 v) const {
     f16x4 vh, vl;
     put_row(g, bz, row, col, v, vh, vl);
-    if (row >= (int)kpad(g.M, P)) return;
+    if (row >= tall(g)) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (col + r < g.N) {
         f16* o = t + bz * ts + (col + r) * ldt + kpos<P>(row);
         o[0] = vh[r];
         if (P == 2) o[32] = vl[r];
+        if (n) {
+          const bool im = col >= n;
+          o = t + bz * ts + (col + r + (im ? -n : n)) * ldt + kpos<P>(row + g.M);
+          o[0] = im ? -vh[r] : vh[r];
+          if (P == 2) o[32] = im ? -vl[r] : vl[r];
+        }
       }
   }
   template <class T>
@@ -437,7 +457,8 @@ struct EpiNext {
       turned.stage(row - m0, col - n0, vh, vl);
     });
     __syncthreads();
-    turned.flush(t + bz * ts, ldt, n0, g.N, m0, (int)kpad(g.M, P));
+    turned.flush(t + bz * ts, ldt, n0, g.N, m0, tall(g));
+    if (n) turned.flush_twin(t + bz * ts, ldt, n0, g.N, m0, g.M, n);
   }
 };
 
@@ -511,17 +532,18 @@ struct EpiOut {
   }
 };
 
-// dG = D / N - G <D, G> / (N^2 |G|)
+// dG = D / N - G <D, G> / (N^2 |G|); d holds D, or D / dnorm
 template <int SRC>
 __global__ __launch_bounds__(256) void grad_out_kernel(Mat gm, const float* d, long long ldd, long long dbs, int m, int n,
-                                                       const double* part, int npart, const float* norm, float eps, void* out,
+                                                       const double* part, int npart, const float* norm, const float* dnorm, float eps, void* out,
                                                        long long rs, long long cs, long long os, int dtype) {
   __shared__ double red[4];
   const int bz = blockIdx.y;
   double s = 0.0;
   for (int k = threadIdx.x; k < npart; k += 256) s += part[(long long)bz * npart + k];
   const double inner = block_sum(s, red), nr = norm[bz], full = nr + (double)eps;
-  const float f1 = full == 0.0 ? 0.f : (float)(1.0 / full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * full * nr));
+  const double by = dnorm ? (double)dnorm[bz] : 1.0;
+  const float f1 = full == 0.0 ? 0.f : (float)(by / full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * nr));
   const long long total = (long long)m * n;
   for (long long k = blockIdx.x * 256ll + threadIdx.x; k < total; k += gridDim.x * 256ll) {
     // the source decides the order: consecutive threads along its contiguous axis
@@ -530,10 +552,70 @@ __global__ __launch_bounds__(256) void grad_out_kernel(Mat gm, const float* d, l
     const float* dd = d + bz * dbs + i * ldd + j;
     const long long at = bz * os + i * rs + j * cs;
     if (SRC == SRC_C64) {
-      ((float2*)out)[at] = make_float2(dd[0] * f1 - g.x * f2, dd[n] * f1 - g.y * f2);
+      ((float2*)out)[at] = make_float2((dd[0] - g.x * f2) * f1, (dd[n] - g.y * f2) * f1);
     } else {
-      put(out, dtype, at, dd[0] * f1 - g.x * f2);
+      put(out, dtype, at, (dd[0] - g.x * f2) * f1);
     }
+  }
+}
+
+// The same two steps, <D, G> and dG, for a G that is contiguous along its columns (a matrix taller than wide): D lies across
+// it, so 64 x 64 tiles of D pass through LDS (62 x 256 x 128 complex64: 17 + 15 us; read across 36 + 29).
+struct TurnedArgs {
+  Mat g;
+  const float* d;
+  long long ldd, dbs;
+  int m, n, tx, tiles, npart;
+  double* part;                  // [batch][npart]; the sums write it, one value a workgroup
+  const float *norm, *dnorm;
+  float eps;
+  void* out;
+  long long rs, cs, os;
+  int dtype;
+};
+
+template <int SRC, bool OUT>
+__global__ __launch_bounds__(256) void turned_kernel(TurnedArgs a) {
+  __shared__ float re[64][65], im[SRC == SRC_C64 ? 64 : 1][65];
+  __shared__ double red[4];
+  const int bz = blockIdx.y, u = threadIdx.x & 63, w = threadIdx.x >> 6;
+  double s = 0.0;
+  float f1 = 0.f, f2 = 0.f;
+  if (OUT) {
+    for (int k = threadIdx.x; k < a.npart; k += 256) s += a.part[(long long)bz * a.npart + k];
+    const double inner = block_sum(s, red), nr = a.norm[bz], full = nr + (double)a.eps, by = a.dnorm ? (double)a.dnorm[bz] : 1.0;
+    f1 = full == 0.0 ? 0.f : (float)(by / full);
+    f2 = nr == 0.0 ? 0.f : (float)(inner / (full * nr));
+  }
+  for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {
+    const int i0 = t / a.tx * 64, j0 = t % a.tx * 64;
+    __syncthreads();
+#pragma unroll 4
+    for (int k = w; k < 64; k += 4)
+      if (i0 + k < a.m && j0 + u < a.n) {
+        const float* p = a.d + bz * a.dbs + (i0 + k) * a.ldd + j0 + u;
+        re[k][u] = p[0];
+        if (SRC == SRC_C64) im[SRC == SRC_C64 ? k : 0][u] = p[a.n];
+      }
+    __syncthreads();
+#pragma unroll 4
+    for (int k = w; k < 64; k += 4) {
+      const int i = i0 + u, j = j0 + k;
+      if (i >= a.m || j >= a.n) continue;
+      const float2 g = fetch<SRC>(a.g.p, bz * a.g.bs + i * a.g.rs + j * a.g.cs);
+      const float x = re[u][k], y = SRC == SRC_C64 ? im[SRC == SRC_C64 ? u : 0][k] : 0.f;
+      if constexpr (OUT) {
+        const long long at = bz * a.os + i * a.rs + j * a.cs;
+        if constexpr (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2((x - g.x * f2) * f1, (y - g.y * f2) * f1);
+        else put(a.out, a.dtype, at, (x - g.x * f2) * f1);
+      } else {
+        s += (double)g.x * x + (double)g.y * y;
+      }
+    }
+  }
+  if (!OUT) {
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) a.part[(long long)bz * gridDim.x + blockIdx.x] = s;
   }
 }
 
@@ -752,7 +834,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs a) {
   }
   const double nrm = sqrt(small_sum(sum, red)), full = nrm + (double)a.eps;
   if (a.norm && threadIdx.x == 0) a.norm[bz] = (float)nrm;
-  const float inv = full == 0.0 ? 0.f : (float)(1.0 / full);
+  const float inv = inverse(full);
   for (int k = threadIdx.x; k < s.R16 * s.ldx; k += SMALL_THREADS) X[k] *= inv;
   __syncthreads();
   for (int t = 0; t < a.steps; ++t) {
@@ -834,14 +916,14 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
     if (SRC == SRC_C64) sum += (double)g.y * D[i * s.ldx + j + s.n];
   }
   const double inner = small_sum(sum, red), nr = a.norm[bz], full = nr + (double)a.eps;
-  const float f1 = full == 0.0 ? 0.f : (float)(1.0 / full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * full * nr));
+  const float f1 = inverse(full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * nr));
   for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
     int i, j;
     place(k, s.m, s.n, a.flat, i, j);
     const float2 g = fetch<SRC>(a.src.p, bz * a.src.bs + i * a.src.rs + j * a.src.cs);
     const long long at = bz * a.obs + i * a.ors + j * a.ocs;
-    const float x = D[i * s.ldx + j] * f1 - g.x * f2;
-    if (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2(x, D[i * s.ldx + j + s.n] * f1 - g.y * f2);
+    const float x = (D[i * s.ldx + j] - g.x * f2) * f1;
+    if (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2(x, (D[i * s.ldx + j + s.n] - g.y * f2) * f1);
     else put(a.out, a.dtype, at, x);
   }
 }
@@ -850,11 +932,11 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
 // Every X of the iteration is a polynomial M of A_0 = X_0 X_0^H times X_0, so for a short side up to 64 (embedded) the steps
 // run on m x m matrices alone: one pass forms G G^H, one workgroup iterates
 //     P = a + b A + c A A,  M <- P M,  A <- P A P
-// and a second pass writes M G.  A_k is no longer formed from X_k: an error of A_0 in a direction of small singular
+// and a second pass writes M X_0.  A_k is no longer formed from X_k: an error of A_0 in a direction of small singular
 // value grows by a^2 a step, 2e4 in five, so everything m x m is f64 (G G^H too: its products are exact, its sums f64).
 // The gradient alike: D_k = U_k dY + V_k X_0 with U <- P U, V <- P V + Q M,
 //     T = (U dY X_0^H + V A_0) M,  S = T + T^H,  Q = b S + c (A S + S A),
-// from one pass for dY G^H and one for U dY + V G.  Bound by the reads of G for long sides, by the chain of small f64
+// from one pass for dY G^H and one for U dY + V X_0.  Bound by the reads of G for long sides, by the chain of small f64
 // products (17 forward, 55 for the gradient) for short ones.  33 x 1088 x 9 f32: 28 us a call (large form: 325); gradient of 38 x 14 x 5789
 // bf16: 157 us, most of it autograd's (3.0 ms).
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -879,7 +961,7 @@ struct ThinArgs {
   double* norm;                  // [batch]
   double* a0;                    // [batch][R16 R16], kept for the gradient (null: not kept)
   double* steps_mem;             // gradient: [batch][steps][3][R16 R16] P, M, A
-  float *m1, *m2;                // [batch][R16 R16]: out = m1 G, or m1 dY + m2 G
+  float *m1, *m2;                // [batch][R16 R16]: out = m1 X_0, or (m1 dY + m2 X_0) / N
 };
 
 __device__ __forceinline__ f64x4 mfma64(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
@@ -1061,8 +1143,7 @@ __device__ __forceinline__ void thin_iterate(const ThinArgs& a, double* A, doubl
   }
   __syncthreads();
   if (!STEPS) {
-    const double n = a.norm[bz] + a.eps, inv = n == 0.0 ? 0.0 : 1.0 / n;
-    for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) a.m1[bz * R16 * R16 + k] = (float)(M[k / R16 * ld + k % R16] * inv);
+    for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) a.m1[bz * R16 * R16 + k] = (float)M[k / R16 * ld + k % R16];
   }
 }
 
@@ -1188,16 +1269,16 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_grad_poly_kernel(ThinArgs a
     tr = s / a.cx;
   }
   __syncthreads();
-  // dG = D / N - G <D, G> / (N^2 |G|), D = U dY + V G / N, <D, G> = N <D, X_0>
-  const double f = nr == 0.0 ? 0.0 : tr * inv / nr;
+  // dG = (D - G <D, G> / (N |G|)) / N, D = U dY + V X_0, <D, G> = N <D, X_0>, G = N X_0
+  const double f = nr == 0.0 ? 0.0 : tr * n / nr;
   for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
     const int i = k / R16, j = k % R16;
-    a.m1[bz * q2 + k] = (float)(U[i * ld + j] * inv);
-    a.m2[bz * q2 + k] = (float)(V[i * ld + j] * inv * inv - (i == j ? f : 0.0));
+    a.m1[bz * q2 + k] = (float)U[i * ld + j];
+    a.m2[bz * q2 + k] = (float)(V[i * ld + j] - (i == j ? f : 0.0));
   }
 }
 
-// out = m1 G, or m1 dY + m2 G, 64 columns a workgroup
+// out = m1 X_0, or (m1 dY + m2 X_0) / N, X_0 = G / N, 64 columns a workgroup
 template <int SRC, bool GRAD>
 __global__ __launch_bounds__(256) void thin_apply_kernel(ThinArgs a) {
   extern __shared__ __attribute__((aligned(16))) float mem[];
@@ -1211,6 +1292,9 @@ __global__ __launch_bounds__(256) void thin_apply_kernel(ThinArgs a) {
   }
   thin_load<SRC, !GRAD>(X, ld, a, a.g, a.flat, bz, j0, false);
   if (GRAD) thin_load<SRC, false>(D, ld, a, a.dy, a.dflat, bz, j0, false);
+  const float inv = inverse(a.norm[bz] + a.eps);
+  for (int k = threadIdx.x; k < R16 * ld; k += 256) X[k] *= inv;
+  __syncthreads();
   f32x4 res[8];                                    // at most 64 x 128 results: 32 tiles, 8 a wave
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
@@ -1242,10 +1326,10 @@ __global__ __launch_bounds__(256) void thin_apply_kernel(ThinArgs a) {
       i = k - j * a.m;
     }
     if (j >= cols) continue;
-    const float x = X[i * ld + j];
+    const float by = GRAD ? inv : 1.f, x = X[i * ld + j] * by;
     const long long at = bz * a.obs + i * a.ors + (long long)(j0 + j) * a.ocs;
     if (SRC == SRC_C64) {
-      ((float2*)a.out)[at] = make_float2(x, X[i * ld + j + THIN_COLS]);
+      ((float2*)a.out)[at] = make_float2(x, X[i * ld + j + THIN_COLS] * by);
     } else if (!GRAD && a.update) {
       const float old = SRC == SRC_F32 ? ((float*)a.out)[at] : SRC == SRC_F16 ? (float)((f16*)a.out)[at] : (float)((__bf16*)a.out)[at];
       put(a.out, a.dtype, at, fmaf(a.rate, x, a.keep * old));
@@ -1324,7 +1408,7 @@ Work take_work(Arena& w, const Shape& s, bool saved) {
   k.split = w.take<float>(PART_BYTES / 4);
   if (!saved) {
     k.p = take_pieces(w, s);
-    if (s.cx == 1) k.t2 = w.take<f16>(s.nc * s.mp * s.batch);
+    k.t2 = w.take<f16>(s.nc * s.mp * s.batch);
   }
   return k;
 }
@@ -1344,7 +1428,7 @@ Saved take_saved(Arena& w, const Shape& s, int steps) {
 struct GradWork {
   double* part;
   float *norm, *carry, *split;
-  f16 *d, *t, *s, *q;
+  f16 *d, *t, *t2, *s, *q;
 };
 
 GradWork take_grad(Arena& w, const Shape& s) {
@@ -1355,24 +1439,29 @@ GradWork take_grad(Arena& w, const Shape& s) {
   k.split = w.take<float>(PART_BYTES / 4);
   k.d = w.take<f16>(s.mr * s.np * s.batch);
   k.t = w.take<f16>(s.nc * s.mp * s.batch);
+  k.t2 = w.take<f16>(s.nc * s.mp * s.batch);
   k.s = w.take<f16>(s.mr * s.mp * s.batch);
   k.q = w.take<f16>(s.mr * s.mp * s.batch);
   return k;
 }
 
-// What bounds the operands of a step whose X has singular values in [0, s]: x for X, A = s^2, B = max |b t + c t^2|, next = max |p|.
+// What bounds the operands of a step whose X has singular values in [0, s]: x for X, A = s^2, B = max |b t + c t^2|, next = max |p|,
+// slope = max |p'|, by which a step can lengthen a derivative: its gains are divided differences of the odd p.
 struct Bound {
-  double x, A, B, next;
+  double x, A, B, next, slope;
 };
 
 Bound bound_of(double s, const double* co) {
   const double a = co[0], b = co[1], c = co[2], t1 = s * s;
-  Bound r{s, t1, fabs(b * t1 + c * t1 * t1), 0.0};
+  Bound r{s, t1, fabs(b * t1 + c * t1 * t1), 0.0, 0.0};
   if (c != 0.0) {
     const double t = -b / (2 * c);
     if (t > 0 && t < t1) r.B = fmax(r.B, fabs(b * t + c * t * t));
   }
   auto p = [&](double t) { return fabs(sqrt(t) * (a + b * t + c * t * t)); };
+  auto slope = [&](double t) { return fabs(a + 3 * b * t + 5 * c * t * t); };
+  r.slope = fmax(slope(0.0), slope(t1));
+  if (c != 0.0 && -0.3 * b / c > 0 && -0.3 * b / c < t1) r.slope = fmax(r.slope, slope(-0.3 * b / c));
   r.next = p(t1);
   const double disc = 9 * b * b - 20 * a * c;
   if (c != 0.0 && disc >= 0) {
@@ -1419,7 +1508,7 @@ hipError_t run(Args& g, bool tri, const Epi& e, hipStream_t st) {
 }
 
 int sum_blocks(const Shape& s) {
-  long long n = (long long)s.m * s.n / 4096;
+  long long n = (long long)s.m * s.n / 1024;
   const int cap = s.batch >= 64 ? 16 : s.batch >= 8 ? 64 : s.batch > 1 ? 256 : MAX_PART;
   return (int)(n < 1 ? 1 : n > cap ? cap : n);
 }
@@ -1622,11 +1711,13 @@ SmallArgs small_args(const Shape& s, const Problem& q) {
   return a;
 }
 
+// the doubled matrix of a complex one has padding that no product writes; else products leave the next step's operands
 bool padded(const Shape& s) { return s.cx == 2 && (s.mp != s.P * s.mr || s.np != s.P * s.nc); }
 
 template <int P>
 hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
   const int nb = sum_blocks(s);
+  const bool fuse = !padded(s);
   SumArgs sa{};
   sa.x = q.g;
   sa.outer = s.m;
@@ -1645,8 +1736,8 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
   }
   for (int i = 0; i < q.steps; ++i) {
     Pieces p = sv ? sv->p[i] : w.p;
-    if (!sv && s.cx == 1 && i % 2) p.t = w.t2;
-    const bool fused = i > 0 && s.cx == 1;           // the step before left this one's operands
+    if (!sv && fuse && i % 2) p.t = w.t2;
+    const bool fused = i > 0 && fuse;                // the step before left this one's operands
     if (padded(s) && (sv || i == 0)) {               // the doubled matrix's padding
       TRY(clear(p.x, s.mr * s.np * s.batch * 2, st));
       TRY(clear(p.t, s.nc * s.mp * s.batch * 2, st));
@@ -1679,10 +1770,11 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
     if (i + 1 < q.steps) {
       Args g = base_args(s, w.split, s.m, s.nc, s.mp, s.mp, qs, ts);
       pair(g, p.b, p.t);
-      if (s.cx == 1) {
+      if (fuse) {
         const Pieces& n = sv ? sv->p[i + 1] : w.p;
         f16* t = !sv && i % 2 == 0 ? w.t2 : n.t;
-        TRY(run<P>(g, false, EpiNext<P>{w.carry, s.ldc, cs, alpha, beta, sc[i + 1].x, n.x, t, s.np, s.mr * s.np, s.mp, ts}, st));
+        TRY(run<P>(g, false, EpiNext<P>{w.carry, s.ldc, cs, alpha, beta, sc[i + 1].x, n.x, t, s.np, s.mr * s.np, s.mp, ts,
+                                               s.cx == 2 ? s.n : 0}, st));
       } else {
         TRY(run<P>(g, false, EpiCarry{w.carry, s.ldc, cs, alpha, beta, nullptr}, st));
       }
@@ -1835,69 +1927,124 @@ hipError_t backward(const Shape& s, const Problem& q, const Mat& dy, const Scale
     TRY(clear(w.d, xs * s.batch * 2, st));
     TRY(clear(w.t, ts * s.batch * 2, st));
   }
-  double bound[TCMI_NS_MAX_STEPS];
-  double sig = 1.0;
+  // The pieces of D are taken under a bound.  Where the steps can lengthen D by 2^10 at most (the default coefficients: 566),
+  // that is |dY| times what the steps allow, and a step leaves the next one's pieces.  Of the 39 binades between f16's largest
+  // value and its smallest step 22 are the pieces' own, so D may stay 2^7 below the bound before an entry of D's mean size
+  // in a 1000 x 1000 matrix loses bits; in fact its part outside G's symmetric directions grows as X does, 2 to 9 times.  A
+  // larger bound would leave too few bits: there D is measured and divided by its norm at every step.
+  double bound[TCMI_NS_MAX_STEPS], dn[TCMI_NS_MAX_STEPS];
+  double sig = 1.0, grown = 1.0;
   for (int i = 0; i < q.steps; ++i) {
     bound[i] = sig * SLACK;
     sig = bound_of(bound[i], q.coef + 3 * i).next;
   }
   for (int i = q.steps - 1; i >= 0; --i) {
+    dn[i] = grown;
+    grown *= fmax(1.0, bound_of(bound[i], q.coef + 3 * i).slope);
+  }
+  const bool fuse = !padded(s) && dn[0] <= 1024.0;
+  float sD[TCMI_NS_MAX_STEPS], sQ[TCMI_NS_MAX_STEPS], sS[TCMI_NS_MAX_STEPS];
+  for (int i = 0; i < q.steps; ++i) {
+    // |S|_F <= 2 x |D|, |Q|_F <= (2 x b + 4 x^3 c) |D|.  B D and Q X share an accumulator, so their scales have to agree:
+    // sB sD = sQ sX.
+    const double x = bound[i], b = fabs(q.coef[3 * i + 1]), c = fabs(q.coef[3 * i + 2]), d = (fuse ? dn[i] : 1.0) * SLACK;
+    const float qmax = scale_for((2 * x * b + 4 * x * x * x * c) * d);
+    sS[i] = scale_for(2 * x * d);
+    sD[i] = scale_for(d);
+    sQ[i] = sc[i].B * sD[i] / sc[i].x;
+    if (sQ[i] > qmax) {
+      sD[i] *= qmax / sQ[i];
+      sQ[i] = qmax;
+    }
+  }
+  for (int i = q.steps - 1; i >= 0; --i) {
     const Pieces& p = sv.p[i];
-    const double x = bound[i], b = fabs(q.coef[3 * i + 1]), c = fabs(q.coef[3 * i + 2]);
-    // D is divided by its own norm before it is cut: |D|_F = 1, |S|_F <= 2 x, |Q|_F <= 2 x b + 4 x^3 c.  B D and Q X share an
-    // accumulator, so their scales have to agree: sB sD = sQ sX.
-    const float sS = scale_for(2 * x * SLACK), qmax = scale_for((2 * x * b + 4 * x * x * x * c) * SLACK);
-    float sD = scale_for(SLACK), sQ = sc[i].B * sD / sc[i].x;
-    if (sQ > qmax) {
-      sD *= qmax / sQ;
-      sQ = qmax;
-    }
-    // |D|
-    SumArgs sa{};
-    sa.outer = s.m;
-    sa.part = w.part;
     const bool first = i == q.steps - 1;
-    if (first) {
-      sa.x = dy;
-      sa.inner = s.n;
-      TRY(launch_sums<0>(q.src, sa, nb, s.batch, st));
-    } else {
-      sa.x = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
-      sa.inner = s.nc;
-      TRY(launch_sums<0>(SRC_F32, sa, nb, s.batch, st));
+    if (first || !fuse) {                            // |D| and D's pieces
+      SumArgs sa{};
+      sa.outer = s.m;
+      sa.part = w.part;
+      PackArgs a{};
+      a.part = w.part;
+      a.npart = nb;
+      a.norm_out = w.norm;
+      a.scale = sD[i];
+      a.x = w.d;
+      a.t = w.t;
+      if (first) {
+        sa.x = a.src = dy;
+        sa.inner = s.n;
+        a.carry = w.carry;
+        a.carry_raw = !fuse;                         // else only its pieces are divided, the epilogue multiplies
+        TRY(launch_sums<0>(q.src, sa, nb, s.batch, st));
+        TRY(launch_pack<2>(q.src, a, s, st));
+      } else {
+        sa.x = a.src = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
+        sa.inner = s.nc;
+        TRY(launch_sums<0>(SRC_F32, sa, nb, s.batch, st));
+        TRY(launch_pack<2>(SRC_PLANAR, a, s, st));
+      }
     }
-    PackArgs a{};
-    a.part = w.part;
-    a.npart = nb;
-    a.norm_out = w.norm;
-    a.scale = sD;
-    a.x = w.d;
-    a.t = w.t;
-    if (first) {
-      a.src = dy;
-      a.carry = w.carry;
-      a.carry_raw = 1;                               // D itself; only its pieces are divided, the epilogue multiplies
-    } else {
-      a.src = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
-    }
-    TRY(launch_pack<2>(first ? q.src : SRC_PLANAR, a, s, st));
     // S = D X^T + X D^T
     Args g = base_args(s, w.split, s.mr, s.mr, s.np, s.np, xs, xs);
     pair(g, w.d, p.x);
     pair(g, p.x, w.d);
-    TRY(run<2>(g, true, EpiSym<2>{w.s, nullptr, s.mp, qs, 1.f / (sD * sc[i].x), 0.f, sS}, st));
+    TRY(run<2>(g, true, EpiSym<2>{w.s, nullptr, s.mp, qs, 1.f / (sD[i] * sc[i].x), 0.f, sS[i]}, st));
     // Q = b S + c (A S + S A)
     g = base_args(s, w.split, s.mr, s.mr, s.mp, s.mp, qs, qs);
     pair(g, p.a, w.s);
     pair(g, w.s, p.a);
-    TRY(run<2>(g, true, EpiSym<2>{w.q, w.s, s.mp, qs, (float)q.coef[3 * i + 2] / (sc[i].A * sS), (float)q.coef[3 * i + 1] / sS, sQ}, st));
-    // D <- a D + |D| (B D + Q X) / |D|
+    TRY(run<2>(g, true, EpiSym<2>{w.q, w.s, s.mp, qs, (float)q.coef[3 * i + 2] / (sc[i].A * sS[i]), (float)q.coef[3 * i + 1] / sS[i], sQ[i]}, st));
+    // D <- a D + B D + Q X (not fused: the products hold D / |D|)
     g = base_args(s, w.split, s.m, s.nc, s.mp, s.mp, qs, ts);
     pair(g, p.b, w.t);
     pair(g, w.q, p.t);
-    TRY(run<2>(g, false, EpiCarry{w.carry, s.ldc, s.m * s.ldc, 1.f / (sc[i].B * sD), (float)q.coef[3 * i], w.norm}, st));
+    const float alpha = 1.f / (sc[i].B * sD[i]), beta = (float)q.coef[3 * i];
+    if (fuse && i > 0) {
+      TRY(run<2>(g, false, EpiNext<2>{w.carry, s.ldc, s.m * s.ldc, alpha, beta, sD[i - 1], w.d, w.t2, s.np, xs, s.mp, ts,
+                                      s.cx == 2 ? s.n : 0}, st));
+      f16* t = w.t;
+      w.t = w.t2;
+      w.t2 = t;
+    } else {
+      TRY(run<2>(g, false, EpiCarry{w.carry, s.ldc, s.m * s.ldc, alpha, beta, fuse ? nullptr : w.norm}, st));
+    }
   }
   // dG
+  if (q.g.rs < q.g.cs) {
+    TurnedArgs a{};
+    a.g = q.g;
+    a.d = w.carry;
+    a.ldd = s.ldc;
+    a.dbs = s.m * s.ldc;
+    a.m = s.m;
+    a.n = s.n;
+    a.tx = (s.n + 63) / 64;
+    a.tiles = a.tx * ((s.m + 63) / 64);
+    a.npart = a.tiles < nb ? a.tiles : nb;
+    a.part = w.part;
+    a.norm = sv.norm;
+    a.dnorm = fuse ? w.norm : nullptr;
+    a.eps = (float)q.eps;
+    a.out = q.out;
+    a.rs = q.ors;
+    a.cs = q.ocs;
+    a.os = q.obs;
+    a.dtype = q.dtype;
+    const dim3 sums(a.npart, s.batch), outs(a.tiles < 4096 ? a.tiles : 4096, s.batch);
+#define GO(SRC)                                                                          \
+  {                                                                                      \
+    hipLaunchKernelGGL((turned_kernel<SRC, false>), sums, dim3(256), 0, st, a);          \
+    TRY(hipGetLastError());                                                              \
+    hipLaunchKernelGGL((turned_kernel<SRC, true>), outs, dim3(256), 0, st, a);           \
+  }
+    if (q.src == SRC_F32) GO(SRC_F32)
+    else if (q.src == SRC_F16) GO(SRC_F16)
+    else if (q.src == SRC_BF16) GO(SRC_BF16)
+    else GO(SRC_C64)
+#undef GO
+    return hipGetLastError();
+  }
   SumArgs sa{};
   sa.x = q.g;
   sa.y = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
@@ -1911,7 +2058,7 @@ hipError_t backward(const Shape& s, const Problem& q, const Mat& dy, const Scale
   const dim3 grid(gx, s.batch);
 #define GO(SRC)                                                                                                            \
   hipLaunchKernelGGL(grad_out_kernel<SRC>, grid, dim3(256), 0, st, q.g, w.carry, s.ldc, s.m * s.ldc, s.m, s.n, w.part, nb, \
-                     sv.norm, (float)q.eps, q.out, q.ors, q.ocs, q.obs, q.dtype)
+                     sv.norm, fuse ? w.norm : nullptr, (float)q.eps, q.out, q.ors, q.ocs, q.obs, q.dtype)
   if (q.src == SRC_F32) GO(SRC_F32);
   else if (q.src == SRC_F16) GO(SRC_F16);
   else if (q.src == SRC_BF16) GO(SRC_BF16);

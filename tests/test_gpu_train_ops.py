@@ -218,6 +218,52 @@ def test_newton_schulz_where_its_forms_meet(shape, dtype):
         assert _rel(got[k], want) < _ns_grad_tol(x[k], dy[k], want, dtype)
 
 
+@pytest.mark.parametrize("power", [-100, 100])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.complex64])
+@pytest.mark.parametrize("shape", [(20, 30), (10, 1500), (150, 140), (160, 128)])
+def test_newton_schulz_does_not_depend_on_the_scale(shape, dtype, power):
+    """without eps a factor 2^k leaves the result alone and divides the gradient, far from where squares overflow"""
+    from tcmi import linalg
+
+    x, dy = _rand(32, *shape, dtype=dtype), _rand(33, *shape, dtype=dtype)
+    leaf = (x * 2.0 ** power).cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf, eps=0.0)
+    (got,) = torch.autograd.grad(out, leaf, dy.cuda())
+    want, grad = _ns64(x, eps=0.0), _ns_grad64(x, dy, eps=0.0)
+    assert _rel(out, want) < _ns_tol(dtype) and _rel(linalg.newton_schulz(leaf.detach(), eps=0.0), want) < _ns_tol(dtype)
+    assert _rel(got * 2.0 ** power, grad) < _ns_grad_tol(x, dy, grad, dtype, eps=0.0)
+    # a tiny and a large cotangent
+    for far in (-100, 60):
+        leaf = x.cuda().requires_grad_()
+        (got,) = torch.autograd.grad(linalg.newton_schulz(leaf, eps=0.0), leaf, (dy * 2.0 ** far).cuda())
+        assert _rel(got * 2.0 ** -far, grad) < _ns_grad_tol(x, dy, grad, dtype, eps=0.0)
+
+
+@pytest.mark.parametrize("coef", [((8.0, -22.0, 16.0),) + ((3.2, -1.408, 0.16384),) * 3, ((1.5, -0.5, 0.0),) * 6, (DEFAULT[0],)])
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (150, 140)), (torch.complex64, (80, 96)), (torch.complex64, (70, 90)), (torch.float32, (200, 333))])
+def test_newton_schulz_grad_with_other_coefficients(dtype, shape, coef):
+    """steps that can lengthen a derivative a lot, ones that cannot, a single one; sides with and without padding"""
+    from tcmi import linalg
+
+    x, dy = _rand(34, 2, *shape, dtype=dtype), _rand(35, 2, *shape, dtype=dtype)
+    leaf = x.cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf, len(coef), coef if len(coef) > 1 else coef[0])
+    (got,) = torch.autograd.grad(out, leaf, dy.cuda())
+    grow, top = 1.0, 1.0
+    for a, b, c in coef:                               # the steps' largest slopes where singular values can lie
+        t = np.linspace(0, 1.02 * top, 1000)
+        grow *= max(1.0, np.abs(a + 3 * b * t ** 2 + 5 * c * t ** 4).max())
+        top = np.abs(a * t + b * t ** 3 + c * t ** 5).max()
+    for k in range(2):
+        want = _ns64(x[k], coef)
+        # the units of the default's tolerance, every step's error times what the steps behind it can make of it
+        assert _rel(out[k], want) < 4 * 2.0 ** -22 * len(coef) * grow + HALF_STEP[dtype]
+        n = torch.linalg.matrix_norm(x[k].to(want.dtype))
+        want = _ns_grad64(x[k], dy[k], coef)
+        tol = 8 * len(coef) * 2.0 ** -22 * grow * torch.linalg.vector_norm(dy[k].to(want.dtype)) / (torch.linalg.vector_norm(want) * n)
+        assert _rel(got[k], want) < float(tol) + HALF_STEP[dtype]
+
+
 def test_newton_schulz_grad_against_differences():
     """and at an isometry, where the gradient of an SVD does not exist"""
     from tcmi import linalg
