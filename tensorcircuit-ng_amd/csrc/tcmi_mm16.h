@@ -37,6 +37,8 @@ struct Args {
   long long sa, sb;            // elements between batch members
   int tm, tn;                  // tiles per matrix
   int tri;                     // 1: C is symmetric, only tiles with row tile >= column tile are computed
+  int doubled;                 // > 0: C = [[R, I], [-I, R]] from a hermitian R + iI of this size
+  int half;                    // `doubled` where tiles end at it: the second R is not computed, the epilogue writes the first one twice
   int tiles;                   // tiles per batch member (tm * tn, or the triangle)
   int batch;
   int split;                   // > 1: the k steps are dealt to `split` workgroups, whose sums join_kernel adds
@@ -60,6 +62,12 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 // tile t of a batch member
 __device__ __forceinline__ void tile_at(const Args& g, unsigned t, int& ti, int& tj) {
   if (g.tri) {
+    const unsigned h = g.half ? (unsigned)g.tm / 2u : 0u, r = h * (h + 1) / 2;
+    if (g.half && t >= r) {                           // below the triangle of R: the square of -I
+      ti = (int)(h + (t - r) / h);
+      tj = (int)((t - r) % h);
+      return;
+    }
     unsigned i = (unsigned)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
     while (i * (i + 1) / 2 > t) --i;
     while ((i + 1) * (i + 2) / 2 <= t) ++i;
@@ -390,10 +398,17 @@ inline double step_us(int per_cu) {
   return per_cu == 1 ? (one ? 0.38 : 0.48) : per_cu == 2 ? (one ? 0.56 : 0.58) : per_cu == 3 ? (one ? 0.68 : 0.70) : (one ? 0.79 : 0.80);
 }
 
+// whether a doubled hermitian result leaves out the second R (up to a quarter of the triangle's tiles): orthogonalising
+// 2048 x 2048 complex64 3.41 -> 2.68 ms; 62 x 256 x 128, bound by the operands' bytes, 2 %
+template <class T>
+inline bool halves(const Args& g, bool tri) {
+  return tri && T::BM == T::BN && g.doubled > 0 && g.doubled % T::BM == 0 && g.M == 2 * g.doubled;
+}
+
 template <class T>
 inline long long tile_count(const Args& g, bool tri) {
   const long long tm = (g.M + T::BM - 1) / T::BM, tn = (g.N + T::BN - 1) / T::BN;
-  return (tri ? tm * (tm + 1) / 2 : tm * tn) * g.batch;
+  return (halves<T>(g, tri) ? tm / 2 * (tm / 2 + 1) / 2 + tm / 2 * (tm / 2) : tri ? tm * (tm + 1) / 2 : tm * tn) * g.batch;
 }
 
 // the cheapest split of a product over tiles T, and its time
@@ -433,7 +448,9 @@ hipError_t launch(Args& g, bool tri, int split, const Epi& e, hipStream_t st) {
   g.tm = (g.M + T::BM - 1) / T::BM;
   g.tn = (g.N + T::BN - 1) / T::BN;
   g.tri = tri ? 1 : 0;
-  const long long tiles = tri ? (long long)g.tm * (g.tm + 1) / 2 : (long long)g.tm * g.tn, units = tiles * g.batch;
+  if (g.batch < 1) return hipErrorInvalidValue;
+  g.half = halves<T>(g, tri) ? g.doubled : 0;
+  const long long units = tile_count<T>(g, tri), tiles = units / g.batch;
   if (units < 1 || units >= (1ll << 24) || g.K < 64 || (g.K & 63) || g.nseg < 1 || g.lda > MAX_ROW || g.ldb > MAX_ROW) return hipErrorInvalidValue;
   g.tiles = (int)tiles;
   g.split = split;

@@ -311,6 +311,9 @@ struct EpiSym {
   float alpha, beta, scale;
   template <class T>
   static constexpr int lds() { return Transposed<T, P>::BYTES; }
+  // the real part of a doubled hermitian result stands in it twice (g.half is a multiple of 64)
+  __device__ __forceinline__ bool twice(const Args& g, int row, int col) const { return row < g.half && col < g.half; }
+  __device__ __forceinline__ long long second(const Args& g) const { return g.half * ld + kpos<P>(g.half); }
   __device__ __forceinline__ void put_row(const Args& g, int bz, int wide, int row, int col, f32x4 v, f16x4& vh, f16x4& vl) const {
     const bool in = row < g.M && col < wide;
     const long long at = bz * bs + row * ld + kpos<P>(col);
@@ -331,6 +334,10 @@ struct EpiSym {
     if (in) {
       *reinterpret_cast<f16x4*>(out + at) = vh;
       if (P == 2) *reinterpret_cast<f16x4*>(out + at + 32) = vl;
+      if (twice(g, row, col)) {
+        *reinterpret_cast<f16x4*>(out + at + second(g)) = vh;
+        if (P == 2) *reinterpret_cast<f16x4*>(out + at + second(g) + 32) = vl;
+      }
     }
   }
   __device__ __forceinline__ void four(const Args& g, int bz, bool mirror, int row, int col, f32x4 v) const {
@@ -344,6 +351,10 @@ struct EpiSym {
           f16* p = out + bz * bs + (col + r) * ld + kpos<P>(row);
           p[0] = vh[r];
           if (P == 2) p[32] = vl[r];
+          if (twice(g, row, col)) {
+            p[second(g)] = vh[r];
+            if (P == 2) p[second(g) + 32] = vl[r];
+          }
         }
     }
   }
@@ -360,6 +371,7 @@ struct EpiSym {
     if (!mirror) return;
     __syncthreads();
     turned.flush(out + bz * bs, ld, n0, g.M, m0, wide);
+    if (twice(g, m0, n0)) turned.flush(out + bz * bs + second(g), ld, n0, g.half, m0, g.half);
   }
 };
 
@@ -1582,6 +1594,7 @@ Args base_args(const Shape& s, float* split, int M, int N, long long K, long lon
   g.sa = sa;
   g.sb = sb;
   g.batch = s.batch;
+  g.doubled = s.cx == 2 ? s.m : 0;
   g.part = split;
   return g;
 }

@@ -264,6 +264,22 @@ def test_newton_schulz_grad_with_other_coefficients(dtype, shape, coef):
         assert _rel(got[k], want) < float(tol) + HALF_STEP[dtype]
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(1, 64, 96), (1, 128, 128), (5, 192, 208), (1, 320, 256), (1, 256, 257), (40, 128, 256), (1, 600, 576)])
+def test_newton_schulz_complex_where_tiles_end_at_the_half(batch, rows, cols):
+    """short sides of whole tiles (the second real part is not computed), of 64 but not of 128, split products and whole ones"""
+    from tcmi import linalg
+
+    x, dy = _rand(36, batch, rows, cols, dtype=torch.complex64), _rand(37, batch, rows, cols, dtype=torch.complex64)
+    leaf = x.cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf)
+    (got,) = torch.autograd.grad(out, leaf, dy.cuda())
+    for k in {0, batch // 2, batch - 1}:
+        want = _ns64(x[k])
+        assert _rel(out[k], want) < _ns_tol(torch.complex64)
+        want = _ns_grad64(x[k], dy[k])
+        assert _rel(got[k], want) < _ns_grad_tol(x[k], dy[k], want, torch.complex64)
+
+
 def test_newton_schulz_grad_against_differences():
     """and at an isometry, where the gradient of an SVD does not exist"""
     from tcmi import linalg
