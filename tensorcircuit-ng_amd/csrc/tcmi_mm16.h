@@ -399,7 +399,7 @@ inline double step_us(int per_cu) {
 }
 
 // whether a doubled hermitian result leaves out the second R (up to a quarter of the triangle's tiles): orthogonalising
-// 2048 x 2048 complex64 3.41 -> 2.68 ms; 62 x 256 x 128, bound by the operands' bytes, 2 %
+// 2048 x 2048 complex64 3.41 -> 2.68 ms; 62 x 256 x 128, one round of tiles either way, 2 %
 template <class T>
 inline bool halves(const Args& g, bool tri) {
   return tri && T::BM == T::BN && g.doubled > 0 && g.doubled % T::BM == 0 && g.M == 2 * g.doubled;
