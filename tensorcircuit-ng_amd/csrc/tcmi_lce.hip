@@ -854,7 +854,9 @@ hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, f
     TRY(run_logits<P>(g, s.dtype, EpiLse<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, 0}, w.part, w.target, in.y}, st));
     tiles = g.tn;
   }
-  if (total && (long long)s.T * tiles <= 8192) {       // 64 KB of statistics
+  // one workgroup for both while its 16 waves have at most four rows each: 7 us for 64 rows (two launches: 3 + 3 and a gap), 26
+  // for 256
+  if (total && s.T <= 64 && (long long)s.T * tiles <= 8192) {       // 64 KB of statistics
     hipLaunchKernelGGL(rowstat_total_kernel, dim3(1), dim3(1024), 0, st, w.part, tiles, w.target, in.y, in.ignore, s.T, s.V, lse, loss, mean,
                        total, count);
     return hipGetLastError();
