@@ -617,9 +617,33 @@ struct EpiGrad {
   int dtype, cols;
   void* db;
   const float *dloss, *count;    // db: the factor all rows share, dloss (/ count), whose mantissa is still missing (null: none)
+  int vec;                       // rows of `out` and `sum` are aligned for four elements
   __device__ __forceinline__ void four(const Args& g, int, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
     const float al = *inv * (1.f / PSCALE);
+    if (vec && col + 3 < cols) {
+      const long long at = (long long)row * cols + col;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] *= al;
+      if (!first) {
+        const f32x4 old = *reinterpret_cast<const f32x4*>(sum + at);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += old[k];
+      }
+      if (!last) {
+        *reinterpret_cast<f32x4*>(sum + at) = v;
+        return;
+      }
+      if (r) {
+        const float f = r[row];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = f == 0.f ? 0.f : v[k] * f;
+      }
+      if (dtype == TCMI_F32) *reinterpret_cast<f32x4*>((float*)out + at) = v;
+      else if (dtype == TCMI_F16) *reinterpret_cast<f16x4*>((f16*)out + at) = __builtin_convertvector(v, f16x4);
+      else *reinterpret_cast<bf16x4*>((__bf16*)out + at) = __builtin_convertvector(v, bf16x4);
+      return;
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (col + k >= g.N) continue;
@@ -914,7 +938,8 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.lda = d.ldb = d.K;
       d.a[0] = w.p;
       d.b[0] = w.wt;
-      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr, nullptr, nullptr}, st));
+      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr, nullptr, nullptr,
+                             vec4(dh, s.D, s.dtype)}, st));
     }
     if (dw) {
       d.M = n;
@@ -924,7 +949,8 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.a[0] = w.pt;
       d.b[0] = w.ht;
       TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype, s.D,
-                            more ? (char*)db + (long long)v0 * size : nullptr, ones == 2 ? dloss : nullptr, count}, st));
+                            more ? (char*)db + (long long)v0 * size : nullptr, ones == 2 ? dloss : nullptr, count,
+                            vec4(dw, s.D, s.dtype)}, st));
     }
     if (db && !ones) {
       hipLaunchKernelGGL(bias_kernel<P>, dim3((n + 3) / 4), dim3(256), 0, st, w.pt, s.tp, w.r, s.T, n, db, s.dtype, v0);
