@@ -397,8 +397,10 @@ int tcmi_comm_destroy(void* comm);
  * (a, b, c) = coef_host[3 i .. 3 i + 2] (host memory, float64).  g: [batch] matrices of rows x cols with element strides
  * rs / cs / bs; out: contiguous, same dtype (TCMI_F32, TCMI_F16, TCMI_BF16 or TCMI_C64).  full = 1: two f16 pieces per
  * operand (f32 accuracy), 0: one (TCMI_BF16 only).  saved (full only, may be NULL): what the gradient needs.
- * Coefficients that let a singular value grow past 64 are refused.  Workspaces: tcmi_ns_work_bytes(.., what) bytes,
- * 256-byte aligned, contents undefined; nothing is kept in them between calls.  A matrix with a non-finite entry gives NaN.
+ * Coefficients that let a singular value grow past 64 are refused.  Workspaces: tcmi_ns_work_bytes_coef(.., what) bytes for
+ * these coefficients, or tcmi_ns_work_bytes(.., what), enough for any; 256-byte aligned, contents undefined; nothing is kept in
+ * them between calls.  A short side up to 64 (complex: 32, gradient: half of that) may be 2^24 long while the steps multiply no
+ * direction by more than 2^18 (ten steps of the default coefficients); others up to 2^21 elements a row (-1 past it).  A matrix with a non-finite entry gives NaN.
  * No counterpart in the reference, whose orthogonal factors come from its backends' svd / qr
  * (tensorcircuit/backends/abstract_backend.py `svd`, `qr`). */
 #define TCMI_NS_MAX_STEPS 16
@@ -407,6 +409,7 @@ int tcmi_comm_destroy(void* comm);
 #define TCMI_NS_SAVED 2         /* `saved` itself */
 #define TCMI_NS_WORK_GRAD 3     /* tcmi_newton_schulz_grad */
 long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full, int dtype, int what);
+long long tcmi_ns_work_bytes_coef(int rows, int cols, int batch, int steps, const double* coef_host, int full, int dtype, int what);
 int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long g_bs, void* out, int rows, int cols, int batch,
                        int steps, const double* coef_host, double eps, int full, void* saved, long long saved_bytes, void* work,
                        long long work_bytes, int dtype, void* stream);

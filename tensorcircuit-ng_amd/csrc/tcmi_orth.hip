@@ -948,7 +948,13 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
 // value grows by a^2 a step, 2e4 in five, so everything m x m is f64 (G G^H too: its products are exact, its sums f64).
 // The gradient alike: D_k = U_k dY + V_k X_0 with U <- P U, V <- P V + Q M,
 //     T = (U dY X_0^H + V A_0) M,  S = T + T^H,  Q = b S + c (A S + S A),
-// from one pass for dY G^H and one for U dY + V X_0.  Bound by the reads of G for long sides, by the chain of small f64
+// from one pass for dY G^H and one for U dY + V X_0.
+// In directions that G does not have M is the product of the steps' a, and what cancels there in M X_0 leaves its rounding
+// behind: f32 sums hold while that product is small (steep), f64 ones (the second pass from 2^-53, 16 products for 1) until the
+// rounding of A_0, which grows by its square, is felt; from there on the iterated forms take over, whose noise the steps
+// themselves keep down.  Rows that occur twice, 32 x 1000, against 64 bits, 5 / 8 / 10 / 12 / 16 steps of the default: f32
+// 9e-6 / 3e-4 / 3e-3 / 3e-2 / 5, f64 1e-13 / 2e-12 / 4e-11 / 6e-10 / 1e-7; of rank one, f64: 4e-13 / 1e-11 / 3e-9 / 5e-6 / 3.
+// Bound by the reads of G for long sides, by the chain of small f64
 // products (17 forward, 55 for the gradient) for short ones.  33 x 1088 x 9 f32: 28 us a call (large form: 325); gradient of 38 x 14 x 5789
 // bf16: 157 us, most of it autograd's (3.0 ms).
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -973,7 +979,7 @@ struct ThinArgs {
   double* norm;                  // [batch]
   double* a0;                    // [batch][R16 R16], kept for the gradient (null: not kept)
   double* steps_mem;             // gradient: [batch][steps][3][R16 R16] P, M, A
-  float *m1, *m2;                // [batch][R16 R16]: out = m1 X_0, or (m1 dY + m2 X_0) / N
+  double *m1, *m2;               // [batch][R16 R16]: out = m1 X_0, or (m1 dY + m2 X_0) / N
 };
 
 __device__ __forceinline__ f64x4 mfma64(double a, double b, f64x4 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
@@ -1104,22 +1110,26 @@ __device__ __forceinline__ void cells64(int i0, int j0, f64x4 v, F f) {        /
   for (int r = 0; r < 4; ++r) f(i0 + g + 4 * r, j0 + l, v[r]);
 }
 
+// A cell on or below the diagonal and its mirror image.  Cells above it in a tile on the diagonal are left out: the rounding of
+// p q and of its transpose differ, and a matrix that holds some of each is not symmetric, which the next products multiply by
+// the square of what M grows to (8 x 1000 of rank 4, ten steps: 6e-5 of the result instead of 3e-9).
+__device__ __forceinline__ void put_sym(double* out, int ld, int i, int j, double x) {
+  if (j > i) return;
+  out[i * ld + j] = x;
+  out[j * ld + i] = x;
+}
+
 // out = sym(p q) for commuting symmetric p, q: lower tiles, written twice
 __device__ __forceinline__ void sym64(const double* p, const double* q, double* out, int ld, int R16) {
   tiles64<true>(R16, [&](int i0, int j0) {
-    cells64(i0, j0, rows64(p + i0 * ld, q + j0 * ld, ld, R16, f64x4{0, 0, 0, 0}), [&](int i, int j, double x) {
-      out[i * ld + j] = x;
-      out[j * ld + i] = x;
-    });
+    cells64(i0, j0, rows64(p + i0 * ld, q + j0 * ld, ld, R16, f64x4{0, 0, 0, 0}), [&](int i, int j, double x) { put_sym(out, ld, i, j, x); });
   });
 }
 
 __device__ __forceinline__ void poly64(const double* A, double* P, int ld, int R16, double a, double b, double c) {
   tiles64<true>(R16, [&](int i0, int j0) {
     cells64(i0, j0, rows64(A + i0 * ld, A + j0 * ld, ld, R16, f64x4{0, 0, 0, 0}), [&](int i, int j, double x) {
-      x = c * x + b * A[i * ld + j] + (i == j ? a : 0.0);
-      P[i * ld + j] = x;
-      P[j * ld + i] = x;
+      put_sym(P, ld, i, j, c * x + b * A[i * ld + j] + (i == j ? a : 0.0));
     });
   });
 }
@@ -1155,7 +1165,7 @@ __device__ __forceinline__ void thin_iterate(const ThinArgs& a, double* A, doubl
   }
   __syncthreads();
   if (!STEPS) {
-    for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) a.m1[bz * R16 * R16 + k] = (float)M[k / R16 * ld + k % R16];
+    for (int k = threadIdx.x; k < R16 * R16; k += THIN_THREADS) a.m1[bz * R16 * R16 + k] = M[k / R16 * ld + k % R16];
   }
 }
 
@@ -1242,11 +1252,7 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_grad_poly_kernel(ThinArgs a
     tiles64<true>(R16, [&](int i0, int j0) {       // Q = b S + c (A S + S A)
       f64x4 v = rows64(A + i0 * ld, S + j0 * ld, ld, R16, zero);
       v = rows64(S + i0 * ld, A + j0 * ld, ld, R16, v);
-      cells64(i0, j0, v, [&](int i, int j, double x) {
-        x = c * x + b * S[i * ld + j];
-        Q[i * ld + j] = x;
-        Q[j * ld + i] = x;
-      });
+      cells64(i0, j0, v, [&](int i, int j, double x) { put_sym(Q, ld, i, j, c * x + b * S[i * ld + j]); });
     });
     __syncthreads();
     sym64(P, U, Z, ld, R16);                       // U <- P U
@@ -1285,46 +1291,72 @@ __global__ __launch_bounds__(THIN_THREADS) void thin_grad_poly_kernel(ThinArgs a
   const double f = nr == 0.0 ? 0.0 : tr * n / nr;
   for (int k = threadIdx.x; k < q2; k += THIN_THREADS) {
     const int i = k / R16, j = k % R16;
-    a.m1[bz * q2 + k] = (float)U[i * ld + j];
-    a.m2[bz * q2 + k] = (float)(V[i * ld + j] - (i == j ? f : 0.0));
+    a.m1[bz * q2 + k] = U[i * ld + j];
+    a.m2[bz * q2 + k] = V[i * ld + j] - (i == j ? f : 0.0);
   }
 }
 
-// out = m1 X_0, or (m1 dY + m2 X_0) / N, X_0 = G / N, 64 columns a workgroup
-template <int SRC, bool GRAD>
+// c += sum_k p[i][k] x[k][j], p in f64, x exact f32
+__device__ __forceinline__ f64x4 rows_cols64(const double* p, int ldp, const float* x, int ldx, int K, f64x4 c) {
+  const int l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+  p += l * ldp + g;
+  x += g * ldx + l;
+  for (int k = 0; k < K; k += 4) c = mfma64(p[k], (double)x[k * ldx], c);
+  return c;
+}
+
+// out = m1 X_0, or (m1 dY + m2 X_0) / N, X_0 = G / N, 64 columns a workgroup.  S: the type of the products and sums; in f64
+// G is divided behind them, as rounding G / N would already cost what f64 is there to save.
+template <int SRC, bool GRAD, class S>
 __global__ __launch_bounds__(256) void thin_apply_kernel(ThinArgs a) {
   extern __shared__ __attribute__((aligned(16))) float mem[];
-  const int R16 = (a.cx * a.m + 15) & ~15, M16 = (a.m + 15) & ~15, w = a.cx * THIN_COLS, ld = w + 4, ldm = R16 + 4;
+  constexpr bool WIDE = std::is_same<S, double>::value;
+  const int R16 = (a.cx * a.m + 15) & ~15, M16 = (a.m + 15) & ~15, w = a.cx * THIN_COLS, ld = w + 4, ldm = R16 + (WIDE ? 2 : 4);
   const long long bz = blockIdx.y;
   const int j0 = blockIdx.x * THIN_COLS, wave = threadIdx.x >> 6, tc = w / 16, tiles = tc * (M16 / 16);
-  float *X = mem, *M1 = X + R16 * ld, *D = M1 + R16 * ldm, *M2 = D + R16 * ld;
+  const int l = threadIdx.x & 15, q = (threadIdx.x & 63) >> 4;
+  float *X = mem, *D = X + R16 * ld;
+  S *M1 = reinterpret_cast<S*>(mem + (GRAD ? 2 : 1) * R16 * ld), *M2 = M1 + R16 * ldm;
   for (int k = threadIdx.x; k < R16 * R16; k += 256) {
-    M1[k / R16 * ldm + k % R16] = a.m1[bz * R16 * R16 + k];
-    if (GRAD) M2[k / R16 * ldm + k % R16] = a.m2[bz * R16 * R16 + k];
+    M1[k / R16 * ldm + k % R16] = (S)a.m1[bz * R16 * R16 + k];
+    if (GRAD) M2[k / R16 * ldm + k % R16] = (S)a.m2[bz * R16 * R16 + k];
   }
   thin_load<SRC, !GRAD>(X, ld, a, a.g, a.flat, bz, j0, false);
   if (GRAD) thin_load<SRC, false>(D, ld, a, a.dy, a.dflat, bz, j0, false);
-  const float inv = inverse(a.norm[bz] + a.eps);
-  for (int k = threadIdx.x; k < R16 * ld; k += 256) X[k] *= inv;
-  __syncthreads();
+  const double full = a.norm[bz] + a.eps;
+  const float inv = inverse(full);
+  const double inv64 = full == 0.0 ? 0.0 : 1.0 / full;
+  if constexpr (!WIDE) {
+    for (int k = threadIdx.x; k < R16 * ld; k += 256) X[k] *= inv;
+    __syncthreads();
+  }
   f32x4 res[8];                                    // at most 64 x 128 results: 32 tiles, 8 a wave
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int t = wave + u * 4;
     if (t >= tiles) continue;
     const int i0 = t / tc * 16, c0 = t % tc * 16;
-    f32x4 v = rows_cols((GRAD ? M2 : M1) + i0 * ldm, ldm, X + c0, ld, R16, f32x4{0.f, 0.f, 0.f, 0.f});
-    if (GRAD) v = rows_cols(M1 + i0 * ldm, ldm, D + c0, ld, R16, v);
-    res[u] = v;
+    if constexpr (WIDE) {
+      f64x4 v = rows_cols64((GRAD ? M2 : M1) + i0 * ldm, ldm, X + c0, ld, R16, f64x4{0.0, 0.0, 0.0, 0.0});
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] *= inv64;
+      if (GRAD) v = rows_cols64(M1 + i0 * ldm, ldm, D + c0, ld, R16, v);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) res[u][r] = (float)v[r];
+    } else {
+      f32x4 v = rows_cols((GRAD ? M2 : M1) + i0 * ldm, ldm, X + c0, ld, R16, f32x4{0.f, 0.f, 0.f, 0.f});
+      if (GRAD) v = rows_cols(M1 + i0 * ldm, ldm, D + c0, ld, R16, v);
+      res[u] = v;
+    }
   }
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const int t = wave + u * 4;
     if (t >= tiles) continue;
-    float* p = X + (t / tc * 16 + 4 * ((threadIdx.x & 63) >> 4)) * ld + t % tc * 16 + (threadIdx.x & 15);
+    float* p = X + t / tc * 16 * ld + t % tc * 16 + l;        // rows 4 q + r of the tile; q + 4 r from the f64 instruction
 #pragma unroll
-    for (int r = 0; r < 4; ++r) p[r * ld] = res[u][r];
+    for (int r = 0; r < 4; ++r) p[(WIDE ? q + 4 * r : 4 * q + r) * ld] = res[u][r];
   }
   __syncthreads();
   const int cols = min(THIN_COLS, a.n - j0);
@@ -1458,17 +1490,21 @@ GradWork take_grad(Arena& w, const Shape& s) {
 }
 
 // What bounds the operands of a step whose X has singular values in [0, s]: x for X, A = s^2, B = max |b t + c t^2|, next = max |p|,
-// slope = max |p'|, by which a step can lengthen a derivative: its gains are divided differences of the odd p.
+// slope = max |p'|, by which a step can lengthen a derivative: its gains are divided differences of the odd p,
+// factor = max |p(t) / t|, what it can multiply a direction by.
 struct Bound {
-  double x, A, B, next, slope;
+  double x, A, B, next, slope, factor;
 };
 
 Bound bound_of(double s, const double* co) {
   const double a = co[0], b = co[1], c = co[2], t1 = s * s;
-  Bound r{s, t1, fabs(b * t1 + c * t1 * t1), 0.0, 0.0};
+  Bound r{s, t1, fabs(b * t1 + c * t1 * t1), 0.0, 0.0, fmax(fabs(a), fabs(a + b * t1 + c * t1 * t1))};
   if (c != 0.0) {
     const double t = -b / (2 * c);
-    if (t > 0 && t < t1) r.B = fmax(r.B, fabs(b * t + c * t * t));
+    if (t > 0 && t < t1) {
+      r.B = fmax(r.B, fabs(b * t + c * t * t));
+      r.factor = fmax(r.factor, fabs(a + b * t + c * t * t));
+    }
   }
   auto p = [&](double t) { return fabs(sqrt(t) * (a + b * t + c * t * t)); };
   auto slope = [&](double t) { return fabs(a + 3 * b * t + 5 * c * t * t); };
@@ -1512,6 +1548,18 @@ bool scales_of(int steps, const double* coef, Scales* out) {
     s = b.next;
   }
   return s * SLACK <= MAX_S;
+}
+
+// what the steps together can multiply a direction by; infinite without coefficients
+double growth_of(int steps, const double* coef) {
+  if (!coef) return INFINITY;
+  double s = 1.0, g = 1.0;
+  for (int i = 0; i < steps; ++i) {
+    const Bound b = bound_of(s * SLACK, coef + 3 * i);
+    g *= fmax(1.0, b.factor);
+    s = b.next;
+  }
+  return g == g ? g : INFINITY;
 }
 
 template <int P, class Epi>
@@ -1607,7 +1655,12 @@ void pair(Args& g, const f16* a, const f16* b) {
 
 constexpr int SMALL_LDS = 156 * 1024;        // of 160 KB: the reductions take a little
 
-bool thin_fits(const Shape& s, bool grad) { return s.mr <= (grad ? THIN_GRAD_R : THIN_R); }
+// The two-pass form's results are off by the growth times the rounding of its last product, 2^-24 in f32 (600 holds five steps
+// of the default, 485, at 9e-6 to 6e-5), and by the growth's square times 2^-53 times the root of the columns: 2^18, ten
+// steps of the default, leaves 1e-3 of its margin at 2^24 columns.
+constexpr double THIN_GROWTH_F32 = 600.0, THIN_GROWTH = 262144.0;
+
+bool thin_fits(const Shape& s, bool grad, double growth) { return growth <= THIN_GROWTH && s.mr <= (grad ? THIN_GRAD_R : THIN_R); }
 
 // Where the two-pass form could take the matrix too, the one-workgroup form stops here: its time grows with the columns, the
 // other's chain of m x m products does not.  Result / gradient of one f32 matrix in us, one workgroup and two passes:
@@ -1616,8 +1669,8 @@ bool thin_fits(const Shape& s, bool grad) { return s.mr <= (grad ? THIN_GRAD_R :
 constexpr int SMALL_COLS = 240;
 
 // bytes of LDS of the one-workgroup form; 0: it does not fit, or another is quicker
-int small_bytes(const Shape& s, bool grad) {
-  if (s.mr > 512 || s.nc > 4096 || (thin_fits(s, grad) && s.nc > SMALL_COLS)) return 0;
+int small_bytes(const Shape& s, bool grad, double growth) {
+  if (s.mr > 512 || s.nc > 4096 || (thin_fits(s, grad, growth) && s.nc > SMALL_COLS)) return 0;
   const SmallShape q = small_shape(s.m, s.n, s.cx);
   if ((q.R16 / 16) * (q.C16 / 16) > SMALL_WAVES * SMALL_TILES) return 0;
   const long long b = 4ll * ((grad ? 2 : 1) * q.R16 * q.ldx + (grad ? 4 : 2) * q.R16 * q.lda);
@@ -1836,8 +1889,7 @@ int thin_parts(const Shape& s) {
 }
 
 struct ThinWork {
-  double *part, *norm, *steps;
-  float *m1, *m2;
+  double *part, *norm, *steps, *m1, *m2;
 };
 
 ThinWork take_thin(Arena& w, const Shape& s, bool grad, int steps) {
@@ -1845,9 +1897,9 @@ ThinWork take_thin(Arena& w, const Shape& s, bool grad, int steps) {
   const long long q = (long long)thin_r16(s) * thin_r16(s) * s.batch;
   k.part = w.take<double>(q * thin_parts(s));
   k.norm = w.take<double>(s.batch);
-  k.m1 = w.take<float>(q);
+  k.m1 = w.take<double>(q);
   if (grad) {
-    k.m2 = w.take<float>(q);
+    k.m2 = w.take<double>(q);
     k.steps = w.take<double>(3 * q * steps);
   }
   return k;
@@ -1899,16 +1951,25 @@ ThinArgs thin_args(const Shape& s, const Problem& q, const ThinWork& w) {
   return a;
 }
 
+template <int SRC, bool GRAD, class S>
+hipError_t thin_apply(const Shape& s, const ThinArgs& a, hipStream_t st) {
+  constexpr int pad = 16 / sizeof(S), size = sizeof(S);
+  const int r = thin_r16(s), ld = s.cx * THIN_COLS + 4, bytes = (GRAD ? 2 : 1) * r * (4 * ld + size * (r + pad));
+  static std::atomic<unsigned long long> done{0};
+  const hipError_t e = raise_lds(reinterpret_cast<const void*>(thin_apply_kernel<SRC, GRAD, S>),
+                                 THIN_R * (4 * (2 * THIN_COLS + 4) + size * (THIN_R + pad)), done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((thin_apply_kernel<SRC, GRAD, S>), dim3(a.chunks, s.batch), dim3(256), bytes, st, a);
+  return hipGetLastError();
+}
+
 template <int SRC, bool GRAD>
-hipError_t thin_launch(const Shape& s, const ThinArgs& a, hipStream_t st) {
-  const int r = thin_r16(s), ld = s.cx * THIN_COLS + 4, gram = (GRAD ? 2 : 1) * r * ld * 4, apply = (GRAD ? 2 : 1) * r * (ld + r + 4) * 4,
-            poly = (GRAD ? 11 : 4) * r * (r + 2) * 8;
-  static std::atomic<unsigned long long> done[3] = {};
-  const int most = THIN_R * (2 * THIN_COLS + 4) * 4 + THIN_R * (THIN_R + 4) * 4;
-  hipError_t e = raise_lds(reinterpret_cast<const void*>(thin_gram_kernel<SRC, GRAD>), most, done[0]);
-  if (e == hipSuccess) e = raise_lds(reinterpret_cast<const void*>(thin_apply_kernel<SRC, GRAD>), most, done[1]);
+hipError_t thin_launch(const Shape& s, const ThinArgs& a, double growth, hipStream_t st) {
+  const int r = thin_r16(s), gram = (GRAD ? 2 : 1) * r * (s.cx * THIN_COLS + 4) * 4, poly = (GRAD ? 11 : 4) * r * (r + 2) * 8;
+  static std::atomic<unsigned long long> done[2] = {};
+  hipError_t e = raise_lds(reinterpret_cast<const void*>(thin_gram_kernel<SRC, GRAD>), THIN_R * (2 * THIN_COLS + 4) * 4, done[0]);
   if (e == hipSuccess)
-    e = raise_lds(GRAD ? reinterpret_cast<const void*>(thin_grad_poly_kernel) : reinterpret_cast<const void*>(thin_poly_kernel), SMALL_LDS, done[2]);
+    e = raise_lds(GRAD ? reinterpret_cast<const void*>(thin_grad_poly_kernel) : reinterpret_cast<const void*>(thin_poly_kernel), SMALL_LDS, done[1]);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((thin_gram_kernel<SRC, GRAD>), dim3(a.parts, s.batch), dim3(256), gram, st, a);
   e = hipGetLastError();
@@ -1917,16 +1978,15 @@ hipError_t thin_launch(const Shape& s, const ThinArgs& a, hipStream_t st) {
   else hipLaunchKernelGGL(thin_poly_kernel, dim3(s.batch), dim3(THIN_THREADS), poly, st, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((thin_apply_kernel<SRC, GRAD>), dim3(a.chunks, s.batch), dim3(256), apply, st, a);
-  return hipGetLastError();
+  return growth <= THIN_GROWTH_F32 ? thin_apply<SRC, GRAD, float>(s, a, st) : thin_apply<SRC, GRAD, double>(s, a, st);
 }
 
 template <bool GRAD>
-hipError_t thin(const Shape& s, int src, const ThinArgs& a, hipStream_t st) {
-  if (src == SRC_F32) return thin_launch<SRC_F32, GRAD>(s, a, st);
-  if (src == SRC_F16) return thin_launch<SRC_F16, GRAD>(s, a, st);
-  if (src == SRC_BF16) return thin_launch<SRC_BF16, GRAD>(s, a, st);
-  return thin_launch<SRC_C64, GRAD>(s, a, st);
+hipError_t thin(const Shape& s, int src, const ThinArgs& a, double growth, hipStream_t st) {
+  if (src == SRC_F32) return thin_launch<SRC_F32, GRAD>(s, a, growth, st);
+  if (src == SRC_F16) return thin_launch<SRC_F16, GRAD>(s, a, growth, st);
+  if (src == SRC_BF16) return thin_launch<SRC_BF16, GRAD>(s, a, growth, st);
+  return thin_launch<SRC_C64, GRAD>(s, a, growth, st);
 }
 
 hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
@@ -2102,26 +2162,35 @@ using namespace tcmi::orth;
 
 extern "C" {
 
-long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full, int dtype, int what) {
+long long tcmi_ns_work_bytes_coef(int rows, int cols, int batch, int steps, const double* coef_host, int full, int dtype, int what) {
   if (!sizes_ok(rows, cols, batch, steps, dtype) || what < 0 || what > 3) return -1;
   const Shape s = shape_of(rows, cols, batch, dtype, full != 0 || what != TCMI_NS_WORK);
-  Arena a{nullptr};
-  if (small_bytes(s, what == TCMI_NS_SAVED || what == TCMI_NS_WORK_GRAD || what == TCMI_NS_WORK_SAVING)) {
-    if (what == TCMI_NS_SAVED) take_small(a, s, steps);
-    else a.take<char>(1);
+  const bool grad = what != TCMI_NS_WORK;
+  auto bytes = [&](double growth) -> long long {
+    Arena a{nullptr};
+    if (small_bytes(s, grad, growth)) {
+      if (what == TCMI_NS_SAVED) take_small(a, s, steps);
+      else a.take<char>(1);
+    } else if (thin_fits(s, grad, growth)) {
+      if (what == TCMI_NS_SAVED) take_thin_saved(a, s);
+      else take_thin(a, s, what == TCMI_NS_WORK_GRAD, steps);
+    } else {
+      if (!rows_ok(s)) return -1;
+      if (what == TCMI_NS_WORK) take_work(a, s, false);
+      else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true);
+      else if (what == TCMI_NS_SAVED) take_saved(a, s, steps);
+      else take_grad(a, s);
+    }
     return a.used;
-  }
-  if (thin_fits(s, what != TCMI_NS_WORK)) {
-    if (what == TCMI_NS_SAVED) take_thin_saved(a, s);
-    else take_thin(a, s, what == TCMI_NS_WORK_GRAD, steps);
-    return a.used;
-  }
-  if (!rows_ok(s)) return -1;
-  if (what == TCMI_NS_WORK) take_work(a, s, false);
-  else if (what == TCMI_NS_WORK_SAVING) take_work(a, s, true);
-  else if (what == TCMI_NS_SAVED) take_saved(a, s, steps);
-  else take_grad(a, s);
-  return a.used;
+  };
+  const long long most = bytes(growth_of(steps, coef_host));
+  if (coef_host) return most;
+  const long long least = bytes(1.0);              // any coefficients: whichever form they lead to
+  return most > least ? most : least;
+}
+
+long long tcmi_ns_work_bytes(int rows, int cols, int batch, int steps, int full, int dtype, int what) {
+  return tcmi_ns_work_bytes_coef(rows, cols, batch, steps, nullptr, full, dtype, what);
 }
 
 int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long g_bs, void* out, int rows, int cols, int batch,
@@ -2132,8 +2201,9 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
   // three forms: one workgroup per matrix; two passes around m x m matrices; a sequence of large products
-  const int small = small_bytes(s, saved != nullptr);
-  const bool narrow = !small && thin_fits(s, saved != nullptr);
+  const double growth = growth_of(steps, coef_host);
+  const int small = small_bytes(s, saved != nullptr, growth);
+  const bool narrow = !small && thin_fits(s, saved != nullptr, growth);
   Arena aw{(char*)work}, av{(char*)saved};
   Work w{};
   Saved sv{};
@@ -2176,7 +2246,7 @@ int tcmi_newton_schulz(const void* g, long long g_rs, long long g_cs, long long 
     ThinArgs a = thin_args(s, q, tw);
     a.a0 = ts.a0;
     if (saved) a.norm = ts.norm;
-    e = thin<false>(s, q.src, a, reinterpret_cast<hipStream_t>(stream));
+    e = thin<false>(s, q.src, a, growth, reinterpret_cast<hipStream_t>(stream));
   } else {
     e = forward(s, q, sc, w, saved ? &sv : nullptr, reinterpret_cast<hipStream_t>(stream));
   }
@@ -2191,8 +2261,9 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_newton_schulz_grad: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype, true);
   Arena aw{(char*)work}, av{(char*)const_cast<void*>(saved)};
-  const int small = small_bytes(s, true);
-  const bool narrow = !small && thin_fits(s, true);
+  const double growth = growth_of(steps, coef_host);
+  const int small = small_bytes(s, true, growth);
+  const bool narrow = !small && thin_fits(s, true, growth);
   GradWork w{};
   Saved sv{};
   SmallSaved ss{};
@@ -2237,7 +2308,7 @@ int tcmi_newton_schulz_grad(const void* g, long long g_rs, long long g_cs, long 
     a.dflat = a.dy.cs <= a.dy.rs;
     a.a0 = ts.a0;
     a.norm = ts.norm;
-    e = thin<true>(s, q.src, a, reinterpret_cast<hipStream_t>(stream));
+    e = thin<true>(s, q.src, a, growth, reinterpret_cast<hipStream_t>(stream));
   } else {
     e = backward(s, q, oriented(dout, d_rs, d_cs, d_bs, s.flip), sc, w, sv, reinterpret_cast<hipStream_t>(stream));
   }
@@ -2252,8 +2323,9 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
       !(momentum >= 0) || !(momentum < 1) || (!full && dtype != TCMI_BF16))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_muon_step: bad argument");
   const Shape s = shape_of(rows, cols, batch, dtype, full != 0);
-  const int small = small_bytes(s, false);
-  const bool narrow = !small && thin_fits(s, false);
+  const double growth = growth_of(steps, coef_host);
+  const int small = small_bytes(s, false, growth);
+  const bool narrow = !small && thin_fits(s, false, growth);
   Arena aw{(char*)work};
   Work w{};
   ThinWork tw{};
@@ -2285,7 +2357,7 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
   q.keep = (float)keep;
   q.rate = (float)rate;
   const hipError_t e = small    ? small_by_type<false>(q.src, small_args(s, q), small, batch, reinterpret_cast<hipStream_t>(stream))
-                       : narrow ? thin<false>(s, q.src, thin_args(s, q, tw), reinterpret_cast<hipStream_t>(stream))
+                       : narrow ? thin<false>(s, q.src, thin_args(s, q, tw), growth, reinterpret_cast<hipStream_t>(stream))
                                 : forward(s, q, sc, w, nullptr, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? TCMI_OK : tcmi_set_error_(TCMI_ERR_HIP, hipGetErrorString(e));
 }

@@ -200,6 +200,7 @@ _SIGNATURES = {
     "tcmi_allreduce_sum": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]),
     "tcmi_comm_destroy": (ctypes.c_int, [ctypes.c_void_p]),
     "tcmi_ns_work_bytes": (ctypes.c_longlong, [ctypes.c_int] * 7),
+    "tcmi_ns_work_bytes_coef": (ctypes.c_longlong, [ctypes.c_int] * 4 + [ctypes.c_void_p] + [ctypes.c_int] * 3),
     "tcmi_newton_schulz": (
         ctypes.c_int,
         [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int,

@@ -436,7 +436,8 @@ def newton_schulz(mat, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float 
 
     ``coefficients``: one triple ``(a, b, c)``, or one per step.  The default drives every singular value into about
     0.7 .. 1.2 in five steps (enough for an optimiser's update); ``(1.5, -0.5, 0)`` converges to the polar factor itself.
-    float32, bfloat16, float16, complex64; up to 65535 matrices; any strides; same shape and dtype out.  Differentiable once, including in
+    float32, bfloat16, float16, complex64; up to 65535 matrices, rows up to 2^21 elements (2^24 beside a short side of 16 and up to
+    ten steps of the default); any strides; same shape and dtype out.  Differentiable once, including in
     ``backend.value_and_grad`` / ``vmap``: unlike the gradient of :func:`svd_trunc` its gradient has no
     ``1 / (s_i^2 - s_j^2)`` and holds at an isometry, where all singular values agree.  A zero matrix gives zero, a
     non-finite entry makes its whole matrix NaN.  Coefficients that let singular values grow past 64 are refused.
@@ -466,18 +467,18 @@ def _newton_schulz_raw(mat, steps, flat, eps, saving):
     if out.numel() == 0:
         return out, torch.empty(0, dtype=torch.uint8, device=mat.device)
     full = int(saving or mat.dtype != torch.bfloat16)
-    L = _lib.lib()
-    nbytes = L.tcmi_ns_work_bytes(m, n, b, steps, full, code, _lib.NS_WORK_SAVING if saving else _lib.NS_WORK)
+    L, coef = _lib.lib(), _host_doubles(flat)
+    nbytes = L.tcmi_ns_work_bytes_coef(m, n, b, steps, coef, full, code, _lib.NS_WORK_SAVING if saving else _lib.NS_WORK)
     if nbytes < 0:
-        raise ValueError(f"newton_schulz: {b} matrices of {m} x {n} are out of range")
+        raise ValueError(f"newton_schulz: {b} matrices of {m} x {n} are out of range ({steps} steps)")
     work = torch.empty(nbytes, dtype=torch.uint8, device=mat.device)
     saved, kept = None, 0
     if saving:
-        kept = L.tcmi_ns_work_bytes(m, n, b, steps, 1, code, _lib.NS_SAVED)
+        kept = L.tcmi_ns_work_bytes_coef(m, n, b, steps, coef, 1, code, _lib.NS_SAVED)
         saved = torch.empty(kept, dtype=torch.uint8, device=mat.device)
     with _on(mat.device):
         _lib.check(L.tcmi_newton_schulz(x.data_ptr(), x.stride(1), x.stride(2), x.stride(0), out.data_ptr(), m, n, b, steps,
-                                        _host_doubles(flat), eps, full, saved.data_ptr() if saving else None, kept,
+                                        coef, eps, full, saved.data_ptr() if saving else None, kept,
                                         work.data_ptr(), nbytes, code, _raw_stream(mat.device)), "tcmi_newton_schulz")
     return out, saved
 
@@ -491,11 +492,11 @@ def _newton_schulz_grad_raw(mat, saved, dout, steps, flat, eps):
     out = torch.empty(mat.shape, dtype=mat.dtype, device=mat.device)
     if out.numel() == 0:
         return out
-    L = _lib.lib()
-    work = torch.empty(L.tcmi_ns_work_bytes(m, n, b, steps, 1, code, _lib.NS_WORK_GRAD), dtype=torch.uint8, device=mat.device)
+    L, coef = _lib.lib(), _host_doubles(flat)
+    work = torch.empty(L.tcmi_ns_work_bytes_coef(m, n, b, steps, coef, 1, code, _lib.NS_WORK_GRAD), dtype=torch.uint8, device=mat.device)
     with _on(mat.device):
         _lib.check(L.tcmi_newton_schulz_grad(x.data_ptr(), x.stride(1), x.stride(2), x.stride(0), d.data_ptr(), d.stride(1),
-                                             d.stride(2), d.stride(0), out.data_ptr(), m, n, b, steps, _host_doubles(flat), eps,
+                                             d.stride(2), d.stride(0), out.data_ptr(), m, n, b, steps, coef, eps,
                                              saved.data_ptr(), saved.numel(), work.data_ptr(), work.numel(), code,
                                              _raw_stream(mat.device)), "tcmi_newton_schulz_grad")
     return out

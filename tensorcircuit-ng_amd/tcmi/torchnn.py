@@ -305,17 +305,17 @@ def muon_step(param: Tensor, grad: Tensor, momentum_buffer: Tensor, lr: float = 
         g = linalg._as_batch(grad.detach())
         b, m, n = p.shape
         full = int(param.dtype != torch.bfloat16)
-        L = _lib.lib()
-        nbytes = L.tcmi_ns_work_bytes(m, n, b, steps, full, code, _lib.NS_WORK)
+        L, coef = _lib.lib(), linalg._host_doubles(flat)
+        nbytes = L.tcmi_ns_work_bytes_coef(m, n, b, steps, coef, full, code, _lib.NS_WORK)
         if nbytes < 0:
-            raise ValueError(f"muon_step: {b} matrices of {m} x {n} are out of range")
+            raise ValueError(f"muon_step: {b} matrices of {m} x {n} are out of range ({steps} steps)")
         work = torch.empty(nbytes, dtype=torch.uint8, device=p.device)
         r = 0.2 * math.sqrt(max(m, n)) if adjust_lr_fn == "match_rms_adamw" else math.sqrt(max(1.0, m / n))
         with linalg._on(p.device):
             _lib.check(L.tcmi_muon_step(
                 p.data_ptr(), p.stride(1), p.stride(2), p.stride(0), g.data_ptr(), g.stride(1), g.stride(2), g.stride(0),
                 v.data_ptr(), v.stride(1), v.stride(2), v.stride(0), m, n, b, float(momentum), int(bool(nesterov)),
-                1.0 - float(lr) * float(weight_decay), -float(lr) * r, steps, linalg._host_doubles(flat), float(eps), full,
+                1.0 - float(lr) * float(weight_decay), -float(lr) * r, steps, coef, float(eps), full,
                 work.data_ptr(), nbytes, code, linalg._raw_stream(p.device)), "tcmi_muon_step")
         torch.autograd.graph.increment_version(param)
         torch.autograd.graph.increment_version(momentum_buffer)

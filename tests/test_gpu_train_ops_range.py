@@ -1,0 +1,177 @@
+"""The training operators on the GPU over the rest of their range: many steps, low rank, features and probabilities of every
+size.  Against plain 64-bit formulas; tolerances are derived at each test from the number formats."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+A, B, C = 3.4445, -4.7750, 2.0315
+DEFAULT = (A, B, C)
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.complex64: 2.0 ** -24}
+
+
+def _rand(seed, *shape, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    wide = torch.complex64 if dtype == torch.complex64 else torch.float32
+    return torch.randn(*shape, generator=g, dtype=wide).to(dtype)
+
+
+def _rel(got, want):
+    got = got.detach().cpu().to(want.dtype)
+    return float(torch.linalg.vector_norm(got - want) / torch.linalg.vector_norm(want))
+
+
+# ----------------------------------------------------------------------------------------- Newton-Schulz, many steps
+def _step64(x, coef):
+    a, b, c = coef
+    s = x @ x.mH
+    return a * x + (b * s + c * s @ s) @ x
+
+
+def _ns64(x, coefs, eps=1e-7):
+    x = x.to(torch.complex128 if x.is_complex() else torch.float64)
+    tall = x.shape[-2] > x.shape[-1]
+    if tall:
+        x = x.mT
+    x = x / (torch.linalg.matrix_norm(x)[..., None, None] + eps)
+    for coef in coefs:
+        x = _step64(x, coef)
+    return x.mT if tall else x
+
+
+def _twice(seed, m, n, dtype):
+    """every row occurs twice"""
+    return torch.cat([_rand(seed, m // 2, n, dtype=dtype)] * 2)
+
+
+def _amplified(x, coefs):
+    """what a relative error made in each step can have grown to at the end, from perturbations of the iterates that leave
+    equal rows equal (as equal arithmetic does), times 4 for directions worse than random ones; relative to the result"""
+    x = x.to(torch.complex128 if x.is_complex() else torch.float64)
+    x = x / torch.linalg.matrix_norm(x)
+    its = [x]
+    for coef in coefs:
+        its.append(_step64(its[-1], coef))
+    total = 0.0
+    for k in range(len(coefs)):
+        d = _twice(1000 + k, *x.shape, dtype=torch.float32).to(x.dtype)
+        d = d * (1e-7 * torch.linalg.matrix_norm(its[k]) / torch.linalg.matrix_norm(d))
+        y = its[k] + d
+        for coef in coefs[k:]:
+            y = _step64(y, coef)
+        total += float((y - its[-1]).norm() / its[-1].norm()) / 1e-7
+    return 4.0 * total
+
+
+def _two_passes(x, coefs, rank):
+    """Two passes in f32 while the steps multiply no direction by more than 600: M's entries and X_0 are rounded, 3 * 2^-24
+    times that factor g times sqrt(rows) against a result of at least 0.7 sqrt(rank).  In f64 (up to 2^18) the same with 2^-53,
+    and the rounding of A_0, which grows by g^2."""
+    g = math.prod(max(abs(c[0]), 1.0) for c in coefs)
+    return 3 * (2.0 ** -24 if g <= 600 else 2.0 ** -53 * g) * g * math.sqrt(min(x.shape) / rank) / 0.7 if g <= 2.0 ** 18 else 0.0
+
+
+def _many_tol(x, coefs, dtype, rank):
+    """two passes, or 4 units of 2^-22 a step where X is iterated; and the rounding to the type returned"""
+    return _two_passes(x, coefs, rank) + 4 * 2.0 ** -22 * _amplified(x, coefs) + HALF_STEP[dtype]
+
+
+@pytest.mark.parametrize("steps", [1, 2, 5, 6, 8, 10, 11, 16])
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (8, 1000)), (torch.float32, (32, 1000)), (torch.float32, (60, 1000)),
+                                         (torch.float32, (24, 28)), (torch.complex64, (16, 900))])
+def test_newton_schulz_many_steps_of_rows_that_occur_twice(shape, dtype, steps):
+    """a direction that G does not have gets a factor a a step in every polynomial of G G^H, and must stay empty all the same"""
+    from tcmi import linalg
+
+    x = _twice(200, *shape, dtype=dtype)
+    coefs = [DEFAULT] * steps
+    want, tol = _ns64(x, coefs), _many_tol(x, coefs, dtype, min(shape) // 2)
+    assert _rel(linalg.newton_schulz(x.cuda(), steps), want) < tol
+    assert _rel(linalg.newton_schulz(x.mT.cuda(), steps), want.mT) < tol
+    leaf = x.cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf, steps)
+    assert _rel(out, want) < tol
+    # The gradient: 8 units of 2^-22 a step, against a cotangent that may grow by a a step where G has nothing.
+    dy = _rand(201, *shape, dtype=dtype)
+    (got,) = torch.autograd.grad(out, leaf, dy.cuda())
+    ref = x.to(want.dtype).requires_grad_()
+    (grad,) = torch.autograd.grad(_ns64(ref, coefs), ref, dy.to(want.dtype))
+    size = torch.linalg.vector_norm(dy.to(want.dtype)) * max(A ** steps, 1.0) / torch.linalg.vector_norm(x.to(want.dtype))
+    assert float(torch.linalg.vector_norm(got.cpu().to(want.dtype) - grad)) < float(size) * (8 * steps * 2.0 ** -22 + HALF_STEP[dtype])
+
+
+@pytest.mark.parametrize("rank", [1, 4])
+@pytest.mark.parametrize("steps", [5, 8, 10, 12, 16])
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (8, 1000)), (torch.float32, (32, 1000)), (torch.float32, (1000, 60)),
+                                         (torch.bfloat16, (32, 1000)), (torch.complex64, (16, 900)), (torch.float32, (70, 500))])
+def test_newton_schulz_many_steps_of_low_rank(shape, dtype, steps, rank):
+    """What the rounding of G's entries adds to its rank grows as in any arithmetic; no singular value may pass the bound that
+    the polynomial keeps them under (max p on [0, 1.21] is 1.2025, and 1.005 of that where operands have 11 bits), and the
+    directions that G has keep theirs."""
+    from tcmi import linalg, torchnn
+
+    m, n = shape
+    wide = torch.complex64 if dtype == torch.complex64 else torch.float32
+    x = (_rand(210, m, rank, dtype=wide) @ _rand(211, rank, n, dtype=wide)).to(dtype)
+    for out in (linalg.newton_schulz(x.cuda(), steps), linalg.newton_schulz(x.cuda().requires_grad_(), steps).detach()):
+        out = out.cpu().to(torch.complex128 if out.is_complex() else torch.float64)
+        assert float(torch.linalg.matrix_norm(out, 2)) < 1.2025 * 1.005 + 1.2 * HALF_STEP[dtype] * math.sqrt(min(m, n))
+    if dtype == torch.float32:
+        p, v = torch.zeros(m, n, device="cuda"), torch.zeros(m, n, device="cuda")
+        torchnn.muon_step(p, x.cuda(), v, lr=1.0, weight_decay=0.0, ns_steps=steps)
+        r = math.sqrt(max(1.0, m / n))
+        assert float(torch.linalg.matrix_norm(p.cpu().double(), 2)) / r < 1.2025 * 1.005
+        if steps <= 10 and min(m, n) <= 64:               # up to here the two passes answer as 64 bits do
+            assert _rel(linalg.newton_schulz(x.cuda(), steps), _ns64(x, [DEFAULT] * steps)) < _two_passes(x, [DEFAULT] * steps, rank) + 2.0 ** -23
+
+
+STEEP = tuple((8.0, -22.0 / t ** 2, 16.0 / t ** 4) for t in (1.0, 2.479, 6.145, 15.233))        # tops of the steps before, 8^4 = 4096
+
+
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (20, 700)), (torch.float32, (700, 6)), (torch.float32, (60, 500)), (torch.complex64, (16, 600))])
+def test_newton_schulz_few_steep_steps(shape, dtype):
+    """four steps that multiply an empty direction by 4096: f64 sums of the two passes (the form goes by the factor)"""
+    from tcmi import linalg
+
+    m, n = min(shape), max(shape)
+    x = _twice(220, m, n, dtype=dtype)
+    want = _ns64(x, STEEP)
+    x, want = (x.mT, want.mT) if shape[0] > shape[1] else (x, want)
+    assert _rel(linalg.newton_schulz(x.cuda(), 4, STEEP), want) < _many_tol(x if shape[0] < shape[1] else x.mT, STEEP, dtype, m // 2)
+
+
+COEFS = [(DEFAULT,), ((1.5, -0.5, 0.0),) * 6, (DEFAULT,) * 3 + ((1.5, -0.5, 0.0),) * 2, (DEFAULT,) * 7, STEEP[:1] + ((3.2, -1.408, 0.16384),) * 3]
+
+
+@pytest.mark.parametrize("coef", COEFS)
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (24, 28)), (torch.float32, (8, 900)), (torch.float32, (31, 700)),
+                                         (torch.float32, (60, 300)), (torch.bfloat16, (40, 260)), (torch.float16, (300, 20)),
+                                         (torch.complex64, (12, 20)), (torch.complex64, (16, 250)), (torch.complex64, (200, 14))])
+def test_newton_schulz_small_and_thin_with_other_coefficients(dtype, shape, coef):
+    """one workgroup and two passes: single steps, triples per step, more than five of them, steep ones"""
+    from tcmi import linalg
+
+    x, dy = _rand(230, 2, *shape, dtype=dtype), _rand(231, 2, *shape, dtype=dtype)
+    steps, co = len(coef), coef if len(set(coef)) > 1 else coef[0]
+    leaf = x.cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf, steps, co)
+    plain = linalg.newton_schulz(x.cuda(), steps, co)
+    (got,) = torch.autograd.grad(out, leaf, dy.cuda())
+    grow, top = 1.0, 1.0
+    for a, b, c in coef:                                  # the steps' largest slopes where singular values can lie
+        t = torch.linspace(0, 1.02 * top, 1000, dtype=torch.float64)
+        grow *= max(1.0, float((a + 3 * b * t ** 2 + 5 * c * t ** 4).abs().max()))
+        top = float((a * t + b * t ** 3 + c * t ** 5).abs().max())
+    for k in range(2):
+        ref = x[k].to(torch.complex128 if dtype == torch.complex64 else torch.float64).requires_grad_()
+        want = _ns64(ref, coef)
+        (grad,) = torch.autograd.grad(want, ref, dy[k].to(ref.dtype))
+        # 4 (gradient: 8) units of 2^-22 a step, each times what the steps behind it can make of it
+        assert _rel(out[k], want.detach()) < 4 * 2.0 ** -22 * steps * grow + HALF_STEP[dtype]
+        if dtype != torch.bfloat16:
+            assert _rel(plain[k], want.detach()) < 4 * 2.0 ** -22 * steps * grow + HALF_STEP[dtype]
+        size = torch.linalg.vector_norm(dy[k].to(ref.dtype)) / torch.linalg.matrix_norm(x[k].to(ref.dtype))
+        assert float(torch.linalg.vector_norm(got[k].cpu().to(ref.dtype) - grad)) < float(size) * 8 * steps * 2.0 ** -22 * grow + HALF_STEP[dtype] * float(grad.norm())

@@ -149,3 +149,20 @@ def test_shared_memory_and_long_sides_are_refused():
     assert lib.tcmi_ns_work_bytes(200, (1 << 21) + 1, 1, 5, 0, _lib.TCMI_BF16, 0) > 0
     assert lib.tcmi_lce_work_bytes(None, 64, None, 64, (1 << 21) + 1, 64, 100, f32, 0) == -1
     assert lib.tcmi_lce_work_bytes(None, 64, None, 64, 1 << 21, 64, 100, f32, 0) > 0
+
+
+def test_newton_schulz_form_goes_by_the_steps_growth():
+    """Two passes keep a polynomial of G G^H apart from G; past 2^18 (ten steps of the default) the iterated form needs its room,
+    and a row longer than that form takes is refused."""
+    lib = _lib.lib()
+    f32 = _lib.TCMI_F32
+
+    def room(rows, cols, steps, what, co=linalg.NS_COEFFICIENTS):
+        return lib.tcmi_ns_work_bytes_coef(rows, cols, 1, steps, linalg._host_doubles(co * steps), 1, f32, what)
+
+    for what in (_lib.NS_WORK, _lib.NS_WORK_SAVING, _lib.NS_SAVED, _lib.NS_WORK_GRAD):
+        assert 0 < room(8, 2000, 10, what) < room(8, 2000, 11, what)
+        assert room(8, 2000, 16, what, (1.5, -0.5, 0.0)) < room(8, 2000, 11, what)
+        assert lib.tcmi_ns_work_bytes(8, 2000, 1, 5, 1, f32, what) >= max(room(8, 2000, 5, what), room(8, 2000, 5, what, (8.0, -2.0, 0.1)))
+        assert room(8, 1 << 24, 10, what) > 0 and room(8, 1 << 24, 11, what) == -1
+    assert room(24, 28, 5, 9) == -1
