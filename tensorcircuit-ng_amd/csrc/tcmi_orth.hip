@@ -1,7 +1,7 @@
 // Newton-Schulz orthogonalisation of (batches of) matrices, its gradient, and the optimiser step built on it.
 //
 //   N = |G|_F + eps,  X_0 = G / N;   A = X X^H,  B = b A + c A A,  X <- a X + B X        (steps times)
-// A and B are symmetric, so only the tiles on and below the diagonal are computed and written twice.  Singular values are
+// A and B are symmetric, so only the tiles on and below the diagonal are computed and written twice (ns_factor).  Singular values are
 // at most 1 at the start (Frobenius norm) and the polynomial bounds them afterwards, so every operand has a bound known
 // on the host: operands are f16 under a power-of-two scale, products run on the f16 matrix pipe (mm16.h).
 //
@@ -1658,7 +1658,7 @@ constexpr int SMALL_LDS = 156 * 1024;        // of 160 KB: the reductions take a
 // The two-pass form's results are off by the growth times the rounding of its last product, 2^-24 in f32 (600 holds five steps
 // of the default, 485, at 9e-6 to 6e-5), and by the growth's square times 2^-53 times the root of the columns: 2^18, ten
 // steps of the default, leaves 1e-3 of its margin at 2^24 columns.
-constexpr double THIN_GROWTH_F32 = 600.0, THIN_GROWTH = 262144.0;
+constexpr double GROWTH_F32 = 600.0, THIN_GROWTH = 262144.0;
 
 bool thin_fits(const Shape& s, bool grad, double growth) { return growth <= THIN_GROWTH && s.mr <= (grad ? THIN_GRAD_R : THIN_R); }
 
@@ -1724,16 +1724,19 @@ hipError_t small_by_type(int src, const SmallArgs& a, int bytes, int batch, hipS
     if (e_ != hipSuccess) return e_;             \
   } while (0)
 
-// A, B of one step from the pieces of X
+// A, B of one step from the pieces of X.  tri: tiles above the diagonal are copies of those below.  Two-piece products add
+// hi lo' before lo hi', so a copy's rounding is that of x y where its neighbours' is that of y x, and rows of G that are equal stop
+// being so: 2^-24 in a direction that G does not have, times a in every step after.  Steps that grow it past 600 (six of the
+// default) compute every tile: 128 x 200 f32 with rows that occur twice, 10 / 16 steps: 5e-4 / 0.8 of the result -> 4e-6 / 7e-6.
 template <int P>
-hipError_t ns_factor(const Shape& s, const Pieces& p, const Scales& c, const double* co, float* split, hipStream_t st) {
+hipError_t ns_factor(const Shape& s, const Pieces& p, const Scales& c, const double* co, bool tri, float* split, hipStream_t st) {
   const long long xs = s.mr * s.np, qs = s.mr * s.mp;
   Args g = base_args(s, split, s.mr, s.mr, s.np, s.np, xs, xs);
   pair(g, p.x, p.x);
-  TRY(run<P>(g, true, EpiSym<P>{p.a, nullptr, s.mp, qs, 1.f / (c.x * c.x), 0.f, c.A}, st));
+  TRY(run<P>(g, tri, EpiSym<P>{p.a, nullptr, s.mp, qs, 1.f / (c.x * c.x), 0.f, c.A}, st));
   g = base_args(s, split, s.mr, s.mr, s.mp, s.mp, qs, qs);
   pair(g, p.a, p.a);
-  return run<P>(g, true, EpiSym<P>{p.b, p.a, s.mp, qs, (float)co[2] / (c.A * c.A), (float)co[1] / c.A, c.B}, st);
+  return run<P>(g, tri, EpiSym<P>{p.b, p.a, s.mp, qs, (float)co[2] / (c.A * c.A), (float)co[1] / c.A, c.B}, st);
 }
 
 struct Problem {
@@ -1783,7 +1786,7 @@ bool padded(const Shape& s) { return s.cx == 2 && (s.mp != s.P * s.mr || s.np !=
 template <int P>
 hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, Saved* sv, hipStream_t st) {
   const int nb = sum_blocks(s);
-  const bool fuse = !padded(s);
+  const bool fuse = !padded(s), tri = P == 1 || growth_of(q.steps, q.coef) <= GROWTH_F32;
   SumArgs sa{};
   sa.x = q.g;
   sa.outer = s.m;
@@ -1830,7 +1833,7 @@ hipError_t forward(const Shape& s, const Problem& q, const Scales* sc, Work& w, 
       a.src = Mat{w.carry, s.ldc, 1, s.m * s.ldc};
       TRY(launch_pack<P>(SRC_PLANAR, a, s, st));
     }
-    TRY(ns_factor<P>(s, p, sc[i], q.coef + 3 * i, w.split, st));
+    TRY(ns_factor<P>(s, p, sc[i], q.coef + 3 * i, tri, w.split, st));
     const float alpha = 1.f / (sc[i].B * sc[i].x), beta = (float)q.coef[3 * i];
     const long long ts = s.nc * s.mp, qs = s.mr * s.mp, cs = s.m * s.ldc;
     if (i + 1 < q.steps) {
@@ -1978,7 +1981,7 @@ hipError_t thin_launch(const Shape& s, const ThinArgs& a, double growth, hipStre
   else hipLaunchKernelGGL(thin_poly_kernel, dim3(s.batch), dim3(THIN_THREADS), poly, st, a);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  return growth <= THIN_GROWTH_F32 ? thin_apply<SRC, GRAD, float>(s, a, st) : thin_apply<SRC, GRAD, double>(s, a, st);
+  return growth <= GROWTH_F32 ? thin_apply<SRC, GRAD, float>(s, a, st) : thin_apply<SRC, GRAD, double>(s, a, st);
 }
 
 template <bool GRAD>

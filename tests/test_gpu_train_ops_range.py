@@ -128,6 +128,21 @@ def test_newton_schulz_many_steps_of_low_rank(shape, dtype, steps, rank):
             assert _rel(linalg.newton_schulz(x.cuda(), steps), _ns64(x, [DEFAULT] * steps)) < _two_passes(x, [DEFAULT] * steps, rank) + 2.0 ** -23
 
 
+@pytest.mark.parametrize("steps", [5, 6, 8, 10, 16])
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (128, 200)), (torch.float32, (130, 260)), (torch.float32, (400, 450)),
+                                         (torch.complex64, (70, 90)), (torch.complex64, (128, 192)), (torch.float16, (144, 150))])
+def test_newton_schulz_many_steps_of_equal_rows_in_different_tiles(shape, dtype, steps):
+    """the products' sums are the same for equal rows wherever they lie, so the direction between them stays empty"""
+    from tcmi import linalg
+
+    x = _twice(202, *shape, dtype=dtype)
+    want = _ns64(x, [DEFAULT] * steps)
+    tol = 4 * 2.0 ** -22 * _amplified(x, [DEFAULT] * steps) + HALF_STEP[dtype]
+    for y, z in ((x, want), (x.mT, want.mT)):
+        assert _rel(linalg.newton_schulz(y.cuda(), steps), z) < tol
+        assert _rel(linalg.newton_schulz(y.cuda().requires_grad_(), steps), z) < tol
+
+
 STEEP = tuple((8.0, -22.0 / t ** 2, 16.0 / t ** 4) for t in (1.0, 2.479, 6.145, 15.233))        # tops of the steps before, 8^4 = 4096
 
 
