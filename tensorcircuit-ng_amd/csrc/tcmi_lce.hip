@@ -75,7 +75,7 @@ __device__ __forceinline__ float scale_of(float top) {
 //   out   the row with k padded.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per row, whose
 //         inverse goes to inv[row] (the second read of the row comes from the cache).
 //   r     h only: the factor of row t in the gradients, from its target and dloss.
-//   part  partial maxima of |x| (h: times |r|, and |r| itself; rows whose factor is zero do not count).
+//   part  partial maxima of |x| (h: times |r|; rows whose factor is zero do not count).
 struct Operand {
   const void* src;
   long long rs;
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
       }
 #pragma unroll
       for (int k = 32; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor(t, k));
-      if (f != 0.f) top = fmaxf(top, (is_h && a.r ? fmaxf(t, 1.f) : t) * fabsf(f));
+      if (f != 0.f) top = fmaxf(top, t * fabsf(f));
     }
     if (!o.out) continue;
     if constexpr (DT == TCMI_F32) {
@@ -161,24 +161,16 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
 
 // out[c][row] = src[row][c] * r[row] * scale as f16 pieces (two for f32), rows padded with zeros.  A zero factor gives zero
 // whatever the row holds; an infinity anywhere else makes everything NaN (no scale would hold the rest beside it).
-// ones: behind the last column one more, the factors themselves (their product with P is the bias's gradient); 2 where all
-// rows that count share one factor: its power of two only, which one piece holds exactly, the epilogue multiplies the rest
-// back (2^-11 of the factor would shift every entry the same way).
 // 64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
 struct Turn {
   const void* src;
   long long rs;
-  int rows, cols, rowsp, vec, ones, tx, tiles;
+  int rows, cols, rowsp, vec, tx, tiles;
   const float *r, *part;
   int nparts;
   f16* out;
   float* inv;
 };
-
-__device__ __forceinline__ float power_of(float f) { return __uint_as_float(__float_as_uint(f) & 0xff800000u); }
-__device__ __forceinline__ float mantissa_of(float f) {
-  return f != f ? f : __uint_as_float((__float_as_uint(f) & 0x007fffffu) | 0x3f800000u);
-}
 
 template <int DT>
 __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
@@ -206,13 +198,8 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
       const float f = a.r ? a.r[row] : 1.f;
       if (f != 0.f) {
         v = fetch_row4<DT>(a.src, row * a.rs, c0 + u, a.cols, a.vec);
-        if (a.ones) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c0 + u + e == a.cols) v[e] = a.ones == 2 ? power_of(f) : f;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (c0 + u + e == a.cols ? v[e] : v[e] * f) * s;
+        for (int e = 0; e < 4; ++e) v[e] = v[e] * f * s;
       }
     }
 #pragma unroll
@@ -222,7 +209,7 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
 #pragma unroll
   for (int k = w; k < 64; k += 16) {
     const int c = c0 + k, row = r0 + u;
-    if (c < a.cols + (a.ones != 0) && row < a.rowsp) {
+    if (c < a.cols && row < a.rowsp) {
       f16x4 hi, lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -605,8 +592,7 @@ struct EpiProb {
   }
 };
 
-// a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor;
-// a column behind the last one is the bias's gradient
+// a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor
 struct EpiGrad {
   static constexpr bool TILE = false, FOUR = true;
   const float* inv;              // inverse of the other operand's scale, on the device
@@ -615,8 +601,6 @@ struct EpiGrad {
   const float* r;                // null: 1
   void* out;
   int dtype, cols;
-  void* db;
-  const float *dloss, *count;    // db: the factor all rows share, dloss (/ count), whose mantissa is still missing (null: none)
   int vec;                       // rows of `out` and `sum` are aligned for four elements
   __device__ __forceinline__ void four(const Args& g, int, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
@@ -648,11 +632,6 @@ struct EpiGrad {
     for (int k = 0; k < 4; ++k) {
       if (col + k >= g.N) continue;
       float x = al * v[k];
-      if (col + k == cols) {
-        if (dloss) x *= mantissa_of(count ? dloss[0] / count[0] : dloss[0]);
-        put(db, dtype, row, x);
-        continue;
-      }
       const long long at = (long long)row * cols + col + k;
       if (!first) x += sum[at];
       if (!last) sum[at] = x;
@@ -763,7 +742,7 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
   w.split = a.take<float>(PART_BYTES / 4);
   w.p = a.take<f16>(s.T * vp * s.P);
   w.pt = a.take<f16>(vc * s.tp * s.P);
-  w.ht = a.take<f16>((long long)(s.D + 1) * s.tp * s.P);
+  w.ht = a.take<f16>((long long)s.D * s.tp * s.P);
   w.wt = a.take<f16>(s.D * vp * s.P);
   return w;
 }
@@ -897,9 +876,6 @@ hipError_t forward(const Shape& s, const In& in, const FwdWork& w, float* lse, f
 template <int P>
 hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float* lse, const float* dloss, int per_row, const float* count,
                     void* dh, void* dw, void* db, hipStream_t st) {
-  // The bias's gradient as one more column of h^T: free where the columns do not fill their tiles, and a further column of
-  // tiles still costs less than reading P^T again (1021 x 512 x 32768 f32: 29 us against 47).
-  const int ones = db && dw ? (per_row ? 1 : 2) : 0, more = ones != 0;
   Prep a{};
   a.y = in.y;
   a.ignore = in.ignore;
@@ -915,11 +891,11 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
     const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P);
     Turn th{}, tw{};
     if (dw && v0 == 0) {
-      th = Turn{in.h, in.hrs, s.T, s.D, s.tp, vec4(in.h, in.hrs, s.dtype), ones, (s.tp + 63) / 64, 0, w.r, w.parth, parts_of(s.T), w.ht, w.invh};
-      th.tiles = th.tx * ((s.D + more + 63) / 64);
+      th = Turn{in.h, in.hrs, s.T, s.D, s.tp, vec4(in.h, in.hrs, s.dtype), (s.tp + 63) / 64, 0, w.r, w.parth, parts_of(s.T), w.ht, w.invh};
+      th.tiles = th.tx * ((s.D + 63) / 64);
     }
     if (dh) {
-      tw = Turn{(const char*)in.w + v0 * in.wrs * size, in.wrs, n, s.D, np, vec4(in.w, in.wrs, s.dtype), 0, (np + 63) / 64, 0, nullptr,
+      tw = Turn{(const char*)in.w + v0 * in.wrs * size, in.wrs, n, s.D, np, vec4(in.w, in.wrs, s.dtype), (np + 63) / 64, 0, nullptr,
                 w.partw, parts_of(s.V), w.wt, w.invw};
       tw.tiles = tw.tx * ((s.D + 63) / 64);
     }
@@ -938,21 +914,19 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.lda = d.ldb = d.K;
       d.a[0] = w.p;
       d.b[0] = w.wt;
-      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr, nullptr, nullptr,
-                             vec4(dh, s.D, s.dtype)}, st));
+      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, vec4(dh, s.D, s.dtype)}, st));
     }
     if (dw) {
       d.M = n;
-      d.N = s.D + more;
+      d.N = s.D;
       d.K = P * s.tp;
       d.lda = d.ldb = d.K;
       d.a[0] = w.pt;
       d.b[0] = w.ht;
       TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype, s.D,
-                            more ? (char*)db + (long long)v0 * size : nullptr, ones == 2 ? dloss : nullptr, count,
                             vec4(dw, s.D, s.dtype)}, st));
     }
-    if (db && !ones) {
+    if (db) {
       hipLaunchKernelGGL(bias_kernel<P>, dim3((n + 3) / 4), dim3(256), 0, st, w.pt, s.tp, w.r, s.T, n, db, s.dtype, v0);
       TRY(hipGetLastError());
     }

@@ -190,3 +190,32 @@ def test_newton_schulz_small_and_thin_with_other_coefficients(dtype, shape, coef
             assert _rel(plain[k], want.detach()) < 4 * 2.0 ** -22 * steps * grow + HALF_STEP[dtype]
         size = torch.linalg.vector_norm(dy[k].to(ref.dtype)) / torch.linalg.matrix_norm(x[k].to(ref.dtype))
         assert float(torch.linalg.vector_norm(got[k].cpu().to(ref.dtype) - grad)) < float(size) * 8 * steps * 2.0 ** -22 * grow + HALF_STEP[dtype] * float(grad.norm())
+
+
+# ------------------------------------------------------------------------------------ cross entropy over its range
+def _head(seed, T, D, V, dtype, bias=True):
+    h, w = _rand(seed, T, D).to(dtype), (_rand(seed + 1, V, D) / math.sqrt(D)).to(dtype)
+    y = torch.randint(0, V, (T,), generator=torch.Generator().manual_seed(seed + 2))
+    return h, w, y, (0.3 * _rand(seed + 3, V)).to(dtype) if bias else None
+
+
+def _grads(h, w, y, b, reduction="mean", dloss=None):
+    from tcmi import torchnn
+
+    leaves = [t.cuda().requires_grad_() for t in (h, w, b) if t is not None]
+    loss = torchnn.linear_cross_entropy(leaves[0], leaves[1], y.cuda(), leaves[2] if b is not None else None, reduction=reduction)
+    return torch.autograd.grad(loss, leaves, None if dloss is None else dloss.cuda())
+
+
+@pytest.mark.parametrize("power", [-60, -30, 30, 60])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype,size", [(torch.float32, (64, 32, 128)), (torch.bfloat16, (64, 32, 128)), (torch.float32, (300, 100, 1000)),
+                                        (torch.bfloat16, (200, 64, 500))])
+def test_head_gradients_do_not_depend_on_the_size_of_the_features(size, dtype, bias, power):
+    """h 2^k against w 2^-k has the same logits: dw goes with 2^k, dh with 2^-k and db stays, bit by bit"""
+    h, w, y, b = _head(300, *size, dtype, bias)
+    one = _grads(h, w, y, b)
+    two = _grads(h * 2.0 ** power, w * 2.0 ** -power, y, b)
+    assert torch.equal(two[0] * 2.0 ** power, one[0]) and torch.equal(two[1] * 2.0 ** -power, one[1])
+    if bias:
+        assert torch.equal(two[2], one[2])
