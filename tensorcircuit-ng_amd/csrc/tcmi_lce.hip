@@ -7,9 +7,10 @@
 // Bound by the matrix pipe: 2 T D V multiply-adds forward, 6 T D V more backward.
 //
 // Operand precision.  bf16 / f16 heads: the logits from the inputs as they are (products exact in the f32 accumulator);
-// P is one f16 piece under 2^14 (2^-11 relative; bf16 would cost 2^-8), h and w enter the two gradient products as f16
-// under a power of two taken from their largest value (exact for 8- and 11-bit significands down to 2^-29 of it).
-// f32 heads: two f16 pieces everywhere (2^-22), three products per product.
+// P is one f16 piece (2^-11 relative; bf16 would cost 2^-8, two pieces a second product), h and w enter the two gradient
+// products as f16 under a power of two taken from their largest value (8- and 11-bit significands down to 2^-29 of it).
+// f32 heads: two f16 pieces everywhere (2^-22 down to 2^-17 of what the scale was taken from, 2^-39 of it below), three
+// products per product.  The scales: h and w in the logits per row, P for dh 2^14 (P lies in [-1, 1]), P^T for dw per class.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -23,7 +24,8 @@ namespace lce {
 
 using namespace mm16;
 
-constexpr float PSCALE = 16384.f;            // P lies in [-1, 1]
+constexpr int PEXP = 14;                     // P lies in [-1, 1]
+constexpr float PSCALE = 1 << PEXP;
 constexpr int PARTS = 1024;                   // partial maxima of an operand
 
 template <int DT>
@@ -531,7 +533,37 @@ __global__ __launch_bounds__(1024) void rowstat_total_kernel(const float2* part,
   total_of(s, c, mean, out, count);
 }
 
-// backward: P as f16 pieces, row-major for dh and transposed for dw, zero in the padding and in ignored rows
+// over the 16 lanes of a lane group, the rows of a fragment: by rotations, in registers
+template <int N>
+__device__ __forceinline__ float turned16(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float max16(float v) {
+  v = fmaxf(v, turned16<8>(v));
+  v = fmaxf(v, turned16<4>(v));
+  v = fmaxf(v, turned16<2>(v));
+  return fmaxf(v, turned16<1>(v));
+}
+__device__ __forceinline__ float sum16(float v) {
+  v += turned16<8>(v);
+  v += turned16<4>(v);
+  v += turned16<2>(v);
+  return v + turned16<1>(v);
+}
+
+// Exponent of a class: P^T's entries leave under 2^(16 k), which brings their largest into [2^-1, 2^15); NO_EXP: all are zero.
+constexpr int NO_EXP = 127, EXP_STEP = 16;
+__device__ __forceinline__ int exp_of(float top) {
+  return top == 0.f ? NO_EXP : (14 + 127 - (int)(__float_as_uint(top) >> 23)) >> 4;
+}
+
+// Backward: P as f16 pieces, row-major for dh and transposed for dw, zero in the padding and in ignored rows.
+//   dh  a row's entries under 2^14: what falls below 2^-39 is lost, where P of the target, 1 less than a probability, is off by
+//       2^-24 in any f32 arithmetic.
+//   dw  a class sees its own column of P only, and most classes of a large head are improbable in every row: each class has its
+//       own power of two.  A wave takes it from its rows and leaves it in `exps`; class_kernel brings the waves' rows of a class
+//       to a common one where they differ (by steps of 2^16, so few do).
+// sums: the wave's rows of P r added up, for the bias's gradient.
 template <int P>
 struct EpiProb {
   static constexpr bool TILE = true, FOUR = false;
@@ -542,6 +574,10 @@ struct EpiProb {
   int V;
   f16 *p, *pt;                   // [T][P * vp], [classes][P * tp]
   int vp, tp;                    // padded classes of the piece, padded rows
+  const float* r;
+  signed char* exps;             // [waves' rows][ldv]
+  float* sums;                   // the same
+  int ldv;
   template <class T>
   static constexpr int lds() { return Transposed<T, P>::BYTES; }
   // P goes out from the registers, eight bytes a lane; P^T through LDS, sixteen (from the registers two, which alone took 50 us
@@ -552,39 +588,70 @@ struct EpiProb {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
     const int cl = wn * T::NI * 16 + 4 * (lane >> 4);
     logits<P, T>(q, g, m0, n0, acc);                 // -inf behind the last class: probability 0
-    __syncthreads();
+    f32x4 top[T::NI] = {}, sum[T::NI] = {};
 #pragma unroll
     for (int i = 0; i < T::MI; ++i) {
-      const int rl = wm * T::MI * 16 + i * 16 + (lane & 15), row = m0 + rl;
+      const int row = m0 + wm * T::MI * 16 + i * 16 + (lane & 15);
       const bool in = row < g.M;
       const long long yt = in ? y[row] : ignore;
       const bool keep = in && yt != ignore;
       // a target outside the classes poisons its row
-      const float l = !keep ? 0.f : yt < 0 || yt >= V ? NAN : lse[row];
+      const float l = !keep ? 0.f : yt < 0 || yt >= V ? NAN : lse[row], f = keep ? r[row] : 0.f;
       const int yl = keep ? local_target(yt, q.v0, g.N) : -8;
 #pragma unroll
       for (int j = 0; j < T::NI; ++j) {
         const f32x4 x = acc[i][j];
         f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = keep ? __expf(x[r] - l) * PSCALE : 0.f;        // whatever an ignored row holds
+        for (int r = 0; r < 4; ++r) v[r] = keep ? __expf(x[r] - l) : 0.f;        // whatever an ignored row holds
         const int k = yl - n0 - cl - 16 * j;
         if ((unsigned)k < 4u) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (r == k) v[r] -= PSCALE;
+            if (r == k) v[r] -= 1.f;
         }
         f16x4 vh, vl;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           f16 a, b;
-          two_pieces(v[r], a, b);
+          two_pieces(v[r] * PSCALE, a, b);
           vh[r] = a;
           vl[r] = b;
+          top[j][r] = fmaxf(top[j][r], fabsf(v[r]));
+          sum[j][r] = fmaf(v[r], f, sum[j][r]);
         }
         const int col = n0 + cl + 16 * j;
         if (in && col < vp) store_four<P>(p + (long long)row * P * vp, col, vh, vl);
-        turned.stage(rl, cl + 16 * j, vh, vl);
+        acc[i][j] = v;
+      }
+    }
+    const long long line = (long long)(m0 / (T::MI * 16) + wm) * ldv;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < T::NI; ++j) {
+      int e[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        e[r] = exp_of(max16(top[j][r]));
+        sum[j][r] = sum16(sum[j][r]);
+      }
+      const int col = n0 + cl + 16 * j;
+      if ((lane & 15) == 0 && col < ldv) {
+        *reinterpret_cast<unsigned*>(exps + line + col) =
+            (e[0] & 255) | (e[1] & 255) << 8 | (e[2] & 255) << 16 | (unsigned)(e[3] & 255) << 24;
+        *reinterpret_cast<f32x4*>(sums + line + col) = sum[j];
+      }
+#pragma unroll
+      for (int i = 0; i < T::MI; ++i) {
+        f16x4 vh, vl;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          f16 a, b;
+          two_pieces(ldexpf(acc[i][j][r], e[r] == NO_EXP ? 0 : EXP_STEP * e[r]), a, b);
+          vh[r] = a;
+          vl[r] = b;
+        }
+        turned.stage(wm * T::MI * 16 + i * 16 + (lane & 15), cl + 16 * j, vh, vl);
       }
     }
     __syncthreads();
@@ -592,7 +659,56 @@ struct EpiProb {
   }
 };
 
-// a gradient: value = inv acc (+ what earlier pieces left in `sum`), kept in `sum` or written out times the row's factor
+// 64 classes a workgroup: the class's exponent, the smallest of its waves' (their largest entry stays where it was, a row's
+// further below may lose its last bits, as in any sum with the largest), its rows of P^T brought to it, and the bias's gradient.
+// Reads one value per wave's rows and class; rewrites 0 to 15 % of P^T.
+template <int P>
+__global__ __launch_bounds__(256) void class_kernel(const signed char* exps, const float* sums, int ldv, int chunks, int rows, int n, f16* pt, int tp,
+                                                    int* cexp, void* db, int dtype, int v0) {
+  __shared__ int lo[4][64];
+  __shared__ double part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, v = blockIdx.x * 64 + lane;        // v < ldv
+  int k = NO_EXP;
+  double s = 0.0;
+  for (int c = wave; c < chunks; c += 4) {
+    k = min(k, (int)exps[(long long)c * ldv + v]);
+    if (db) s += sums[(long long)c * ldv + v];
+  }
+  lo[wave][lane] = k;
+  part[wave][lane] = s;
+  __syncthreads();
+  k = min(min(lo[0][lane], lo[1][lane]), min(lo[2][lane], lo[3][lane]));
+  if (wave == 0 && v < n) {
+    if (cexp) cexp[v] = k == NO_EXP ? 0 : EXP_STEP * k;
+    if (db) put(db, dtype, (long long)v0 + v, (float)(part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]));
+  }
+  if (!cexp) return;
+  for (int c = wave; c < chunks; c += 4) {
+    const int e = exps[(long long)c * ldv + v], less = v >= n || e == NO_EXP ? 0 : e - k;
+    unsigned long long todo = __ballot(less > 0);
+    const int len = P * min(rows, tp - c * rows);
+    while (todo) {                                   // four classes at a time, 16 lanes each
+      int mine = -1;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (q == lane >> 4 && todo) mine = __ffsll((long long)todo) - 1;
+        todo &= todo - 1;
+      }
+      const int by = -EXP_STEP * __shfl(less, mine < 0 ? 0 : mine);
+      if (mine < 0) continue;
+      f16* p = pt + (long long)(blockIdx.x * 64 + mine) * P * tp + (long long)P * c * rows;
+      for (int i = 4 * (lane & 15); i < len; i += 64) {
+        f16x4 x = *reinterpret_cast<f16x4*>(p + i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = (f16)ldexpf((float)x[r], by);
+        *reinterpret_cast<f16x4*>(p + i) = x;
+      }
+    }
+  }
+}
+
+// a gradient: value = inv acc 2^-(rexp or 14) (+ what earlier pieces left in `sum`), kept in `sum` or written out times the
+// row's factor
 struct EpiGrad {
   static constexpr bool TILE = false, FOUR = true;
   const float* inv;              // inverse of the other operand's scale, on the device
@@ -601,14 +717,16 @@ struct EpiGrad {
   const float* r;                // null: 1
   void* out;
   int dtype, cols;
+  const int* rexp;               // exponents of the rows of the other operand (null: PSCALE's)
   int vec;                       // rows of `out` and `sum` are aligned for four elements
   __device__ __forceinline__ void four(const Args& g, int, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
-    const float al = *inv * (1.f / PSCALE);
+    const int ex = rexp ? rexp[row] : PEXP;
+    const float al = *inv;
     if (vec && col + 3 < cols) {
       const long long at = (long long)row * cols + col;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] *= al;
+      for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k] * al, -ex);
       if (!first) {
         const f32x4 old = *reinterpret_cast<const f32x4*>(sum + at);
 #pragma unroll
@@ -631,7 +749,7 @@ struct EpiGrad {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (col + k >= g.N) continue;
-      float x = al * v[k];
+      float x = ldexpf(v[k] * al, -ex);
       const long long at = (long long)row * cols + col + k;
       if (!first) x += sum[at];
       if (!last) sum[at] = x;
@@ -639,26 +757,6 @@ struct EpiGrad {
     }
   }
 };
-
-// db_v = sum_t P[t][v] r_t from the transposed pieces (zero behind the last row): one wave per class
-template <int P>
-__global__ __launch_bounds__(256) void bias_kernel(const f16* pt, int tp, const float* r, int T, int vc, void* out, int dtype, int v0) {
-  const int v = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (v >= vc) return;
-  const f16* q = pt + (long long)v * P * tp;
-  float s = 0.f;
-  for (int t = 4 * lane; t < tp; t += 256) {
-    const f16x4 hi = *reinterpret_cast<const f16x4*>(q + kpos<P>(t));
-    f32x4 p = __builtin_convertvector(hi, f32x4);
-    if (P == 2) p += __builtin_convertvector(*reinterpret_cast<const f16x4*>(q + kpos<P>(t) + 32), f32x4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (t + e < T) s = fmaf(p[e], r[t + e], s);
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (lane == 0) put(out, dtype, (long long)v0 + v, s * (1.f / PSCALE));
-}
 
 // ---------------------------------------------------------------------------------------------------------- host side
 struct Arena {
@@ -727,7 +825,13 @@ struct BwdWork {
   Rows rows;
   float *r, *parth, *partw, *invh, *invw, *sum, *split;
   f16 *p, *pt, *ht, *wt;                           // P, P^T, h^T, w^T of the piece
+  signed char* exps;                               // EpiProb's, and what class_kernel makes of them
+  float* sums;
+  int* cexp;
 };
+
+int chunks_of(const Shape& s) { return (s.T + 127) / 128 * 4; }        // at most: the fewest rows a wave has are 32
+
 
 BwdWork take_bwd(Arena& a, const Shape& s) {
   BwdWork w{};
@@ -744,6 +848,10 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
   w.pt = a.take<f16>(vc * s.tp * s.P);
   w.ht = a.take<f16>((long long)s.D * s.tp * s.P);
   w.wt = a.take<f16>(s.D * vp * s.P);
+  const long long ldv = (vc + 63) & ~63ll;
+  w.exps = a.take<signed char>(chunks_of(s) * ldv);
+  w.sums = a.take<float>(chunks_of(s) * ldv);
+  w.cexp = a.take<int>(ldv);
   return w;
 }
 
@@ -888,7 +996,7 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
   TRY(prepare(s, in, w.rows, a, st));
   const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
   for (int v0 = 0; v0 < s.V; v0 += vc) {
-    const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P);
+    const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P), ldv = (n + 63) & ~63;
     Turn th{}, tw{};
     if (dw && v0 == 0) {
       th = Turn{in.h, in.hrs, s.T, s.D, s.tp, vec4(in.h, in.hrs, s.dtype), (s.tp + 63) / 64, 0, w.r, w.parth, parts_of(s.T), w.ht, w.invh};
@@ -902,7 +1010,12 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
     TRY(turn(s, th, tw, st));
     Args g = logit_args(s, in, w.rows, v0, n);
     TRY(run_logits<P>(g, s.dtype,
-                      EpiProb<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.p, w.pt, np, s.tp}, st));
+                      EpiProb<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.p, w.pt, np, s.tp, w.r, w.exps, w.sums, ldv}, st));
+    if (dw || db) {
+      hipLaunchKernelGGL(class_kernel<P>, dim3(ldv / 64), dim3(256), 0, st, w.exps, w.sums, ldv, (s.T + g.wave_rows - 1) / g.wave_rows, g.wave_rows, n,
+                         w.pt, s.tp, dw ? w.cexp : nullptr, db, s.dtype, v0);
+      TRY(hipGetLastError());
+    }
     Args d{};
     d.batch = 1;
     d.nseg = 1;
@@ -914,7 +1027,7 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.lda = d.ldb = d.K;
       d.a[0] = w.p;
       d.b[0] = w.wt;
-      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, vec4(dh, s.D, s.dtype)}, st));
+      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr, vec4(dh, s.D, s.dtype)}, st));
     }
     if (dw) {
       d.M = n;
@@ -923,12 +1036,8 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.lda = d.ldb = d.K;
       d.a[0] = w.pt;
       d.b[0] = w.ht;
-      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype, s.D,
+      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype, s.D, w.cexp,
                             vec4(dw, s.D, s.dtype)}, st));
-    }
-    if (db) {
-      hipLaunchKernelGGL(bias_kernel<P>, dim3((n + 3) / 4), dim3(256), 0, st, w.pt, s.tp, w.r, s.T, n, db, s.dtype, v0);
-      TRY(hipGetLastError());
     }
   }
   return hipSuccess;

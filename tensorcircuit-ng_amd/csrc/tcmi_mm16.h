@@ -43,6 +43,7 @@ struct Args {
   int batch;
   int split;                   // > 1: the k steps are dealt to `split` workgroups, whose sums join_kernel adds
   float* part;                 // [split][batch * tiles][BM * BN]
+  int wave_rows;               // rows of C that one wave holds: an epilogue may leave something per wave and column
 };
 
 // where logical k lies in a row of P pieces (the low piece 32 further), and the padded length of a row
@@ -448,6 +449,7 @@ hipError_t launch(Args& g, bool tri, int split, const Epi& e, hipStream_t st) {
   g.tm = (g.M + T::BM - 1) / T::BM;
   g.tn = (g.N + T::BN - 1) / T::BN;
   g.tri = tri ? 1 : 0;
+  g.wave_rows = T::MI * 16;
   if (g.batch < 1) return hipErrorInvalidValue;
   g.half = halves<T>(g, tri) ? g.doubled : 0;
   const long long units = tile_count<T>(g, tri), tiles = units / g.batch;

@@ -219,3 +219,90 @@ def test_head_gradients_do_not_depend_on_the_size_of_the_features(size, dtype, b
     assert torch.equal(two[0] * 2.0 ** power, one[0]) and torch.equal(two[1] * 2.0 ** -power, one[1])
     if bias:
         assert torch.equal(two[2], one[2])
+
+
+def _head64(h, w, y, b, scale=None):
+    """P with its row factors in 64 bits, on the inputs' device: mean over the rows, or `scale` per row"""
+    z = h.double() @ w.double().T + (0 if b is None else b.double())
+    p = torch.softmax(z, 1)
+    p[torch.arange(len(y)), y] = -torch.where(torch.nn.functional.one_hot(y, z.shape[1]).bool(), 0.0, p).sum(1)
+    r = (torch.full((len(y),), 1.0 / len(y)) if scale is None else scale).to(z)
+    return z, p * r[:, None]
+
+
+def _check_every_class(h, w, y, b, dtype, dloss=None):
+    """Each class's row of dw (and entry of db) against its own size.  P[t][v] is off by twice its logit's error (two pieces
+    per operand: 2^-22 of sum |h||w|, and the sum's sqrt(D) 2^-24; half a step of the logit and of the row's log sum), 2^-22 a unit
+    of exp's argument, and 2^-21 (f32: two pieces and the factor) or 2^-11 (one f16 piece); the target's entry by 2^-23 of 1
+    where the log sum's rounding meets 1 - p; an entry by 2^-24 of its class's largest; the sum over rows by sqrt(T) 2^-22."""
+    from tcmi import torchnn
+
+    leaves = [t.cuda().requires_grad_() for t in (h, w, b) if t is not None]
+    loss = torchnn.linear_cross_entropy(leaves[0], leaves[1], y.cuda(), leaves[2] if b is not None else None, reduction="mean" if dloss is None else "none")
+    got = torch.autograd.grad(loss, leaves, None if dloss is None else dloss.cuda())
+    h, w, y, b = (t if t is None else t.cuda() for t in (h, w, y, b))
+    z, pr = _head64(h, w, y, b, None if dloss is None else dloss.cuda())
+    T, D = h.shape
+    top = float((h.double().abs() @ w.double().abs().T).max())
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    logit = (2.0 ** -22 + math.sqrt(D) * 2.0 ** -24) * top + 2.0 ** -24 * (z.abs() + lse.abs())
+    rel = 2 * logit + 2.0 ** -22 * (z - lse).abs() + (2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11) + math.sqrt(T) * 2.0 ** -22
+    r = (torch.full((T,), 1.0 / T) if dloss is None else dloss).cuda().double().abs()
+    err = pr.abs() * rel
+    rows = torch.arange(T)
+    err[rows, y] += r * (2.0 ** -23 + 2 * logit[rows, y])
+    err += 2.0 ** -24 * pr.abs().amax(0, keepdim=True)
+    half = HALF_STEP[dtype]
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    ref = pr.T @ h.double()
+    slack = torch.linalg.vector_norm(err.T @ h.double().abs(), dim=1) + half * torch.linalg.vector_norm(ref, dim=1) + tiny * math.sqrt(D)
+    off = torch.linalg.vector_norm(got[1].double() - ref, dim=1)
+    assert bool((off <= slack).all()), float((off / slack).max())
+    if b is not None:
+        ref = pr.sum(0)
+        assert bool(((got[2].double() - ref).abs() <= err.sum(0) + half * ref.abs() + tiny).all())
+    return got, pr
+
+
+FALL = (0, 3, 10, 16, 20, 24, 28, 32, 36, 40, 50, 70, 90)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [(1, 24, 650), (70, 40, 650), (300, 64, 1300), (200, 520, 2600)])
+def test_head_gradients_of_improbable_classes(size, dtype):
+    """classes of probability 2^-3 to 2^-90 in every row, each held to its own size"""
+    h, w, y, b = _head(310, *size, dtype)
+    b = (b.float() - math.log(2.0) * torch.tensor(FALL).float().repeat(size[2] // len(FALL))).to(dtype)
+    y = y // len(FALL) * len(FALL)                        # targets among the probable ones
+    got, pr = _check_every_class(h, w, y, b, dtype)
+    if dtype != torch.float16:
+        assert bool((got[1] != 0).any(1).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [40, 129, 300, 1000])
+def test_head_gradients_of_classes_that_few_rows_know(T, dtype):
+    """a class is probable in some rows and at 2^-30 .. 2^-60 in the others, in the same and in other groups of rows"""
+    D, V = 40, 700
+    h, w, y, b = _head(320, T, D, V, dtype)
+    for k, rows in enumerate((slice(0, 20), slice(0, None, 64), slice(T // 2, None), slice(T - 1, None))):
+        h[:, k] = 0.0
+        h[rows, k] = 1.0
+        w[:, k] = -24.0
+        w[torch.arange(k, V, 5), k] = 8.0
+    _check_every_class(h, w, y, b, dtype)
+    g = torch.Generator().manual_seed(321)
+    _check_every_class(h, w, y, b, dtype, dloss=torch.randn(T, generator=g))
+
+
+def test_head_gradients_of_a_million_equal_classes():
+    h, w, y, _ = _head(330, 40, 16, 1 << 20, torch.float32, bias=False)
+    _check_every_class(h * 0.25, w * 0.25, y, None, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_head_gradients_of_certain_rows(dtype):
+    """rows whose loss is 1e-9 to 1e-13: the other classes' gradients against their own size"""
+    h, w, y, _ = _head(340, 96, 64, 500, dtype, bias=False)
+    h = (h.float() * 0.3 + torch.linspace(26.0, 34.0, 96)[:, None] * w[y].float()).to(dtype)
+    _check_every_class(h, w, y, None, dtype)
