@@ -1,6 +1,6 @@
 // Softmax cross entropy of a linear head over many classes, without its logits:
 //   l[t][v] = <h_t, w_v> + b_v,   loss_t = log sum_v exp l[t][v] - l[t][y_t],
-//   P = exp(l - lse) - onehot(y),  dh_t = r_t P_t w,  dw = P^T (r h),  db = P^T r      (r_t = dloss_t, 0 for ignored rows)
+//   P = exp(l - lse) - onehot(y),  dh_t = r_t P_t w,  dw = (r P)^T h,  db = P^T r      (r_t = dloss_t, 0 for ignored rows)
 // Forward: one product on the matrix pipe whose epilogue keeps, per row and tile of classes, the running maximum and the
 // sum of exponentials (T x V / 128 pairs instead of T x V logits).  Backward: per piece of the classes the logits are
 // formed again, become P (f16, row-major and transposed) in the epilogue, and two products use it while it is there.
@@ -10,7 +10,7 @@
 // P is one f16 piece (2^-11 relative; bf16 would cost 2^-8, two pieces a second product), h and w enter the two gradient
 // products as f16 under a power of two taken from their largest value (8- and 11-bit significands down to 2^-29 of it).
 // f32 heads: two f16 pieces everywhere (2^-22 down to 2^-17 of what the scale was taken from, 2^-39 of it below), three
-// products per product.  The scales: h and w in the logits per row, P for dh 2^14 (P lies in [-1, 1]), P^T for dw per class.
+// products per product.  The scales: h and w in the logits per row, P for dh 2^14 (P lies in [-1, 1]), (r P)^T for dw per class.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -77,7 +77,7 @@ __device__ __forceinline__ float scale_of(float top) {
 //   out   the row with k padded.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per row, whose
 //         inverse goes to inv[row] (the second read of the row comes from the cache).
 //   r     h only: the factor of row t in the gradients, from its target and dloss.
-//   part  partial maxima of |x| (h: times |r|; rows whose factor is zero do not count).
+//   part  partial maxima of |x| (h: rows whose factor is zero do not count).
 struct Operand {
   const void* src;
   long long rs;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
       }
 #pragma unroll
       for (int k = 32; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor(t, k));
-      if (f != 0.f) top = fmaxf(top, t * fabsf(f));
+      if (f != 0.f) top = fmaxf(top, t);
     }
     if (!o.out) continue;
     if constexpr (DT == TCMI_F32) {
@@ -161,8 +161,8 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
   if (threadIdx.x == 0) o.part[block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// out[c][row] = src[row][c] * r[row] * scale as f16 pieces (two for f32), rows padded with zeros.  A zero factor gives zero
-// whatever the row holds; an infinity anywhere else makes everything NaN (no scale would hold the rest beside it).
+// out[c][row] = src[row][c] * scale as f16 pieces (two for f32), rows padded with zeros.  A row whose factor r is zero gives
+// zero whatever it holds; an infinity anywhere else makes everything NaN (no scale would hold the rest beside it).
 // 64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
 struct Turn {
   const void* src;
@@ -197,11 +197,10 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
     const int row = r0 + k;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     if (row < a.rows) {
-      const float f = a.r ? a.r[row] : 1.f;
-      if (f != 0.f) {
+      if (!a.r || a.r[row] != 0.f) {
         v = fetch_row4<DT>(a.src, row * a.rs, c0 + u, a.cols, a.vec);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = v[e] * f * s;
+        for (int e = 0; e < 4; ++e) v[e] *= s;
       }
     }
 #pragma unroll
@@ -561,9 +560,10 @@ __device__ __forceinline__ int exp_of(float top) {
 //   dh  a row's entries under 2^14: what falls below 2^-39 is lost, where P of the target, 1 less than a probability, is off by
 //       2^-24 in any f32 arithmetic.
 //   dw  a class sees its own column of P only, and most classes of a large head are improbable in every row: each class has its
-//       own power of two.  A wave takes it from its rows and leaves it in `exps`; class_kernel brings the waves' rows of a class
+//       own power of two.  The rows' factors are in it too: h stays as it is, and a row of a small factor is small in the classes
+//       that others know better, not in all.  A wave takes it from its rows and leaves it in `exps`; class_kernel brings the waves' rows of a class
 //       to a common one where they differ (by steps of 2^16, so few do).
-// sums: the wave's rows of P r added up, for the bias's gradient.
+// sums: the wave's rows added up, for the bias's gradient.
 template <int P>
 struct EpiProb {
   static constexpr bool TILE = true, FOUR = false;
@@ -617,8 +617,9 @@ struct EpiProb {
           two_pieces(v[r] * PSCALE, a, b);
           vh[r] = a;
           vl[r] = b;
+          v[r] = f == 0.f ? 0.f : v[r] * f;
           top[j][r] = fmaxf(top[j][r], fabsf(v[r]));
-          sum[j][r] = fmaf(v[r], f, sum[j][r]);
+          sum[j][r] += v[r];
         }
         const int col = n0 + cl + 16 * j;
         if (in && col < vp) store_four<P>(p + (long long)row * P * vp, col, vh, vl);

@@ -306,3 +306,47 @@ def test_head_gradients_of_certain_rows(dtype):
     h, w, y, _ = _head(340, 96, 64, 500, dtype, bias=False)
     h = (h.float() * 0.3 + torch.linspace(26.0, 34.0, 96)[:, None] * w[y].float()).to(dtype)
     _check_every_class(h, w, y, None, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("power", [-20, -36, -60, 40])
+def test_head_gradients_with_row_factors_of_every_size(dtype, power):
+    """rows 64 .. with a factor of 2^power; classes that only they know, and classes that only the others know"""
+    h, w, y, b = _head(350, 128, 40, 300, dtype)
+    h[:, :2] = 0.0
+    h[:64, 0], h[64:, 1] = 1.0, 1.0
+    w[:, :2] = 4.0
+    w[::3, 0], w[1::3, 1] = -40.0, -40.0
+    y[:64], y[64:] = 1 + y[:64] // 3 * 3, y[64:] // 3 * 3
+    g = torch.Generator().manual_seed(351)
+    d = torch.randn(128, generator=g)
+    d[64:] *= 2.0 ** power
+    d[5] = d[70] = 0.0
+    _check_every_class(h, w, y, b, dtype, dloss=d)
+
+
+@pytest.mark.parametrize("factor", [1.0, 1.0 / 1371, 0.7])
+def test_head_gradients_round_the_probability_and_not_the_features(factor):
+    """one float16 row: dw[v][d] = P_v r h_d is off by one piece of P r (2^-11), by the rounding to float16 (2^-11) and by the
+    logit (2^-24 sum |h||w| (1 + sqrt(D)), twice), element by element; no factor touches h"""
+    h, w, y, _ = _head(360, 1, 200, 900, torch.float16, bias=False)
+    got = _grads(h, w, y, None, "none", torch.tensor([factor]))[1].cpu().double()
+    z, pr = _head64(h, w, y, None, torch.tensor([factor]))
+    want = pr.T @ h.double()
+    top = float((h.double().abs() @ w.double().abs().T).max())
+    rel = (1 + 2.0 ** -11) ** 2 - 1 + 4 * (1 + math.sqrt(200)) * 2.0 ** -24 * top + 2.0 ** -21 * float((z - torch.logsumexp(z, 1, keepdim=True)).abs().max())
+    assert bool(((got - want).abs() <= rel * want.abs() + 2.0 ** -25).all())
+
+
+def test_head_gradients_of_a_row_without_a_share():
+    """a loss factor of zero leaves a row out of every gradient, whatever it holds"""
+    h, w, y, b = _head(370, 50, 32, 200, torch.float32)
+    d = _rand(371, 50)
+    d[7] = d[20] = 0.0
+    bad = h.clone()
+    bad[7, 3], bad[20] = math.nan, math.inf
+    one, two = _grads(h, w, y, b, "none", d), _grads(bad, w, y, b, "none", d)
+    keep = torch.arange(50) != 7
+    keep[20] = False
+    assert torch.equal(one[0][keep], two[0][keep]) and bool((two[0][~keep] == 0).all())
+    assert torch.equal(one[1], two[1]) and torch.equal(one[2], two[2])
