@@ -8,9 +8,11 @@
 //
 // Operand precision.  bf16 / f16 heads: the logits from the inputs as they are (products exact in the f32 accumulator);
 // P is one f16 piece (2^-11 relative; bf16 would cost 2^-8, two pieces a second product), h and w enter the two gradient
-// products as f16 under a power of two taken from their largest value (8- and 11-bit significands down to 2^-29 of it).
+// products as f16, each feature under a power of two taken from its largest value (exact down to 2^-29 of it for 11 bits).
 // f32 heads: two f16 pieces everywhere (2^-22 down to 2^-17 of what the scale was taken from, 2^-39 of it below), three
-// products per product.  The scales: h and w in the logits per row, P for dh 2^14 (P lies in [-1, 1]), (r P)^T for dw per class.
+// products per product.  The scales: h and w in the logits per row, in the gradients per feature, P for dh 2^14 (P lies in [-1, 1]),
+// (r P)^T for dw per class.  So a logit is off by 2^-22 sum |h||w| of the rows' largest, an entry of dw by that share of its class's
+// largest r P times its feature's largest h, of dh by that of the largest w of its feature.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -26,7 +28,7 @@ using namespace mm16;
 
 constexpr int PEXP = 14;                     // P lies in [-1, 1]
 constexpr float PSCALE = 1 << PEXP;
-constexpr int PARTS = 1024;                   // partial maxima of an operand
+constexpr int PARTS = 1024;                   // workgroups of a pass over an operand
 
 template <int DT>
 __device__ __forceinline__ float fetch(const void* p, long long at) {
@@ -77,13 +79,13 @@ __device__ __forceinline__ float scale_of(float top) {
 //   out   the row with k padded.  16-bit types are copied; f32 rows are cut into two pieces under a power of two per row, whose
 //         inverse goes to inv[row] (the second read of the row comes from the cache).
 //   r     h only: the factor of row t in the gradients, from its target and dloss.
-//   part  partial maxima of |x| (h: rows whose factor is zero do not count).
+//   top   cleared, for top_kernel: a word per feature and one more.
 struct Operand {
   const void* src;
   long long rs;
   int rows, cols, colsp, vec, blocks;
   f16* out;
-  float *inv, *part;
+  float* inv;
 };
 
 struct Prep {
@@ -93,25 +95,26 @@ struct Prep {
   const float *dloss, *count;
   int per_row;
   float* r;                      // null: no factors (forward)
+  unsigned* top;
+  int tops;
 };
 
 template <int DT>
 __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
-  __shared__ float red[4];
+  for (int k = blockIdx.x * 256 + threadIdx.x; k < a.tops; k += gridDim.x * 256) a.top[k] = 0;
   const bool is_h = (int)blockIdx.x < a.h.blocks;
   const Operand& o = is_h ? a.h : a.w;
   const int block = is_h ? blockIdx.x : blockIdx.x - a.h.blocks, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float top = 0.f;
   for (int row = block * 4 + wave; row < o.rows; row += o.blocks * 4) {
     const long long in = row * o.rs;
-    float f = 1.f;
     if (is_h && a.r) {
-      f = a.per_row ? a.dloss[row] : a.count ? a.dloss[0] / a.count[0] : a.dloss[0];
+      float f = a.per_row ? a.dloss[row] : a.count ? a.dloss[0] / a.count[0] : a.dloss[0];
       if (a.y[row] == a.ignore) f = 0.f;
       if (lane == 0) a.r[row] = f;
     }
-    float t = 0.f;
-    if ((o.part && f != 0.f) || (o.out && DT == TCMI_F32)) {
+    if (!o.out) continue;
+    if constexpr (DT == TCMI_F32) {
+      float t = 0.f;
 #pragma unroll 4
       for (int c = 4 * lane; c < o.cols; c += 256) {
         const f32x4 v = fetch_row4<DT>(o.src, in, c, o.cols, o.vec);
@@ -119,10 +122,6 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
       }
 #pragma unroll
       for (int k = 32; k > 0; k >>= 1) t = fmaxf(t, __shfl_xor(t, k));
-      if (f != 0.f) top = fmaxf(top, t);
-    }
-    if (!o.out) continue;
-    if constexpr (DT == TCMI_F32) {
       const float s = scale_of(t);
       f16* q = o.out + (long long)row * 2 * o.colsp;
       for (int c = 4 * lane; c < o.colsp; c += 256) {
@@ -155,43 +154,91 @@ __global__ __launch_bounds__(256) void prep_kernel(Prep a) {
       }
     }
   }
-  if (!o.part) return;
-  if (lane == 0) red[wave] = top;
-  __syncthreads();
-  if (threadIdx.x == 0) o.part[block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 
-// out[c][row] = src[row][c] * scale as f16 pieces (two for f32), rows padded with zeros.  A row whose factor r is zero gives
+// Largest |x| of every feature, over the rows that count, and of the whole operand behind them: the gradients' products take
+// each feature under its own power of two.  A thread holds four features and walks down the rows; workgroups join by atomic
+// maxima (of non-negative floats as whole numbers: the order does not matter).  h and w in one launch, at most 64 shares of
+// the rows: 512 of them waited 60 us for each other's atomics.  Bound by its reads.
+struct Top {
+  const void* src;
+  long long rs;
+  int rows, cols, vec, lanes, panels, blocks;        // lanes: threads along a row; panels: of 4 lanes features; blocks = panels * shares of the rows
+  const float* r;                // rows with r = 0 do not count (null: all do)
+  unsigned* top;                 // [cols + 1]
+};
+
+constexpr int TOP_THREADS = 1024, TOP_SHARES = 64;
+
+template <int DT>
+__global__ __launch_bounds__(TOP_THREADS) void top_kernel(Top x, Top y) {
+  __shared__ f32x4 red[TOP_THREADS];
+  const bool first = (int)blockIdx.x < x.blocks;
+  const Top& a = first ? x : y;
+  const int block = first ? blockIdx.x : blockIdx.x - x.blocks, share = block / a.panels, shares = a.blocks / a.panels;
+  const int per = TOP_THREADS / a.lanes, lane = threadIdx.x % a.lanes, c = (block % a.panels * a.lanes + lane) * 4;
+  f32x4 t = {0.f, 0.f, 0.f, 0.f};
+  const bool whole = a.vec && c + 3 < a.cols;
+  if (c < a.cols)
+    for (int row = share * per + threadIdx.x / a.lanes; row < a.rows; row += 8 * shares * per) {
+      f32x4 v[8];                                    // eight rows under way at once; behind the last one that one again
+      float f[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const long long at = min((long long)row + (long long)u * shares * per, a.rows - 1ll);
+        v[u] = whole ? fetch4<DT>(a.src, at * a.rs + c, true) : fetch_row4<DT>(a.src, at * a.rs, c, a.cols, false);
+        f[u] = a.r ? a.r[at] : 1.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], f[u] == 0.f ? 0.f : fabsf(v[u][k]));
+    }
+  red[threadIdx.x] = t;
+  __syncthreads();
+  if ((int)threadIdx.x >= a.lanes || c >= a.cols) return;
+  for (int q = 1; q < per; ++q) {
+    const f32x4 v = red[threadIdx.x + q * a.lanes];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], v[k]);
+  }
+  float all = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (c + k < a.cols) {
+      atomicMax(a.top + c + k, __float_as_uint(t[k]));
+      all = fmaxf(all, t[k]);
+    }
+  if (all == INFINITY) atomicMax(a.top + a.cols, __float_as_uint(all));      // only whether it is finite matters
+}
+
+// the power of two that brings a feature's largest value into [2^14, 2^15)
+__device__ __forceinline__ int feature_exp(unsigned top) { return 14 + 127 - (int)(top >> 23); }
+
+// out[c][row] = src[row][c] 2^exp[c] as f16 pieces (two for f32), rows padded with zeros.  A row whose factor r is zero gives
 // zero whatever it holds; an infinity anywhere else makes everything NaN (no scale would hold the rest beside it).
 // 64 x 64 tiles through LDS, four elements a thread on both sides; h and w in one launch.
 struct Turn {
   const void* src;
   long long rs;
   int rows, cols, rowsp, vec, tx, tiles;
-  const float *r, *part;
-  int nparts;
+  const float* r;
+  const unsigned* top;
   f16* out;
-  float* inv;
 };
 
 template <int DT>
 __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
   constexpr int P = DT == TCMI_F32 ? 2 : 1;
   __shared__ float tile[64][65];
-  __shared__ float red[4];
   const bool first = (int)blockIdx.x < x.tiles;
   const Turn& a = first ? x : y;
   const int tid = threadIdx.x, block = first ? blockIdx.x : blockIdx.x - x.tiles;
-  float top = 0.f;
-  for (int k = tid; k < a.nparts; k += 256) top = fmaxf(top, a.part[k]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if ((tid & 63) == 0) red[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float s = top == INFINITY ? NAN : scale_of(top);
+  const bool lost = a.top[a.cols] != 0;            // an infinity
   const int r0 = block % a.tx * 64, c0 = block / a.tx * 64, u = (tid & 15) * 4, w = tid >> 4;
-  if (block == 0 && tid == 0) *a.inv = 1.f / s;
+  int ex[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) ex[e] = c0 + u + e < a.cols ? feature_exp(a.top[c0 + u + e]) : 0;
 #pragma unroll
   for (int k = w; k < 64; k += 16) {
     const int row = r0 + k;
@@ -200,7 +247,7 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn x, Turn y) {
       if (!a.r || a.r[row] != 0.f) {
         v = fetch_row4<DT>(a.src, row * a.rs, c0 + u, a.cols, a.vec);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= s;
+        for (int e = 0; e < 4; ++e) v[e] = lost ? NAN : ldexpf(v[e], ex[e]);
       }
     }
 #pragma unroll
@@ -708,11 +755,11 @@ __global__ __launch_bounds__(256) void class_kernel(const signed char* exps, con
   }
 }
 
-// a gradient: value = inv acc 2^-(rexp or 14) (+ what earlier pieces left in `sum`), kept in `sum` or written out times the
-// row's factor
+// a gradient: value = acc 2^-(rexp or 14, + the feature's) (+ what earlier pieces left in `sum`), kept in `sum` or written out
+// times the row's factor
 struct EpiGrad {
   static constexpr bool TILE = false, FOUR = true;
-  const float* inv;              // inverse of the other operand's scale, on the device
+  const unsigned* top;           // largest value of each feature of the other operand
   float* sum;                    // f32 [rows][cols] (null: only one piece)
   int first, last;
   const float* r;                // null: 1
@@ -723,11 +770,21 @@ struct EpiGrad {
   __device__ __forceinline__ void four(const Args& g, int, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
     const int ex = rexp ? rexp[row] : PEXP;
-    const float al = *inv;
+    int e4[4];
+    if (col + 3 < cols) {
+      const uint4 t = *reinterpret_cast<const uint4*>(top + col);
+      e4[0] = -(ex + feature_exp(t.x));
+      e4[1] = -(ex + feature_exp(t.y));
+      e4[2] = -(ex + feature_exp(t.z));
+      e4[3] = -(ex + feature_exp(t.w));
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) e4[k] = -(ex + feature_exp(top[min(col + k, cols - 1)]));
+    }
     if (vec && col + 3 < cols) {
       const long long at = (long long)row * cols + col;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k] * al, -ex);
+      for (int k = 0; k < 4; ++k) v[k] = ldexpf(v[k], e4[k]);
       if (!first) {
         const f32x4 old = *reinterpret_cast<const f32x4*>(sum + at);
 #pragma unroll
@@ -750,7 +807,7 @@ struct EpiGrad {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (col + k >= g.N) continue;
-      float x = ldexpf(v[k] * al, -ex);
+      float x = ldexpf(v[k], e4[k]);
       const long long at = (long long)row * cols + col + k;
       if (!first) x += sum[at];
       if (!last) sum[at] = x;
@@ -824,12 +881,15 @@ int piece_of(const Shape& s) {
 
 struct BwdWork {
   Rows rows;
-  float *r, *parth, *partw, *invh, *invw, *sum, *split;
+  float *r, *sum, *split;
+  unsigned* top;                                   // of h's features, then of w's
   f16 *p, *pt, *ht, *wt;                           // P, P^T, h^T, w^T of the piece
   signed char* exps;                               // EpiProb's, and what class_kernel makes of them
   float* sums;
   int* cexp;
 };
+
+int tops_of(const Shape& s) { return (s.D + 4) & ~3; }                // a word per feature and one more, aligned for four
 
 int chunks_of(const Shape& s) { return (s.T + 127) / 128 * 4; }        // at most: the fewest rows a wave has are 32
 
@@ -839,10 +899,7 @@ BwdWork take_bwd(Arena& a, const Shape& s) {
   const long long vc = piece_of(s), vp = kpad(vc, s.P);
   w.rows = take_rows(a, s);
   w.r = a.take<float>(s.T);
-  w.parth = a.take<float>(PARTS);
-  w.partw = a.take<float>(PARTS);
-  w.invh = a.take<float>(1);
-  w.invw = a.take<float>(1);
+  w.top = a.take<unsigned>(2ll * tops_of(s));
   w.sum = vc < s.V ? a.take<float>((long long)s.T * s.D) : nullptr;
   w.split = a.take<float>(PART_BYTES / 4);
   w.p = a.take<f16>(s.T * vp * s.P);
@@ -897,7 +954,7 @@ hipError_t prepare(const Shape& s, const In& in, const Rows& rows, Prep a, hipSt
     o.vec = vec4(src, rs, s.dtype);
     o.out = out;
     o.inv = inv;
-    const bool work = out || o.part || (&o == &a.h && a.r);
+    const bool work = out || (&o == &a.h && a.r);
     o.blocks = !work ? 0 : n / 4 < 1 ? 1 : n / 4 > PARTS ? PARTS : n / 4;
   };
   one(a.h, in.h, in.hrs, s.T, rows.h, rows.hs);
@@ -910,7 +967,25 @@ hipError_t prepare(const Shape& s, const In& in, const Rows& rows, Prep a, hipSt
   return hipGetLastError();
 }
 
-int parts_of(int rows) { return rows / 4 < 1 ? 1 : rows / 4 > PARTS ? PARTS : rows / 4; }
+// workgroups of the pass for the features' largest values
+Top top_of(const Shape& s, const void* src, long long rs, int rows, const float* r, unsigned* top) {
+  Top t{src, rs, rows, s.D, vec4(src, rs, s.dtype), 64, 0, 0, r, top};
+  while (t.lanes > 1 && t.lanes * 2 >= s.D) t.lanes /= 2;        // half of 4 lanes would do
+  t.panels = (s.D + 4 * t.lanes - 1) / (4 * t.lanes);
+  const int per = TOP_THREADS / t.lanes;
+  const int shares = (rows + 8 * per - 1) / (8 * per);           // eight rows a thread at least
+  t.blocks = t.panels * (shares < TOP_SHARES ? shares : TOP_SHARES);
+  return t;
+}
+
+hipError_t tops(const Shape& s, const Top& x, const Top& y, hipStream_t st) {
+  const int blocks = x.blocks + y.blocks;
+  if (!blocks) return hipSuccess;
+  if (s.dtype == TCMI_F32) hipLaunchKernelGGL(top_kernel<TCMI_F32>, dim3(blocks), dim3(TOP_THREADS), 0, st, x, y);
+  else if (s.dtype == TCMI_F16) hipLaunchKernelGGL(top_kernel<TCMI_F16>, dim3(blocks), dim3(TOP_THREADS), 0, st, x, y);
+  else hipLaunchKernelGGL(top_kernel<TCMI_BF16>, dim3(blocks), dim3(TOP_THREADS), 0, st, x, y);
+  return hipGetLastError();
+}
 
 hipError_t turn(const Shape& s, const Turn& x, const Turn& y, hipStream_t st) {
   const int blocks = x.tiles + y.tiles;
@@ -992,20 +1067,21 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
   a.count = count;
   a.per_row = per_row;
   a.r = w.r;
-  if (dw) a.h.part = w.parth;
-  if (dh) a.w.part = w.partw;
+  a.top = w.top;
+  a.tops = 2 * tops_of(s);
   TRY(prepare(s, in, w.rows, a, st));
+  TRY(tops(s, dw ? top_of(s, in.h, in.hrs, s.T, w.r, w.top) : Top{}, dh ? top_of(s, in.w, in.wrs, s.V, nullptr, w.top + tops_of(s)) : Top{}, st));
   const int size = s.dtype == TCMI_F32 ? 4 : 2, vc = piece_of(s);
   for (int v0 = 0; v0 < s.V; v0 += vc) {
     const int n = s.V - v0 < vc ? s.V - v0 : vc, np = (int)kpad(n, P), ldv = (n + 63) & ~63;
     Turn th{}, tw{};
     if (dw && v0 == 0) {
-      th = Turn{in.h, in.hrs, s.T, s.D, s.tp, vec4(in.h, in.hrs, s.dtype), (s.tp + 63) / 64, 0, w.r, w.parth, parts_of(s.T), w.ht, w.invh};
+      th = Turn{in.h, in.hrs, s.T, s.D, s.tp, vec4(in.h, in.hrs, s.dtype), (s.tp + 63) / 64, 0, w.r, w.top, w.ht};
       th.tiles = th.tx * ((s.D + 63) / 64);
     }
     if (dh) {
       tw = Turn{(const char*)in.w + v0 * in.wrs * size, in.wrs, n, s.D, np, vec4(in.w, in.wrs, s.dtype), (np + 63) / 64, 0, nullptr,
-                w.partw, parts_of(s.V), w.wt, w.invw};
+                w.top + tops_of(s), w.wt};
       tw.tiles = tw.tx * ((s.D + 63) / 64);
     }
     TRY(turn(s, th, tw, st));
@@ -1028,7 +1104,7 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.lda = d.ldb = d.K;
       d.a[0] = w.p;
       d.b[0] = w.wt;
-      TRY(run<P>(d, EpiGrad{w.invw, w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr, vec4(dh, s.D, s.dtype)}, st));
+      TRY(run<P>(d, EpiGrad{w.top + tops_of(s), w.sum, v0 == 0, v0 + vc >= s.V, w.r, dh, s.dtype, s.D, nullptr, vec4(dh, s.D, s.dtype)}, st));
     }
     if (dw) {
       d.M = n;
@@ -1037,7 +1113,7 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
       d.lda = d.ldb = d.K;
       d.a[0] = w.pt;
       d.b[0] = w.ht;
-      TRY(run<P>(d, EpiGrad{w.invh, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype, s.D, w.cexp,
+      TRY(run<P>(d, EpiGrad{w.top, nullptr, 1, 1, nullptr, (char*)dw + (long long)v0 * s.D * size, s.dtype, s.D, w.cexp,
                             vec4(dw, s.D, s.dtype)}, st));
     }
   }

@@ -350,3 +350,31 @@ def test_head_gradients_of_a_row_without_a_share():
     keep[20] = False
     assert torch.equal(one[0][keep], two[0][keep]) and bool((two[0][~keep] == 0).all())
     assert torch.equal(one[1], two[1]) and torch.equal(one[2], two[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [(70, 40, 300), (1, 5, 7), (130, 300, 260), (40, 1030, 600), (200, 33, 5000)])
+def test_head_gradients_of_features_of_every_size(size, dtype):
+    """Features from 2^-60 to 1 of the largest, each column of dw and dh against its own size: columns are held under their own
+    powers of two.  The slack: _check_every_class's, and for dh 2^-39 a class where P lies far below 1."""
+    T, D, V = size
+    h, w, y, b = _head(380, T, D, V, dtype)
+    g = torch.Generator().manual_seed(381)
+    h = h * torch.exp2(-torch.randint(0, 61, (D,), generator=g).float()).to(dtype)
+    w = w * torch.exp2(-torch.randint(0, 61, (D,), generator=g).float()).to(dtype)
+    if D > 4:
+        h[:, 3] = 0.0
+        w[:, 4] = 0.0
+    got = [t.double() for t in _grads(h, w, y, b)]
+    h, w, y, b = (t.cuda() for t in (h, w, y, b))
+    z, pr = _head64(h, w, y, b)
+    top = float((h.double().abs() @ w.double().abs().T).max())
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    logit = (2.0 ** -22 + math.sqrt(D) * 2.0 ** -24) * top + 2.0 ** -24 * (z.abs() + lse.abs())
+    err = pr.abs() * (2 * logit + 2.0 ** -22 * (z - lse).abs() + (2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11) + math.sqrt(max(T, V)) * 2.0 ** -22)
+    rows = torch.arange(T)
+    err[rows, y] += (2.0 ** -23 + 2 * logit[rows, y]) / T
+    for k, (mine, ref, slack) in enumerate(((got[1], pr.T @ h.double(), (err + 2.0 ** -24 * pr.abs().amax(0)).T @ h.double().abs()),
+                                            (got[0], pr @ w.double(), (err + 2.0 ** -39 / T) @ w.double().abs()))):
+        off, size = torch.linalg.vector_norm(mine - ref, dim=0), torch.linalg.vector_norm(slack, dim=0) + HALF_STEP[dtype] * torch.linalg.vector_norm(ref, dim=0)
+        assert bool((off <= size).all()), (k, float((off / size).max()))
