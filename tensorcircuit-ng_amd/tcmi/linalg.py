@@ -52,11 +52,26 @@ def _workspace(kind, nbytes, device):
     return w
 
 
+def _no_tangent(*ts) -> None:
+    """refuses operands of ``torch.autograd.forward_ad`` (``torch.func``'s own wrappers refuse by themselves)"""
+    import torch
+    from torch.autograd import forward_ad
+
+    if forward_ad._current_level < 0:                # outside every dual_level
+        return
+    for t in ts:
+        if torch.is_tensor(t) and not torch._C._functorch.is_functorch_wrapped_tensor(t) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("forward-mode derivatives (torch.autograd.forward_ad) are not offered: use backend.jvp, "
+                                      "or reverse mode")
+
+
 def _tracked(*ts) -> bool:
     """True when a result must stay on torch's autograd tape: an operand requires grad (and grad mode is
-    on) or is a ``torch.func`` wrapper, whose storage the C ABI cannot be handed directly."""
+    on) or is a ``torch.func`` wrapper, whose storage the C ABI cannot be handed directly.  A forward-mode tangent would be
+    lost on the way: refused."""
     import torch
 
+    _no_tangent(*ts)
     for t in ts:
         if torch.is_tensor(t):
             if torch._C._functorch.is_functorch_wrapped_tensor(t):

@@ -297,6 +297,7 @@ def muon_step(param: Tensor, grad: Tensor, momentum_buffer: Tensor, lr: float = 
             raise ValueError(f"muon_step: {name} has elements that share memory")
     if momentum_buffer.numel() and momentum_buffer.data_ptr() in (param.data_ptr(), grad.data_ptr()):
         raise ValueError("muon_step: momentum_buffer must not share memory with param or grad")
+    linalg._no_tangent(param, grad, momentum_buffer)
     linalg._need_gpu("muon_step", param, grad, momentum_buffer)
     if param.numel() == 0:
         return

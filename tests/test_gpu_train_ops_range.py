@@ -378,3 +378,22 @@ def test_head_gradients_of_features_of_every_size(size, dtype):
                                             (got[0], pr @ w.double(), (err + 2.0 ** -39 / T) @ w.double().abs()))):
         off, size = torch.linalg.vector_norm(mine - ref, dim=0), torch.linalg.vector_norm(slack, dim=0) + HALF_STEP[dtype] * torch.linalg.vector_norm(ref, dim=0)
         assert bool((off <= size).all()), (k, float((off / size).max()))
+
+
+def test_forward_mode_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    from tcmi import linalg, torchnn
+
+    h, w, y, b = (t.cuda() for t in _head(390, 20, 8, 30, torch.float32))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: linalg.newton_schulz(dual(h)), lambda: torchnn.linear_cross_entropy(dual(h), w, y),
+                     lambda: torchnn.linear_cross_entropy(h, dual(w), y), lambda: torchnn.linear_cross_entropy(h, w, y, dual(b)),
+                     lambda: linalg.matmul(dual(h), dual(w).mT)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert bool(torch.isfinite(linalg.newton_schulz(h)).all())
+    for f in (lambda t: linalg.newton_schulz(t), lambda t: torchnn.linear_cross_entropy(t, w, y)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(f, (h,), (h,))

@@ -166,3 +166,23 @@ def test_newton_schulz_form_goes_by_the_steps_growth():
         assert lib.tcmi_ns_work_bytes(8, 2000, 1, 5, 1, f32, what) >= max(room(8, 2000, 5, what), room(8, 2000, 5, what, (8.0, -2.0, 0.1)))
         assert room(8, 1 << 24, 10, what) > 0 and room(8, 1 << 24, 11, what) == -1
     assert room(24, 28, 5, 9) == -1
+
+
+def test_forward_mode_tangents_are_refused():
+    """the kernels know no tangent: without a refusal it would vanish and the derivative be zero"""
+    from torch.autograd import forward_ad
+
+    x, t = torch.ones(3, 4), torch.ones(3, 4)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, t)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            linalg._tracked(dual)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            linalg._tracked(x, None, dual)
+        for k in range(3):
+            args = [torch.zeros(3, 4) for _ in range(3)]
+            args[k] = forward_ad.make_dual(args[k], t)
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torchnn.muon_step(*args)
+        assert not linalg._tracked(x, 3.0)
+    assert not linalg._tracked(x)
