@@ -95,7 +95,7 @@ def _lce_grad_raw(h, w, target, bias, stat, dloss, ignore_index, reduction, need
     if t == 0:
         return tuple(torch.empty(0, device=dev) if o is None else o.zero_() for o in outs)
     code = linalg._train_code(h)
-    dloss = dloss.to(torch.float32).contiguous()
+    dloss = dloss.to(torch.float32).resolve_neg().contiguous()        # a view that only carries its sign (of an imaginary part)
     L = _lib.lib()
     hp, hs, wp, ws, lse = h.data_ptr(), _row_stride(h), w.data_ptr(), _row_stride(w), stat.data_ptr()
     nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_GRAD)
@@ -214,12 +214,12 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, target: Tensor, bias: Op
     if target.dtype != torch.int64:
         raise TypeError(f"linear_cross_entropy: target must be int64, got {target.dtype}")
     linalg._need_gpu("linear_cross_entropy", input, weight, target, bias)
+    input, w = input.resolve_neg(), weight.resolve_neg()
     h = input if input.dim() == 2 else input.reshape(-1, input.shape[-1])
-    w = weight
     # features contiguous, rows apart (a broadcast or transposed operand is copied; autograd takes its gradient back)
     h = h if h.stride(1) == 1 and h.stride(0) >= h.shape[1] else h.contiguous()
     w = w if w.stride(1) == 1 and w.stride(0) >= w.shape[1] else w.contiguous()
-    b = None if bias is None else bias.contiguous()
+    b = None if bias is None else bias.resolve_neg().contiguous()
     y = (target if target.dim() == 1 else target.reshape(-1)).contiguous()
     args = (h, w, y, b, int(ignore_index), reduction)
     if not linalg._tracked(h, w, b, y):
@@ -293,6 +293,8 @@ def muon_step(param: Tensor, grad: Tensor, momentum_buffer: Tensor, lr: float = 
         raise ValueError(f"muon_step: momentum must lie in [0, 1), lr and weight_decay be finite (got {momentum}, {lr}, {weight_decay})")
     steps, flat = linalg._ns_coefficients(ns_steps, ns_coefficients, eps)
     for name, x in (("param", param), ("momentum_buffer", momentum_buffer)):
+        if x.is_neg():
+            raise ValueError(f"muon_step: {name} is a view that negates its memory")
         if torch._debug_has_internal_overlap(x) == 1:
             raise ValueError(f"muon_step: {name} has elements that share memory")
     if momentum_buffer.numel() and momentum_buffer.data_ptr() in (param.data_ptr(), grad.data_ptr()):

@@ -397,3 +397,29 @@ def test_forward_mode_tangents_are_refused():
     for f in (lambda t: linalg.newton_schulz(t), lambda t: torchnn.linear_cross_entropy(t, w, y)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             torch.func.jvp(f, (h,), (h,))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_head_with_views_that_negate(reduction):
+    """the imaginary part of a conjugate keeps its sign in the view and not in memory: as cotangent, feature, weight, bias"""
+    from tcmi import torchnn
+
+    T = 1 if reduction == "none" else 12
+    h, w, y, b = (t.cuda() for t in _head(400, T, 8, 30, torch.float32))
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = torchnn.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction=reduction)
+    plain = torch.autograd.grad(loss.sum(), leaves, retain_graph=True)
+    # Re(conj(i loss) (1 + 2i)) = 2 loss: the cotangent arrives as the imaginary part of a conjugate
+    twice = (torch.complex(torch.zeros_like(loss), loss).conj() * (1 + 2j)).real.sum()
+    for a, e in zip(torch.autograd.grad(twice, leaves), plain):
+        assert torch.equal(a, 2 * e)
+    base = torchnn.linear_cross_entropy(h, w, y, b, reduction=reduction)
+    for k in range(3):
+        args = [h, w, b]
+        args[k] = torch._neg_view(-args[k])
+        assert args[k].is_neg()
+        assert torch.equal(torchnn.linear_cross_entropy(args[0], args[1], y, args[2], reduction=reduction), base)
+        args[k].requires_grad_()
+        mine = torchnn.linear_cross_entropy(args[0], args[1], y, args[2], reduction=reduction)
+        assert torch.equal(mine.detach(), loss.detach())
+        assert torch.equal(torch.autograd.grad(mine.sum(), args[k])[0], plain[k])

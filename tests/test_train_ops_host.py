@@ -186,3 +186,11 @@ def test_forward_mode_tangents_are_refused():
                 torchnn.muon_step(*args)
         assert not linalg._tracked(x, 3.0)
     assert not linalg._tracked(x)
+
+
+def test_muon_refuses_views_that_negate():
+    z = torch.zeros(3, 4, dtype=torch.complex64).conj().imag
+    assert z.is_neg()
+    for args in ((z, torch.zeros(3, 4), torch.zeros(3, 4)), (torch.zeros(3, 4), torch.zeros(3, 4), z)):
+        with pytest.raises(ValueError, match="negates"):
+            torchnn.muon_step(*args)
