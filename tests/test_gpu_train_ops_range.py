@@ -423,3 +423,108 @@ def test_head_with_views_that_negate(reduction):
         mine = torchnn.linear_cross_entropy(args[0], args[1], y, args[2], reduction=reduction)
         assert torch.equal(mine.detach(), loss.detach())
         assert torch.equal(torch.autograd.grad(mine.sum(), args[k])[0], plain[k])
+
+
+# ------------------------------------------------- float32 stays float32: against the same formula evaluated in float32
+@pytest.mark.parametrize("size", [(16, 257, 130), (17, 257, 130), (64, 64, 128), (129, 100, 257), (33, 192, 1000), (300, 64, 129),
+                                  (257, 320, 3001), (2000, 300, 9000), (130, 65, 70000), (1021, 28, 16384), (4100, 640, 3300), (600, 4096, 90)])
+def test_head_gradients_are_as_near_as_float32(size):
+    """Two-piece products are off by 3 * 2^-22 of their operands at most, where one piece would be by 2.5e-4: the distance to 64
+    bits stays within that and four times what the formula in float32 is off by."""
+    h, w, y, b = _head(410, *size, torch.float32)
+    h[::5] += (3 * math.sqrt(size[1])) * w[y[::5]]
+    got = _grads(h, w, y, b)
+    h, w, y, b = (t.cuda() for t in (h, w, y, b))
+    exact, plain = [], []
+    for out, up in ((exact, torch.float64), (plain, torch.float32)):
+        x, v = h.to(up), w.to(up)
+        p = torch.softmax(x @ v.T + b.to(up), 1)
+        p[torch.arange(len(y)), y] -= 1
+        p /= len(y)
+        out += [p @ v, p.T @ x, p.sum(0)]
+    for mine, want, f32 in zip(got, exact, plain):
+        n = torch.linalg.vector_norm(want)
+        off, usual = float(torch.linalg.vector_norm(mine.double() - want) / n), float(torch.linalg.vector_norm(f32.double() - want) / n)
+        assert off <= 4 * usual + 3 * 2.0 ** -22, (off, usual)
+
+
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (24, 28)), (torch.float32, (31, 700)), (torch.float32, (130, 65)), (torch.float32, (129, 200)),
+                                         (torch.float32, (500, 300)), (torch.float32, (700, 900)), (torch.float32, (1030, 1100)),
+                                         (torch.complex64, (14, 100)), (torch.complex64, (80, 96)), (torch.complex64, (256, 128)), (torch.complex64, (333, 300))])
+def test_newton_schulz_is_as_near_as_float32(shape, dtype):
+    """the result and its gradient, five steps: 20 (40) units of 2^-22, and four times what float32 is off by"""
+    from tcmi import linalg
+
+    x, dy = _rand(420, *shape, dtype=dtype).cuda(), _rand(421, *shape, dtype=dtype).cuda()
+    leaf = x.clone().requires_grad_()
+    out = linalg.newton_schulz(leaf)
+    (grad,) = torch.autograd.grad(out, leaf, dy)
+    refs = []
+    for up in ((torch.complex128, torch.complex64) if x.is_complex() else (torch.float64, torch.float32)):
+        z = x.to(up).requires_grad_()
+        v = z.mT if shape[0] > shape[1] else z
+        v = v / (torch.linalg.matrix_norm(v) + 1e-7)
+        for _ in range(5):
+            s = v @ v.mH
+            v = A * v + (B * s + C * (s @ s)) @ v
+        v = v.mT if shape[0] > shape[1] else v
+        refs.append((v.detach(), torch.autograd.grad(v, z, dy.to(up))[0]))
+    for k, mine in enumerate((out.detach(), grad)):
+        want, f32 = refs[0][k], refs[1][k]
+        n = torch.linalg.vector_norm(want)
+        off, usual = float(torch.linalg.vector_norm(mine.to(want.dtype) - want) / n), float(torch.linalg.vector_norm(f32.to(want.dtype) - want) / n)
+        assert off <= 4 * usual + 20 * (k + 1) * 2.0 ** -22, (k, off, usual)
+
+
+# -------------------------------------------------------------------------------------- the head in torch.func's transforms
+def test_head_in_the_backend_transforms():
+    """vmap over inputs with a shared head, over heads, over everything; value_and_grad, gradients of sums, create_graph refused"""
+    import tcmi as tc
+    from tcmi import torchnn
+
+    T, D, V = 14, 20, 70
+    hs, ws = torch.stack([_rand(430 + k, T, D) for k in range(3)]).cuda(), torch.stack([_rand(440 + k, V, D) / 4 for k in range(3)]).cuda()
+    bs = _rand(450, 3, V).cuda()
+    ys = torch.randint(0, V, (3, T), generator=torch.Generator().manual_seed(451)).cuda()
+    ys[1, 4] = -100
+
+    def one(h, w, y, b, reduction="mean"):
+        return torchnn.linear_cross_entropy(h, w, y, b, reduction=reduction)
+
+    def eager(k, j, i, reduction="mean", cot=None):
+        leaves = [t.detach().clone().requires_grad_() for t in (hs[k], ws[j], bs[j])]
+        loss = one(leaves[0], leaves[1], ys[i], leaves[2], reduction)
+        return loss.detach(), torch.autograd.grad(loss, leaves, torch.ones_like(loss) if cot is None else cot)
+
+    for reduction in ("mean", "sum", "none"):
+        out = torch.func.vmap(lambda h, w, y, b: one(h, w, y, b, reduction))(hs, ws, ys, bs)
+        shared = torch.func.vmap(lambda h, y: one(h, ws[0], y, bs[0], reduction))(hs, ys)
+        heads = torch.func.vmap(lambda w, b: one(hs[0], w, ys[0], b, reduction))(ws, bs)
+        for k in range(3):
+            assert torch.equal(out[k], eager(k, k, k, reduction)[0]) and torch.equal(shared[k], eager(k, 0, k, reduction)[0])
+            assert torch.equal(heads[k], eager(0, k, 0, reduction)[0])
+    v, g = tc.backend.value_and_grad(lambda h, w, b: one(h, w, ys[0], b), argnums=(0, 1, 2))(hs[0], ws[0], bs[0])
+    want, grads = eager(0, 0, 0)
+    assert torch.equal(v, want) and all(torch.equal(a, e) for a, e in zip(g, grads))
+    # per-sample gradients of a shared head
+    per = torch.func.vmap(torch.func.grad(lambda w, b, h, y: one(h, w, y, b), argnums=(0, 1)), in_dims=(None, None, 0, 0))(ws[0], bs[0], hs, ys)
+    for k in range(3):
+        _, (_, dw, db) = eager(k, 0, k)
+        assert torch.equal(per[0][k], dw) and torch.equal(per[1][k], db)
+    # many cotangents of one loss per row
+    _, pull = torch.func.vjp(lambda h, w: one(h, w, ys[1], bs[1], "none"), hs[1], ws[1])
+    cot = _rand(452, 4, T).cuda()
+    dh, dw = torch.func.vmap(pull)(cot)
+    for k in range(4):
+        _, (eh, ew, _) = eager(1, 1, 1, "none", cot[k])
+        assert torch.equal(dh[k], eh) and torch.equal(dw[k], ew)
+    # without a gradient, above the rows of the kernel for few
+    big = _rand(453, 2, 40, D).cuda()
+    yb = torch.randint(0, V, (2, 40), generator=torch.Generator().manual_seed(454)).cuda()
+    out = tc.backend.vmap(lambda h, y: one(h, ws[0], y, bs[0]), vectorized_argnums=(0, 1))(big, yb)
+    for k in range(2):
+        assert torch.equal(out[k], one(big[k], ws[0], yb[k], bs[0]))
+    leaf = hs[0].clone().requires_grad_()
+    (g,) = torch.autograd.grad(one(leaf, ws[0], ys[0], bs[0]), leaf, create_graph=True)
+    with pytest.raises(NotImplementedError, match="once"):
+        g.sum().backward()
