@@ -141,8 +141,25 @@ __global__ __launch_bounds__(256) void sums_kernel(SumArgs a) {
   if (threadIdx.x == 0) a.part[(long long)blockIdx.y * gridDim.x + blockIdx.x] = s;
 }
 
-// 1 / d as f32; 0 for 0, and finite for norms that only subnormal numbers have
-__device__ __forceinline__ float inverse(double d) { return d == 0.0 ? 0.f : d < 3e-39 ? 3e38f : (float)(1.0 / d); }
+// A factor m 2^e, 0.5 <= |m| <= 1: norms and their inverses leave f32's range long before the entries that they scale.
+struct Factor {
+  float m;
+  int e;
+};
+__device__ __forceinline__ float times(float x, Factor f) { return ldexpf(x, f.e) * f.m; }
+__device__ __forceinline__ Factor factor_of(double d) {
+  if (!(fabs(d) < INFINITY)) return {(float)d, 0};
+  int k;
+  const double f = frexp(d, &k);
+  return {(float)f, k};
+}
+// 1 / d; 0 for 0
+__device__ __forceinline__ Factor inverse(double d) {
+  if (d == 0.0 || !(d < INFINITY)) return {d == 0.0 ? 0.f : (float)(1.0 / d), 0};
+  int k;
+  const double f = frexp(d, &k);
+  return {(float)(0.5 / f), 1 - k};
+}
 
 // Operand layout: a 64 x 64 tile of the source becomes f16 pieces, row-major and transposed (both k-contiguous for the
 // products that read them), zero beyond the matrix up to the padded length, and the f32 carry.  Bound by its writes.
@@ -153,7 +170,7 @@ struct PackArgs {
   const double* part;
   int npart;
   float eps, scale;                        // pieces = value * scale
-  float* norm_out;                         // [batch] the norm without eps (may be null)
+  double* norm_out;                        // [batch] the norm without eps (may be null)
   const float* buf;                        // momentum (null: none)
   long long brs, bcs, bbs;
   float rest;
@@ -173,12 +190,12 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
   __shared__ double red[4];
   const unsigned tiles = (unsigned)a.tx * a.ty;
   const int bz = blockIdx.x / tiles, t = blockIdx.x % tiles, i0 = (t / a.tx) * 64, j0 = (t % a.tx) * 64;
-  float inv = 1.f;
+  Factor inv = {1.f, 0};
   if (a.part) {
     double s = 0.0;
     for (int k = threadIdx.x; k < a.npart; k += 256) s += a.part[(long long)bz * a.npart + k];
     const double nrm = sqrt(block_sum(s, red));
-    if (a.norm_out && t == 0 && threadIdx.x == 0) a.norm_out[bz] = (float)nrm;
+    if (a.norm_out && t == 0 && threadIdx.x == 0) a.norm_out[bz] = nrm;
     inv = inverse(nrm + (double)a.eps);
   }
   // 16 threads along an axis, four elements each, 16 lines at a time
@@ -224,7 +241,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     }
   }
   __syncthreads();
-  const float cinv = a.carry_raw ? 1.f : inv;
+  const Factor cinv = a.carry_raw ? Factor{1.f, 0} : inv;
   const bool twice = MAYBE_COMPLEX && a.embed;
   const int mrows = twice ? a.m : (int)kpad(a.m, P), ncols = twice ? a.n : (int)kpad(a.n, P);
   f16 *px = a.x + (long long)bz * a.os, *pt = a.t + (long long)bz * a.ts;
@@ -234,7 +251,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       f16 h, l;
-      two_pieces(v[e] * inv * a.scale, h, l);
+      two_pieces(times(v[e], inv) * a.scale, h, l);
       hi[e] = h;
       lo[e] = l;
     }
@@ -250,12 +267,14 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     }
   };
   auto carry = [&](float* q, int left, f32x4 v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = times(v[e], cinv);
     if (left > 3 && ((uintptr_t)q & 15) == 0) {
-      *reinterpret_cast<f32x4*>(q) = v * cinv;
+      *reinterpret_cast<f32x4*>(q) = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e < left) q[e] = v[e] * cinv;
+        if (e < left) q[e] = v[e];
     }
   };
 #pragma unroll
@@ -381,10 +400,10 @@ struct EpiCarry {
   float* carry;
   long long ld, bs;
   float alpha, beta;
-  const float* dev;              // [batch] further factor of acc held on the device (null: none)
+  const double* dev;             // [batch] further factor of acc held on the device (null: none)
   __device__ __forceinline__ void four(const Args& g, int bz, bool, int row, int col, f32x4 v) const {
     if (row >= g.M) return;
-    const float al = dev ? alpha * dev[bz] : alpha;
+    const float al = dev ? (float)(alpha * dev[bz]) : alpha;
     float* p = carry + bz * bs + row * ld + col;
     if (col + 3 < g.N) {
       f32x4 x = *reinterpret_cast<f32x4*>(p);
@@ -544,18 +563,18 @@ struct EpiOut {
   }
 };
 
-// dG = D / N - G <D, G> / (N^2 |G|); d holds D, or D / dnorm
+// dG = (D - X_0 <D, G> / |G|) / N, X_0 = G / N; d holds D, or D / dnorm
 template <int SRC>
 __global__ __launch_bounds__(256) void grad_out_kernel(Mat gm, const float* d, long long ldd, long long dbs, int m, int n,
-                                                       const double* part, int npart, const float* norm, const float* dnorm, float eps, void* out,
+                                                       const double* part, int npart, const double* norm, const double* dnorm, float eps, void* out,
                                                        long long rs, long long cs, long long os, int dtype) {
   __shared__ double red[4];
   const int bz = blockIdx.y;
   double s = 0.0;
   for (int k = threadIdx.x; k < npart; k += 256) s += part[(long long)bz * npart + k];
   const double inner = block_sum(s, red), nr = norm[bz], full = nr + (double)eps;
-  const double by = dnorm ? (double)dnorm[bz] : 1.0;
-  const float f1 = full == 0.0 ? 0.f : (float)(by / full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * nr));
+  const Factor inv = inverse(full), f1 = factor_of(full == 0.0 ? 0.0 : (dnorm ? dnorm[bz] : 1.0) / full);
+  const float f2 = nr == 0.0 ? 0.f : (float)(inner / nr);
   const long long total = (long long)m * n;
   for (long long k = blockIdx.x * 256ll + threadIdx.x; k < total; k += gridDim.x * 256ll) {
     // the source decides the order: consecutive threads along its contiguous axis
@@ -564,9 +583,9 @@ __global__ __launch_bounds__(256) void grad_out_kernel(Mat gm, const float* d, l
     const float* dd = d + bz * dbs + i * ldd + j;
     const long long at = bz * os + i * rs + j * cs;
     if (SRC == SRC_C64) {
-      ((float2*)out)[at] = make_float2((dd[0] - g.x * f2) * f1, (dd[n] - g.y * f2) * f1);
+      ((float2*)out)[at] = make_float2(times(dd[0] - times(g.x, inv) * f2, f1), times(dd[n] - times(g.y, inv) * f2, f1));
     } else {
-      put(out, dtype, at, (dd[0] - g.x * f2) * f1);
+      put(out, dtype, at, times(dd[0] - times(g.x, inv) * f2, f1));
     }
   }
 }
@@ -579,7 +598,7 @@ struct TurnedArgs {
   long long ldd, dbs;
   int m, n, tx, tiles, npart;
   double* part;                  // [batch][npart]; the sums write it, one value a workgroup
-  const float *norm, *dnorm;
+  const double *norm, *dnorm;
   float eps;
   void* out;
   long long rs, cs, os;
@@ -592,12 +611,14 @@ __global__ __launch_bounds__(256) void turned_kernel(TurnedArgs a) {
   __shared__ double red[4];
   const int bz = blockIdx.y, u = threadIdx.x & 63, w = threadIdx.x >> 6;
   double s = 0.0;
-  float f1 = 0.f, f2 = 0.f;
+  Factor inv = {0.f, 0}, f1 = {0.f, 0};
+  float f2 = 0.f;
   if (OUT) {
     for (int k = threadIdx.x; k < a.npart; k += 256) s += a.part[(long long)bz * a.npart + k];
-    const double inner = block_sum(s, red), nr = a.norm[bz], full = nr + (double)a.eps, by = a.dnorm ? (double)a.dnorm[bz] : 1.0;
-    f1 = full == 0.0 ? 0.f : (float)(by / full);
-    f2 = nr == 0.0 ? 0.f : (float)(inner / (full * nr));
+    const double inner = block_sum(s, red), nr = a.norm[bz], full = nr + (double)a.eps;
+    inv = inverse(full);
+    f1 = factor_of(full == 0.0 ? 0.0 : (a.dnorm ? a.dnorm[bz] : 1.0) / full);
+    f2 = nr == 0.0 ? 0.f : (float)(inner / nr);
   }
   for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {
     const int i0 = t / a.tx * 64, j0 = t % a.tx * 64;
@@ -618,8 +639,8 @@ __global__ __launch_bounds__(256) void turned_kernel(TurnedArgs a) {
       const float x = re[u][k], y = SRC == SRC_C64 ? im[SRC == SRC_C64 ? u : 0][k] : 0.f;
       if constexpr (OUT) {
         const long long at = bz * a.os + i * a.rs + j * a.cs;
-        if constexpr (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2((x - g.x * f2) * f1, (y - g.y * f2) * f1);
-        else put(a.out, a.dtype, at, (x - g.x * f2) * f1);
+        if constexpr (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2(times(x - times(g.x, inv) * f2, f1), times(y - times(g.y, inv) * f2, f1));
+        else put(a.out, a.dtype, at, times(x - times(g.x, inv) * f2, f1));
       } else {
         s += (double)g.x * x + (double)g.y * y;
       }
@@ -673,7 +694,7 @@ struct SmallArgs {
   int dtype, update;
   float keep, rate;
   float* saved;                            // [batch][steps][m][C] iterates, then the norm: [batch] (null: not kept)
-  float* norm;
+  double* norm;
 };
 
 __device__ __forceinline__ f32x4 mfma4(f32x4 a, f32x4 b, f32x4 c) {
@@ -845,9 +866,9 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_kernel(SmallArgs a) {
     embed(X, s.ldx, s, i, j, v);
   }
   const double nrm = sqrt(small_sum(sum, red)), full = nrm + (double)a.eps;
-  if (a.norm && threadIdx.x == 0) a.norm[bz] = (float)nrm;
-  const float inv = inverse(full);
-  for (int k = threadIdx.x; k < s.R16 * s.ldx; k += SMALL_THREADS) X[k] *= inv;
+  if (a.norm && threadIdx.x == 0) a.norm[bz] = nrm;
+  const Factor inv = inverse(full);
+  for (int k = threadIdx.x; k < s.R16 * s.ldx; k += SMALL_THREADS) X[k] = times(X[k], inv);
   __syncthreads();
   for (int t = 0; t < a.steps; ++t) {
     if (a.saved) {
@@ -928,14 +949,15 @@ __global__ __launch_bounds__(SMALL_THREADS) void small_grad_kernel(SmallArgs a) 
     if (SRC == SRC_C64) sum += (double)g.y * D[i * s.ldx + j + s.n];
   }
   const double inner = small_sum(sum, red), nr = a.norm[bz], full = nr + (double)a.eps;
-  const float f1 = inverse(full), f2 = nr == 0.0 ? 0.f : (float)(inner / (full * nr));
+  const Factor f1 = inverse(full);
+  const float f2 = nr == 0.0 ? 0.f : (float)(inner / nr);
   for (int k = threadIdx.x; k < s.m * s.n; k += SMALL_THREADS) {
     int i, j;
     place(k, s.m, s.n, a.flat, i, j);
     const float2 g = fetch<SRC>(a.src.p, bz * a.src.bs + i * a.src.rs + j * a.src.cs);
     const long long at = bz * a.obs + i * a.ors + j * a.ocs;
-    const float x = (D[i * s.ldx + j] - g.x * f2) * f1;
-    if (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2(x, (D[i * s.ldx + j + s.n] - g.y * f2) * f1);
+    const float x = times(D[i * s.ldx + j] - times(g.x, f1) * f2, f1);
+    if (SRC == SRC_C64) ((float2*)a.out)[at] = make_float2(x, times(D[i * s.ldx + j + s.n] - times(g.y, f1) * f2, f1));
     else put(a.out, a.dtype, at, x);
   }
 }
@@ -1324,10 +1346,10 @@ __global__ __launch_bounds__(256) void thin_apply_kernel(ThinArgs a) {
   thin_load<SRC, !GRAD>(X, ld, a, a.g, a.flat, bz, j0, false);
   if (GRAD) thin_load<SRC, false>(D, ld, a, a.dy, a.dflat, bz, j0, false);
   const double full = a.norm[bz] + a.eps;
-  const float inv = inverse(full);
+  const Factor inv = inverse(full);
   const double inv64 = full == 0.0 ? 0.0 : 1.0 / full;
   if constexpr (!WIDE) {
-    for (int k = threadIdx.x; k < R16 * ld; k += 256) X[k] *= inv;
+    for (int k = threadIdx.x; k < R16 * ld; k += 256) X[k] = times(X[k], inv);
     __syncthreads();
   }
   f32x4 res[8];                                    // at most 64 x 128 results: 32 tiles, 8 a wave
@@ -1370,10 +1392,11 @@ __global__ __launch_bounds__(256) void thin_apply_kernel(ThinArgs a) {
       i = k - j * a.m;
     }
     if (j >= cols) continue;
-    const float by = GRAD ? inv : 1.f, x = X[i * ld + j] * by;
+    const Factor by = GRAD ? inv : Factor{1.f, 0};
+    const float x = times(X[i * ld + j], by);
     const long long at = bz * a.obs + i * a.ors + (long long)(j0 + j) * a.ocs;
     if (SRC == SRC_C64) {
-      ((float2*)a.out)[at] = make_float2(x, X[i * ld + j + THIN_COLS] * by);
+      ((float2*)a.out)[at] = make_float2(x, times(X[i * ld + j + THIN_COLS], by));
     } else if (!GRAD && a.update) {
       const float old = SRC == SRC_F32 ? ((float*)a.out)[at] : SRC == SRC_F16 ? (float)((f16*)a.out)[at] : (float)((__bf16*)a.out)[at];
       put(a.out, a.dtype, at, fmaf(a.rate, x, a.keep * old));
@@ -1438,8 +1461,8 @@ Pieces take_pieces(Arena& w, const Shape& s) {
 constexpr int MAX_PART = 1024;
 
 struct Work {
-  double* part;
-  float *norm, *carry, *split;
+  double *part, *norm;
+  float *carry, *split;
   Pieces p;
   f16* t2;                        // X^T changes places with this: a step's product reads one while it writes the other
 };
@@ -1447,7 +1470,7 @@ struct Work {
 Work take_work(Arena& w, const Shape& s, bool saved) {
   Work k{};
   k.part = w.take<double>((long long)s.batch * MAX_PART);
-  k.norm = w.take<float>(s.batch);
+  k.norm = w.take<double>(s.batch);
   k.carry = w.take<float>(s.m * s.ldc * s.batch);
   k.split = w.take<float>(PART_BYTES / 4);
   if (!saved) {
@@ -1458,27 +1481,27 @@ Work take_work(Arena& w, const Shape& s, bool saved) {
 }
 
 struct Saved {
-  float* norm;
+  double* norm;
   Pieces p[TCMI_NS_MAX_STEPS];
 };
 
 Saved take_saved(Arena& w, const Shape& s, int steps) {
   Saved v{};
-  v.norm = w.take<float>(s.batch);
+  v.norm = w.take<double>(s.batch);
   for (int i = 0; i < steps; ++i) v.p[i] = take_pieces(w, s);
   return v;
 }
 
 struct GradWork {
-  double* part;
-  float *norm, *carry, *split;
+  double *part, *norm;
+  float *carry, *split;
   f16 *d, *t, *t2, *s, *q;
 };
 
 GradWork take_grad(Arena& w, const Shape& s) {
   GradWork k{};
   k.part = w.take<double>((long long)s.batch * MAX_PART);
-  k.norm = w.take<float>(s.batch);
+  k.norm = w.take<double>(s.batch);
   k.carry = w.take<float>(s.m * s.ldc * s.batch);
   k.split = w.take<float>(PART_BYTES / 4);
   k.d = w.take<f16>(s.mr * s.np * s.batch);
@@ -1679,12 +1702,13 @@ int small_bytes(const Shape& s, bool grad, double growth) {
 
 // the saved block of the one-workgroup form: norms, then the iterates
 struct SmallSaved {
-  float *norm, *x;
+  double* norm;
+  float* x;
 };
 
 SmallSaved take_small(Arena& w, const Shape& s, int steps) {
   SmallSaved v;
-  v.norm = w.take<float>(s.batch);
+  v.norm = w.take<double>(s.batch);
   v.x = w.take<float>((long long)s.batch * steps * s.m * s.nc);
   return v;
 }

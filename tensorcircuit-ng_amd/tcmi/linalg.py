@@ -55,8 +55,8 @@ def _workspace(kind, nbytes, device):
 def _no_tangent(*ts) -> None:
     """refuses operands of ``torch.autograd.forward_ad`` (``torch.func``'s own wrappers refuse by themselves)"""
     import torch
-    from torch.autograd import forward_ad
 
+    forward_ad = torch.autograd.forward_ad
     if forward_ad._current_level < 0:                # outside every dual_level
         return
     for t in ts:

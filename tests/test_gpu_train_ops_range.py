@@ -528,3 +528,38 @@ def test_head_in_the_backend_transforms():
     (g,) = torch.autograd.grad(one(leaf, ws[0], ys[0], bs[0]), leaf, create_graph=True)
     with pytest.raises(NotImplementedError, match="once"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("power", [-145, -135, 118, 126])
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (20, 30)), (torch.float32, (10, 1500)), (torch.float32, (150, 140)), (torch.float32, (160, 128)),
+                                         (torch.bfloat16, (150, 140)), (torch.complex64, (10, 14)), (torch.complex64, (90, 100)), (torch.complex64, (100, 96))])
+def test_newton_schulz_at_the_ends_of_float32(dtype, shape, power):
+    """entries down to the smallest numbers and up to the largest, where the norm or its inverse is no float32: without eps the
+    result is that of the same entries in the middle of the range"""
+    from tcmi import linalg
+
+    if dtype == torch.bfloat16:                           # its smallest step: below it k 2^power is another matrix
+        power = max(power, -133)
+    # a few bits each, so that no entry rounds at the lower end; 1 to 2.25 at the upper
+    k = torch.randint(-8, 9, shape, generator=torch.Generator().manual_seed(460)).float()
+    x = (k if power < 0 else torch.sign(k + 0.5) * (1 + k.abs() / 8)).to(dtype)
+    if dtype == torch.complex64:
+        x = torch.complex(x.real, torch.randint(-8, 9, shape, generator=torch.Generator().manual_seed(461)).float() / (1 if power < 0 else 16))
+    far = torch.ldexp(torch.view_as_real(x) if x.is_complex() else x.float(), torch.tensor(power if power < 0 else power - 1))
+    far = (torch.view_as_complex(far) if x.is_complex() else far).to(dtype)
+    assert bool((far.abs() > 0).any()) and bool(torch.isfinite(torch.view_as_real(far) if x.is_complex() else far).all())
+    leaf = far.cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf, eps=0.0)
+    near = x.cuda().requires_grad_()
+    ref = linalg.newton_schulz(near, eps=0.0)
+    # the same sums and products up to powers of two; the factor's mantissa may round once more
+    assert _rel(out, ref.detach().cpu()) < 2.0 ** -20 + HALF_STEP[dtype]
+    assert _rel(linalg.newton_schulz(far.cuda(), eps=0.0), linalg.newton_schulz(x.cuda(), eps=0.0).cpu()) < 2.0 ** -20 + HALF_STEP[dtype]
+    # a cotangent that keeps the gradient in range
+    dy = _rand(462, *shape, dtype=dtype).cuda()
+    back = -20 if power < 0 else 20
+    (got,) = torch.autograd.grad(out, leaf, dy * 2.0 ** (back + (-40 if power < 0 else 40)))
+    (want,) = torch.autograd.grad(ref, near, dy * 2.0 ** (back + (-40 if power < 0 else 40)))
+    p = power if power < 0 else power - 1
+    got, want = (torch.view_as_real(t) if t.is_complex() else t for t in (got.cpu(), want.cpu()))
+    assert _rel(torch.ldexp(got.double(), torch.tensor(p)), want.double()) < 2.0 ** -18 + HALF_STEP[dtype]
