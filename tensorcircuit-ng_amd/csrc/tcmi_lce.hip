@@ -494,7 +494,9 @@ __global__ __launch_bounds__(256) void few_kernel(FewArgs<DT> a) {
   a.part[(long long)threadIdx.x * gridDim.x + blockIdx.x] = make_float2(top, sum);
 }
 
-// the loss of row t from its tiles' statistics, by one wave
+// the loss of row t from its tiles' statistics, by one wave.  lse: the log sum as a value and its remainder.  In one float it would
+// be off by 2^-24 of itself, which of a row that is certain to 1e-6 at logits of 20 leaves nothing in 1 - p; with the
+// remainder what is left is the sum's own rounding, 2^-24.
 __device__ __forceinline__ float row_loss(const float2* part, int tiles, const float* target, const long long* y, long long ignore, int t,
                                           int V, float* lse) {
   const int lane = threadIdx.x & 63;
@@ -511,10 +513,10 @@ __device__ __forceinline__ float row_loss(const float2* part, int tiles, const f
   for (int k = lane; k < tiles; k += 64) sum += p[k].x == -INFINITY ? 0.f : p[k].y * expf(p[k].x - at);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  const float l = at + logf(sum);
-  if (lane == 0) lse[t] = l;
+  const float ls = logf(sum), l = at + ls, b = l - at, rest = fabsf(l) < INFINITY ? (at - (l - b)) + (ls - b) : 0.f;
+  if (lane == 0) reinterpret_cast<float2*>(lse)[t] = make_float2(l, rest);
   const long long yt = y[t];
-  return yt == ignore ? 0.f : yt < 0 || yt >= V ? NAN : l - target[t];
+  return yt == ignore ? 0.f : yt < 0 || yt >= V ? NAN : (l - target[t]) + rest;
 }
 
 // sum or mean over the rows that count, in f64 and a fixed order; 16 waves
@@ -615,7 +617,7 @@ template <int P>
 struct EpiProb {
   static constexpr bool TILE = true, FOUR = false;
   Logits q;
-  const float* lse;
+  const float2* lse;
   const long long* y;
   long long ignore;
   int V;
@@ -643,19 +645,20 @@ struct EpiProb {
       const long long yt = in ? y[row] : ignore;
       const bool keep = in && yt != ignore;
       // a target outside the classes poisons its row
-      const float l = !keep ? 0.f : yt < 0 || yt >= V ? NAN : lse[row], f = keep ? r[row] : 0.f;
+      const float2 l = !keep ? float2{0.f, 0.f} : yt < 0 || yt >= V ? float2{NAN, NAN} : lse[row];
+      const float f = keep ? r[row] : 0.f;
       const int yl = keep ? local_target(yt, q.v0, g.N) : -8;
 #pragma unroll
       for (int j = 0; j < T::NI; ++j) {
         const f32x4 x = acc[i][j];
         f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = keep ? __expf(x[r] - l) : 0.f;        // whatever an ignored row holds
+        for (int r = 0; r < 4; ++r) v[r] = keep ? __expf((x[r] - l.x) - l.y) : 0.f;        // whatever an ignored row holds
         const int k = yl - n0 - cl - 16 * j;
         if ((unsigned)k < 4u) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (r == k) v[r] -= 1.f;
+            if (r == k) v[r] = expm1f((x[r] - l.x) - l.y);
         }
         f16x4 vh, vl;
 #pragma unroll
@@ -1087,7 +1090,7 @@ hipError_t backward(const Shape& s, const In& in, const BwdWork& w, const float*
     TRY(turn(s, th, tw, st));
     Args g = logit_args(s, in, w.rows, v0, n);
     TRY(run_logits<P>(g, s.dtype,
-                      EpiProb<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, lse, in.y, in.ignore, s.V, w.p, w.pt, np, s.tp, w.r, w.exps, w.sums, ldv}, st));
+                      EpiProb<P>{{w.rows.hs, w.rows.ws, in.bias, s.dtype, v0}, reinterpret_cast<const float2*>(lse), in.y, in.ignore, s.V, w.p, w.pt, np, s.tp, w.r, w.exps, w.sums, ldv}, st));
     if (dw || db) {
       hipLaunchKernelGGL(class_kernel<P>, dim3(ldv / 64), dim3(256), 0, st, w.exps, w.sums, ldv, (s.T + g.wave_rows - 1) / g.wave_rows, g.wave_rows, n,
                          w.pt, s.tp, dw ? w.cexp : nullptr, db, s.dtype, v0);

@@ -54,7 +54,7 @@ def _row_stride(x):
 
 def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
     """(loss, stat): h [T, D], w [V, D], target [T]; loss is per row for reduction "none".  stat, what the gradient needs: the
-    rows' log sums, how many rows count, and (not "none") the rows' losses"""
+    rows' log sums in two floats, how many rows count, and (not "none") the rows' losses"""
     t, d = h.shape
     v = w.shape[0]
     code = linalg._train_code(h)
@@ -70,7 +70,7 @@ def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
     nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_FOR_GRAD if for_grad else _lib.LCE_ALONE)
     if nbytes < 0:
         raise ValueError(f"linear_cross_entropy: {t} rows, {d} features, {v} classes are out of range")
-    floats = t + 1 if per_row else 2 * t + 1
+    floats = 2 * t + 1 if per_row else 3 * t + 1
     if for_grad:
         stat = torch.empty(floats, dtype=torch.float32, device=h.device)
         work = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
@@ -81,7 +81,7 @@ def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
     with linalg._on(h.device):
         _lib.check(L.tcmi_linear_cross_entropy(
             hp, hs, wp, ws, None if bias is None else bias.data_ptr(), target.data_ptr(), ignore_index, t, d, v, lse,
-            loss.data_ptr() if per_row else lse + 4 * (t + 1), None if per_row else loss.data_ptr(), lse + 4 * t,
+            loss.data_ptr() if per_row else lse + 4 * (2 * t + 1), None if per_row else loss.data_ptr(), lse + 8 * t,
             int(reduction == "mean"), int(for_grad), work.data_ptr(), nbytes, code, linalg._raw_stream(h.device)),
             "tcmi_linear_cross_entropy")
     return loss, stat
@@ -104,7 +104,7 @@ def _lce_grad_raw(h, w, target, bias, stat, dloss, ignore_index, reduction, need
     with linalg._on(dev):
         _lib.check(L.tcmi_linear_cross_entropy_grad(
             hp, hs, wp, ws, None if bias is None else bias.data_ptr(), target.data_ptr(), ignore_index, t, d, v, lse,
-            dloss.data_ptr(), int(reduction == "none"), lse + 4 * t if reduction == "mean" else None, *ptrs, work.data_ptr(),
+            dloss.data_ptr(), int(reduction == "none"), lse + 8 * t if reduction == "mean" else None, *ptrs, work.data_ptr(),
             nbytes, code, linalg._raw_stream(dev)), "tcmi_linear_cross_entropy_grad")
     return tuple(torch.empty(0, device=dev) if o is None else o for o in outs)
 

@@ -563,3 +563,36 @@ def test_newton_schulz_at_the_ends_of_float32(dtype, shape, power):
     p = power if power < 0 else power - 1
     got, want = (torch.view_as_real(t) if t.is_complex() else t for t in (got.cpu(), want.cpu()))
     assert _rel(torch.ldexp(got.double(), torch.tensor(p)), want.double()) < 2.0 ** -18 + HALF_STEP[dtype]
+
+
+@pytest.mark.parametrize("T", [1, 30, 200])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_head_of_rows_that_are_nearly_certain(T, dtype):
+    """Rows with 1 - p of 1e-3 to 1e-6 at logits of 50 to 70.  The sum of exponentials is 1 and a little, off by a few of its
+    rounding, 2^-24 (eight are allowed), and that is all that is lost of 1 - p besides the logits' own error; 2^-24 of the log
+    sum, 64, would be more than 1e-6."""
+    from tcmi import torchnn
+
+    D, V = 100, 2000
+    for k in range(3):
+        h, w, y, _ = _head(470 + 10 * k, T, D, V, dtype, bias=False)
+        wy = w[y].float()
+        h = (torch.linspace(16.0, 23.0, T)[:, None] * wy / wy.square().sum(1, keepdim=True)).to(dtype)
+        leaves = [t.cuda().requires_grad_() for t in (h, w, torch.full((V,), 40.0).to(dtype))]
+        loss = torchnn.linear_cross_entropy(leaves[0], leaves[1], y.cuda(), leaves[2], reduction="none")
+        dh, dw, db = (t.double() for t in torch.autograd.grad(loss.sum(), leaves))
+        h, w, y = h.cuda(), w.cuda(), y.cuda()
+        z, pr = _head64(h, w, y, leaves[2].detach(), torch.ones(T))
+        rows = torch.arange(T)
+        little = -pr[rows, y]
+        assert 1e-8 < float(little.min()) and float(little.max()) < 1e-2
+        top = float((h.double().abs() @ w.double().abs().T).max())
+        logit = (2.0 ** -22 + math.sqrt(D) * 2.0 ** -24) * top + 2.0 ** -24 * 70
+        rel = 2 * logit + 8 * 2.0 ** -24 / little + 2.0 ** -22 * 30 + (2.0 ** -21 if dtype == torch.float32 else 2.0 ** -11)
+        want = -torch.log1p(-little)
+        assert bool(((loss.detach().double() - want).abs() <= little * (2 * logit) + 8 * 2.0 ** -24 + 2.0 ** -23 * want).all())
+        err = pr.abs() * rel[:, None]
+        for mine, ref, slack in ((dh, pr @ w.double(), (err + 2.0 ** -39) @ w.double().abs()),
+                                 (dw, pr.T @ h.double(), (err + 2.0 ** -24 * pr.abs().amax(0)).T @ h.double().abs()), (db, pr.sum(0), err.sum(0))):
+            tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+            assert bool(((mine - ref).abs() <= slack + HALF_STEP[dtype] * ref.abs() + tiny).all())
