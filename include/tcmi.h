@@ -430,8 +430,8 @@ int tcmi_muon_step(void* param, long long p_rs, long long p_cs, long long p_bs, 
 
 /* Softmax cross entropy of a linear head, logits never stored: h [tokens][features], w [classes][features] (row strides
  * h_rs, w_rs; features contiguous), bias [classes] or NULL, all of one dtype (TCMI_F32 / F16 / BF16); target int64.
- * Writes lse[2 tokens] (per row the log of the sum of exponentials, and what its rounding left over), loss[tokens] (f32; 0 for target == ignore_index, NaN for any other target outside [0, classes)) and,
- * with `total` given, the sum (mean = 0) or mean over the rows that count, and their number.  for_grad = 1: lse goes to
+ * Writes lse[2 tokens] (per row the log of the sum of exponentials, and what its rounding left over; 8-byte aligned), loss[tokens]
+ * (f32; 0 for target == ignore_index, NaN for any other target outside [0, classes)) and, with `total` given, the sum (mean = 0) or mean over the rows that count, and their number.  for_grad = 1: lse goes to
  * tcmi_linear_cross_entropy_grad and is formed from the product that forms its logits (0: up to 16 rows read w once, uncopied).
  * No counterpart in the reference: it leaves classical heads to the host framework (tensorcircuit/torchnn.py). */
 #define TCMI_LCE_ALONE 0      /* tcmi_lce_work_bytes' `what`: tcmi_linear_cross_entropy with for_grad = 0 */

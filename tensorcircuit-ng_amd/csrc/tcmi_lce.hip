@@ -1170,7 +1170,7 @@ int tcmi_linear_cross_entropy(const void* h, long long h_rs, const void* w, long
                               long long ignore_index, int tokens, int features, int classes, float* lse, float* loss, float* total,
                               float* count, int mean, int for_grad, void* work, long long work_bytes, int dtype, void* stream) {
   if (!shape_ok(tokens, features, classes, dtype) || !h || !w || !target || !lse || !loss || !work || (total && !count) || h_rs < features ||
-      w_rs < features)
+      w_rs < features || ((uintptr_t)lse & 7))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy: bad argument");
   const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype),
                            !for_grad);
@@ -1188,7 +1188,7 @@ int tcmi_linear_cross_entropy_grad(const void* h, long long h_rs, const void* w,
                                    const float* lse, const float* dloss, int per_row, const float* count, void* dh, void* dw, void* db,
                                    void* work, long long work_bytes, int dtype, void* stream) {
   if (!shape_ok(tokens, features, classes, dtype) || !h || !w || !target || !lse || !dloss || !work || (!dh && !dw && !db) ||
-      h_rs < features || w_rs < features)
+      h_rs < features || w_rs < features || ((uintptr_t)lse & 7))
     return tcmi_set_error_(TCMI_ERR_ARG, "tcmi_linear_cross_entropy_grad: bad argument");
   const Shape s = shape_of(tokens, features, classes, dtype, direct(h, h_rs, features, dtype), direct(w, w_rs, features, dtype), false);
   Arena a{(char*)work};

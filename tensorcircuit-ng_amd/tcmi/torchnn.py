@@ -70,7 +70,7 @@ def _lce_raw(h, w, target, bias, ignore_index, reduction, for_grad):
     nbytes = L.tcmi_lce_work_bytes(hp, hs, wp, ws, t, d, v, code, _lib.LCE_FOR_GRAD if for_grad else _lib.LCE_ALONE)
     if nbytes < 0:
         raise ValueError(f"linear_cross_entropy: {t} rows, {d} features, {v} classes are out of range")
-    floats = 2 * t + 1 if per_row else 3 * t + 1
+    floats = 2 * t + 2 if per_row else 3 * t + 1 + (t + 1) % 2        # even: vmap cuts stacks of them, and the log sums need 8 bytes
     if for_grad:
         stat = torch.empty(floats, dtype=torch.float32, device=h.device)
         work = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
@@ -190,7 +190,17 @@ def linear_cross_entropy(input: Tensor, weight: Tensor, target: Tensor, bias: Op
     over no rows is NaN (its gradients are zero).  Any other target outside ``0 .. classes - 1`` gives NaN, in the loss and
     in the gradients (checked where the targets live, nothing is read out of range).  Classes may be masked by a bias
     of ``-inf``.  A non-finite feature or weight of a row that counts gives NaN, or where the logits it makes are ``-inf`` a
-    class without probability and gradients of NaN.  float64 (``tc.set_dtype("complex128")``) is refused.
+    class without probability and gradients of NaN.  float64 (``tc.set_dtype("complex128")``) is refused, and so are
+    forward-mode tangents.
+
+    The loss stores no logits.  Its gradient stores the probabilities of as many classes as 1 GiB holds, twice (a training step
+    with few rows takes more than its logits would), and copies of operands that are float32 or whose rows are no whole
+    number of 64 features.  ``vmap`` runs one call per element.
+
+    A logit of a float32 head is held to ``2 ** -22`` of its terms, ``2 ** -39`` of its row's largest feature times largest weight:
+    features that are ``2 ** 17`` and more apart and weighted the other way round should be brought to like sizes.  Gradients
+    are held by class and feature, whatever their sizes; those of 16-bit heads multiply probabilities of 11 bits, which
+    with float16 costs up to as much as the rounding of the result.
 
     A training step may be captured into a graph (``torch.cuda.graph``).  As with any operator, let go of eager losses of the
     same leaves first (torch ties a leaf's gradient to the stream of its oldest living graph), or capture

@@ -596,3 +596,33 @@ def test_head_of_rows_that_are_nearly_certain(T, dtype):
                                  (dw, pr.T @ h.double(), (err + 2.0 ** -24 * pr.abs().amax(0)).T @ h.double().abs()), (db, pr.sum(0), err.sum(0))):
             tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
             assert bool(((mine - ref).abs() <= slack + HALF_STEP[dtype] * ref.abs() + tiny).all())
+
+
+@pytest.mark.parametrize("steps", [1, 3, 8, 16])
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (24, 28)), (torch.float32, (9, 2000)), (torch.float32, (1500, 60)), (torch.bfloat16, (40, 900)),
+                                         (torch.float16, (3, 20, 700)), (torch.float32, (2, 100, 90))])
+def test_muon_with_other_numbers_of_steps(shape, dtype, steps):
+    """every form of the orthogonalisation under the optimiser step; the tolerance: 4 units of 2^-22 a step times what the steps
+    can make of them (from the slopes on the singular values that these matrices have), and the rounding of param"""
+    from tcmi import torchnn
+
+    p, g, v = (0.1 * _rand(480, *shape)).to(dtype), _rand(481, *shape).to(dtype), _rand(482, *shape)
+    pd, vd = p.cuda(), v.cuda()
+    torchnn.muon_step(pd, g.cuda(), vd, lr=0.02, weight_decay=0.1, momentum=0.9, ns_steps=steps)
+    wv = 0.9 * v.double() + 0.1 * g.double()
+    u = 0.1 * g.double() + 0.9 * wv
+    m, n = shape[-2:]
+    o = _ns64(u, [DEFAULT] * steps)
+    rate = 0.02 * math.sqrt(max(1.0, m / n))
+    want = (1 - 0.02 * 0.1) * p.double() - rate * o
+    assert float((vd.cpu().double() - wv).norm()) <= 2.0 ** -22 * float(wv.norm())
+    s = torch.linalg.svdvals(u / torch.linalg.matrix_norm(u)[..., None, None]).reshape(-1)
+    grow, total = torch.ones_like(s), torch.ones_like(s)
+    for _ in range(steps):
+        grow = grow * (A + 3 * B * s ** 2 + 5 * C * s ** 4).abs().clamp_min(1.0)
+        total = total + grow
+        s = A * s + B * s ** 3 + C * s ** 5
+    one_piece = 3 * steps * 2.2 * 2.0 ** -11 if dtype == torch.bfloat16 else 0.0
+    tol = min(4 * 2.0 ** -22 * float(total.max()), 1.0) + one_piece
+    half = HALF_STEP[dtype]
+    assert float((pd.cpu().double() - want).norm()) <= rate * tol * float(o.norm()) + (half + 2.0 ** -23) * float(want.norm())
