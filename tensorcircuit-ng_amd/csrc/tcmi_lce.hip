@@ -712,7 +712,7 @@ struct EpiProb {
 
 // 64 classes a workgroup: the class's exponent, the smallest of its waves' (their largest entry stays where it was, a row's
 // further below may lose its last bits, as in any sum with the largest), its rows of P^T brought to it, and the bias's gradient.
-// Reads one value per wave's rows and class; rewrites 0 to 15 % of P^T.
+// Reads one value per wave's rows and class, rewrites what differs: 8192 x 65536 bf16 a tenth of P^T, 2 x 100 us; 15 us at 1021 x 32768.
 template <int P>
 __global__ __launch_bounds__(256) void class_kernel(const signed char* exps, const float* sums, int ldv, int chunks, int rows, int n, f16* pt, int tp,
                                                     int* cexp, void* db, int dtype, int v0) {
