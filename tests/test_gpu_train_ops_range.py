@@ -626,3 +626,39 @@ def test_muon_with_other_numbers_of_steps(shape, dtype, steps):
     tol = min(4 * 2.0 ** -22 * float(total.max()), 1.0) + one_piece
     half = HALF_STEP[dtype]
     assert float((pd.cpu().double() - want).norm()) <= rate * tol * float(o.norm()) + (half + 2.0 ** -23) * float(want.norm())
+
+
+@pytest.mark.parametrize("steps", [11, 16])
+@pytest.mark.parametrize("dtype,shape", [(torch.float32, (1, 3000)), (torch.float32, (5000, 3)), (torch.float32, (3, 8, 5000)), (torch.float16, (33, 2000)),
+                                         (torch.bfloat16, (16, 4500)), (torch.complex64, (1, 2100)), (torch.complex64, (2, 11, 3000)), (torch.float32, (2, 5, 900))])
+def test_newton_schulz_iterated_for_few_rows(dtype, shape, steps):
+    """short sides whose steps are too many for two passes: any number of rows, in the result and its gradient.  4 (8) units of
+    2^-22 a step times what the steps behind it make of them at these singular values; one-piece operands 2^-11 alike"""
+    from tcmi import linalg
+
+    x, dy = _rand(490, *shape, dtype=dtype), _rand(491, *shape, dtype=dtype)
+    coefs = [DEFAULT] * steps
+    leaf = x.cuda().requires_grad_()
+    out = linalg.newton_schulz(leaf, steps)
+    (got,) = torch.autograd.grad(out, leaf, dy.cuda())
+    plain = linalg.newton_schulz(x.cuda(), steps)
+    ref = x.to(torch.complex128 if x.is_complex() else torch.float64).requires_grad_()
+    want = _ns64(ref, coefs)
+    (grad,) = torch.autograd.grad(want, ref, dy.to(ref.dtype))
+    want, r = want.detach(), ref.detach()
+    n = torch.linalg.matrix_norm(r)[..., None, None]
+    s = torch.linalg.svdvals(r / n).reshape(-1)
+    slopes = []
+    for _ in range(steps):
+        slopes.append((A + 3 * B * s ** 2 + 5 * C * s ** 4).abs())
+        s = A * s + B * s ** 3 + C * s ** 5
+    behind, total = torch.ones_like(s), torch.ones_like(s)
+    for slope in reversed(slopes):
+        behind = behind * slope.clamp_min(1.0)
+        total = total + behind
+    unit = float(total.max()) * 4 * 2.0 ** -22
+    half = HALF_STEP[dtype]
+    assert _rel(out, want) < unit + half
+    assert _rel(plain, want) < unit + half + (float(total.max()) * 3 * 2.0 ** -11 if dtype == torch.bfloat16 else 0.0)
+    size = float((torch.linalg.vector_norm(dy.to(ref.dtype)) / n.min()).abs()) * A ** steps
+    assert float(torch.linalg.vector_norm(got.cpu().to(ref.dtype) - grad)) < size * 8 * steps * 2.0 ** -22 + half * float(grad.norm())
